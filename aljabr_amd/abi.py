@@ -98,6 +98,16 @@ class LlamaTensors(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    """aljabr_rocm_kv4_cache: the planes and shape of a 4-bit KV cache."""
+    _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("block_table", _P),
+                ("sequences", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("rows", ctypes.c_int32), ("num_blocks", ctypes.c_int32), ("max_blocks", ctypes.c_int32)]
+
+
+_KV = ctypes.POINTER(Kv4Cache)
+
+
 # name -> (restype, argtypes); every symbol declared in include/aljabr_rocm.h.
 class KernelStat(ctypes.Structure):
     """aljabr_rocm_kernel_stat: one launch group of a profiled decode step."""
@@ -139,6 +149,11 @@ SIGNATURES = {
     "aljabr_rocm_quantize": (_I, [_P, _P, _P, _LL, _I, _I]),
     "aljabr_rocm_attention_gqa": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I]),
     "aljabr_rocm_attention_gqa_noalloc": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I]),
+    "aljabr_rocm_kv4_cache_bytes": (_I, [_KV, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]),
+    "aljabr_rocm_kv4_write": (_I, [_KV, _P, _P, _P, _P, _I, _LL, _LL, _LL, _I]),
+    "aljabr_rocm_kv4_read": (_I, [_P, _P, _KV, _P, _P, _I, _LL, _LL, _LL, _I]),
+    "aljabr_rocm_kv4_attention": (_I, [_P, _P, _KV, _P, _P, _I, _I, _F, _I, _I, _F, _P, _SZ]),
+    "aljabr_rocm_kv4_attention_workspace": (_I, [_KV, _I, _I, ctypes.POINTER(_SZ)]),
     "aljabr_rocm_matvec_tb_pair": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
     "aljabr_rocm_matvec_tb_triple": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I]),
     "aljabr_rocm_matvec_tb_triple_batch": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I]),

@@ -1,0 +1,676 @@
+// kv4_attention.hip - attention over the 4-bit KV cache (layout: kv4.hpp).
+//
+//   out[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(s_j - max s),
+//   s_j = cap(scale * q[t, h] . k_j), over the keys j that row t sees.
+//
+// The rows of a KV head are stacked, r = t * G + g (G = Hq / Hkv). A wave walks
+// tiles of 32 keys and keeps 8 rows as the 16 columns of
+// v_mfma_f32_16x16x32_f16: columns c and c + 8 carry row c's two fp16 parts,
+// so the matrix cores' idle columns buy fp32 accuracy. Both products take the
+// decoded codes as their other operand, straight from the cache:
+//   S[key][row]  = K Q^T: lane (n, h) of a 16-key half holds key n, dwords
+//     [h D/32, (h+1) D/32) of its row: one 16-byte load at D = 128;
+//   O^T[d][row] += V^T P^T: lane (n, h) holds the codes of 8 dims (dword n of
+//     a row) for the 8 keys whose weights its lane group computed, so V is
+//     transposed in registers by taking nibble j of 8 dwords.
+// Any order of the contraction will do as long as both operands agree on it,
+// and the order of the dims in O is undone when it is stored.
+//
+// Decoding: a nibble under an exponent is 1024 + q or 64 + q; subtracting 1032
+// or 72 is exact, times the scale is the value (kv4.hpp): three packed fp16
+// instructions a pair of values.
+//
+// Precision: K and V enter as the fp16 numbers they stand for. A query row is
+// scaled by a power of two to a largest magnitude in [2^14, 2^15) and split
+// into two fp16 parts (2^-23 of each element), a weight times 2^11 likewise;
+// sums are fp32.
+//
+// Keys a row does not see get weight 0, and V rows past a sequence's end may
+// hold anything: their scales are taken as 0. Where a row's tile has a scale
+// that is not finite among keys that only some rows see, the tile's V product
+// is done once per token with that token's keys alone.
+#include <algorithm>
+#include <cmath>
+
+#include "device.hpp"
+#include "internal.hpp"
+#include "kv4.hpp"
+
+namespace aljabr {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kTile = 32;                    // keys a wave takes at once
+constexpr int kMinTiles = kWaves;            // tiles of a workgroup at the least
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kWeightScale = 2048.0f;
+
+struct Params {
+    Kv4View v;
+    float *out;
+    const float *q;
+    const int *lens, *counts;
+    int T, Hq, G, row_groups;
+    float scale, soft_cap;
+    int causal, window;
+    int splits;
+    float *part_o, *part_ml;                 // [b][t][hq][split][D] and (m, l), or null with one split
+};
+
+// A sequence's keys and its rows.
+struct Seq {
+    int n, cnt;
+};
+__device__ __forceinline__ Seq sequence(const Params &p, int b) {
+    Seq s;
+    s.n = min(max(p.lens[b], 0), kv4_capacity(p.v));
+    s.cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+    return s;
+}
+
+// Keys [lo, hi) that row t sees.
+__device__ __forceinline__ void key_range(const Params &p, const Seq &s, int t, int &lo, int &hi) {
+    const int pos = s.n - s.cnt + t;
+    hi = p.causal ? max(pos + 1, 0) : s.n;
+    lo = p.window > 0 ? max(pos - p.window + 1, 0) : 0;
+}
+
+// The tiles of split `split` of rows [r0, r1) (stacked), and how many splits have any.
+__device__ __forceinline__ void split_range(const Params &p, const Seq &s, int r0, int r1, int split, int &t0, int &t1,
+                                            int &used) {
+    int lo, hi, x;
+    key_range(p, s, r0 / p.G, lo, x);
+    key_range(p, s, (r1 - 1) / p.G, x, hi);
+    const int a = lo / kTile, z = hi > lo ? (hi + kTile - 1) / kTile : a;
+    const int per = max(kMinTiles, (z - a + p.splits - 1) / p.splits);
+    used = (z - a + per - 1) / per;
+    t0 = a + split * per;
+    t1 = min(t0 + per, z);
+}
+
+__device__ __forceinline__ half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
+__device__ __forceinline__ uint32_t as_u32(half2v h) { return __builtin_bit_cast(uint32_t, h); }
+__device__ __forceinline__ half2v pair(float a, float b) {
+    return half2v{static_cast<_Float16>(a), static_cast<_Float16>(b)};
+}
+
+// The 8 nibbles of the 16-bit halves of w, in pairs (nibble i of the low half,
+// nibble i of the high half), times the pair of scales d.
+__device__ __forceinline__ void decode8(uint32_t w, half2v d, uint32_t (&r)[4]) {
+    const half2v o10 = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+    const half2v o6 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+    const uint32_t x = w >> 8;
+    r[0] = as_u32((as_half2((w & 0x000f000fu) | 0x64006400u) + o10) * d);
+    r[1] = as_u32((as_half2((w & 0x00f000f0u) | 0x54005400u) + o6) * d);
+    r[2] = as_u32((as_half2((x & 0x000f000fu) | 0x64006400u) + o10) * d);
+    r[3] = as_u32((as_half2((x & 0x00f000f0u) | 0x54005400u) + o6) * d);
+}
+
+__device__ __forceinline__ half8 frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(half8, make_uint4(a, b, c, d));
+}
+
+// x of the lane 8 columns away (the row's other fp16 part).
+__device__ __forceinline__ float other_part(float x) { return dpp_f32<0x128>(x); }
+
+// One lane's share of a tile as loaded.
+template <int D>
+struct Tile {
+    uint32_t k[2][D / 32];       // per 16-key half: this lane's dwords of key n
+    uint32_t v[2][4][D == 256 ? 2 : 1];   // per half and key 4h + r: dword(s) of its dims
+    uint16_t ks[2][D == 256 ? 2 : 1];
+    uint2 vs[2];                 // scales of keys 4h .. 4h + 3
+    bool ok[2];                  // the half's block exists (uniform)
+};
+
+template <int D, bool PAGED>
+__device__ __forceinline__ void load_tile(const Params &p, int b, int kvh, int n_keys, int kt, int n, int h, Tile<D> &x) {
+    constexpr int ND = D / 32;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        int key = kt * kTile + 16 * u;
+        if (key >= n_keys) key = kt * kTile;               // past the end: the tile's first half again, masked
+        int s = b, row = key;
+        x.ok[u] = true;
+        if constexpr (PAGED) {
+            const int blk = key / p.v.R;
+            s = p.v.table[static_cast<long long>(b) * p.v.max_blocks + blk];
+            row = key - blk * p.v.R;
+            x.ok[u] = s >= 0 && s < p.v.num_blocks;
+            if (!x.ok[u]) s = 0;
+        }
+        const long long head = static_cast<long long>(s) * p.v.H + kvh;
+        const uint8_t *kc = p.v.kc + (head * p.v.R + row) * (D / 2);
+        const uint8_t *vc = p.v.vc + (head * p.v.R + row) * (D / 2);
+        const uint16_t *ks = p.v.ks + head * ND * p.v.R + row;
+        const uint16_t *vs = p.v.vs + head * ND * p.v.R + row;
+        const uint32_t *kr = reinterpret_cast<const uint32_t *>(kc + n * (D / 2)) + h * ND;
+        if constexpr (D == 64) {
+            const uint2 a = *reinterpret_cast<const uint2 *>(kr);
+            x.k[u][0] = a.x;
+            x.k[u][1] = a.y;
+            x.ks[u][0] = ks[static_cast<long long>(h >> 1) * p.v.R + n];
+        } else if constexpr (D == 128) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(kr);
+            x.k[u][0] = a.x; x.k[u][1] = a.y; x.k[u][2] = a.z; x.k[u][3] = a.w;
+            x.ks[u][0] = ks[static_cast<long long>(h) * p.v.R + n];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 a = *reinterpret_cast<const uint4 *>(kr + 4 * i);
+                x.k[u][4 * i] = a.x; x.k[u][4 * i + 1] = a.y; x.k[u][4 * i + 2] = a.z; x.k[u][4 * i + 3] = a.w;
+                x.ks[u][i] = ks[static_cast<long long>(2 * h + i) * p.v.R + n];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t *vr = reinterpret_cast<const uint32_t *>(vc + (4 * h + r) * (D / 2));
+            if constexpr (D == 64) {
+                x.v[u][r][0] = vr[n >> 1];
+            } else if constexpr (D == 128) {
+                x.v[u][r][0] = vr[n];
+            } else {
+                const uint2 a = *reinterpret_cast<const uint2 *>(vr + 2 * n);
+                x.v[u][r][0] = a.x;
+                x.v[u][r][1] = a.y;
+            }
+        }
+        const int vg = D == 128 ? n >> 2 : D == 64 ? n >> 3 : n >> 1;
+        x.vs[u] = *reinterpret_cast<const uint2 *>(vs + static_cast<long long>(vg) * p.v.R + 4 * h);
+    }
+}
+
+// O += V^T P^T of a tile: NT column tiles, output tile j holds nibble j of the
+// lanes' dwords (D = 256: j / 8 picks the dword). vd: scales of key pairs.
+template <int D, int NT>
+__device__ __forceinline__ void add_values(const Tile<D> &x, const half2v (&vd)[4], const half8 (&pw)[NT], uint32_t vsel,
+                                           f32x4 (&o)[NT][D / 16]) {
+#pragma unroll
+    for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
+#pragma unroll
+        for (int half = 0; half < (D == 64 ? 1 : 2); ++half) {
+            uint32_t f[4][4];                              // [key pair][nibble]
+#pragma unroll
+            for (int pr = 0; pr < 4; ++pr) {
+                const uint32_t w0 = x.v[pr >> 1][2 * (pr & 1)][i], w1 = x.v[pr >> 1][2 * (pr & 1) + 1][i];
+                const uint32_t sel = D == 64 ? vsel : half ? 0x07060302u : 0x05040100u;
+                decode8(__builtin_amdgcn_perm(w1, w0, sel), vd[pr], f[pr]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const half8 a = frag(f[0][j], f[1][j], f[2][j], f[3][j]);
+#pragma unroll
+                for (int c = 0; c < NT; ++c) {
+                    f32x4 &acc = o[c][8 * i + 4 * half + j];
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pw[c], acc, 0, 0, 0);
+                }
+            }
+        }
+    }
+}
+
+// grid: x split, y KV head * row groups, z sequence.
+template <int D, int NT, bool PAGED>
+__global__ __launch_bounds__(kWaves * 64) void kv4_split_kernel(Params p) {
+    constexpr int ND = D / 32, ROWS = 8 * NT, OT = D / 16;
+    extern __shared__ float smem[];                        // [kWaves][ROWS][D + 2]
+    const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.x, b = blockIdx.z;
+    const int kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y - kvh * p.row_groups) * ROWS;
+    const Seq seq = sequence(p, b);
+    const int total = seq.cnt * p.G;
+    if (r0 >= total) return;
+    const int r1 = min(r0 + ROWS, total);
+    int t0, t1, used;
+    split_range(p, seq, r0, r1, split, t0, t1, used);
+    if (split >= max(used, 1)) return;                     // rows with no key at all: split 0 writes them
+
+    // This lane's columns: row, visible keys, query parts (dword i of the lane's share of a row).
+    int lo[NT], hi[NT];
+    half8 qf[NT][ND];
+    float unscale[NT];
+    int full_lo = 0, full_hi = 0x7fffffff;                 // keys that every row sees
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const int r = min(r0 + 8 * c + (n & 7), r1 - 1);   // columns past the rows repeat the last and are not stored
+        const int t = r / p.G, g = r - t * p.G;
+        key_range(p, seq, t, lo[c], hi[c]);
+        const float *qr = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D;
+        float x[ND][8], top = 0.0f;
+        const float qs = p.scale * kLog2e;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            const int w = h * ND + i;
+            const float4 a = *reinterpret_cast<const float4 *>(qr + 32 * (w >> 2) + 4 * (w & 3));
+            const float4 e = *reinterpret_cast<const float4 *>(qr + 32 * (w >> 2) + 4 * (w & 3) + 16);
+            // decode8's order: nibbles 0 4 1 5 2 6 3 7; even nibbles are dims 0..3 of the dword, odd ones 16..19.
+            x[i][0] = a.x; x[i][1] = a.z; x[i][2] = e.x; x[i][3] = e.z;
+            x[i][4] = a.y; x[i][5] = a.w; x[i][6] = e.y; x[i][7] = e.w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32)) * qs;
+        int e = 0;
+        if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
+        e = e < -100 ? -100 : e;
+        const float up = ldexpf(1.0f, 15 - e);
+        unscale[c] = ldexpf(1.0f, e - 15);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[i][j] * qs * up;
+                const _Float16 first = static_cast<_Float16>(y);
+                qf[c][i][j] = n < 8 ? first : static_cast<_Float16>(y - static_cast<float>(first));
+            }
+    }
+    {
+        int first_lo, first_hi, last_lo, last_hi;
+        key_range(p, seq, r0 / p.G, first_lo, first_hi);
+        key_range(p, seq, (r1 - 1) / p.G, last_lo, last_hi);
+        full_lo = last_lo;
+        full_hi = first_hi;
+    }
+    const float lo_part = n < 8 ? 0.0f : 1.0f;
+    const uint32_t vsel = n & 1 ? 0x07060302u : 0x05040100u;
+
+    f32x4 o[NT][OT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        m[c] = -INFINITY;
+        l[c] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < OT; ++j) o[c][j] = f32x4{};
+    }
+
+    Tile<D> next;
+    if (t0 + wave < t1) load_tile<D, PAGED>(p, b, kvh, seq.n, t0 + wave, n, h, next);
+    for (int kt = t0 + wave; kt < t1; kt += kWaves) {
+        const Tile<D> x = next;
+        if (kt + kWaves < t1) load_tile<D, PAGED>(p, b, kvh, seq.n, kt + kWaves, n, h, next);
+        const int k0 = kt * kTile;
+        const bool whole = k0 >= full_lo && k0 + kTile <= full_hi && x.ok[0] && x.ok[1];   // every row sees every key
+
+        // S of the two halves: accumulator r is key k0 + 16u + 4h + r of this lane's column.
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) s[c][u] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                const _Float16 d1 = __builtin_bit_cast(_Float16, x.ks[u][D == 256 ? i / 4 : 0]);
+                uint32_t f[4];
+                decode8(x.k[u][i], half2v{d1, d1}, f);
+                const half8 a = frag(f[0], f[1], f[2], f[3]);
+#pragma unroll
+                for (int c = 0; c < NT; ++c) s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[c][i], s[c][u], 0, 0, 0);
+            }
+        }
+        half8 pw[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            float y[8], mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float raw = s[c][i >> 2][i & 3];
+                y[i] = (raw + other_part(raw)) * unscale[c];
+            }
+            if (p.soft_cap > 0.0f) {
+                const float cap = p.soft_cap * kLog2e;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = cap * tanhf(y[i] / cap);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = k0 + 16 * (i >> 2) + 4 * h + (i & 3);
+                    if (key < lo[c] || key >= hi[c] || !x.ok[i >> 2]) y[i] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, y[i]);
+            // The reference m of a column is raised only when a score exceeds it by more than 2.
+            if (__any(mx > m[c] + 2.0f)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                if (mx > m[c] + 2.0f) {
+                    const float alpha = __builtin_amdgcn_exp2f(m[c] - mx);       // 0 while m is -inf
+                    l[c] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < OT; ++j) o[c][j] *= alpha;
+                    m[c] = mx;
+                }
+            }
+            const float ref = m[c] == -INFINITY ? 0.0f : m[c];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = __builtin_amdgcn_exp2f(y[i] - ref) * kWeightScale;
+                l[c] += y[i];
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const half2v first = pair(y[2 * i], y[2 * i + 1]);
+                w[i] = as_u32(pair(fmaf(static_cast<float>(first[0]), -lo_part, y[2 * i]),
+                                   fmaf(static_cast<float>(first[1]), -lo_part, y[2 * i + 1])));
+            }
+            pw[c] = frag(w[0], w[1], w[2], w[3]);
+        }
+
+        half2v vd[4] = {as_half2(x.vs[0].x), as_half2(x.vs[0].y), as_half2(x.vs[1].x), as_half2(x.vs[1].y)};
+        if (whole) {
+            add_values<D, NT>(x, vd, pw, vsel, o);
+        } else {
+            // Scales of keys outside every row's range, or on no block, are 0.
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = k0 + 16 * (i >> 2) + 4 * h + (i & 3);
+                if (key >= seq.n || !x.ok[i >> 2]) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
+                const uint16_t bits = __builtin_bit_cast(uint16_t, vd[i >> 1][i & 1]);
+                odd |= (bits & 0x7c00u) == 0x7c00u;
+            }
+            if (!__any(odd)) {
+                add_values<D, NT>(x, vd, pw, vsel, o);
+            } else {
+                // Token by token: its keys' values alone, and only its rows take the sums.
+                for (int t = r0 / p.G; t <= (r1 - 1) / p.G; ++t) {
+                    int a, z;
+                    key_range(p, seq, t, a, z);
+                    half2v mine[4];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int key = k0 + 16 * (i >> 2) + 4 * h + (i & 3);
+                        mine[i >> 1][i & 1] = key >= a && key < z ? vd[i >> 1][i & 1] : static_cast<_Float16>(0.0f);
+                    }
+                    f32x4 sum[NT][OT];
+#pragma unroll
+                    for (int c = 0; c < NT; ++c)
+#pragma unroll
+                        for (int j = 0; j < OT; ++j) sum[c][j] = o[c][j];
+                    add_values<D, NT>(x, mine, pw, vsel, sum);
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) {
+                        const int r = min(r0 + 8 * c + (n & 7), r1 - 1);
+                        if (r / p.G == t)
+#pragma unroll
+                            for (int j = 0; j < OT; ++j) o[c][j] = sum[c][j];
+                    }
+                }
+            }
+        }
+    }
+
+    // The wave's state to LDS: O^T tile j, accumulator r: nibble j of dword 4h + r (D = 64: of 16-bit piece 4h + r;
+    // D = 256: of dword 2 (4h + r) + j / 8).
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        if (m[c] == -INFINITY && l[c] != l[c]) m[c] = 0.0f;   // a NaN score alone leaves no reference: any finite one carries it
+        float *st = smem + (wave * ROWS + 8 * c + (n & 7)) * (D + 2);
+#pragma unroll
+        for (int j = 0; j < OT; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float val = o[c][j][r] + other_part(o[c][j][r]);
+                const int piece = 4 * h + r;
+                const int w = D == 128 ? piece : D == 64 ? piece >> 1 : 2 * piece + (j >> 3);
+                const int x = D == 64 ? 4 * (piece & 1) + j : j & 7;           // nibble of dword w
+                if (n < 8) st[32 * (w >> 2) + 16 * (x & 1) + 4 * (w & 3) + (x >> 1)] = val;
+            }
+        if (lane < 8) {
+            st[D] = m[c];
+            st[D + 1] = l[c];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * D; i += kWaves * 64) {
+        const int r = r0 + i / D, dd = i % D;
+        if (r >= r1) break;
+        float M = -INFINITY, mw[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            mw[w] = smem[(w * ROWS + i / D) * (D + 2) + D];
+            M = fmaxf(M, mw[w]);
+        }
+        float L = 0.0f, O = 0.0f;
+        if (M != -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float *st = smem + (w * ROWS + i / D) * (D + 2);
+                const float f = mw[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw[w] - M);
+                L = fmaf(st[D + 1], f, L);
+                O = fmaf(st[dd], f, O);
+            }
+        }
+        const int t = r / p.G, g = r - t * p.G;
+        const long long row = (static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g;
+        if (p.splits == 1) {
+            p.out[row * D + dd] = L == 0.0f ? 0.0f : O / L;
+        } else {
+            p.part_o[(row * p.splits + split) * D + dd] = O;
+            if (dd == 0) {
+                p.part_ml[(row * p.splits + split) * 2] = M;
+                p.part_ml[(row * p.splits + split) * 2 + 1] = L;
+            }
+        }
+    }
+}
+
+// One workgroup a row: D/4 lanes take a split's partial as float4s, 256 / (D/4)
+// splits at once, folded in split order and then across the lane groups.
+// `rows_per_group`: stacked rows whose splits the split kernel chose together.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(Params p, int rows_per_group) {
+    constexpr int LPS = D / 4, SG = 256 / LPS;
+    __shared__ float st[SG * (D + 2)];
+    const int hq = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
+    const Seq seq = sequence(p, b);
+    if (t >= seq.cnt) return;
+    const int total = seq.cnt * p.G, r = t * p.G + hq % p.G;
+    const int r0 = r / rows_per_group * rows_per_group, r1 = min(r0 + rows_per_group, total);
+    int t0, t1, used;
+    split_range(p, seq, r0, r1, 0, t0, t1, used);
+    used = max(used, 1);
+    const long long row = (static_cast<long long>(b) * p.T + t) * p.Hq + hq;
+    const float *po = p.part_o + row * p.splits * D, *pm = p.part_ml + row * p.splits * 2;
+    const int sg = threadIdx.x / LPS, j = threadIdx.x % LPS;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int U = 8;                                   // splits in flight per lane group
+    for (int s0 = sg; s0 < used; s0 += U * SG) {
+        float ms[U], ls[U];
+        float4 os[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + u * SG < used ? s0 + u * SG : sg;
+            ms[u] = pm[2 * s];
+            ls[u] = pm[2 * s + 1];
+            os[u] = *reinterpret_cast<const float4 *>(po + s * D + 4 * j);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u * SG >= used) break;
+            const float mn = fmaxf(m, ms[u]);
+            if (mn == -INFINITY) continue;
+            const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float e = ms[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[u] - mn);
+            l = fmaf(l, a, ls[u] * e);
+            o.x = fmaf(o.x, a, os[u].x * e);
+            o.y = fmaf(o.y, a, os[u].y * e);
+            o.z = fmaf(o.z, a, os[u].z * e);
+            o.w = fmaf(o.w, a, os[u].w * e);
+            m = mn;
+        }
+    }
+    float *my = st + sg * (D + 2);
+    my[4 * j] = o.x;
+    my[4 * j + 1] = o.y;
+    my[4 * j + 2] = o.z;
+    my[4 * j + 3] = o.w;
+    if (j == 0) {
+        my[D] = m;
+        my[D + 1] = l;
+    }
+    __syncthreads();
+    for (int dd = threadIdx.x; dd < D; dd += 256) {
+        float M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int g = 0; g < SG; ++g) M = fmaxf(M, st[g * (D + 2) + D]);
+        if (M != -INFINITY) {
+#pragma unroll
+            for (int g = 0; g < SG; ++g) {
+                const float mg = st[g * (D + 2) + D];
+                if (mg == -INFINITY) continue;
+                const float e = __builtin_amdgcn_exp2f(mg - M);
+                L = fmaf(st[g * (D + 2) + D + 1], e, L);
+                O = fmaf(st[g * (D + 2) + dd], e, O);
+            }
+        }
+        p.out[row * D + dd] = L == 0.0f ? 0.0f : O / L;
+    }
+}
+
+// Rows a workgroup of the split kernel stacks: 16 where there are more than 8 (and the state fits LDS).
+int stacked_rows(int rows, int D) { return rows > 8 && D < 256 ? 16 : 8; }
+
+template <int D, int NT>
+void launch_split(const Params &p, hipStream_t s) {
+    const size_t lds = static_cast<size_t>(kWaves) * 8 * NT * (D + 2) * sizeof(float);
+    const dim3 grid(p.splits, p.v.H * p.row_groups, p.v.B);
+    if (p.v.table)
+        hipLaunchKernelGGL((kv4_split_kernel<D, NT, true>), grid, dim3(kWaves * 64), lds, s, p);
+    else
+        hipLaunchKernelGGL((kv4_split_kernel<D, NT, false>), grid, dim3(kWaves * 64), lds, s, p);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((kv4_merge_kernel<D>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p, 8 * NT);
+}
+
+// Splits: enough workgroups for two a CU, none below kMinTiles tiles of the longest sequence.
+int choose_splits(const Kv4View &v, int T, int Hq) {
+    const int rows = T * (Hq / v.H), per = stacked_rows(rows, v.D);
+    const long long items = static_cast<long long>(v.B) * v.H * ((rows + per - 1) / per);
+    const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    const long long most = (kv4_capacity(v) + kTile * kMinTiles - 1) / (kTile * kMinTiles);
+    long long splits = (2 * cus + items - 1) / items;
+    splits = std::min(splits, most);
+    return static_cast<int>(std::max(splits, 1LL));
+}
+
+}  // namespace
+
+size_t kv4_attention_scratch_bytes(const Kv4View &v, int T, int Hq) {
+    const int splits = choose_splits(v, T, Hq);
+    return splits > 1 ? static_cast<size_t>(v.B) * T * Hq * splits * (v.D + 2) * sizeof(float) : 0;
+}
+
+int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
+    Params p{};
+    p.v = v;
+    p.out = a.out;
+    p.q = a.q;
+    p.lens = a.lens;
+    p.counts = a.counts;
+    p.T = a.T;
+    p.Hq = a.Hq;
+    p.G = a.Hq / v.H;
+    p.scale = a.scale;
+    p.soft_cap = a.soft_cap;
+    p.causal = a.causal;
+    p.window = a.window;
+    const long long rows = static_cast<long long>(a.T) * p.G;
+    const int per = stacked_rows(static_cast<int>(rows), v.D);
+    const long long groups = (rows + per - 1) / per * v.H;
+    if (a.T > 65535 || a.Hq > 65535 || groups > 65535)
+        return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv4_attention: %lld stacked rows are more than one launch takes", rows * v.H);
+    p.row_groups = static_cast<int>((rows + per - 1) / per);
+    p.splits = choose_splits(v, a.T, a.Hq);
+    const size_t one = static_cast<size_t>(v.B) * a.T * a.Hq * (v.D + 2) * sizeof(float);
+    float *part = a.scratch;
+    if (p.splits > 1) {
+        if (a.scratch) {
+            const size_t fit = a.scratch_bytes / one;
+            if (static_cast<size_t>(p.splits) > fit) p.splits = fit < 2 ? 1 : static_cast<int>(fit);
+        } else {
+            part = static_cast<float *>(stream_scratch(one * p.splits));
+            if (!part) return ALJABR_ROCM_ERR_BUFFER;
+        }
+    }
+    if (p.splits > 1) {
+        p.part_o = part;
+        p.part_ml = part + static_cast<size_t>(v.B) * a.T * a.Hq * p.splits * v.D;
+    }
+    hipStream_t s = current_stream();
+    if (v.D == 64) per == 8 ? launch_split<64, 1>(p, s) : launch_split<64, 2>(p, s);
+    else if (v.D == 128) per == 8 ? launch_split<128, 1>(p, s) : launch_split<128, 2>(p, s);
+    else launch_split<256, 1>(p, s);
+    return ALJABR_ROCM_OK;
+}
+
+}  // namespace aljabr
+
+using namespace aljabr;
+
+namespace {
+
+int check_attention(const aljabr_rocm_kv4_cache *cache, int T, int Hq, Kv4View &v) {
+    const int rc = kv4_view(cache, "kv4_attention", v);
+    if (rc != ALJABR_ROCM_OK) return rc;
+    ALJ_REQUIRE(T > 0 && Hq > 0 && Hq % v.H == 0, "kv4_attention: T = %d must be positive and Hq = %d a multiple of %d KV heads",
+                T, Hq, v.H);
+    ALJ_REQUIRE(static_cast<long long>(T) * Hq <= (1 << 30), "kv4_attention: T * Hq exceeds 2^30");
+    return ALJABR_ROCM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int aljabr_rocm_kv4_attention_workspace(const aljabr_rocm_kv4_cache *cache, int T, int Hq, size_t *bytes) {
+    ALJ_REQUIRE(bytes, "kv4_attention_workspace: bytes is null");
+    Kv4View v;
+    const int rc = check_attention(cache, T, Hq, v);
+    if (rc != ALJABR_ROCM_OK) return rc;
+    ALJ_CHECK_READY();
+    *bytes = kv4_attention_scratch_bytes(v, T, Hq);
+    return ALJABR_ROCM_OK;
+}
+
+int aljabr_rocm_kv4_attention(void *out, const void *Q, const aljabr_rocm_kv4_cache *cache, const int *context_lens,
+                              const int *counts, int T, int Hq, float scale, int is_causal, int window, float soft_cap,
+                              void *workspace, size_t workspace_bytes) {
+    Kv4View v;
+    int rc = check_attention(cache, T, Hq, v);
+    if (rc != ALJABR_ROCM_OK) return rc;
+    ALJ_REQUIRE(out && Q && context_lens, "kv4_attention: out, Q and context_lens must be device pointers");
+    ALJ_REQUIRE(aligned(out, 16) && aligned(Q, 16) && aligned(workspace, 16),
+                "kv4_attention: out, Q and workspace must be 16-byte aligned");
+    ALJ_REQUIRE(std::isfinite(scale) && std::isfinite(soft_cap), "kv4_attention: scale and soft_cap must be finite");
+    ALJ_CHECK_READY();
+    Kv4Attention a{};
+    a.out = static_cast<float *>(out);
+    a.q = static_cast<const float *>(Q);
+    a.lens = context_lens;
+    a.counts = counts;
+    a.T = T;
+    a.Hq = Hq;
+    a.scale = scale > 0.0f ? scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(v.D)));
+    a.causal = is_causal != 0;
+    a.window = window;
+    a.soft_cap = soft_cap;
+    a.scratch = static_cast<float *>(workspace);
+    a.scratch_bytes = workspace ? workspace_bytes : 0;
+    rc = enqueue_kv4_attention(v, a);
+    return rc == ALJABR_ROCM_OK ? finish_launch("kv4_attention") : rc;
+}
+
+}  // extern "C"

@@ -250,6 +250,76 @@ int aljabr_rocm_paged_attention_gqa_windowed(void *out, const void *Q, const voi
                                              float soft_cap);
 
 /* ======================================================================== */
+/* 4-bit KV cache                                                            */
+/* ======================================================================== */
+/*
+ * A cache of K and V rows in 4 bits (no counterpart in the reference, whose
+ * caches are fp32): head_dim values as blocks of 32 codes of 4 bits with one
+ * fp16 scale each, value = (code - 8) * scale (rounded to fp16 where a scale
+ * of more than 8 significant bits makes it inexact; aljabr_rocm_kv4_write
+ * makes none). 72 bytes a row of 128 values, 256 in fp16. Planes:
+ *   codes   u8  [S][n_kv_heads][rows][head_dim / 2], byte j of a block:
+ *           code j | code (j + 16) << 4, Q4_0's order
+ *   scales  f16 [S][n_kv_heads][head_dim / 32][rows]
+ * Without a block table S = sequences and a sequence holds `rows` positions.
+ * With one S = num_blocks: position j of sequence b is row j % rows of block
+ * block_table[b * max_blocks + j / rows], as in the paged attention. rows is a
+ * multiple of 16, head_dim 64, 128 or 256 (else -3), planes 16-byte aligned.
+ *
+ * The calls below read positions, lengths and the table on the device, wait
+ * for nothing there and can be captured: a position outside the cache, or on a
+ * block index outside [0, num_blocks), is a row that the cache does not have.
+ */
+typedef struct aljabr_rocm_kv4_cache {
+    void *k_codes, *k_scales, *v_codes, *v_scales;   /* device */
+    const void *block_table;                         /* device int32 [sequences][max_blocks], or NULL */
+    int32_t sequences, n_kv_heads, head_dim;
+    int32_t rows;                                    /* positions of a sequence, or of a block */
+    int32_t num_blocks, max_blocks;                  /* with a block table */
+} aljabr_rocm_kv4_cache;
+
+/* Bytes of one codes and one scales plane (K's; V's are alike) of a cache with
+ * this shape: num_blocks > 0 counts blocks, else sequences. The pointers are
+ * not read; no device is needed. */
+int aljabr_rocm_kv4_cache_bytes(const aljabr_rocm_kv4_cache *cache, size_t *codes_bytes, size_t *scales_bytes);
+/* Quantises K and V rows [sequences][T][n_kv_heads][head_dim] (type F32 or
+ * F16; element strides of a sequence, a token and a head, the values of a row
+ * adjacent; all three 0: dense) into the cache: row t of sequence b goes to
+ * position positions[b] + t, for t < counts[b] (counts NULL: T). Rows that the
+ * cache does not have are dropped. K or V may be NULL: only the other is
+ * written. Rows of one call must be different rows of the cache.
+ * Per block: top = its smallest value if that is at least as large in
+ * magnitude as its largest, else its largest; scale = -top / 8 rounded to 8
+ * significant bits (ties to even; a multiple of 2^-24; at most 8160); code =
+ * floor(x / scale + 1/2), exactly, clamped to [-8, 7], plus 8. A block with an
+ * infinity or NaN becomes NaN. */
+int aljabr_rocm_kv4_write(const aljabr_rocm_kv4_cache *cache, const void *K, const void *V, const int *positions,
+                          const int *counts, int T, long long stride_b, long long stride_t, long long stride_h,
+                          int type);
+/* The values of rows positions[b] + t, t < counts[b], as F32 or F16 (both
+ * exact), with the layout rules of kv4_write. Rows that the cache does not
+ * have read as zeros; rows from counts[b] on are left as they were. */
+int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, const int *positions, const int *counts,
+                         int T, long long stride_b, long long stride_t, long long stride_h, int type);
+/* GQA attention over the cache: Q and out [sequences][T][Hq][head_dim] fp32,
+ * Hq a multiple of n_kv_heads. Sequence b has context_lens[b] keys (clamped to
+ * what it can hold), the last counts[b] (NULL: T) of them its rows' own: row t
+ * sits at position p = context_lens[b] - counts[b] + t and sees keys j <= p
+ * when is_causal, and j > p - window when window > 0. T = 1 decodes, a few
+ * rows verify a draft, many are a prompt or a chunk of one. soft_cap > 0 caps
+ * scores as cap * tanh(score / cap); scale <= 0: 1 / sqrt(head_dim). A row
+ * that sees no key gives zeros; rows from counts[b] on are left as they were.
+ * Keys on a bad block are not seen. fp32-accurate.
+ * workspace: device scratch for split partials, of
+ * aljabr_rocm_kv4_attention_workspace bytes (fewer: fewer splits), not shared
+ * by calls that may run at once, captured graphs among them. NULL: the
+ * stream's scratch, which a call under stream capture is refused (-4). */
+int aljabr_rocm_kv4_attention(void *out, const void *Q, const aljabr_rocm_kv4_cache *cache, const int *context_lens,
+                              const int *counts, int T, int Hq, float scale, int is_causal, int window, float soft_cap,
+                              void *workspace, size_t workspace_bytes);
+int aljabr_rocm_kv4_attention_workspace(const aljabr_rocm_kv4_cache *cache, int T, int Hq, size_t *bytes);
+
+/* ======================================================================== */
 /* Several matrices over one input (replaces MTLC/aljabr_metal_matvec_api.h: */
 /* 83-120): device pointers; types F32 0, F16 1, Q4_0 2, Q8_0 8, Q4_K 12,    */
 /* Q6_K 14. Matrices of one type share a launch.                             */

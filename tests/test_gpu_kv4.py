@@ -1,0 +1,474 @@
+"""The 4-bit KV cache on the GPU: rows written and read bit for bit, attention
+against float64 within the bound that ``kv4_plain.attention`` derives, bad
+pages, garbage past a sequence's end, capture into graphs, several streams."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_plain as plain
+from conftest import fresh_thread, scratch_held
+
+pytestmark = pytest.mark.gpu
+
+F32, F16 = 0, 1
+POISON = -77.0
+
+
+class Device:
+    """A host cache's planes on the GPU and the description the calls take."""
+
+    def __init__(self, rocm, host):
+        put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+        self.host, self.abi = host, rocm
+        self.codes = {w: put(host.codes[w]) for w in "kv"}
+        self.scales = {w: put(host.scales[w]) for w in "kv"}
+        self.table = None if host.table is None else put(host.table)
+        self.desc = rocm.Kv4Cache(self.codes["k"].data_ptr(), self.scales["k"].data_ptr(), self.codes["v"].data_ptr(),
+                                  self.scales["v"].data_ptr(), None if self.table is None else self.table.data_ptr(),
+                                  host.seqs, host.heads, host.d, host.rows, host.s if host.page else 0,
+                                  host.per if host.page else 0)
+        torch.cuda.synchronize()
+
+    def ref(self):
+        return ctypes.byref(self.desc)
+
+    def planes_equal(self):
+        torch.cuda.synchronize()
+        for w in "kv":
+            assert np.array_equal(self.codes[w].cpu().numpy(), self.host.codes[w])
+            assert np.array_equal(self.scales[w].cpu().numpy(), self.host.scales[w], equal_nan=True)
+
+
+def ints(x):
+    return None if x is None else torch.tensor(np.asarray(x), dtype=torch.int32).cuda()
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def attend(rocm, dev, q, lens, counts=None, causal=1, window=0, cap=0.0, scale=0.0, workspace=None):
+    B, T, Hq, _ = q.shape
+    qd, ld, cd = torch.from_numpy(q).cuda(), ints(lens), ints(counts)
+    out = torch.full(q.shape, POISON, device="cuda")
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_attention", out.data_ptr(), qd.data_ptr(), dev.ref(), ld.data_ptr(), ptr(cd), T, Hq, scale,
+              causal, window, cap, ptr(workspace), 0 if workspace is None else workspace.numel())
+    torch.cuda.synchronize()
+    return out.cpu().numpy()
+
+
+def check(got, want, bound, live):
+    assert (got[~live] == POISON).all(), "rows behind a sequence's last were written"
+    err = np.abs(got.astype(np.float64) - want)[live]
+    assert (err <= bound[live] + 1e-30).all(), (np.nanmax(err), np.nanmax(err / (bound[live] + 1e-30)), np.isnan(err).sum())
+
+
+# ---- rows --------------------------------------------------------------------------
+
+def rows(seed, b, t, h, d):
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((b, t, h, d)) * np.exp(rng.uniform(-3, 3, (b, t, h, 1)))).astype(np.float32)
+    flat = x.reshape(-1, 32)
+    special = [np.zeros(32), np.where(np.arange(32) == 7, 3.0, 0), np.arange(32) - 15.5, -(np.arange(32) - 15.5),
+               (rng.integers(-16, 17, 32) / 2.0), np.full(32, -1e-7), np.linspace(-3e-6, 2e-6, 32), np.linspace(-1e30, 7e29, 32),
+               np.full(32, 70000.0), np.linspace(-65280, 65279, 32), np.full(32, 5e-324), np.linspace(1, 2, 32),
+               np.where(np.arange(32) % 2, 8.0, -8.0), np.where(np.arange(32) == 31, np.inf, 1.0),
+               np.where(np.arange(32) == 0, np.nan, 1.0), np.full(32, -0.0), 1 + np.arange(32) * 2.0 ** -23]
+    for i, s in enumerate(special):
+        flat[(i * 5 + seed) % len(flat)] = s
+    return x
+
+
+def lay_out(x, layout):
+    """A float array [B, T, H, D] as (device tensor, pointer offset in elements, strides)."""
+    b, t, h, d = x.shape
+    if layout == "dense":
+        return x.copy(), 0, (0, 0, 0)
+    if layout == "heads":
+        return np.ascontiguousarray(x.transpose(0, 2, 1, 3)), 0, (h * t * d, d, t * d)
+    pad = 5 if layout == "odd" else 8                       # odd: rows off the wide loads' alignment
+    row = h * d + pad
+    out = np.full((b, t, row), 9.0, x.dtype)
+    out[:, :, pad - 1 if layout == "odd" else 4:][:, :, :h * d] = x.reshape(b, t, -1)
+    return out, pad - 1 if layout == "odd" else 4, (t * row, row, d)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,page,dtype,layout", [(1, 0, F32, "dense"), (1, 16, F16, "heads"), (5, 48, F32, "odd"),
+                                                 (15, 0, F16, "odd"), (16, 32, F32, "row"), (37, 16, F32, "heads"),
+                                                 (70, 0, F16, "dense"), (33, 64, F16, "row")])
+@pytest.mark.parametrize("h", [1, 3])
+def test_write_and_read_bit_for_bit(rocm, d, t, page, dtype, layout, h):
+    b, np_t = 3, np.float32 if dtype == F32 else np.float16
+    with np.errstate(over="ignore"):
+        k, v = (rows(s, b, t, h, d).astype(np_t) for s in (1, 2))
+    host = plain.Cache(b, h, d, 96, page)
+    dev = Device(rocm, host)
+    start, counts = [0, 11, 96 - t], [t, max(t - 2, 0), t]
+    for s in range(b):
+        for i in range(counts[s]):
+            for w, x in (("k", k), ("v", v)):
+                host.write(w, s, start[s] + i, x[s, i])
+    bufs = [lay_out(x, layout) for x in (k, v)]
+    devs = [torch.from_numpy(x[0]).cuda() for x in bufs]
+    off, strides = bufs[0][1] * np_t().itemsize, bufs[0][2]
+    pos, cnt = ints(start), ints(counts)
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_write", dev.ref(), devs[0].data_ptr() + off, devs[1].data_ptr() + off, pos.data_ptr(),
+              cnt.data_ptr(), t, *strides, dtype)
+    dev.planes_equal()
+    for out_t in (F32, F16):
+        outs = [torch.full((b, t, h, d), POISON, device="cuda", dtype=torch.float32 if out_t == F32 else torch.float16)
+                for _ in "kv"]
+        torch.cuda.synchronize()
+        rocm.call("aljabr_rocm_kv4_read", outs[0].data_ptr(), outs[1].data_ptr(), dev.ref(), pos.data_ptr(), cnt.data_ptr(), t,
+                  0, 0, 0, out_t)
+        for w, o in zip("kv", outs):
+            got = o.cpu().numpy()
+            for s in range(b):
+                want, _ = host.rows_of(w, s, start[s] + counts[s])
+                assert np.array_equal(got[s, :counts[s]].astype(np.float64),
+                                      want[:, start[s]:].transpose(1, 0, 2).astype(np.float64), equal_nan=True)
+                assert (got[s, counts[s]:] == POISON).all()
+
+
+@pytest.mark.parametrize("layout", ["heads", "odd"])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_read_into_strided_rows(rocm, layout, dtype):
+    b, t, h, d = 2, 21, 3, 128
+    np_t = np.float32 if dtype == F32 else np.float16
+    host = plain.Cache(b, h, d, 64, 16)
+    host.fill([30, 40])
+    dev = Device(rocm, host)
+    blank, off, strides = lay_out(np.full((b, t, h, d), POISON, np_t), layout)
+    outs = [torch.from_numpy(blank).cuda() for _ in "kv"]
+    pos = ints([3, 19])
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_read", outs[0].data_ptr() + off * np_t().itemsize, outs[1].data_ptr() + off * np_t().itemsize,
+              dev.ref(), pos.data_ptr(), None, t, *strides, dtype)
+    for w, o in zip("kv", outs):
+        want = np.stack([host.rows_of(w, s, p + t)[0][:, p:].transpose(1, 0, 2) for s, p in ((0, 3), (1, 19))]).astype(np_t)
+        assert np.array_equal(o.cpu().numpy(), lay_out(want, layout)[0])
+
+
+def test_rows_that_the_cache_does_not_have(rocm):
+    b, t, h, d = 4, 8, 2, 64
+    host = plain.Cache(b, h, d, 48, 16)
+    host.fill([48, 48, 48, 48])
+    host.table[0, 1], host.table[1, 0], host.table[2, 2] = -1, host.s, 2 ** 31 - 1
+    dev = Device(rocm, host)
+    x = rows(5, b, t, h, d)
+    start = [12, 12, -3, 44]
+    for s in range(b):
+        for i in range(t):
+            host.write("k", s, start[s] + i, x[s, i])
+            host.write("v", s, start[s] + i, x[s, i])
+    xd, pos = torch.from_numpy(x).cuda(), ints(start)
+    outs = [torch.full((b, t, h, d), POISON, device="cuda") for _ in "kv"]
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_write", dev.ref(), xd.data_ptr(), xd.data_ptr(), pos.data_ptr(), None, t, 0, 0, 0, F32)
+    dev.planes_equal()
+    rocm.call("aljabr_rocm_kv4_read", outs[0].data_ptr(), outs[1].data_ptr(), dev.ref(), pos.data_ptr(), None, t, 0, 0, 0, F32)
+    got = outs[0].cpu().numpy()
+    for s in range(b):
+        for i in range(t):
+            at = host.at(s, start[s] + i)
+            want = 0.0 if at is None else plain.decode(host.codes["k"][at[0], :, at[1]], host.scales["k"][at[0], :, :, at[1]])
+            assert np.array_equal(got[s, i].astype(np.float64), np.broadcast_to(want, (h, d)).astype(np.float64), equal_nan=True)
+
+
+def test_one_of_k_and_v(rocm):
+    b, t, h, d = 1, 3, 2, 128
+    host = plain.Cache(b, h, d, 16)
+    dev = Device(rocm, host)
+    x = rows(6, b, t, h, d)
+    xd, pos = torch.from_numpy(x).cuda(), ints([2])
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_write", dev.ref(), None, xd.data_ptr(), pos.data_ptr(), None, t, 0, 0, 0, F32)
+    for i in range(t):
+        host.write("v", 0, 2 + i, x[0, i])
+    dev.planes_equal()
+    rocm.call("aljabr_rocm_kv4_write", dev.ref(), xd.data_ptr(), None, pos.data_ptr(), None, t, 0, 0, 0, F32)
+    for i in range(t):
+        host.write("k", 0, 2 + i, x[0, i])
+    dev.planes_equal()
+    out = torch.full((b, t, h, d), POISON, device="cuda")
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_read", None, out.data_ptr(), dev.ref(), pos.data_ptr(), None, t, 0, 0, 0, F32)
+    assert np.array_equal(out.cpu().numpy()[0], host.rows_of("v", 0, 5)[0][:, 2:].transpose(1, 0, 2).astype(np.float32), equal_nan=True)
+
+
+# ---- attention ---------------------------------------------------------------------
+
+def query(seed, b, t, hq, d):
+    return np.random.default_rng(seed).standard_normal((b, t, hq, d)).astype(np.float32)
+
+
+SHAPES = [(1, 1), (8, 4), (4, 8), (2, 3), (1, 16), (3, 7)]           # (KV heads, query heads of each)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hkv,g", SHAPES)
+@pytest.mark.parametrize("page", [0, 16, 48])
+def test_decode(rocm, d, hkv, g, page):
+    lens = [1, 33, 200, 0]
+    host = plain.Cache(4, hkv, d, 208, page)
+    host.fill(lens)
+    q = query(d + g, 4, 1, hkv * g, d)
+    got = attend(rocm, Device(rocm, host), q, lens)
+    check(got, *plain.attention(host, q, lens))
+    assert not got[3].any()                                           # no key: zeros
+
+
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 127, 128, 129, 255, 257, 511, 1000, 2047])
+def test_lengths(rocm, n):
+    host = plain.Cache(1, 2, 128, 2048)
+    host.fill([n], seed=n)
+    q = query(n, 1, 1, 8, 128)
+    check(attend(rocm, Device(rocm, host), q, [n]), *plain.attention(host, q, [n]))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,hkv,g", [(2, 2, 4), (5, 2, 2), (8, 1, 8), (9, 2, 1), (17, 2, 4), (40, 1, 3), (70, 2, 2)])
+@pytest.mark.parametrize("causal,window,cap", [(1, 0, 0.0), (0, 0, 0.0), (1, 20, 0.0), (0, 24, 0.0), (1, 40, 5.0), (1, 1, 0.0)])
+def test_several_rows(rocm, d, t, hkv, g, causal, window, cap):
+    lens, counts = [t, 100, 3, 150], [t, max(t - 3, 1), t, 0]         # the third: more rows than keys
+    host = plain.Cache(4, hkv, d, 160, 16 if t % 2 else 0)
+    host.fill(lens)
+    q = query(t, 4, t, hkv * g, d)
+    got = attend(rocm, Device(rocm, host), q, lens, counts, causal, window, cap)
+    check(got, *plain.attention(host, q, lens, counts, bool(causal), window, cap))
+
+
+def test_scale_and_large_scores(rocm):
+    host = plain.Cache(1, 2, 128, 304)
+    host.fill([300])
+    dev = Device(rocm, host)
+    for scale, size in ((0.5, 1.0), (2.0, 30.0), (1e-3, 1e-20), (1e-4, 1e6)):
+        q = query(3, 1, 2, 4, 128) * np.float32(size)
+        check(attend(rocm, dev, q, [300], scale=scale), *plain.attention(host, q, [300], scale=scale))
+
+
+def test_scales_of_any_fp16_number(rocm):
+    """Scales that kv4_write would not make: values are the products rounded to fp16."""
+    host = plain.Cache(1, 2, 128, 112)
+    rng = np.random.default_rng(9)
+    for w in "kv":
+        host.codes[w][:] = rng.integers(0, 256, host.codes[w].shape)
+        host.scales[w][:] = (rng.standard_normal(host.scales[w].shape) * 0.2).astype(np.float16)
+    q = query(4, 1, 3, 8, 128)
+    dev = Device(rocm, host)
+    check(attend(rocm, dev, q, [101]), *plain.attention(host, q, [101]))
+    out = torch.empty(1, 112, 2, 128, device="cuda", dtype=torch.float16)
+    pos = ints([0])
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_read", out.data_ptr(), None, dev.ref(), pos.data_ptr(), None, 112, 0, 0, 0, F16)
+    assert np.array_equal(out.cpu().numpy()[0].transpose(1, 0, 2), host.rows_of("k", 0, 112)[0])
+
+
+def test_small_values(rocm):
+    """Scales down in fp16's subnormal numbers."""
+    host = plain.Cache(1, 1, 128, 64)
+    rng = np.random.default_rng(2)
+    for w in "kv":
+        for pos in range(64):
+            host.write(w, 0, pos, (rng.standard_normal((1, 128)) * 2e-5).astype(np.float32))
+    q = query(5, 1, 1, 4, 128) * np.float32(3e4)
+    check(attend(rocm, Device(rocm, host), q, [64]), *plain.attention(host, q, [64]))
+
+
+@pytest.mark.parametrize("t", [1, 6, 40])
+def test_bad_blocks_hold_no_keys(rocm, t):
+    lens = [90, 90, 90, 20]
+    host = plain.Cache(4, 2, 128, 96, 16)
+    host.fill(lens)
+    host.table[0, 2], host.table[1, 0], host.table[1, 5], host.table[3, :] = -1, host.s, 2 ** 31 - 1, -5
+    q = query(6, 4, t, 8, 128)
+    got = attend(rocm, Device(rocm, host), q, lens)
+    check(got, *plain.attention(host, q, lens))
+    assert not got[3].any()
+
+
+def test_lengths_past_the_cache_are_clamped(rocm):
+    host = plain.Cache(2, 2, 64, 32)
+    host.fill([32, 32])
+    q = query(7, 2, 1, 4, 64)
+    got = attend(rocm, Device(rocm, host), q, [2 ** 31 - 1, -7])
+    want, bound, live = plain.attention(host, q, [32, 0])
+    check(got, want, bound, live)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("t", [4, 40])
+def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(rocm, which, t):
+    host = plain.Cache(1, 2, 128, 128)
+    host.fill([100])
+    q = query(8, 1, t, 8, 128)
+    want, bound, live = plain.attention(host, q, [100])
+    bad = 98                                                           # seen by the last two rows
+    x = np.random.default_rng(0).standard_normal((2, 128)).astype(np.float32)
+    x[1, 37] = np.nan                                                  # one block of one head
+    host.write(which, 0, bad, x)
+    got = attend(rocm, Device(rocm, host), q, [100])
+    check(got[:, :t - 2], want[:, :t - 2], bound[:, :t - 2], live[:, :t - 2])
+    want2, bound2, _ = plain.attention(host, q, [100])
+    assert np.array_equal(np.isnan(got), np.isnan(want2))
+    ok = ~np.isnan(want2)
+    assert (np.abs(got - want2)[ok] <= bound2[ok]).all()
+
+
+def test_window_leaves_nan_behind(rocm):
+    host = plain.Cache(1, 1, 64, 128)
+    host.fill([120])
+    host.write("v", 0, 70, np.full((1, 64), np.nan, np.float32))       # outside the windows of all rows but the first
+    q = query(9, 1, 3, 4, 64)
+    got = attend(rocm, Device(rocm, host), q, [120], window=48)        # rows at 117..119 see 70.., 71.., 72..
+    want, bound, _ = plain.attention(host, q, [120], window=48)
+    assert np.isnan(got[0, 0]).all() and np.isnan(want[0, 0]).all()
+    check(got[:, 1:], want[:, 1:], bound[:, 1:], np.ones((1, 2), bool))
+
+
+@pytest.mark.parametrize("t", [1, 20])
+def test_workspace_of_any_size(rocm, t):
+    host = plain.Cache(2, 2, 128, 1024, 32)
+    lens = [1000, 700]
+    host.fill(lens)
+    dev = Device(rocm, host)
+    q = query(10, 2, t, 8, 128)
+    want = plain.attention(host, q, lens)
+    n = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv4_attention_workspace", dev.ref(), t, 8, ctypes.byref(n))
+    assert n.value > 0
+    for size in (n.value, n.value // 2, n.value // 3, 16, 0):
+        ws = torch.full((max(size, 16) + 64,), 0xCD, dtype=torch.uint8, device="cuda")
+        got = attend(rocm, dev, q, lens, workspace=ws[:size] if size else None)
+        check(got, *want)
+        assert (ws[size:] == 0xCD).all()
+    check(attend(rocm, dev, q, lens), *want)
+
+
+def test_same_call_same_bits(rocm):
+    host = plain.Cache(2, 4, 128, 1024)
+    host.fill([1024, 513])
+    dev = Device(rocm, host)
+    for t in (1, 30):
+        q = query(11, 2, t, 16, 128)
+        first = attend(rocm, dev, q, [1024, 513])
+        for _ in range(3):
+            assert np.array_equal(first, attend(rocm, dev, q, [1024, 513]))
+
+
+# ---- together, as a serving program runs them ------------------------------------------
+
+def test_capture_without_workspace_is_refused(rocm):
+    host = plain.Cache(1, 2, 128, 2048)
+    host.fill([2000])
+    dev, q, lens = Device(rocm, host), torch.from_numpy(query(1, 1, 1, 8, 128)).cuda(), ints([2000])
+    out = torch.zeros(1, 1, 8, 128, device="cuda")
+    lib, s = rocm.load(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def body():
+        rocm.call("aljabr_rocm_set_stream", s.cuda_stream)
+        rocm.call("aljabr_rocm_set_sync_mode", 0)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s, capture_error_mode="thread_local"):
+            out.add_(0)
+            rc = lib.aljabr_rocm_kv4_attention(out.data_ptr(), q.data_ptr(), dev.ref(), lens.data_ptr(), None, 1, 8, 0.0, 1, 0,
+                                               0.0, None, 0)
+        rocm.call("aljabr_rocm_set_stream", None)
+        rocm.call("aljabr_rocm_set_sync_mode", 1)
+        return rc
+
+    assert fresh_thread(body) == -4
+
+
+@pytest.mark.parametrize("t", [1, 12])
+def test_captured_steps_write_and_attend(rocm, t):
+    """Write, attend and read back in one graph, replayed while the cache grows, against eager calls and float64."""
+    b, hkv, g, d, page, cap = 3, 2, 4, 128, 16, 256
+    steps = 4
+    host = plain.Cache(b, hkv, d, cap, page)
+    start = [100, 3, 37]
+    host.fill(start)
+    dev = Device(rocm, host)
+    pos, lens = ints(start), ints([s + t for s in start])
+    k, v, q = (torch.empty(b, t, n, d, device="cuda") for n in (hkv, hkv, hkv * g))
+    out, back = torch.zeros(b, t, hkv * g, d, device="cuda"), torch.zeros(b, t, hkv, d, device="cuda")
+    n = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv4_attention_workspace", dev.ref(), t, hkv * g, ctypes.byref(n))
+    ws = torch.zeros(max(n.value, 16), dtype=torch.uint8, device="cuda")
+
+    def step():
+        rocm.call("aljabr_rocm_kv4_write", dev.ref(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), None, t, 0, 0, 0, F32)
+        rocm.call("aljabr_rocm_kv4_attention", out.data_ptr(), q.data_ptr(), dev.ref(), lens.data_ptr(), None, t, hkv * g, 0.0,
+                  1, 0, 0.0, ws.data_ptr(), ws.numel())
+        rocm.call("aljabr_rocm_kv4_read", back.data_ptr(), None, dev.ref(), pos.data_ptr(), None, t, 0, 0, 0, F32)
+
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def body():
+        rocm.call("aljabr_rocm_set_stream", s.cuda_stream)
+        rocm.call("aljabr_rocm_set_sync_mode", 0)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+            step()
+        assert scratch_held(rocm) == 0
+        at = list(start)
+        for i in range(steps):
+            rng = np.random.default_rng(50 + i)
+            kh, vh = (rng.standard_normal((b, t, hkv, d)).astype(np.float32) for _ in "kv")
+            qh = rng.standard_normal((b, t, hkv * g, d)).astype(np.float32)
+            for dst, src in ((k, kh), (v, vh), (q, qh)):
+                dst.copy_(torch.from_numpy(src))
+            pos.copy_(ints(at))
+            lens.copy_(ints([a + t for a in at]))
+            out.fill_(POISON)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for j in range(b):
+                for r in range(t):
+                    host.write("k", j, at[j] + r, kh[j, r])
+                    host.write("v", j, at[j] + r, vh[j, r])
+            dev.planes_equal()
+            got = out.cpu().numpy()
+            check(got, *plain.attention(host, qh, [a + t for a in at]))
+            for j in range(b):
+                assert np.array_equal(back[j].cpu().numpy(),
+                                      host.rows_of("k", j, at[j] + t)[0][:, at[j]:].transpose(1, 0, 2).astype(np.float32))
+            with torch.cuda.stream(s):
+                out.fill_(POISON)
+            step()                                                     # eager, between the replays
+            torch.cuda.synchronize()
+            assert np.array_equal(got, out.cpu().numpy())
+            at = [a + t for a in at]
+        rocm.call("aljabr_rocm_set_stream", None)
+        rocm.call("aljabr_rocm_set_sync_mode", 1)
+        return True
+
+    assert fresh_thread(body)
+
+
+def test_two_streams_at_once(rocm):
+    """Calls of two threads on streams of their own share nothing but the cache they read."""
+    host = plain.Cache(2, 4, 128, 1024)
+    host.fill([1024, 900])
+    dev = Device(rocm, host)
+    qs = [query(20 + i, 2, t, 16, 128) for i, t in enumerate((1, 20))]
+    want = [attend(rocm, dev, q, [1024, 900]) for q in qs]
+
+    def work(i):
+        return [attend(rocm, dev, qs[i], [1024, 900]) for _ in range(6)]
+
+    import concurrent.futures as cf
+    with cf.ThreadPoolExecutor(2) as pool:
+        for i, outs in enumerate(pool.map(work, (0, 1))):
+            for got in outs:
+                assert np.array_equal(got, want[i])

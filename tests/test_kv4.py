@@ -1,0 +1,98 @@
+"""The 4-bit KV cache without a GPU: sizes, refusals, and the plain encoder's own rules."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv4_plain as plain
+from aljabr_amd import abi
+
+
+def cache(**kw):
+    """A description of a cache whose planes are never touched."""
+    base = dict(k_codes=0x10000, k_scales=0x20000, v_codes=0x30000, v_scales=0x40000, block_table=None, sequences=2,
+                n_kv_heads=8, head_dim=128, rows=64, num_blocks=0, max_blocks=0)
+    base.update(kw)
+    return abi.Kv4Cache(*[base[n] for n, _ in abi.Kv4Cache._fields_])
+
+
+def test_cache_bytes():
+    lib = abi.load()
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    assert lib.aljabr_rocm_kv4_cache_bytes(ctypes.byref(cache()), ctypes.byref(codes), ctypes.byref(scales)) == 0
+    assert (codes.value, scales.value) == (2 * 8 * 64 * 64, 2 * 8 * 64 * 4 * 2)
+    big = cache(sequences=1, num_blocks=1 << 20, rows=128, head_dim=256)
+    assert lib.aljabr_rocm_kv4_cache_bytes(ctypes.byref(big), ctypes.byref(codes), ctypes.byref(scales)) == 0
+    assert codes.value == (1 << 20) * 8 * 128 * 128                      # past 32 bits
+    for bad in (dict(rows=40), dict(rows=0), dict(n_kv_heads=0), dict(sequences=0)):
+        assert lib.aljabr_rocm_kv4_cache_bytes(ctypes.byref(cache(**bad)), ctypes.byref(codes), ctypes.byref(scales)) == -2
+    assert lib.aljabr_rocm_kv4_cache_bytes(ctypes.byref(cache(head_dim=96)), ctypes.byref(codes), ctypes.byref(scales)) == -3
+    assert lib.aljabr_rocm_kv4_cache_bytes(None, ctypes.byref(codes), ctypes.byref(scales)) == -2
+
+
+BAD_CACHES = [
+    (dict(k_codes=None), -2), (dict(v_scales=None), -2), (dict(sequences=0), -2), (dict(sequences=70000), -2),
+    (dict(n_kv_heads=-1), -2), (dict(rows=24), -2), (dict(rows=0), -2), (dict(k_codes=0x10008), -2), (dict(v_scales=0x40002), -2),
+    (dict(block_table=0x50000), -2), (dict(block_table=0x50000, num_blocks=4), -2),
+    (dict(block_table=0x50000, num_blocks=4, max_blocks=1 << 27), -2), (dict(head_dim=96), -3), (dict(head_dim=512), -3),
+]
+P = 0x60000
+
+
+@pytest.mark.parametrize("bad,status", BAD_CACHES)
+def test_bad_caches_are_refused_by_every_call(bad, status):
+    lib, c = abi.load(), ctypes.byref(cache(**bad))
+    n = ctypes.c_size_t()
+    assert lib.aljabr_rocm_kv4_write(c, P, P, P, None, 1, 0, 0, 0, abi.TYPE_F32) == status
+    assert lib.aljabr_rocm_kv4_read(P, P, c, P, None, 1, 0, 0, 0, abi.TYPE_F32) == status
+    assert lib.aljabr_rocm_kv4_attention(P, P, c, P, None, 1, 32, 0.0, 1, 0, 0.0, None, 0) == status
+    assert lib.aljabr_rocm_kv4_attention_workspace(c, 1, 32, ctypes.byref(n)) == status
+    assert abi.last_error()
+
+
+def test_bad_arguments_are_refused():
+    lib, c = abi.load(), ctypes.byref(cache())
+    write, read, att = lib.aljabr_rocm_kv4_write, lib.aljabr_rocm_kv4_read, lib.aljabr_rocm_kv4_attention
+    for fn in (lambda k, v, pos, t, sb, st, sh, ty: write(c, k, v, pos, None, t, sb, st, sh, ty),
+               lambda k, v, pos, t, sb, st, sh, ty: read(k, v, c, pos, None, t, sb, st, sh, ty)):
+        assert fn(None, None, P, 1, 0, 0, 0, 0) == -2          # neither K nor V
+        assert fn(P, P, None, 1, 0, 0, 0, 0) == -2
+        assert fn(P, P, P, 0, 0, 0, 0, 0) == -2
+        assert fn(P, P, P, -3, 0, 0, 0, 0) == -2
+        assert fn(P, P, P, 1, 0, -128, 0, 0) == -2
+        assert fn(P + 2, P, P, 1, 0, 0, 0, 0) == -2            # fp32 off its element
+        assert fn(P, P, P, 1, 0, 0, 0, abi.TYPE_Q8_0) == -3
+    bad = [dict(out=None), dict(q=None), dict(lens=None), dict(t=0), dict(hq=12), dict(hq=0), dict(out=P + 4), dict(q=P + 8),
+           dict(ws=P + 4), dict(scale=float("nan")), dict(cap=float("inf"))]
+    for b in bad:
+        a = dict(out=P, q=P, lens=P, t=1, hq=32, scale=0.0, cap=0.0, ws=None)
+        a.update(b)
+        assert att(a["out"], a["q"], c, a["lens"], None, a["t"], a["hq"], a["scale"], 1, 0, a["cap"], a["ws"], 0) == -2, b
+    assert lib.aljabr_rocm_kv4_attention_workspace(c, 1, 32, None) == -2
+
+
+def test_encoder_rules():
+    x = np.zeros((4, 64), np.float32)
+    x[0, 3], x[0, 40] = -4.0, 4.0                              # the largest magnitude takes code 0 whatever its sign
+    x[1, :32] = np.arange(32) - 16
+    x[2, 5], x[2, 6] = 8.0, -8.0                               # two alike: the negative one
+    x[3, 0] = np.inf
+    codes, scales = plain.encode(x)
+    v = plain.decode(codes, scales).astype(np.float64)
+    assert v[0, 3] == -4.0 and v[0, 40] == 4.0 and scales[0, 0] == 0.5 and scales[0, 1] == -0.5
+    assert np.array_equal(v[1, ::2], x[1, ::2]) and scales[1, 0] == 2.0
+    assert scales[2, 0] == 1.0 and v[2, 6] == -8.0 and v[2, 5] == 7.0
+    assert np.isnan(v[3, :32]).all() and not v[3, 32:].any()
+
+
+def test_encoder_is_within_half_a_step():
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal((64, 256)) * np.exp(rng.uniform(-20, 9, (64, 1)))).astype(np.float32)
+    codes, scales = plain.encode(x)
+    err = np.abs(plain.decode(codes, scales).astype(np.float64) - x).reshape(64, 8, 32)
+    step = np.abs(scales.astype(np.float64))[..., None]
+    # Half a step; a whole one and the scale's rounding (2^-9 of 8 steps) for a value as large as the top one, of the other sign.
+    top = np.abs(x).reshape(64, 8, 32) > 7.5 * step * (1 - 2.0 ** -8)
+    assert (err <= np.where(top, 1 + 2.0 ** -6, 0.5) * step + 2.0 ** -25 * 8).all()
