@@ -263,7 +263,7 @@ int kv4_view(const aljabr_rocm_kv4_cache *c, const char *who, Kv4View &v) {
                 who);
     ALJ_REQUIRE(c->sequences > 0 && c->n_kv_heads > 0 && c->head_dim > 0 && c->rows > 0,
                 "%s: sequences, n_kv_heads, head_dim and rows must be positive", who);
-    ALJ_REQUIRE(c->rows % 16 == 0, "%s: rows = %d must be a multiple of 16", who, c->rows);
+    ALJ_REQUIRE(c->rows % 16 == 0 && c->rows <= (1 << 26), "%s: rows = %d must be a multiple of 16, at most 2^26", who, c->rows);
     if (c->block_table)
         ALJ_REQUIRE(c->num_blocks > 0 && c->max_blocks > 0 && static_cast<long long>(c->max_blocks) * c->rows < (1LL << 31),
                     "%s: a paged cache needs num_blocks and max_blocks, max_blocks * rows below 2^31", who);

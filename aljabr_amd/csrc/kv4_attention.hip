@@ -17,18 +17,19 @@
 // and the order of the dims in O is undone when it is stored.
 //
 // Decoding: a nibble under an exponent is 1024 + q or 64 + q; subtracting 1032
-// or 72 is exact, times the scale is the value (kv4.hpp): three packed fp16
-// instructions a pair of values.
+// or 72 is exact, times the scale is the value (kv4.hpp): three instructions a
+// pair of values, and a shift for every other one.
 //
 // Precision: K and V enter as the fp16 numbers they stand for. A query row is
 // scaled by a power of two to a largest magnitude in [2^14, 2^15) and split
-// into two fp16 parts (2^-23 of each element), a weight times 2^11 likewise;
-// sums are fp32.
+// into two fp16 parts (2^-22 of each element), a weight, scaled to at most
+// 2^15, likewise; sums are fp32. The sum of the weights is one more row of the
+// V product, of ones, so numerator and denominator hold the same weights.
 //
 // Keys a row does not see get weight 0, and V rows past a sequence's end may
-// hold anything: their scales are taken as 0. Where a row's tile has a scale
-// that is not finite among keys that only some rows see, the tile's V product
-// is done once per token with that token's keys alone.
+// hold anything: their scales are taken as 0. A scale that is not finite among
+// keys that only some rows see is taken as 0 too and remembered for the rows
+// that see it: their values of its block are made NaN at the end.
 #include <algorithm>
 #include <cmath>
 
@@ -47,7 +48,7 @@ constexpr int kWaves = 4;
 constexpr int kTile = 32;                    // keys a wave takes at once
 constexpr int kMinTiles = kWaves;            // tiles of a workgroup at the least
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kWeightScale = 2048.0f;
+constexpr float kWeightScale = 8192.0f;      // weights are at most 4
 
 struct Params {
     Kv4View v;
@@ -98,38 +99,75 @@ __device__ __forceinline__ half2v pair(float a, float b) {
     return half2v{static_cast<_Float16>(a), static_cast<_Float16>(b)};
 }
 
+// Masks in scalar and exponents in vector registers: one v_and_or_b32 each.
+struct Magic {
+    uint32_t m0 = 0x000f000fu, m4 = 0x00f000f0u, e10 = 0x64006400u, e6 = 0x54005400u;
+    __device__ __forceinline__ Magic() { asm("" : "+s"(m0), "+s"(m4), "+v"(e10), "+v"(e6)); }
+};
+
 // The 8 nibbles of the 16-bit halves of w, in pairs (nibble i of the low half,
 // nibble i of the high half), times the pair of scales d.
-__device__ __forceinline__ void decode8(uint32_t w, half2v d, uint32_t (&r)[4]) {
+__device__ __forceinline__ void decode8(const Magic &g, uint32_t w, half2v d, uint32_t (&r)[4]) {
     const half2v o10 = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
     const half2v o6 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
     const uint32_t x = w >> 8;
-    r[0] = as_u32((as_half2((w & 0x000f000fu) | 0x64006400u) + o10) * d);
-    r[1] = as_u32((as_half2((w & 0x00f000f0u) | 0x54005400u) + o6) * d);
-    r[2] = as_u32((as_half2((x & 0x000f000fu) | 0x64006400u) + o10) * d);
-    r[3] = as_u32((as_half2((x & 0x00f000f0u) | 0x54005400u) + o6) * d);
+    r[0] = as_u32((as_half2((w & g.m0) | g.e10) + o10) * d);
+    r[1] = as_u32((as_half2((w & g.m4) | g.e6) + o6) * d);
+    r[2] = as_u32((as_half2((x & g.m0) | g.e10) + o10) * d);
+    r[3] = as_u32((as_half2((x & g.m4) | g.e6) + o6) * d);
 }
 
 __device__ __forceinline__ half8 frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(half8, make_uint4(a, b, c, d));
 }
 
+__device__ __forceinline__ bool not_finite(_Float16 x) {
+    return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) == 0x7c00u;
+}
+
 // x of the lane 8 columns away (the row's other fp16 part).
 __device__ __forceinline__ float other_part(float x) { return dpp_f32<0x128>(x); }
 
-// One lane's share of a tile as loaded.
-template <int D>
-struct Tile {
-    uint32_t k[2][D / 32];       // per 16-key half: this lane's dwords of key n
-    uint32_t v[2][4][D == 256 ? 2 : 1];   // per half and key 4h + r: dword(s) of its dims
-    uint16_t ks[2][D == 256 ? 2 : 1];
-    uint2 vs[2];                 // scales of keys 4h .. 4h + 3
-    bool ok[2];                  // the half's block exists (uniform)
+// Where a tile's two 16-key halves are (uniform over the wave).
+struct Place {
+    long long row[2];            // first key's row in the codes planes
+    long long scale[2];          // and in the scales planes
+    bool ok[2];                  // the half's block exists
 };
 
+// One lane's share of a tile as loaded.
+template <int D>
+struct Keys {
+    uint32_t k[2][D / 32];       // per half: this lane's dwords of key n
+    uint32_t s[2][D == 256 ? 2 : 1];
+};
+template <int D>
+struct Values {
+    uint32_t v[2][4][D == 256 ? 2 : 1];   // per half and key 4h + r: dword(s) of its dims
+    uint2 s[2];                  // scales of keys 4h .. 4h + 3
+};
+
+// Bytes from a half's first row to this lane's pieces (a plane of one head is
+// below 2^31 bytes: rows are at most 2^26).
+template <int D>
+struct LaneOffsets {
+    uint32_t k, v, ks, vs;
+    __device__ __forceinline__ LaneOffsets(int n, int h, int R) {
+        k = n * (D / 2) + h * (D / 8);
+        v = 4 * h * (D / 2) + (D == 64 ? 4 * (n >> 1) : D == 128 ? 4 * n : 8 * n);
+        ks = 2 * ((D == 64 ? h >> 1 : D == 128 ? h : 2 * h) * R + n);
+        vs = 2 * ((D == 64 ? n >> 3 : D == 128 ? n >> 2 : n >> 1) * R + 4 * h);
+    }
+};
+
+template <class T>
+__device__ __forceinline__ T load_at(const void *base, uint32_t off) {
+    return *reinterpret_cast<const T *>(static_cast<const char *>(base) + off);
+}
+
 template <int D, bool PAGED>
-__device__ __forceinline__ void load_tile(const Params &p, int b, int kvh, int n_keys, int kt, int n, int h, Tile<D> &x) {
-    constexpr int ND = D / 32;
+__device__ __forceinline__ Place place(const Params &p, int b, int kvh, int n_keys, int kt) {
+    Place x;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         int key = kt * kTile + 16 * u;
@@ -144,51 +182,58 @@ __device__ __forceinline__ void load_tile(const Params &p, int b, int kvh, int n
             if (!x.ok[u]) s = 0;
         }
         const long long head = static_cast<long long>(s) * p.v.H + kvh;
-        const uint8_t *kc = p.v.kc + (head * p.v.R + row) * (D / 2);
-        const uint8_t *vc = p.v.vc + (head * p.v.R + row) * (D / 2);
-        const uint16_t *ks = p.v.ks + head * ND * p.v.R + row;
-        const uint16_t *vs = p.v.vs + head * ND * p.v.R + row;
-        const uint32_t *kr = reinterpret_cast<const uint32_t *>(kc + n * (D / 2)) + h * ND;
+        x.row[u] = head * p.v.R + row;
+        x.scale[u] = head * (D / 32) * p.v.R + row;
+    }
+    return x;
+}
+
+template <int D>
+__device__ __forceinline__ void load_keys(const Params &p, const Place &w, const LaneOffsets<D> &at, Keys<D> &x) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const uint8_t *kc = p.v.kc + w.row[u] * (D / 2);
+        const uint16_t *ks = p.v.ks + w.scale[u];
         if constexpr (D == 64) {
-            const uint2 a = *reinterpret_cast<const uint2 *>(kr);
+            const uint2 a = load_at<uint2>(kc, at.k);
             x.k[u][0] = a.x;
             x.k[u][1] = a.y;
-            x.ks[u][0] = ks[static_cast<long long>(h >> 1) * p.v.R + n];
-        } else if constexpr (D == 128) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(kr);
-            x.k[u][0] = a.x; x.k[u][1] = a.y; x.k[u][2] = a.z; x.k[u][3] = a.w;
-            x.ks[u][0] = ks[static_cast<long long>(h) * p.v.R + n];
         } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 a = *reinterpret_cast<const uint4 *>(kr + 4 * i);
+            for (int i = 0; i < D / 128; ++i) {
+                const uint4 a = load_at<uint4>(kc, at.k + 16 * i);
                 x.k[u][4 * i] = a.x; x.k[u][4 * i + 1] = a.y; x.k[u][4 * i + 2] = a.z; x.k[u][4 * i + 3] = a.w;
-                x.ks[u][i] = ks[static_cast<long long>(2 * h + i) * p.v.R + n];
             }
         }
+        x.s[u][0] = load_at<uint16_t>(ks, at.ks);
+        if constexpr (D == 256) x.s[u][1] = load_at<uint16_t>(ks + p.v.R, at.ks);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void load_values(const Params &p, const Place &w, const LaneOffsets<D> &at, Values<D> &x) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const uint8_t *vc = p.v.vc + w.row[u] * (D / 2);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const uint32_t *vr = reinterpret_cast<const uint32_t *>(vc + (4 * h + r) * (D / 2));
-            if constexpr (D == 64) {
-                x.v[u][r][0] = vr[n >> 1];
-            } else if constexpr (D == 128) {
-                x.v[u][r][0] = vr[n];
-            } else {
-                const uint2 a = *reinterpret_cast<const uint2 *>(vr + 2 * n);
+            if constexpr (D == 256) {
+                const uint2 a = load_at<uint2>(vc, at.v + r * (D / 2));
                 x.v[u][r][0] = a.x;
                 x.v[u][r][1] = a.y;
+            } else {
+                x.v[u][r][0] = load_at<uint32_t>(vc, at.v + r * (D / 2));
             }
         }
-        const int vg = D == 128 ? n >> 2 : D == 64 ? n >> 3 : n >> 1;
-        x.vs[u] = *reinterpret_cast<const uint2 *>(vs + static_cast<long long>(vg) * p.v.R + 4 * h);
+        x.s[u] = load_at<uint2>(p.v.vs + w.scale[u], at.vs);
     }
 }
 
 // O += V^T P^T of a tile: NT column tiles, output tile j holds nibble j of the
 // lanes' dwords (D = 256: j / 8 picks the dword). vd: scales of key pairs.
 template <int D, int NT>
-__device__ __forceinline__ void add_values(const Tile<D> &x, const half2v (&vd)[4], const half8 (&pw)[NT], uint32_t vsel,
-                                           f32x4 (&o)[NT][D / 16]) {
+__device__ __forceinline__ void add_values(const Magic &g, const Values<D> &x, const half2v (&vd)[4], const half8 (&pw)[NT],
+                                           uint32_t vsel, f32x4 (&o)[NT][D / 16]) {
 #pragma unroll
     for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
 #pragma unroll
@@ -198,7 +243,7 @@ __device__ __forceinline__ void add_values(const Tile<D> &x, const half2v (&vd)[
             for (int pr = 0; pr < 4; ++pr) {
                 const uint32_t w0 = x.v[pr >> 1][2 * (pr & 1)][i], w1 = x.v[pr >> 1][2 * (pr & 1) + 1][i];
                 const uint32_t sel = D == 64 ? vsel : half ? 0x07060302u : 0x05040100u;
-                decode8(__builtin_amdgcn_perm(w1, w0, sel), vd[pr], f[pr]);
+                decode8(g, __builtin_amdgcn_perm(w1, w0, sel), vd[pr], f[pr]);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -214,8 +259,8 @@ __device__ __forceinline__ void add_values(const Tile<D> &x, const half2v (&vd)[
 }
 
 // grid: x split, y KV head * row groups, z sequence.
-template <int D, int NT, bool PAGED>
-__global__ __launch_bounds__(kWaves * 64) void kv4_split_kernel(Params p) {
+template <int D, int NT, bool PAGED, bool CAP>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : NT == 1 ? 4 : D == 64 ? 3 : 2) void kv4_split_kernel(Params p) {
     constexpr int ND = D / 32, ROWS = 8 * NT, OT = D / 16;
     extern __shared__ float smem[];                        // [kWaves][ROWS][D + 2]
     const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
@@ -280,23 +325,35 @@ __global__ __launch_bounds__(kWaves * 64) void kv4_split_kernel(Params p) {
     const float lo_part = n < 8 ? 0.0f : 1.0f;
     const uint32_t vsel = n & 1 ? 0x07060302u : 0x05040100u;
 
-    f32x4 o[NT][OT];
-    float m[NT], l[NT];
+    f32x4 o[NT][OT], l[NT];                                // l: the sum of the weights, in every accumulator
+    float m[NT];
+    uint32_t poison[NT];                                   // per lane n: its block of a key this column sees is not finite
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         m[c] = -INFINITY;
-        l[c] = 0.0f;
+        poison[c] = 0;
+        l[c] = f32x4{};
 #pragma unroll
         for (int j = 0; j < OT; ++j) o[c][j] = f32x4{};
     }
+    const Magic g;
+    const half8 ones = frag(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u);
 
-    Tile<D> next;
-    if (t0 + wave < t1) load_tile<D, PAGED>(p, b, kvh, seq.n, t0 + wave, n, h, next);
+    const LaneOffsets<D> at(n, h, p.v.R);
+    Place here, next;
+    Keys<D> xk;
+    Values<D> xv;
+    if (t0 + wave < t1) {
+        here = place<D, PAGED>(p, b, kvh, seq.n, t0 + wave);
+        load_keys<D>(p, here, at, xk);
+        load_values<D>(p, here, at, xv);
+    }
+    // A tile's K registers are refilled with the next tile's as soon as S is done, V's after its product.
     for (int kt = t0 + wave; kt < t1; kt += kWaves) {
-        const Tile<D> x = next;
-        if (kt + kWaves < t1) load_tile<D, PAGED>(p, b, kvh, seq.n, kt + kWaves, n, h, next);
         const int k0 = kt * kTile;
-        const bool whole = k0 >= full_lo && k0 + kTile <= full_hi && x.ok[0] && x.ok[1];   // every row sees every key
+        const bool more = kt + kWaves < t1;
+        if (more) next = place<D, PAGED>(p, b, kvh, seq.n, kt + kWaves);
+        const bool whole = k0 >= full_lo && k0 + kTile <= full_hi && here.ok[0] && here.ok[1];   // every row sees every key
 
         // S of the two halves: accumulator r is key k0 + 16u + 4h + r of this lane's column.
         f32x4 s[NT][2];
@@ -304,16 +361,19 @@ __global__ __launch_bounds__(kWaves * 64) void kv4_split_kernel(Params p) {
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) s[c][u] = f32x4{};
+            half2v kd[D == 256 ? 2 : 1];
+#pragma unroll
+            for (int i = 0; i < (D == 256 ? 2 : 1); ++i) kd[i] = as_half2(__builtin_amdgcn_perm(xk.s[u][i], xk.s[u][i], 0x01000100u));
 #pragma unroll
             for (int i = 0; i < ND; ++i) {
-                const _Float16 d1 = __builtin_bit_cast(_Float16, x.ks[u][D == 256 ? i / 4 : 0]);
                 uint32_t f[4];
-                decode8(x.k[u][i], half2v{d1, d1}, f);
+                decode8(g, xk.k[u][i], kd[D == 256 ? i / 4 : 0], f);
                 const half8 a = frag(f[0], f[1], f[2], f[3]);
 #pragma unroll
                 for (int c = 0; c < NT; ++c) s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[c][i], s[c][u], 0, 0, 0);
             }
         }
+        if (more) load_keys<D>(p, next, at, xk);
         half8 pw[NT];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
@@ -321,115 +381,99 @@ __global__ __launch_bounds__(kWaves * 64) void kv4_split_kernel(Params p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float raw = s[c][i >> 2][i & 3];
-                y[i] = (raw + other_part(raw)) * unscale[c];
+                y[i] = raw + other_part(raw);
             }
-            if (p.soft_cap > 0.0f) {
-                const float cap = p.soft_cap * kLog2e;
+            if constexpr (CAP) {
+                const float cap = p.soft_cap * kLog2e, in = unscale[c] / cap;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = cap * tanhf(y[i] / cap);
+                for (int i = 0; i < 8; ++i) y[i] = cap * tanhf(y[i] * in);
             }
+            const float us = CAP ? 1.0f : unscale[c];
             if (!whole) {
+                const int first = lo[c] - k0 - 4 * h, end = hi[c] - k0 - 4 * h;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = k0 + 16 * (i >> 2) + 4 * h + (i & 3);
-                    if (key < lo[c] || key >= hi[c] || !x.ok[i >> 2]) y[i] = -INFINITY;
-                }
+                for (int i = 0; i < 8; ++i)
+                    if (16 * (i >> 2) + (i & 3) < first || 16 * (i >> 2) + (i & 3) >= end || !here.ok[i >> 2]) y[i] = -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) mx = fmaxf(mx, y[i]);
+            mx *= us;
             // The reference m of a column is raised only when a score exceeds it by more than 2.
             if (__any(mx > m[c] + 2.0f)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
-                if (mx > m[c] + 2.0f) {
-                    const float alpha = __builtin_amdgcn_exp2f(m[c] - mx);       // 0 while m is -inf
-                    l[c] *= alpha;
+                const float up = mx > m[c] + 2.0f ? mx : m[c];
+                const float alpha = up == m[c] ? 1.0f : __builtin_amdgcn_exp2f(m[c] - up);     // 0 while m is -inf
+                l[c] *= alpha;
 #pragma unroll
-                    for (int j = 0; j < OT; ++j) o[c][j] *= alpha;
-                    m[c] = mx;
-                }
+                for (int j = 0; j < OT; ++j) o[c][j] *= alpha;
+                m[c] = up;
             }
             const float ref = m[c] == -INFINITY ? 0.0f : m[c];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[i] = __builtin_amdgcn_exp2f(y[i] - ref) * kWeightScale;
-                l[c] += y[i];
-            }
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half2v first = pair(y[2 * i], y[2 * i + 1]);
-                w[i] = as_u32(pair(fmaf(static_cast<float>(first[0]), -lo_part, y[2 * i]),
-                                   fmaf(static_cast<float>(first[1]), -lo_part, y[2 * i + 1])));
+                float e[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) e[k] = __builtin_amdgcn_exp2f(fmaf(y[2 * i + k], us, -ref)) * kWeightScale;
+                const half2v first = pair(e[0], e[1]);
+                w[i] = as_u32(pair(fmaf(static_cast<float>(first[0]), -lo_part, e[0]),
+                                   fmaf(static_cast<float>(first[1]), -lo_part, e[1])));
             }
             pw[c] = frag(w[0], w[1], w[2], w[3]);
+            l[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pw[c], l[c], 0, 0, 0);
         }
-
-        half2v vd[4] = {as_half2(x.vs[0].x), as_half2(x.vs[0].y), as_half2(x.vs[1].x), as_half2(x.vs[1].y)};
-        if (whole) {
-            add_values<D, NT>(x, vd, pw, vsel, o);
-        } else {
-            // Scales of keys outside every row's range, or on no block, are 0.
+        half2v vd[4] = {as_half2(xv.s[0].x), as_half2(xv.s[0].y), as_half2(xv.s[1].x), as_half2(xv.s[1].y)};
+        if (!whole) {
             bool odd = false;
+            const int end = seq.n - k0 - 4 * h;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int key = k0 + 16 * (i >> 2) + 4 * h + (i & 3);
-                if (key >= seq.n || !x.ok[i >> 2]) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
-                const uint16_t bits = __builtin_bit_cast(uint16_t, vd[i >> 1][i & 1]);
-                odd |= (bits & 0x7c00u) == 0x7c00u;
+                if (16 * (i >> 2) + (i & 3) >= end || !here.ok[i >> 2]) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
+                odd |= not_finite(vd[i >> 1][i & 1]);
             }
-            if (!__any(odd)) {
-                add_values<D, NT>(x, vd, pw, vsel, o);
-            } else {
-                // Token by token: its keys' values alone, and only its rows take the sums.
-                for (int t = r0 / p.G; t <= (r1 - 1) / p.G; ++t) {
-                    int a, z;
-                    key_range(p, seq, t, a, z);
-                    half2v mine[4];
+            if (__any(odd)) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int key = k0 + 16 * (i >> 2) + 4 * h + (i & 3);
-                        mine[i >> 1][i & 1] = key >= a && key < z ? vd[i >> 1][i & 1] : static_cast<_Float16>(0.0f);
+                for (int i = 0; i < 8; ++i) {
+                    const uint64_t bad = __ballot(not_finite(vd[i >> 1][i & 1]));
+#pragma unroll 1
+                    for (int hh = 0; hh < 4; ++hh) {
+                        const int key = k0 + 16 * (i >> 2) + 4 * hh + (i & 3);
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+                            if (key >= lo[c] && key < hi[c]) poison[c] |= static_cast<uint32_t>(bad >> (16 * hh)) & 0xffffu;
                     }
-                    f32x4 sum[NT][OT];
-#pragma unroll
-                    for (int c = 0; c < NT; ++c)
-#pragma unroll
-                        for (int j = 0; j < OT; ++j) sum[c][j] = o[c][j];
-                    add_values<D, NT>(x, mine, pw, vsel, sum);
-#pragma unroll
-                    for (int c = 0; c < NT; ++c) {
-                        const int r = min(r0 + 8 * c + (n & 7), r1 - 1);
-                        if (r / p.G == t)
-#pragma unroll
-                            for (int j = 0; j < OT; ++j) o[c][j] = sum[c][j];
-                    }
+                    if (not_finite(vd[i >> 1][i & 1])) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
                 }
             }
         }
+        add_values<D, NT>(g, xv, vd, pw, vsel, o);
+        if (more) load_values<D>(p, next, at, xv);
+        here = next;
     }
 
     // The wave's state to LDS: O^T tile j, accumulator r: nibble j of dword 4h + r (D = 64: of 16-bit piece 4h + r;
     // D = 256: of dword 2 (4h + r) + j / 8).
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
-        l[c] += __shfl_xor(l[c], 16);
-        l[c] += __shfl_xor(l[c], 32);
-        if (m[c] == -INFINITY && l[c] != l[c]) m[c] = 0.0f;   // a NaN score alone leaves no reference: any finite one carries it
+        const float sum = l[c][0] + other_part(l[c][0]);
+        if (m[c] == -INFINITY && sum != sum) m[c] = 0.0f;  // a NaN score alone leaves no reference: any finite one carries it
         float *st = smem + (wave * ROWS + 8 * c + (n & 7)) * (D + 2);
 #pragma unroll
-        for (int j = 0; j < OT; ++j)
+        for (int r = 0; r < 4; ++r) {
+            const int piece = 4 * h + r;                   // the lane n whose V codes these are
+            const float bad = poison[c] >> (D == 64 ? piece & 8 : D == 128 ? piece & 12 : piece & 14) & 1 ? NAN : 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float val = o[c][j][r] + other_part(o[c][j][r]);
-                const int piece = 4 * h + r;
+            for (int j = 0; j < OT; ++j) {
+                const float val = o[c][j][r] + other_part(o[c][j][r]) + bad;
                 const int w = D == 128 ? piece : D == 64 ? piece >> 1 : 2 * piece + (j >> 3);
                 const int x = D == 64 ? 4 * (piece & 1) + j : j & 7;           // nibble of dword w
                 if (n < 8) st[32 * (w >> 2) + 16 * (x & 1) + 4 * (w & 3) + (x >> 1)] = val;
             }
+        }
         if (lane < 8) {
             st[D] = m[c];
-            st[D + 1] = l[c];
+            st[D + 1] = sum;
         }
     }
     __syncthreads();
@@ -543,16 +587,21 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Params p, int rows_per_g
 // Rows a workgroup of the split kernel stacks: 16 where there are more than 8 (and the state fits LDS).
 int stacked_rows(int rows, int D) { return rows > 8 && D < 256 ? 16 : 8; }
 
-template <int D, int NT>
+template <int D, int NT, bool PAGED>
 void launch_split(const Params &p, hipStream_t s) {
     const size_t lds = static_cast<size_t>(kWaves) * 8 * NT * (D + 2) * sizeof(float);
     const dim3 grid(p.splits, p.v.H * p.row_groups, p.v.B);
-    if (p.v.table)
-        hipLaunchKernelGGL((kv4_split_kernel<D, NT, true>), grid, dim3(kWaves * 64), lds, s, p);
+    if (p.soft_cap > 0.0f)
+        hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, true>), grid, dim3(kWaves * 64), lds, s, p);
     else
-        hipLaunchKernelGGL((kv4_split_kernel<D, NT, false>), grid, dim3(kWaves * 64), lds, s, p);
+        hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, false>), grid, dim3(kWaves * 64), lds, s, p);
     if (p.splits > 1)
         hipLaunchKernelGGL((kv4_merge_kernel<D>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p, 8 * NT);
+}
+
+template <int D, int NT>
+void launch(const Params &p, hipStream_t s) {
+    p.v.table ? launch_split<D, NT, true>(p, s) : launch_split<D, NT, false>(p, s);
 }
 
 // Splits: enough workgroups for two a CU, none below kMinTiles tiles of the longest sequence.
@@ -610,9 +659,9 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
         p.part_ml = part + static_cast<size_t>(v.B) * a.T * a.Hq * p.splits * v.D;
     }
     hipStream_t s = current_stream();
-    if (v.D == 64) per == 8 ? launch_split<64, 1>(p, s) : launch_split<64, 2>(p, s);
-    else if (v.D == 128) per == 8 ? launch_split<128, 1>(p, s) : launch_split<128, 2>(p, s);
-    else launch_split<256, 1>(p, s);
+    if (v.D == 64) per == 8 ? launch<64, 1>(p, s) : launch<64, 2>(p, s);
+    else if (v.D == 128) per == 8 ? launch<128, 1>(p, s) : launch<128, 2>(p, s);
+    else launch<256, 1>(p, s);
     return ALJABR_ROCM_OK;
 }
 
