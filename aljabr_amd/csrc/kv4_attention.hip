@@ -44,9 +44,9 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
 constexpr int kTile = 32;                    // keys a wave takes at once
-constexpr int kMinTiles = kWaves;            // tiles of a workgroup at the least
+// Waves of a workgroup, and tiles it takes at the least (two at D = 256, whose ring of tiles is twice as large).
+__host__ __device__ constexpr int waves(int D) { return D == 256 ? 2 : 4; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightScale = 8192.0f;      // weights are at most 4
 
@@ -81,13 +81,13 @@ __device__ __forceinline__ void key_range(const Params &p, const Seq &s, int t, 
 }
 
 // The tiles of split `split` of rows [r0, r1) (stacked), and how many splits have any.
-__device__ __forceinline__ void split_range(const Params &p, const Seq &s, int r0, int r1, int split, int &t0, int &t1,
-                                            int &used) {
+__device__ __forceinline__ void split_range(const Params &p, const Seq &s, int r0, int r1, int split, int least, int &t0,
+                                            int &t1, int &used) {
     int lo, hi, x;
     key_range(p, s, r0 / p.G, lo, x);
     key_range(p, s, (r1 - 1) / p.G, x, hi);
     const int a = lo / kTile, z = hi > lo ? (hi + kTile - 1) / kTile : a;
-    const int per = max(kMinTiles, (z - a + p.splits - 1) / p.splits);
+    const int per = max(least, (z - a + p.splits - 1) / p.splits);
     used = (z - a + per - 1) / per;
     t0 = a + split * per;
     t1 = min(t0 + per, z);
@@ -121,6 +121,10 @@ __device__ __forceinline__ half8 frag(uint32_t a, uint32_t b, uint32_t c, uint32
     return __builtin_bit_cast(half8, make_uint4(a, b, c, d));
 }
 
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)p));
+}
+
 __device__ __forceinline__ bool not_finite(_Float16 x) {
     return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) == 0x7c00u;
 }
@@ -147,22 +151,65 @@ struct Values {
     uint2 s[2];                  // scales of keys 4h .. 4h + 3
 };
 
-// Bytes from a half's first row to this lane's pieces (a plane of one head is
-// below 2^31 bytes: rows are at most 2^26).
+// A tile on its way: copied to LDS as it is (16 bytes a lane, whole lines: the
+// fragments' own order would touch a line for every 16 bytes), two tiles ahead
+// in a ring that is the wave's own. Per half of 16 keys: K and V codes as
+// 16-byte chunks, then the scales of both.
+//   K: row r's chunk c at 16 (CPR r + (c ^ swizzle(r))): the 16-byte reads of
+//      eight neighbouring rows take eight different bank groups;
+//   V: rows rotated by r / 4 within their four: the four rows that a read
+//      takes are in different banks;
+//   scales: [K, V][D/32][16].
 template <int D>
-struct LaneOffsets {
-    uint32_t k, v, ks, vs;
-    __device__ __forceinline__ LaneOffsets(int n, int h, int R) {
-        k = n * (D / 2) + h * (D / 8);
-        v = 4 * h * (D / 2) + (D == 64 ? 4 * (n >> 1) : D == 128 ? 4 * n : 8 * n);
-        ks = 2 * ((D == 64 ? h >> 1 : D == 128 ? h : 2 * h) * R + n);
-        vs = 2 * ((D == 64 ? n >> 3 : D == 128 ? n >> 2 : n >> 1) * R + 4 * h);
+struct Ring {
+    static constexpr int CPR = D / 32;                     // chunks of a row
+    static constexpr int kHalf = 16 * 16 * CPR;            // bytes of K's codes (and of V's) of a half
+    static constexpr int kLoads = 2 * kHalf / 1024;        // wave-wide copies of both
+    static constexpr int kScaleLoads = D == 256 ? 2 : 1;
+    static constexpr int kScales = 256 * kScaleLoads;
+    static constexpr int kSlot = 2 * (2 * kHalf + kScales);
+    static constexpr int kTileLoads = 2 * (kLoads + kScaleLoads);
+    static constexpr int kBytes = 2 * kSlot;               // of a wave
+    __device__ static __forceinline__ int swizzle(int r) { return D == 256 ? r & 7 : D == 128 ? r >> 1 & 3 : r >> 2 & 1; }
+
+    const uint8_t *codes[kLoads];                          // this lane's source in row 0 of the planes
+    const uint8_t *scales[kScaleLoads];
+    uint32_t base;                                         // LDS address of the ring
+
+    __device__ __forceinline__ Ring(const Kv4View &v, int lane, uint32_t lds) : base(lds) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int i = 64 * j + lane, c = i % (16 * CPR);
+            const bool is_v = i >= 16 * CPR;
+            const int at = c / CPR;
+            const int row = is_v ? (at & ~3) | ((at - (at >> 2)) & 3) : at;
+            const int chunk = is_v ? c % CPR : c % CPR ^ swizzle(at);
+            codes[j] = (is_v ? v.vc : v.kc) + row * (D / 2) + 16 * chunk;
+        }
+#pragma unroll
+        for (int j = 0; j < kScaleLoads; ++j) {
+            const int i = (64 * j + lane) % (16 * CPR), g = i % (8 * CPR) >> 3;
+            const uint16_t *s = i >= 8 * CPR ? v.vs : v.ks;
+            scales[j] = reinterpret_cast<const uint8_t *>(s + static_cast<long long>(g) * v.R + 2 * (i & 7));
+        }
+    }
+    // The copies of a tile into slot `slot` of the ring.
+    __device__ __forceinline__ void fetch(const Place &w, int slot) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t dst = base + slot * kSlot + u * (kSlot / 2);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) dma16(codes[j] + w.row[u] * (D / 2), dst + 1024 * j);
+#pragma unroll
+            for (int j = 0; j < kScaleLoads; ++j) dma4(scales[j] + w.scale[u] * 2, dst + 2 * kHalf + 256 * j);
+        }
     }
 };
 
-template <class T>
-__device__ __forceinline__ T load_at(const void *base, uint32_t off) {
-    return *reinterpret_cast<const T *>(static_cast<const char *>(base) + off);
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    static_assert(N < 64, "vmcnt range");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
 
 template <int D, bool PAGED>
@@ -176,7 +223,8 @@ __device__ __forceinline__ Place place(const Params &p, int b, int kvh, int n_ke
         x.ok[u] = true;
         if constexpr (PAGED) {
             const int blk = key / p.v.R;
-            s = p.v.table[static_cast<long long>(b) * p.v.max_blocks + blk];
+            // A scalar load: nothing writes the table while the kernel runs.
+            s = ((const __attribute__((address_space(4))) int *)p.v.table)[static_cast<long long>(b) * p.v.max_blocks + blk];
             row = key - blk * p.v.R;
             x.ok[u] = s >= 0 && s < p.v.num_blocks;
             if (!x.ok[u]) s = 0;
@@ -188,44 +236,44 @@ __device__ __forceinline__ Place place(const Params &p, int b, int kvh, int n_ke
     return x;
 }
 
+template <class T>
+__device__ __forceinline__ T lds_at(const char *slot, int off) {
+    return *reinterpret_cast<const T *>(slot + off);
+}
+
+// A tile from its slot of the ring.
 template <int D>
-__device__ __forceinline__ void load_keys(const Params &p, const Place &w, const LaneOffsets<D> &at, Keys<D> &x) {
+__device__ __forceinline__ void read_tile(const char *slot, int n, int h, Keys<D> &xk, Values<D> &xv) {
+    using R = Ring<D>;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const uint8_t *kc = p.v.kc + w.row[u] * (D / 2);
-        const uint16_t *ks = p.v.ks + w.scale[u];
+        const char *half = slot + u * (R::kSlot / 2), *sc = half + 2 * R::kHalf;
         if constexpr (D == 64) {
-            const uint2 a = load_at<uint2>(kc, at.k);
-            x.k[u][0] = a.x;
-            x.k[u][1] = a.y;
+            const uint2 a = lds_at<uint2>(half, 32 * n + 16 * (h >> 1 ^ R::swizzle(n)) + 8 * (h & 1));
+            xk.k[u][0] = a.x;
+            xk.k[u][1] = a.y;
+            xk.s[u][0] = lds_at<uint16_t>(sc, 32 * (h >> 1) + 2 * n);
         } else {
 #pragma unroll
             for (int i = 0; i < D / 128; ++i) {
-                const uint4 a = load_at<uint4>(kc, at.k + 16 * i);
-                x.k[u][4 * i] = a.x; x.k[u][4 * i + 1] = a.y; x.k[u][4 * i + 2] = a.z; x.k[u][4 * i + 3] = a.w;
+                const int c = D / 128 * h + i;
+                const uint4 a = lds_at<uint4>(half, 16 * (R::CPR * n + (c ^ R::swizzle(n))));
+                xk.k[u][4 * i] = a.x; xk.k[u][4 * i + 1] = a.y; xk.k[u][4 * i + 2] = a.z; xk.k[u][4 * i + 3] = a.w;
+                xk.s[u][i] = lds_at<uint16_t>(sc, 32 * c + 2 * n);
             }
         }
-        x.s[u][0] = load_at<uint16_t>(ks, at.ks);
-        if constexpr (D == 256) x.s[u][1] = load_at<uint16_t>(ks + p.v.R, at.ks);
-    }
-}
-
-template <int D>
-__device__ __forceinline__ void load_values(const Params &p, const Place &w, const LaneOffsets<D> &at, Values<D> &x) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const uint8_t *vc = p.v.vc + w.row[u] * (D / 2);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+            const int at = R::kHalf + (4 * h + (r + h & 3)) * (D / 2);
             if constexpr (D == 256) {
-                const uint2 a = load_at<uint2>(vc, at.v + r * (D / 2));
-                x.v[u][r][0] = a.x;
-                x.v[u][r][1] = a.y;
+                const uint2 a = lds_at<uint2>(half, at + 8 * n);
+                xv.v[u][r][0] = a.x;
+                xv.v[u][r][1] = a.y;
             } else {
-                x.v[u][r][0] = load_at<uint32_t>(vc, at.v + r * (D / 2));
+                xv.v[u][r][0] = lds_at<uint32_t>(half, at + (D == 64 ? 4 * (n >> 1) : 4 * n));
             }
         }
-        x.s[u] = load_at<uint2>(p.v.vs + w.scale[u], at.vs);
+        xv.s[u] = lds_at<uint2>(sc, 32 * (R::CPR + (D == 64 ? n >> 3 : D == 128 ? n >> 2 : n >> 1)) + 8 * h);
     }
 }
 
@@ -260,9 +308,9 @@ __device__ __forceinline__ void add_values(const Magic &g, const Values<D> &x, c
 
 // grid: x split, y KV head * row groups, z sequence.
 template <int D, int NT, bool PAGED, bool CAP>
-__global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : NT == 1 ? 4 : D == 64 ? 3 : 2) void kv4_split_kernel(Params p) {
-    constexpr int ND = D / 32, ROWS = 8 * NT, OT = D / 16;
-    extern __shared__ float smem[];                        // [kWaves][ROWS][D + 2]
+__global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 3 : 2) void kv4_split_kernel(Params p) {
+    constexpr int ND = D / 32, ROWS = 8 * NT, OT = D / 16, kWaves = waves(D);
+    extern __shared__ float smem[];                        // the waves' rings, then their states [kWaves][ROWS][D + 2]
     const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int split = blockIdx.x, b = blockIdx.z;
@@ -272,8 +320,21 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : NT == 1 ? 4 : D == 64 ?
     if (r0 >= total) return;
     const int r1 = min(r0 + ROWS, total);
     int t0, t1, used;
-    split_range(p, seq, r0, r1, split, t0, t1, used);
+    split_range(p, seq, r0, r1, split, kWaves, t0, t1, used);
     if (split >= max(used, 1)) return;                     // rows with no key at all: split 0 writes them
+
+    // The first two tiles go out before anything else is read.
+    const Ring<D> ring(p.v, lane, lds_address(smem) + wave * Ring<D>::kBytes);
+    const char *slots = reinterpret_cast<const char *>(smem) + wave * Ring<D>::kBytes;
+    Place here, next;
+    if (t0 + wave < t1) {
+        here = place<D, PAGED>(p, b, kvh, seq.n, t0 + wave);
+        ring.fetch(here, 0);
+    }
+    if (t0 + wave + kWaves < t1) {
+        next = place<D, PAGED>(p, b, kvh, seq.n, t0 + wave + kWaves);
+        ring.fetch(next, 1);
+    }
 
     // This lane's columns: row, visible keys, query parts (dword i of the lane's share of a row).
     int lo[NT], hi[NT];
@@ -339,20 +400,20 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : NT == 1 ? 4 : D == 64 ?
     const Magic g;
     const half8 ones = frag(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u);
 
-    const LaneOffsets<D> at(n, h, p.v.R);
-    Place here, next;
-    Keys<D> xk;
-    Values<D> xv;
-    if (t0 + wave < t1) {
-        here = place<D, PAGED>(p, b, kvh, seq.n, t0 + wave);
-        load_keys<D>(p, here, at, xk);
-        load_values<D>(p, here, at, xv);
-    }
-    // A tile's K registers are refilled with the next tile's as soon as S is done, V's after its product.
-    for (int kt = t0 + wave; kt < t1; kt += kWaves) {
+    int slot = 0;
+    for (int kt = t0 + wave; kt < t1; kt += kWaves, slot ^= 1) {
         const int k0 = kt * kTile;
-        const bool more = kt + kWaves < t1;
-        if (more) next = place<D, PAGED>(p, b, kvh, seq.n, kt + kWaves);
+        Keys<D> xk;
+        Values<D> xv;
+        if (kt + kWaves < t1) wait_copies<Ring<D>::kTileLoads>();
+        else wait_copies<0>();
+        read_tile<D>(slots + slot * Ring<D>::kSlot, n, h, xk, xv);
+        Place after;
+        if (kt + 2 * kWaves < t1) {
+            after = place<D, PAGED>(p, b, kvh, seq.n, kt + 2 * kWaves);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the slot has been read
+            ring.fetch(after, slot);
+        }
         const bool whole = k0 >= full_lo && k0 + kTile <= full_hi && here.ok[0] && here.ok[1];   // every row sees every key
 
         // S of the two halves: accumulator r is key k0 + 16u + 4h + r of this lane's column.
@@ -373,7 +434,6 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : NT == 1 ? 4 : D == 64 ?
                 for (int c = 0; c < NT; ++c) s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[c][i], s[c][u], 0, 0, 0);
             }
         }
-        if (more) load_keys<D>(p, next, at, xk);
         half8 pw[NT];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
@@ -448,9 +508,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : NT == 1 ? 4 : D == 64 ?
             }
         }
         add_values<D, NT>(g, xv, vd, pw, vsel, o);
-        if (more) load_values<D>(p, next, at, xv);
         here = next;
+        next = after;
     }
+    __syncthreads();                                       // every wave has left its ring (its last copies were waited for)
 
     // The wave's state to LDS: O^T tile j, accumulator r: nibble j of dword 4h + r (D = 64: of 16-bit piece 4h + r;
     // D = 256: of dword 2 (4h + r) + j / 8).
@@ -523,7 +584,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Params p, int rows_per_g
     const int total = seq.cnt * p.G, r = t * p.G + hq % p.G;
     const int r0 = r / rows_per_group * rows_per_group, r1 = min(r0 + rows_per_group, total);
     int t0, t1, used;
-    split_range(p, seq, r0, r1, 0, t0, t1, used);
+    split_range(p, seq, r0, r1, 0, waves(D), t0, t1, used);
     used = max(used, 1);
     const long long row = (static_cast<long long>(b) * p.T + t) * p.Hq + hq;
     const float *po = p.part_o + row * p.splits * D, *pm = p.part_ml + row * p.splits * 2;
@@ -589,7 +650,9 @@ int stacked_rows(int rows, int D) { return rows > 8 && D < 256 ? 16 : 8; }
 
 template <int D, int NT, bool PAGED>
 void launch_split(const Params &p, hipStream_t s) {
-    const size_t lds = static_cast<size_t>(kWaves) * 8 * NT * (D + 2) * sizeof(float);
+    constexpr int kWaves = waves(D), states = kWaves * 8 * NT * (D + 2) * 4, rings = kWaves * Ring<D>::kBytes;
+    constexpr size_t lds = states > rings ? states : rings;
+    static_assert(lds <= 65536, "LDS of a workgroup");
     const dim3 grid(p.splits, p.v.H * p.row_groups, p.v.B);
     if (p.soft_cap > 0.0f)
         hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, true>), grid, dim3(kWaves * 64), lds, s, p);
@@ -604,12 +667,12 @@ void launch(const Params &p, hipStream_t s) {
     p.v.table ? launch_split<D, NT, true>(p, s) : launch_split<D, NT, false>(p, s);
 }
 
-// Splits: enough workgroups for two a CU, none below kMinTiles tiles of the longest sequence.
+// Splits: enough workgroups for two a CU, none below a tile a wave of the longest sequence.
 int choose_splits(const Kv4View &v, int T, int Hq) {
     const int rows = T * (Hq / v.H), per = stacked_rows(rows, v.D);
     const long long items = static_cast<long long>(v.B) * v.H * ((rows + per - 1) / per);
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const long long most = (kv4_capacity(v) + kTile * kMinTiles - 1) / (kTile * kMinTiles);
+    const long long most = (kv4_capacity(v) + kTile * waves(v.D) - 1) / (kTile * waves(v.D));
     long long splits = (2 * cus + items - 1) / items;
     splits = std::min(splits, most);
     return static_cast<int>(std::max(splits, 1LL));
