@@ -50,16 +50,32 @@ __host__ __device__ constexpr int waves(int D) { return D == 256 ? 2 : 4; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightScale = 8192.0f;      // weights are at most 4
 
+// n / d for 0 <= n < 2^31 without a division.
+struct FastDiv {
+    uint32_t mul, shift;
+    void set(uint32_t d) {
+        uint32_t l = 0;
+        while ((uint64_t{1} << l) < d) ++l;
+        shift = 31 + l;
+        mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);   // off by less than 1: n / 2^shift of it is below 1 / d
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul >> shift);
+    }
+};
+
 struct Params {
     Kv4View v;
     float *out;
     const float *q;
     const int *lens, *counts;
     int T, Hq, G, row_groups;
+    FastDiv by_g, by_groups, by_rows, by_chunks, by_items;   // G, row_groups, rows of a block, chunks that vary fastest, H * row_groups
     float scale, soft_cap;
     int causal, window;
-    int splits;
-    float *part_o, *part_ml;                 // [b][t][hq][split][D] and (m, l), or null with one split
+    int quota;                               // chunks that the keys of all sequences are cut into (about), 0: one each
+    float *part_o, *part_ml;                 // per chunk, KV head, row group and stacked row: D sums, and (m, l)
+    int2 *chunks;                            // per sequence, KV head and row group: its first chunk and their number
 };
 
 // A sequence's keys and its rows.
@@ -80,17 +96,113 @@ __device__ __forceinline__ void key_range(const Params &p, const Seq &s, int t, 
     lo = p.window > 0 ? max(pos - p.window + 1, 0) : 0;
 }
 
-// The tiles of split `split` of rows [r0, r1) (stacked), and how many splits have any.
-__device__ __forceinline__ void split_range(const Params &p, const Seq &s, int r0, int r1, int split, int least, int &t0,
-                                            int &t1, int &used) {
+// The tiles [a, z) that rows [r0, r0 + rows) of a sequence see together; false when it has none of the rows.
+__device__ __forceinline__ bool row_tiles(const Params &p, const Seq &s, int r0, int rows, int &a, int &z) {
+    a = z = 0;
+    if (r0 >= s.cnt * p.G) return false;
     int lo, hi, x;
-    key_range(p, s, r0 / p.G, lo, x);
-    key_range(p, s, (r1 - 1) / p.G, x, hi);
-    const int a = lo / kTile, z = hi > lo ? (hi + kTile - 1) / kTile : a;
-    const int per = max(least, (z - a + p.splits - 1) / p.splits);
-    used = (z - a + per - 1) / per;
-    t0 = a + split * per;
-    t1 = min(t0 + per, z);
+    key_range(p, s, p.by_g(r0), lo, x);
+    key_range(p, s, min(p.by_g(r0 + rows - 1), s.cnt - 1), x, hi);
+    a = lo / kTile;
+    z = hi > lo ? (hi + kTile - 1) / kTile : a;
+    return true;
+}
+
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // row 0's and 2's sums into 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // the first half's into the second
+    return v;
+}
+
+// One chunk of the work of a row group: tiles [t0, t1) of sequence b. The
+// tiles of all sequences are cut into chunks of one size, a multiple of
+// `least`, about `quota` of them: a batch of uneven lengths keeps every
+// workgroup busy alike. Chunks are numbered through the sequences.
+struct Chunk {
+    int b, t0, t1;
+    int first, count;        // of the sequence's chunks
+    Seq seq;
+};
+
+// Chunk number w; b < 0 past the end. Called by whole waves.
+__device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int rows, int least) {
+    Chunk c{-1, 0, 0, 0, 0, {0, 0}};
+    const int lane = threadIdx.x & 63, B = p.v.B;
+    if (p.quota == 0 || B == 1) {
+        const int b = p.quota ? 0 : w;
+        int a, z;
+        c.seq = sequence(p, b);
+        if (!row_tiles(p, c.seq, r0, rows, a, z)) return c;
+        int per = max(z - a, 1);
+        if (p.quota) {
+            per = max(p.by_chunks(z - a + p.quota - 1), least);
+            per = (per + least - 1) / least * least;
+            c.count = max((z - a + per - 1) / per, 1);
+        } else {
+            c.count = 1;
+        }
+        const int i = p.quota ? w : 0;
+        if (i >= c.count) return c;
+        c.b = b;
+        c.first = p.quota ? 0 : b;
+        c.t0 = a + i * per;
+        c.t1 = min(c.t0 + per, z);
+        return c;
+    }
+    // A lane a sequence; the last (for B <= 64 the only) 64 stay in registers.
+    const int last = (B - 1) & ~63;
+    Seq s{0, 0};
+    int a = 0, z = 0, total = 0;
+    for (int b0 = 0; b0 <= last; b0 += 64) {
+        a = z = 0;
+        if (b0 + lane < B) {
+            s = sequence(p, b0 + lane);
+            row_tiles(p, s, r0, rows, a, z);
+        }
+        total += __builtin_amdgcn_readlane(wave_scan(z - a), 63);
+    }
+    int per = max(p.by_chunks(total + p.quota - 1), least);
+    per = (per + least - 1) / least * least;
+    const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
+    int before = 0;
+    for (int b0 = 0; b0 <= last; b0 += 64) {
+        if (last) {
+            a = z = 0;
+            s.cnt = 0;
+            if (b0 + lane < B) {
+                s = sequence(p, b0 + lane);
+                row_tiles(p, s, r0, rows, a, z);
+            }
+        }
+        // ceil((z - a) / per): the estimate is at most one off.
+        int n = static_cast<int>(static_cast<float>(z - a) * inv);
+        n += n * per < z - a ? 1 : 0;
+        n -= n > 0 && (n - 1) * per >= z - a ? 1 : 0;
+        n += n * per < z - a ? 1 : 0;
+        n = r0 < s.cnt * p.G ? max(n, 1) : 0;
+        const int end = before + wave_scan(n);
+        const uint64_t hit = __ballot(w >= end - n && w < end);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            c.count = __builtin_amdgcn_readlane(n, l);
+            c.first = __builtin_amdgcn_readlane(end, l) - c.count;
+            a = __builtin_amdgcn_readlane(a, l);
+            z = __builtin_amdgcn_readlane(z, l);
+            c.seq.n = __builtin_amdgcn_readlane(s.n, l);
+            c.seq.cnt = __builtin_amdgcn_readlane(s.cnt, l);
+            c.b = b0 + l;
+            c.t0 = a + (w - c.first) * per;
+            c.t1 = min(c.t0 + per, z);
+            return c;
+        }
+        before = __builtin_amdgcn_readlane(end, 63);
+    }
+    return c;
 }
 
 __device__ __forceinline__ half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
@@ -222,7 +334,7 @@ __device__ __forceinline__ Place place(const Params &p, int b, int kvh, int n_ke
         int s = b, row = key;
         x.ok[u] = true;
         if constexpr (PAGED) {
-            const int blk = key / p.v.R;
+            const int blk = p.by_rows(key);
             // A scalar load: nothing writes the table while the kernel runs.
             s = ((const __attribute__((address_space(4))) int *)p.v.table)[static_cast<long long>(b) * p.v.max_blocks + blk];
             row = key - blk * p.v.R;
@@ -306,22 +418,29 @@ __device__ __forceinline__ void add_values(const Magic &g, const Values<D> &x, c
     }
 }
 
-// grid: x split, y KV head * row groups, z sequence.
+// grid: `quota` chunks of every KV head and row group, the chunk varying fastest,
+// then the numbers that only uneven batches need (no CU is left half full by
+// workgroups that find none).
 template <int D, int NT, bool PAGED, bool CAP>
 __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 3 : 2) void kv4_split_kernel(Params p) {
     constexpr int ND = D / 32, ROWS = 8 * NT, OT = D / 16, kWaves = waves(D);
     extern __shared__ float smem[];                        // the waves' rings, then their states [kWaves][ROWS][D + 2]
     const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int split = blockIdx.x, b = blockIdx.z;
-    const int kvh = blockIdx.y / p.row_groups, r0 = (blockIdx.y - kvh * p.row_groups) * ROWS;
-    const Seq seq = sequence(p, b);
-    const int total = seq.cnt * p.G;
-    if (r0 >= total) return;
-    const int r1 = min(r0 + ROWS, total);
-    int t0, t1, used;
-    split_range(p, seq, r0, r1, split, kWaves, t0, t1, used);
-    if (split >= max(used, 1)) return;                     // rows with no key at all: split 0 writes them
+    const int most = p.quota ? p.quota : p.v.B, items = p.v.H * p.row_groups;
+    int item = p.by_chunks(blockIdx.x), w = blockIdx.x - item * most;
+    if (item >= items) {
+        w = most + p.by_items(blockIdx.x - items * most);
+        item = blockIdx.x - w * items;
+    }
+    const int kvh = p.by_groups(item), r0 = (item - kvh * p.row_groups) * ROWS;
+    const Chunk chunk = find_chunk(p, w, r0, ROWS, kWaves);
+    if (chunk.b < 0) return;
+    const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
+    if (p.quota && w == chunk.first && threadIdx.x == 0)
+        p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.first, chunk.count);
+    const Seq seq = chunk.seq;
+    const int r1 = min(r0 + ROWS, seq.cnt * p.G);
 
     // The first two tiles go out before anything else is read.
     const Ring<D> ring(p.v, lane, lds_address(smem) + wave * Ring<D>::kBytes);
@@ -344,7 +463,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         const int r = min(r0 + 8 * c + (n & 7), r1 - 1);   // columns past the rows repeat the last and are not stored
-        const int t = r / p.G, g = r - t * p.G;
+        const int t = p.by_g(r), g = r - t * p.G;
         key_range(p, seq, t, lo[c], hi[c]);
         const float *qr = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D;
         float x[ND][8], top = 0.0f;
@@ -378,8 +497,8 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
     }
     {
         int first_lo, first_hi, last_lo, last_hi;
-        key_range(p, seq, r0 / p.G, first_lo, first_hi);
-        key_range(p, seq, (r1 - 1) / p.G, last_lo, last_hi);
+        key_range(p, seq, p.by_g(r0), first_lo, first_hi);
+        key_range(p, seq, p.by_g(r1 - 1), last_lo, last_hi);
         full_lo = last_lo;
         full_hi = first_hi;
     }
@@ -557,37 +676,34 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
                 O = fmaf(st[dd], f, O);
             }
         }
-        const int t = r / p.G, g = r - t * p.G;
-        const long long row = (static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g;
-        if (p.splits == 1) {
-            p.out[row * D + dd] = L == 0.0f ? 0.0f : O / L;
+        if (chunk.count == 1) {
+            const int t = p.by_g(r), g = r - t * p.G;
+            p.out[((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D + dd] = L == 0.0f ? 0.0f : O / L;
         } else {
-            p.part_o[(row * p.splits + split) * D + dd] = O;
-            if (dd == 0) {
-                p.part_ml[(row * p.splits + split) * 2] = M;
-                p.part_ml[(row * p.splits + split) * 2 + 1] = L;
-            }
+            const long long row = (static_cast<long long>(w) * items + item) * ROWS + i / D;
+            p.part_o[row * D + dd] = O;
+            if (dd == 0) *reinterpret_cast<float2 *>(p.part_ml + row * 2) = make_float2(M, L);
         }
     }
 }
 
-// One workgroup a row: D/4 lanes take a split's partial as float4s, 256 / (D/4)
-// splits at once, folded in split order and then across the lane groups.
-// `rows_per_group`: stacked rows whose splits the split kernel chose together.
-template <int D>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Params p, int rows_per_group) {
+// One workgroup a row of a sequence with several chunks: D/4 lanes take a
+// chunk's partial as float4s, 256 / (D/4) chunks at once, folded in order and
+// then across the lane groups.
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(Params p) {
     constexpr int LPS = D / 4, SG = 256 / LPS;
     __shared__ float st[SG * (D + 2)];
     const int hq = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-    const Seq seq = sequence(p, b);
-    if (t >= seq.cnt) return;
-    const int total = seq.cnt * p.G, r = t * p.G + hq % p.G;
-    const int r0 = r / rows_per_group * rows_per_group, r1 = min(r0 + rows_per_group, total);
-    int t0, t1, used;
-    split_range(p, seq, r0, r1, 0, waves(D), t0, t1, used);
-    used = max(used, 1);
+    const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
+    const int group = r / ROWS;
+    const int2 chunk = p.chunks[(static_cast<long long>(kvh) * p.row_groups + group) * p.v.B + b];   // only read for rows that exist
+    if (t >= sequence(p, b).cnt || chunk.y <= 1) return;   // no row, or the split kernel wrote it itself
+    const int used = chunk.y;
     const long long row = (static_cast<long long>(b) * p.T + t) * p.Hq + hq;
-    const float *po = p.part_o + row * p.splits * D, *pm = p.part_ml + row * p.splits * 2;
+    const long long step = static_cast<long long>(p.v.H) * p.row_groups * ROWS;      // rows from chunk to chunk
+    const long long first = chunk.x * step + (static_cast<long long>(kvh) * p.row_groups + group) * ROWS + r % ROWS;
+    const float *po = p.part_o + first * D, *pm = p.part_ml + first * 2;
     const int sg = threadIdx.x / LPS, j = threadIdx.x % LPS;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -597,10 +713,11 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Params p, int rows_per_g
         float4 os[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = s0 + u * SG < used ? s0 + u * SG : sg;
-            ms[u] = pm[2 * s];
-            ls[u] = pm[2 * s + 1];
-            os[u] = *reinterpret_cast<const float4 *>(po + s * D + 4 * j);
+            const long long s = s0 + u * SG < used ? s0 + u * SG : s0;
+            const float2 ml = *reinterpret_cast<const float2 *>(pm + 2 * s * step);
+            ms[u] = ml.x;
+            ls[u] = ml.y;
+            os[u] = *reinterpret_cast<const float4 *>(po + s * step * D + 4 * j);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -646,20 +763,19 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Params p, int rows_per_g
 }
 
 // Rows a workgroup of the split kernel stacks: 16 where there are more than 8 (and the state fits LDS).
-int stacked_rows(int rows, int D) { return rows > 8 && D < 256 ? 16 : 8; }
+int stacked_rows(long long rows, int D) { return rows > 8 && D < 256 ? 16 : 8; }
 
 template <int D, int NT, bool PAGED>
 void launch_split(const Params &p, hipStream_t s) {
     constexpr int kWaves = waves(D), states = kWaves * 8 * NT * (D + 2) * 4, rings = kWaves * Ring<D>::kBytes;
     constexpr size_t lds = states > rings ? states : rings;
     static_assert(lds <= 65536, "LDS of a workgroup");
-    const dim3 grid(p.splits, p.v.H * p.row_groups, p.v.B);
+    const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
     if (p.soft_cap > 0.0f)
         hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, true>), grid, dim3(kWaves * 64), lds, s, p);
     else
         hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, false>), grid, dim3(kWaves * 64), lds, s, p);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((kv4_merge_kernel<D>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p, 8 * NT);
+    if (p.quota) hipLaunchKernelGGL((kv4_merge_kernel<D, 8 * NT>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
 }
 
 template <int D, int NT>
@@ -667,22 +783,36 @@ void launch(const Params &p, hipStream_t s) {
     p.v.table ? launch_split<D, NT, true>(p, s) : launch_split<D, NT, false>(p, s);
 }
 
-// Splits: enough workgroups for two a CU, none below a tile a wave of the longest sequence.
-int choose_splits(const Kv4View &v, int T, int Hq) {
-    const int rows = T * (Hq / v.H), per = stacked_rows(rows, v.D);
-    const long long items = static_cast<long long>(v.B) * v.H * ((rows + per - 1) / per);
+// How a call's work is laid out: stacked rows of a workgroup, row groups, and
+// the chunks that the keys are cut into (all sequences together, per KV head
+// and row group): two workgroups a CU.
+struct Plan {
+    int rows, groups, quota;
+};
+Plan make_plan(const Kv4View &v, int T, int Hq) {
+    Plan s;
+    const long long rows = static_cast<long long>(T) * (Hq / v.H);
+    s.rows = stacked_rows(rows, v.D);
+    s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
+    const long long items = static_cast<long long>(v.H) * s.groups;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const long long most = (kv4_capacity(v) + kTile * waves(v.D) - 1) / (kTile * waves(v.D));
-    long long splits = (2 * cus + items - 1) / items;
-    splits = std::min(splits, most);
-    return static_cast<int>(std::max(splits, 1LL));
+    const long long most = v.B * ((static_cast<long long>(kv4_capacity(v)) + kTile * waves(v.D) - 1) / (kTile * waves(v.D)));
+    s.quota = static_cast<int>(std::min(2 * cus / items, most));
+    if (s.quota <= 1) s.quota = 0;                         // heads and row groups fill the chip, or there is one chunk
+    return s;
+}
+
+// Bytes of partials with this many chunks.
+size_t partial_bytes(const Kv4View &v, const Plan &s, int quota) {
+    return static_cast<size_t>(v.H) * s.groups * ((static_cast<size_t>(quota) + v.B) * s.rows * (v.D + 2) * sizeof(float) +
+                                                  v.B * sizeof(int2));
 }
 
 }  // namespace
 
 size_t kv4_attention_scratch_bytes(const Kv4View &v, int T, int Hq) {
-    const int splits = choose_splits(v, T, Hq);
-    return splits > 1 ? static_cast<size_t>(v.B) * T * Hq * splits * (v.D + 2) * sizeof(float) : 0;
+    const Plan s = make_plan(v, T, Hq);
+    return s.quota ? partial_bytes(v, s, s.quota) : 0;
 }
 
 int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
@@ -699,28 +829,33 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.soft_cap = a.soft_cap;
     p.causal = a.causal;
     p.window = a.window;
-    const long long rows = static_cast<long long>(a.T) * p.G;
-    const int per = stacked_rows(static_cast<int>(rows), v.D);
-    const long long groups = (rows + per - 1) / per * v.H;
-    if (a.T > 65535 || a.Hq > 65535 || groups > 65535)
-        return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv4_attention: %lld stacked rows are more than one launch takes", rows * v.H);
-    p.row_groups = static_cast<int>((rows + per - 1) / per);
-    p.splits = choose_splits(v, a.T, a.Hq);
-    const size_t one = static_cast<size_t>(v.B) * a.T * a.Hq * (v.D + 2) * sizeof(float);
-    float *part = a.scratch;
-    if (p.splits > 1) {
+    const Plan plan = make_plan(v, a.T, a.Hq);
+    if (a.T > 65535 || static_cast<double>(v.H) * plan.groups * (plan.quota + static_cast<double>(v.B)) > 0x7fffff)
+        return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv4_attention: T = %d rows of %d heads are more than one launch takes", a.T, a.Hq);
+    p.row_groups = plan.groups;
+    p.quota = plan.quota;
+    p.by_g.set(p.G);
+    p.by_groups.set(plan.groups);
+    p.by_rows.set(v.R);
+    p.by_items.set(v.H * plan.groups);
+    if (p.quota) {
+        float *part = a.scratch;
         if (a.scratch) {
-            const size_t fit = a.scratch_bytes / one;
-            if (static_cast<size_t>(p.splits) > fit) p.splits = fit < 2 ? 1 : static_cast<int>(fit);
+            // As many chunks as the caller's workspace holds the partials of.
+            const size_t none = partial_bytes(v, plan, 0), one = partial_bytes(v, plan, 1) - none;
+            const size_t fit = a.scratch_bytes < none ? 0 : (a.scratch_bytes - none) / one;
+            if (fit < static_cast<size_t>(p.quota)) p.quota = fit < 2 ? 0 : static_cast<int>(fit);
         } else {
-            part = static_cast<float *>(stream_scratch(one * p.splits));
+            part = static_cast<float *>(stream_scratch(partial_bytes(v, plan, p.quota)));
             if (!part) return ALJABR_ROCM_ERR_BUFFER;
         }
-    }
-    if (p.splits > 1) {
         p.part_o = part;
-        p.part_ml = part + static_cast<size_t>(v.B) * a.T * a.Hq * p.splits * v.D;
+        const size_t all = (static_cast<size_t>(p.quota) + v.B) * v.H * plan.groups * plan.rows;
+        p.part_ml = part + all * v.D;
+        p.chunks = reinterpret_cast<int2 *>(p.part_ml + 2 * all);
     }
+    p.by_chunks.set(p.quota ? p.quota : v.B);
+    const int per = plan.rows;
     hipStream_t s = current_stream();
     if (v.D == 64) per == 8 ? launch<64, 1>(p, s) : launch<64, 2>(p, s);
     else if (v.D == 128) per == 8 ? launch<128, 1>(p, s) : launch<128, 2>(p, s);
