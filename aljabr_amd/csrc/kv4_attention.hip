@@ -525,6 +525,9 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.by_rows.set(v.R);
     p.by_items.set(v.H * plan.groups);
     p.by_heads.set(v.H);
+    // Two workgroups a CU, all there at once, each with its row group's keys whole.
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    if (!p.quota && a.causal && v.B == 1 && cus % v.H == 0 && static_cast<long long>(v.H) * plan.groups <= 2 * cus) p.pairs = cus / v.H;
     if (p.quota) {
         float *part = a.scratch;
         if (a.scratch) {

@@ -46,6 +46,7 @@ struct Params {
     int causal, window;
     int quota;                               // chunks that the keys of all sequences are cut into (about), 0: one each
     float *part_o, *part_ml;                 // per chunk, KV head, row group and stacked row: D sums, and (m, l)
+    int pairs;                               // rows kernel: see group_of
     int2 *chunks;                            // per sequence, KV head and row group: its first chunk and their number
 };
 
@@ -246,13 +247,6 @@ __device__ __forceinline__ Place place(const Params &p, int b, int kvh, int n_ke
     return x;
 }
 
-// Work items are numbered head by head; in the rows kernel by row group, the
-// last (of most keys, when causal) first, all heads of it together.
-template <int ROWS>
-__device__ __forceinline__ int item_of(const Params &p, int kvh, int group) {
-    return ROWS == kRowsBlock ? (p.row_groups - 1 - group) * p.v.H + kvh : kvh * p.row_groups + group;
-}
-
 // The item and chunk number of a workgroup: `quota` chunks of every item, the
 // chunk varying fastest, then the numbers that only uneven batches need (no CU
 // is left half full by workgroups that find none).
@@ -266,6 +260,20 @@ __device__ __forceinline__ void work_of(const Params &p, int id, int &item, int 
     }
 }
 
+// Folds the state (m2, l2, o2) into (m, l, o); a state without keys has m = -inf.
+__device__ __forceinline__ void fold(float &m, float &l, float4 &o, float m2, float l2, const float4 &o2) {
+    const float mn = fmaxf(m, m2);
+    if (mn == -INFINITY) return;
+    const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float e = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
+    l = fmaf(l, a, l2 * e);
+    o.x = fmaf(o.x, a, o2.x * e);
+    o.y = fmaf(o.y, a, o2.y * e);
+    o.z = fmaf(o.z, a, o2.z * e);
+    o.w = fmaf(o.w, a, o2.w * e);
+    m = mn;
+}
+
 // One workgroup a row of a sequence with several chunks: D/4 lanes take a
 // chunk's partial as float4s, 256 / (D/4) chunks at once, folded in order and
 // then across the lane groups.
@@ -275,7 +283,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Params p) {
     __shared__ float st[SG * (D + 2)];
     const int hq = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
     const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
-    const int item = item_of<ROWS>(p, kvh, r / ROWS);
+    const int item = kvh * p.row_groups + r / ROWS;
     const int2 chunk = p.chunks[static_cast<long long>(item) * p.v.B + b];   // written for the rows that exist
     if (t >= sequence(p, b).cnt || chunk.y <= 1) return;   // no row, or its one chunk wrote it
     const int used = chunk.y;
@@ -301,16 +309,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Params p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s0 + u * SG >= used) break;
-            const float mn = fmaxf(m, ms[u]);
-            if (mn == -INFINITY) continue;
-            const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            const float e = ms[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[u] - mn);
-            l = fmaf(l, a, ls[u] * e);
-            o.x = fmaf(o.x, a, os[u].x * e);
-            o.y = fmaf(o.y, a, os[u].y * e);
-            o.z = fmaf(o.z, a, os[u].z * e);
-            o.w = fmaf(o.w, a, os[u].w * e);
-            m = mn;
+            fold(m, l, o, ms[u], ls[u], os[u]);
         }
     }
     float *my = st + sg * (D + 2);

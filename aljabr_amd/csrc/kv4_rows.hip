@@ -149,6 +149,14 @@ __device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, int
         }
 }
 
+// The row group of the item group i (and the other way round): the last, of
+// most keys when causal, first. With p.pairs, one workgroup a CU and then the
+// other: the second half of the items, from p.pairs groups on, runs from the
+// first group up, so that a CU's two workgroups have a like sum of keys.
+__device__ __forceinline__ int group_of(const Params &p, int i) {
+    return p.pairs && i >= p.pairs ? i - p.pairs : p.row_groups - 1 - i;
+}
+
 template <int D, bool PAGED, bool CAP>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Params p) {
     constexpr int STEPS = D / 16, DT = D / 32, KS = Shape<D>::kKStride, BUFS = Shape<D>::kBuffers;
@@ -158,7 +166,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int item, w;
     work_of(p, blockIdx.x, item, w);
-    const int group = p.row_groups - 1 - p.by_heads(item), kvh = item - p.by_heads(item) * p.v.H;
+    const int group = group_of(p, p.by_heads(item)), kvh = item - p.by_heads(item) * p.v.H;
     const int r0 = group * kRowsBlock;
     const Chunk chunk = find_chunk(p, w, r0, kRowsBlock, 4);
     if (chunk.b < 0) return;
@@ -226,6 +234,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     float m = -INFINITY, l = 0.0f;
     uint32_t poison = 0;                                                   // blocks of 32 dims with a visible key that is not finite
 
+    auto read_values = [&](const _Float16 *vl, int dt, int j) __attribute__((always_inline)) {
+        const _Float16 *at = vl + (32 * dt + nl) * kVStride + 16 * j + 4 * h;
+        const half4 a0 = *reinterpret_cast<const half4 *>(at), a1 = *reinterpret_cast<const half4 *>(at + 8);
+        return half8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+    };
     auto edge_of = [&](int kt) { return kt * kTile < all_lo || kt * kTile + kTile > all_hi; };
     bool ok = true, ok_next = true;                                        // both halves of the tile exist
     if (BUFS == 2 && t0 < t1) {
@@ -239,7 +252,14 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
         __syncthreads();                                                   // this tile is decoded; the other buffer is free
         const _Float16 *kl = lds + (BUFS == 2 ? ((kt - t0) & 1) * Shape<D>::kHalves : 0), *vl = kl + kTile * KS;
         ok = ok_next;
+        half8 ka[STEPS];
+        auto read_keys = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) ka[st] = *reinterpret_cast<const half8 *>(kl + nl * KS + 16 * st + 8 * h);
+            __builtin_amdgcn_sched_barrier(0);
+        };
         if constexpr (BUFS == 2) {
+            read_keys();                                                   // they arrive while the next tile is decoded
             if (tid < 8) bad[ahead == 2 ? 0 : ahead + 1][tid] = 0;         // the tile before this one's
             if (kt + 1 < t1) {
                 ok_next = both_ok<PAGED>(p, b, seq.n, kt + 1);
@@ -253,16 +273,29 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             decode_tile<D>(g, raw, k0, seq.n, edge_of(kt) || !ok, tid, lds, bad[i]);
             if (kt + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 1, tid, raw);
             __syncthreads();
+            read_keys();
         }
         if (idle || k0 >= w_hi || k0 + kTile <= w_lo) continue;
         // S^T: accumulator j is key k0 + 8 (j / 4) + 4h + j % 4 of this lane's row.
-        f32x16 s = {};
+        // Two chains: a product that waits for the one before it takes twice its time.
+        f32x16 s = {}, s1 = {};
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
-            const half8 a = *reinterpret_cast<const half8 *>(kl + nl * KS + 16 * st + 8 * h);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[st], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[st], s, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], s1, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], s, 0, 0, 0);
         }
+        // V's fragments arrive while the weights are computed.
+        half8 va[2][DT];
+        if constexpr (D < 256) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) va[j][dt] = read_values(vl, dt, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] += s1[j];
         if constexpr (CAP) {
             const float cap = p.soft_cap * kLog2e, in = unscale / cap;
 #pragma unroll
@@ -320,41 +353,111 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         // Lane half h supplies contraction entries 0..3 -> key 16j + 4h + e and 4..7 -> key 16j + 8 + 4h + e - 4.
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int j = 0; j < 2; ++j) {
+            if constexpr (D == 256) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const _Float16 *at = vl + (32 * dt + nl) * kVStride + 16 * j + 4 * h;
-                const half4 a0 = *reinterpret_cast<const half4 *>(at), a1 = *reinterpret_cast<const half4 *>(at + 8);
-                const half8 a = half8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j], o[dt], 0, 0, 0);
+                for (int dt = 0; dt < DT; ++dt) va[j][dt] = read_values(vl, dt, j);
             }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[j][dt], pl[j], o[dt], 0, 0, 0);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[j][dt], ph[j], o[dt], 0, 0, 0);
+        }
     }
 
     l += __shfl_xor(l, 32);
     if (m == -INFINITY && l != l) m = 0.0f;                                // a NaN score alone leaves no reference
-    if (w0 + nl >= r1) return;
     const bool whole = chunk.count == 1;
-    const long long row = (static_cast<long long>(w) * p.v.H * p.row_groups + item) * kRowsBlock + 32 * wave + nl;
-    float *dst = whole ? p.out + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D : p.part_o + row * D;
     const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-    // Accumulator j of tile dt is row 32 dt + 8 (j / 4) + 4h + j % 4 of V^T: nibble 2 dt + j / 8 of piece n.
+    const long long part = (static_cast<long long>(w) * p.v.H * p.row_groups + item) * kRowsBlock + 32 * wave;
+    if (!whole && h == 0 && w0 + nl < r1) *reinterpret_cast<float2 *>(p.part_ml + (part + nl) * 2) = make_float2(m, l);
+    __syncthreads();                                                       // every wave is done with the tiles
+    // O through LDS, so that whole lines are stored: rounds of two blocks of dims (D = 64: of one), a wave's own
+    // [32 rows][block of h][32]. Accumulator j of tile dt is row 32 dt + 8 (j / 4) + 4h + j % 4 of V^T: nibble
+    // 2 dt + j / 8 of piece n = 8 (j / 4 % 2) + 4h + j % 4.
+    constexpr int SPAN = D == 64 ? 32 : 64, STRIDE = SPAN + 4, ROUNDS = D / SPAN, LPR = SPAN / 4;
+    float *st = reinterpret_cast<float *>(lds) + wave * 32 * STRIDE;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const int n = 8 * (j >> 2 & 1) + 4 * h + (j & 3), odd = j >> 3;
-        const int block = D == 64 ? n >> 3 : D == 128 ? n >> 2 : n >> 1;
-        const float nan = poison >> block & 1 ? NAN : 0.0f;
-        if constexpr (D == 64) {
-            *reinterpret_cast<float2 *>(dst + 32 * block + 16 * odd + 4 * (n >> 1 & 3) + 2 * (n & 1)) =
-                make_float2(o[0][j] * f + nan, o[1][j] * f + nan);
-        } else {
+    for (int rd = 0; rd < ROUNDS; ++rd) {
+        const int u = D == 256 ? rd >> 1 : rd, sub = rd & 1;               // D = 256: j % 4 / 2 == sub
 #pragma unroll
-            for (int c = 0; c < DT / 4; ++c)
-                *reinterpret_cast<float4 *>(dst + 32 * block + 16 * odd + (D == 128 ? 4 * (n & 3) : 8 * (n & 1) + 4 * c)) = make_float4(
-                    o[4 * c][j] * f + nan, o[4 * c + 1][j] * f + nan, o[4 * c + 2][j] * f + nan, o[4 * c + 3][j] * f + nan);
+        for (int j = 0; j < 16; ++j) {
+            if ((j >> 2 & 1) != u || (D == 256 && (j >> 1 & 1) != sub)) continue;
+            const int odd = j >> 3;
+            if constexpr (D == 64) {
+                *reinterpret_cast<float2 *>(st + nl * STRIDE + 16 * odd + 4 * (2 * h + (j >> 1 & 1)) + 2 * (j & 1)) =
+                    make_float2(o[0][j] * f, o[1][j] * f);
+            } else {
+#pragma unroll
+                for (int c = 0; c < DT / 4; ++c)
+                    *reinterpret_cast<float4 *>(st + nl * STRIDE + 32 * h + 16 * odd +
+                                                (D == 128 ? 4 * (j & 3) : 8 * (j & 1) + 4 * c)) =
+                        make_float4(o[4 * c][j] * f, o[4 * c + 1][j] * f, o[4 * c + 2][j] * f, o[4 * c + 3][j] * f);
+            }
         }
+        if (poison && (D != 64 || h == 0)) {
+            const int own = D == 64 ? u : D == 128 ? 2 * u + h : 4 * u + 2 * h + sub;
+            if (poison >> own & 1)
+                for (int i = 0; i < 32; ++i) st[nl * STRIDE + (D == 64 ? 0 : 32 * h) + i] = NAN;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the wave's own writes
+#pragma unroll
+        for (int i = 0; i < 32 * LPR / 64; ++i) {
+            const int lr = (64 * i + lane) / LPR, d = 4 * ((64 * i + lane) % LPR), rr = w0 + lr;
+            if (rr < r1) {
+                const float4 val = *reinterpret_cast<const float4 *>(st + lr * STRIDE + d);
+                const int block = D == 64 ? u : D == 128 ? 2 * u + (d >> 5) : 4 * u + 2 * (d >> 5) + sub;
+                const int tt = p.by_g(rr);
+                float *dst = whole ? p.out + ((static_cast<long long>(b) * p.T + tt) * p.Hq + kvh * p.G + (rr - tt * p.G)) * D
+                                   : p.part_o + (part + lr) * D;
+                *reinterpret_cast<float4 *>(dst + 32 * block + (d & 31)) = val;
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // read before the next round's writes
     }
-    if (!whole && h == 0) *reinterpret_cast<float2 *>(p.part_ml + row * 2) = make_float2(m, l);
+}
+
+// A wave a row of a sequence with several chunks: D/4 lanes take a chunk's
+// partial as float4s (64 / (D/4) chunks at once), folded in order, then across
+// the lane groups.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_merge_rows_kernel(Params p, long long rows) {
+    constexpr int LPS = D / 4, SG = 64 / LPS;
+    const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int bt = static_cast<int>(row / p.Hq), hq = static_cast<int>(row - static_cast<long long>(bt) * p.Hq);
+    const int b = bt / p.T, t = bt - b * p.T;
+    const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
+    const int item = group_of(p, r / kRowsBlock) * p.v.H + kvh;
+    const int2 chunk = p.chunks[static_cast<long long>(item) * p.v.B + b];   // written for the rows that exist
+    if (t >= sequence(p, b).cnt || chunk.y <= 1) return;   // no row, or its one chunk wrote it
+    const long long step = static_cast<long long>(p.v.H) * p.row_groups * kRowsBlock;
+    const long long first = chunk.x * step + static_cast<long long>(item) * kRowsBlock + r % kRowsBlock;
+    const int lane = threadIdx.x & 63, sg = lane / LPS, j = lane % LPS;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int U = 4;                                   // chunks in flight per lane group
+    for (int s0 = sg; s0 < chunk.y; s0 += U * SG) {
+        float2 ml[U];
+        float4 os[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long s = s0 + u * SG < chunk.y ? s0 + u * SG : s0;
+            ml[u] = *reinterpret_cast<const float2 *>(p.part_ml + (first + s * step) * 2);
+            os[u] = *reinterpret_cast<const float4 *>(p.part_o + (first + s * step) * D + 4 * j);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u * SG < chunk.y) fold(m, l, o, ml[u].x, ml[u].y, os[u]);
+    }
+#pragma unroll
+    for (int off = LPS; off < 64; off <<= 1) {
+        const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+        const float4 o2 = make_float4(__shfl_xor(o.x, off), __shfl_xor(o.y, off), __shfl_xor(o.z, off), __shfl_xor(o.w, off));
+        fold(m, l, o, m2, l2, o2);
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    if (sg == 0) *reinterpret_cast<float4 *>(p.out + row * D + 4 * j) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 }
 
 template <int D, bool PAGED>
@@ -364,7 +467,9 @@ void launch_typed(const Params &p, hipStream_t s) {
         hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, true>), grid, dim3(kThreads), 0, s, p);
     else
         hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, false>), grid, dim3(kThreads), 0, s, p);
-    if (p.quota) hipLaunchKernelGGL((kv4_merge_kernel<D, kRowsBlock>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
+    const long long rows = static_cast<long long>(p.v.B) * p.T * p.Hq;
+    if (p.quota)
+        hipLaunchKernelGGL((kv4_merge_rows_kernel<D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, p, rows);
 }
 
 template <int D>
