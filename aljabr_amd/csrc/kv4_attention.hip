@@ -471,7 +471,7 @@ void launch(const Params &p, hipStream_t s) {
 
 // How a call's work is laid out: stacked rows of a workgroup, row groups, and
 // the chunks that the keys are cut into (all sequences together, per KV head
-// and row group): two workgroups a CU.
+// and row group): two workgroups a CU, in the rows kernel one.
 struct Plan {
     int rows, groups, quota;
 };
@@ -483,7 +483,7 @@ Plan make_plan(const Kv4View &v, int T, int Hq) {
     const long long items = static_cast<long long>(v.H) * s.groups;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const long long most = v.B * ((static_cast<long long>(kv4_capacity(v)) + kTile * waves(v.D) - 1) / (kTile * waves(v.D)));
-    s.quota = static_cast<int>(std::min(2 * cus / items, most));
+    s.quota = static_cast<int>(std::min((s.rows == kRowsBlock ? 1 : 2) * cus / items, most));
     if (s.quota <= 1) s.quota = 0;                         // heads and row groups fill the chip, or there is one chunk
     return s;
 }
@@ -525,9 +525,9 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.by_rows.set(v.R);
     p.by_items.set(v.H * plan.groups);
     p.by_heads.set(v.H);
-    // Two workgroups a CU, all there at once, each with its row group's keys whole.
+    // A causal prompt's row groups in pairs of many and few keys, where that still leaves every CU a workgroup.
     const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    if (!p.quota && a.causal && v.B == 1 && cus % v.H == 0 && static_cast<long long>(v.H) * plan.groups <= 2 * cus) p.pairs = cus / v.H;
+    p.pairs = plan.rows == kRowsBlock && !p.quota && a.causal && static_cast<long long>(v.H) * plan.groups * v.B > cus;
     if (p.quota) {
         float *part = a.scratch;
         if (a.scratch) {
