@@ -46,7 +46,6 @@ struct Params {
     int causal, window;
     int quota;                               // chunks that the keys of all sequences are cut into (about), 0: one each
     float *part_o, *part_ml;                 // per chunk, KV head, row group and stacked row: D sums, and (m, l)
-    int pairs;                               // rows kernel: a workgroup takes two row groups
     int2 *chunks;                            // per sequence, KV head and row group: its first chunk and their number
 };
 

@@ -2,21 +2,18 @@
 // chunks of prompts, drafts of large groups (kv4_attention.hip has the
 // formulas, the precision and the treatment of keys that are not finite).
 //
-// A workgroup takes 128 stacked rows. Two groups of four waves (one at D = 256,
-// whose accumulators leave room for one wave a SIMD) take every other tile of
-// 32 keys, a wave 32 rows. The group decodes its tile once for its four waves,
-// into LDS as the fragments that v_mfma_f32_32x32x16_f16 takes:
+// A workgroup takes 128 stacked rows, 32 a wave, and walks tiles of 32 keys.
+// Its four waves decode a tile once for all of them, into LDS as the fp16
+// fragments that v_mfma_f32_32x32x16_f16 takes:
 //   K   [key][D + 8]: dword w of a row as the 8 halves at 8w, in decode8's
 //       order, which the query's fragments follow;
 //   V^T [16 x + n][36]: nibble x of dword n (D = 64: 16-bit piece n) of 32
 //       keys, so that a thread that holds two keys' dword n writes a pair of
 //       keys for each nibble.
-// A tile is a phase of matrix products (O^T += V^T P^T of the tile before, then
-// S^T = K Q^T) and a phase of vector work (the softmax, the decoding of the next
-// tile), a barrier between them, and the two groups are a phase apart: on every
-// SIMD one wave has the matrix cores while the other has the vector ALU. At the
-// end the groups' states are joined through LDS. Rows run along the lanes: a
-// row's query parts, maximum and sum stay in its two lanes.
+// The next tile is decoded into the other buffer before this one is used, and
+// the one after that is on its way in registers: one barrier a tile.
+//   S^T = K Q^T, O^T += V^T P^T, rows along the lanes: a row's query parts,
+// maximum and sum stay in its two lanes.
 #include "kv4_attention.hpp"
 
 namespace aljabr {
@@ -28,16 +25,16 @@ namespace {
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kGroup = 256;                  // threads that share a tile
+constexpr int kThreads = 256;
 constexpr int kVStride = kTile + 4;          // halves: 72-byte rows
 
 template <int D>
 struct Shape {
-    static constexpr int kGroups = D == 256 ? 1 : 2;
-    static constexpr int kThreads = kGroup * kGroups;
     static constexpr int kKStride = D + 8;                                 // halves
-    static constexpr int kK = kTile * kKStride, kV = D * kVStride;         // halves of a tile's fragments
-    static constexpr int kHalves = kK + 2 * kV;                            // a group's: V stays while the next tile is decoded
+    static constexpr int kHalves = kTile * kKStride + D * kVStride;        // of a decoded tile
+    static constexpr int kBuffers = D == 256 ? 1 : 2;                      // as many as fit 64 KB
+    static constexpr int kDwords = D / 64;                                 // of K a thread decodes
+    static constexpr int kPieces = D == 256 ? 2 : 1;                       // dwords of a V row a thread decodes
 };
 
 // A thread's share of a tile: dwords of one K row, and of two V rows.
@@ -49,15 +46,10 @@ struct Raw {
     bool ok;                                 // the rows' block exists (uniform)
 };
 
-template <class T>
-__device__ __forceinline__ T load_at(const void *base, uint32_t off) {
-    return *reinterpret_cast<const T *>(static_cast<const char *>(base) + off);
-}
-
-// `tid` is the thread's number in its group. Threads of a wave hold 8 neighbouring keys, of one 16-key half: key 8w + i / 8 of K, 8w + 2 (i / 16) of V.
+// Threads of a wave hold 8 neighbouring keys, of one 16-key half: key 8w + i / 8 of K, 8w + 2 (i / 16) of V.
 template <int D, bool PAGED>
 __device__ __forceinline__ void load_raw(const Params &p, int b, int kvh, int n_keys, int kt, int tid, Raw<D> &x) {
-    const int u = __builtin_amdgcn_readfirstlane(tid >> 7);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), u = wave >> 1;
     int key = kt * kTile + 16 * u;
     if (key >= n_keys) key = kt * kTile;
     int s = b, row = key;
@@ -72,30 +64,32 @@ __device__ __forceinline__ void load_raw(const Params &p, int b, int kvh, int n_
     const long long head = static_cast<long long>(s) * p.v.H + kvh;
     const uint8_t *kc = p.v.kc + (head * p.v.R + row) * (D / 2), *vc = p.v.vc + (head * p.v.R + row) * (D / 2);
     const uint16_t *ks = p.v.ks + head * (D / 32) * p.v.R + row, *vs = p.v.vs + head * (D / 32) * p.v.R + row;
-    // K row of the half and its first dword; first V row of the half.
-    const uint32_t kk = tid >> 3 & 15, kd = (tid & 7) * (D / 64), vk = 2 * (tid >> 4 & 7), n = tid & 15;
-    const uint32_t kat = kk * (D / 2) + 4 * kd, vat = vk * (D / 2) + (D == 64 ? 4 * (n >> 1) : D == 128 ? 4 * n : 8 * n);
+    const int kk = (tid >> 3) & 15, kd = (tid & 7) * (D / 64);             // K row of the half, first dword
+    const uint32_t *ksrc = reinterpret_cast<const uint32_t *>(kc + kk * (D / 2)) + kd;
     if constexpr (D == 64) {
-        x.k[0] = load_at<uint32_t>(kc, kat);
+        x.k[0] = ksrc[0];
     } else if constexpr (D == 128) {
-        const uint2 a = load_at<uint2>(kc, kat);
+        const uint2 a = *reinterpret_cast<const uint2 *>(ksrc);
         x.k[0] = a.x; x.k[1] = a.y;
     } else {
-        const uint4 a = load_at<uint4>(kc, kat);
+        const uint4 a = *reinterpret_cast<const uint4 *>(ksrc);
         x.k[0] = a.x; x.k[1] = a.y; x.k[2] = a.z; x.k[3] = a.w;
     }
-    x.ks = load_at<uint16_t>(ks, 2 * ((kd >> 2) * p.v.R + kk));
+    x.ks = ks[static_cast<uint32_t>(kd >> 2) * p.v.R + kk];
+    const int vk = 2 * ((tid >> 4) & 7), n = tid & 15;                     // first V row of the half
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+        const uint32_t *vsrc = reinterpret_cast<const uint32_t *>(vc + (vk + r) * (D / 2));
         if constexpr (D == 256) {
-            const uint2 a = load_at<uint2>(vc, vat + r * (D / 2));
+            const uint2 a = *reinterpret_cast<const uint2 *>(vsrc + 2 * n);
             x.v[r][0] = a.x;
             x.v[r][1] = a.y;
         } else {
-            x.v[r][0] = load_at<uint32_t>(vc, vat + r * (D / 2));
+            x.v[r][0] = vsrc[D == 64 ? n >> 1 : n];
         }
     }
-    x.vs = load_at<uint32_t>(vs, 2 * ((D == 64 ? n >> 3 : D == 128 ? n >> 2 : n >> 1) * p.v.R + vk));
+    const int vg = D == 64 ? n >> 3 : D == 128 ? n >> 2 : n >> 1;
+    x.vs = *reinterpret_cast<const uint32_t *>(vs + static_cast<uint32_t>(vg) * p.v.R + vk);
 }
 
 // Bit u: half u of a tile is on a block that exists (a half past the end counts as the first).
@@ -120,14 +114,14 @@ __device__ __forceinline__ bool both_ok(const Params &p, int b, int n_keys, int 
 // the end, or on no block, are then taken as 0, and one that is not finite too, with its key's bit set in bad[block].
 template <int D>
 __device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, int k0, int n_keys, bool edge, int tid,
-                                            _Float16 *kbuf, _Float16 *vbuf, uint32_t *bad) {
+                                            _Float16 *buf, uint32_t *bad) {
     const int key = tid >> 3, kd = (tid & 7) * (D / 64);
     const half2v kdup = as_half2(__builtin_amdgcn_perm(x.ks, x.ks, 0x01000100u));
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         uint32_t f[4];
         decode8(g, x.k[i], kdup, f);
-        *reinterpret_cast<uint4 *>(kbuf + key * Shape<D>::kKStride + 8 * (kd + i)) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4 *>(buf + key * Shape<D>::kKStride + 8 * (kd + i)) = make_uint4(f[0], f[1], f[2], f[3]);
     }
     const int pr = tid >> 4, n = tid & 15;                                 // pair of keys 2 pr, 2 pr + 1
     half2v vd = as_half2(x.vs);
@@ -142,9 +136,9 @@ __device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, int
             }
         }
     }
-    _Float16 *vt = vbuf + n * kVStride + 2 * pr;
+    _Float16 *vt = buf + kTile * Shape<D>::kKStride + n * kVStride + 2 * pr;
 #pragma unroll
-    for (int i = 0; i < (D == 256 ? 2 : 1); ++i)
+    for (int i = 0; i < Shape<D>::kPieces; ++i)
 #pragma unroll
         for (int half = 0; half < (D == 64 ? 1 : 2); ++half) {
             const uint32_t sel = D == 64 ? (n & 1 ? 0x07060302u : 0x05040100u) : half ? 0x07060302u : 0x05040100u;
@@ -155,48 +149,33 @@ __device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, int
         }
 }
 
-// The row group of the i-th set of items: the last, of most keys when causal, first.
+// The row group of the item group i, and the other way round: the last, of most keys when causal, first.
 __device__ __forceinline__ int group_of(const Params &p, int i) { return p.row_groups - 1 - i; }
 
 template <int D, bool PAGED, bool CAP>
-__global__ __launch_bounds__(Shape<D>::kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Params p) {
-    constexpr int STEPS = D / 16, DT = D / 32, KS = Shape<D>::kKStride, GROUPS = Shape<D>::kGroups;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[GROUPS * Shape<D>::kHalves];
-    __shared__ uint32_t bad[GROUPS][3][8];                                 // per tile in flight and block: keys not finite
-    __shared__ float joint[3][kRowsBlock];                                 // the second group's m, l and poison
-    const int lane = threadIdx.x & 63, h = lane >> 5, nl = lane & 31;
-    const int grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kGroup), tid = threadIdx.x % kGroup;
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Params p) {
+    constexpr int STEPS = D / 16, DT = D / 32, KS = Shape<D>::kKStride, BUFS = Shape<D>::kBuffers;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[BUFS * Shape<D>::kHalves];
+    __shared__ uint32_t bad[3][8];                                         // per tile in flight and block: keys not finite
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, nl = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    _Float16 *kbuf = lds + grp * Shape<D>::kHalves, *vbufs = kbuf + Shape<D>::kK;
-    const Magic g;
-
-    // With p.pairs a workgroup takes a row group of many keys and then one of few, so that all have alike.
-    for (int pass = 0; pass < (p.pairs ? 2 : 1); ++pass) {
     int item, w;
     work_of(p, blockIdx.x, item, w);
-    if (pass) {
-        const int i = p.by_heads(item), other = p.row_groups - 1 - i;
-        if (other <= i) return;
-        item += (other - i) * p.v.H;
-        __syncthreads();                                                   // the first pass has left LDS
-    }
     const int group = group_of(p, p.by_heads(item)), kvh = item - p.by_heads(item) * p.v.H;
     const int r0 = group * kRowsBlock;
     const Chunk chunk = find_chunk(p, w, r0, kRowsBlock, 4);
-    if (chunk.b < 0) {
-        if (p.pairs) continue;
-        return;
-    }
+    if (chunk.b < 0) return;
     const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
-    if (p.quota && w == chunk.first && threadIdx.x == 0)
+    if (p.quota && w == chunk.first && tid == 0)
         p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.first, chunk.count);
     const Seq seq = chunk.seq;
     const int r1 = min(r0 + kRowsBlock, seq.cnt * p.G);
     const int w0 = r0 + 32 * wave;
-    if (tid < 24) (&bad[grp][0][0])[tid] = 0;
+    const Magic g;
+    if (tid < 24) (&bad[0][0])[tid] = 0;
 
     Raw<D> raw;
-    if (t0 + grp < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, t0 + grp, tid, raw);
+    if (t0 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, t0, tid, raw);
 
     // This lane's row, its keys, and the wave's and the workgroup's.
     const int r = min(w0 + nl, r1 - 1);                                    // lanes past the rows repeat the last and are not stored
@@ -217,10 +196,15 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D == 256 ? 1 : 2) void kv4_rows
         const float *qr = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D + 4 * h;
         const float qs = p.scale * kLog2e;
         float top = 0.0f;
+        float4 qa[STEPS], qc[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const float4 a = *reinterpret_cast<const float4 *>(qr + 32 * (s >> 1) + 8 * (s & 1));
-            const float4 c = *reinterpret_cast<const float4 *>(qr + 32 * (s >> 1) + 8 * (s & 1) + 16);
+            qa[s] = *reinterpret_cast<const float4 *>(qr + 32 * (s >> 1) + 8 * (s & 1));
+            qc[s] = *reinterpret_cast<const float4 *>(qr + 32 * (s >> 1) + 8 * (s & 1) + 16);
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const float4 a = qa[s], c = qc[s];
             top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
                                    fmaxf(fmaxf(fabsf(c.x), fabsf(c.y)), fmaxf(fabsf(c.z), fabsf(c.w)))));
         }
@@ -232,8 +216,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D == 256 ? 1 : 2) void kv4_rows
         unscale = ldexpf(1.0f, e - 15);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const float4 a = *reinterpret_cast<const float4 *>(qr + 32 * (s >> 1) + 8 * (s & 1));
-            const float4 c = *reinterpret_cast<const float4 *>(qr + 32 * (s >> 1) + 8 * (s & 1) + 16);
+            const float4 a = qa[s], c = qc[s];
             const float y[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -250,228 +233,183 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D == 256 ? 1 : 2) void kv4_rows
     float m = -INFINITY, l = 0.0f;
     uint32_t poison = 0;                                                   // blocks of 32 dims with a visible key that is not finite
 
-    auto edge_of = [&](int kt) { return kt * kTile < all_lo || kt * kTile + kTile > all_hi || !both_ok<PAGED>(p, b, seq.n, kt); };
-    auto live_of = [&](int kt) { return !idle && kt < t1 && kt * kTile < w_hi && kt * kTile + kTile > w_lo; };
-    auto decode = [&](int kt, int j, int slot) __attribute__((always_inline)) {
-        decode_tile<D>(g, raw, kt * kTile, seq.n, edge_of(kt), tid, kbuf, vbufs + (j & 1) * Shape<D>::kV, bad[grp][slot]);
+    auto read_values = [&](const _Float16 *vl, int dt, int j) __attribute__((always_inline)) {
+        const _Float16 *at = vl + (32 * dt + nl) * kVStride + 16 * j + 4 * h;
+        const half4 a0 = *reinterpret_cast<const half4 *>(at), a1 = *reinterpret_cast<const half4 *>(at + 8);
+        return half8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
     };
-    half8 ph[2], pl[2];                                                    // the weights as two fp16 parts
-    // O^T += V^T P^T: lane half h supplies contraction entries 0..3 -> key 16j + 4h + e and 4..7 -> key 16j + 8 + 4h + e - 4.
-    auto add_values = [&](int j2) __attribute__((always_inline)) {
-        const _Float16 *vl = vbufs + (j2 & 1) * Shape<D>::kV;
+    auto edge_of = [&](int kt) { return kt * kTile < all_lo || kt * kTile + kTile > all_hi; };
+    bool ok = true, ok_next = true;                                        // both halves of the tile exist
+    if (BUFS == 2 && t0 < t1) {
+        __syncthreads();                                                   // `bad` is clear
+        ok_next = both_ok<PAGED>(p, b, seq.n, t0);
+        decode_tile<D>(g, raw, t0 * kTile, seq.n, edge_of(t0) || !ok_next, tid, lds, bad[0]);
+        if (t0 + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, t0 + 1, tid, raw);
+    }
+    for (int kt = t0, i = 0; kt < t1; ++kt, i = i == 2 ? 0 : i + 1) {
+        const int k0 = kt * kTile, ahead = i == 2 ? 0 : i + 1;
+        __syncthreads();                                                   // this tile is decoded; the other buffer is free
+        const _Float16 *kl = lds + (BUFS == 2 ? ((kt - t0) & 1) * Shape<D>::kHalves : 0), *vl = kl + kTile * KS;
+        ok = ok_next;
+        half8 ka[STEPS];
+        auto read_keys = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) ka[st] = *reinterpret_cast<const half8 *>(kl + nl * KS + 16 * st + 8 * h);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if constexpr (BUFS == 2) {
+            read_keys();                                                   // they arrive while the next tile is decoded
+            if (tid < 8) bad[ahead == 2 ? 0 : ahead + 1][tid] = 0;         // the tile before this one's
+            if (kt + 1 < t1) {
+                ok_next = both_ok<PAGED>(p, b, seq.n, kt + 1);
+                decode_tile<D>(g, raw, k0 + kTile, seq.n, edge_of(kt + 1) || !ok_next, tid,
+                               lds + ((kt + 1 - t0) & 1) * Shape<D>::kHalves, bad[ahead]);
+                if (kt + 2 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 2, tid, raw);
+            }
+        } else {
+            ok = both_ok<PAGED>(p, b, seq.n, kt);
+            if (tid < 8) bad[ahead][tid] = 0;
+            decode_tile<D>(g, raw, k0, seq.n, edge_of(kt) || !ok, tid, lds, bad[i]);
+            if (kt + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 1, tid, raw);
+            __syncthreads();
+            read_keys();
+        }
+        if (idle || k0 >= w_hi || k0 + kTile <= w_lo) continue;
+        // S^T: accumulator j is key k0 + 8 (j / 4) + 4h + j % 4 of this lane's row.
+        f32x16 s = {};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], s, 0, 0, 0);
+        }
+        // V's fragments arrive while the weights are computed.
+        half8 va[2][DT];
+        if constexpr (D < 256) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) va[j][dt] = read_values(vl, dt, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (CAP) {
+            const float cap = p.soft_cap * kLog2e, in = unscale / cap;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = cap * tanhf(s[j] * in);
+        }
+        const float us = CAP ? 1.0f : unscale;
+        if (k0 < full_lo || k0 + kTile > full_hi || !ok) {
+            const int first = lo - k0 - 4 * h, end = hi - k0 - 4 * h;
+            uint32_t there = 0xffffffffu;                                  // keys on blocks that exist
+            if (!ok) there = half_ok<PAGED>(p, b, seq.n, kt);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int c = 8 * (j >> 2) + (j & 3);
+                if (c < first || c >= end || !(there >> (j >> 3) & 1)) s[j] = -INFINITY;
+            }
+        }
+        if (edge_of(kt) || !ok) {
+            // Keys of this tile that the row sees, against the ones that are not finite.
+            const int a = max(lo - k0, 0), z = min(hi - k0, kTile);
+            const uint32_t see = z <= a ? 0 : (z == 32 ? 0xffffffffu : (1u << z) - 1) & ~((1u << a) - 1);
+#pragma unroll
+            for (int q = 0; q < DT; ++q) poison |= bad[i][q] & see ? 1u << q : 0;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+        mx *= us;
+        if (__any(mx > m + 2.0f)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float up = mx > m + 2.0f ? mx : m;
+            const float alpha = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);                  // 0 while m is -inf
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+            m = up;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        half8 ph[2], pl[2];
+        float sum[4] = {};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float e[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                e[c] = __builtin_amdgcn_exp2f(fmaf(s[2 * j + c], us, -ref)) * kWeightScale;
+                sum[(2 * j + c) & 3] += e[c];
+            }
+            const half2v first = pair(e[0], e[1]);
+            const half2v rest = pair(e[0] - static_cast<float>(first[0]), e[1] - static_cast<float>(first[1]));
+            ph[j >> 2][2 * (j & 3)] = first[0];
+            ph[j >> 2][2 * (j & 3) + 1] = first[1];
+            pl[j >> 2][2 * (j & 3)] = rest[0];
+            pl[j >> 2][2 * (j & 3) + 1] = rest[1];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // Lane half h supplies contraction entries 0..3 -> key 16j + 4h + e and 4..7 -> key 16j + 8 + 4h + e - 4.
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            half8 a[DT];
+            if constexpr (D == 256) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const _Float16 *at = vl + (32 * dt + nl) * kVStride + 16 * j + 4 * h;
-                const half4 a0 = *reinterpret_cast<const half4 *>(at), a1 = *reinterpret_cast<const half4 *>(at + 8);
-                a[dt] = half8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+                for (int dt = 0; dt < DT; ++dt) va[j][dt] = read_values(vl, dt, j);
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[dt], pl[j], o[dt], 0, 0, 0);
+            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[j][dt], pl[j], o[dt], 0, 0, 0);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[dt], ph[j], o[dt], 0, 0, 0);
+            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[j][dt], ph[j], o[dt], 0, 0, 0);
         }
-    };
-
-    const int tiles = (t1 - t0 + GROUPS - 1) / GROUPS;                     // of a group, the second's last may not exist
-    __syncthreads();                                                       // `bad` is clear
-    if (t0 + grp < t1) {
-        decode(t0 + grp, 0, 0);
-        if (t0 + grp + GROUPS < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, t0 + grp + GROUPS, tid, raw);
     }
-    __syncthreads();
-    if (grp) __syncthreads();                                              // a phase behind the first group
-    bool pending = false;                                                  // ph and pl hold weights of the tile before
-    for (int j = 0, slot = 0; j < tiles; ++j, slot = slot == 2 ? 0 : slot + 1) {
-        const int kt = t0 + grp + GROUPS * j, k0 = kt * kTile, slot1 = slot == 2 ? 0 : slot + 1;
-        // ---- matrix products
-        const bool live = live_of(kt);
-        if (pending) add_values(j - 1);
-        f32x16 s = {};
-        if (live) {
-            // S^T in two chains (a product that waits for the one before it takes twice its time): accumulator i is
-            // key k0 + 8 (i / 4) + 4h + i % 4 of this lane's row.
-            f32x16 s1 = {};
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-                const half8 a = *reinterpret_cast<const half8 *>(kbuf + nl * KS + 16 * st + 8 * h);
-                s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[st], s1, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[st], s, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] += s1[i];
-        }
-        __syncthreads();
-        // ---- vector work
-        if (tid < 8) bad[grp][slot1 == 2 ? 0 : slot1 + 1][tid] = 0;        // the tile before's
-        if (kt + GROUPS < t1) {
-            decode(kt + GROUPS, j + 1, slot1);
-            if (kt + 2 * GROUPS < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 2 * GROUPS, tid, raw);
-        }
-        pending = live;
-        if (live) {
-            const float us = CAP ? 1.0f : unscale;
-            if constexpr (CAP) {
-                const float cap = p.soft_cap * kLog2e, in = unscale / cap;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = cap * tanhf(s[i] * in);
-            }
-            const bool ok = both_ok<PAGED>(p, b, seq.n, kt);
-            if (k0 < full_lo || k0 + kTile > full_hi || !ok) {
-                const int first = lo - k0 - 4 * h, end = hi - k0 - 4 * h;
-                const uint32_t there = ok ? 3 : half_ok<PAGED>(p, b, seq.n, kt);          // halves on blocks that exist
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int c = 8 * (i >> 2) + (i & 3);
-                    if (c < first || c >= end || !(there >> (i >> 3) & 1)) s[i] = -INFINITY;
-                }
-            }
-            if (edge_of(kt)) {
-                // Keys of this tile that the row sees, against the ones that are not finite.
-                const int a = max(lo - k0, 0), z = min(hi - k0, kTile);
-                const uint32_t see = z <= a ? 0 : (z == 32 ? 0xffffffffu : (1u << z) - 1) & ~((1u << a) - 1);
-#pragma unroll
-                for (int q = 0; q < DT; ++q) poison |= bad[grp][slot][q] & see ? 1u << q : 0;
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-            mx *= us;
-            // The row's reference m is raised only when a score exceeds it by more than 2.
-            if (__any(mx > m + 2.0f)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float up = mx > m + 2.0f ? mx : m;
-                const float alpha = up == m ? 1.0f : __builtin_amdgcn_exp2f(m - up);              // 0 while m is -inf
-                l *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-                m = up;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            float sum[4] = {};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float e[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    e[c] = __builtin_amdgcn_exp2f(fmaf(s[2 * i + c], us, -ref)) * kWeightScale;
-                    sum[(2 * i + c) & 3] += e[c];
-                }
-                const half2v first = pair(e[0], e[1]);
-                const half2v rest = pair(e[0] - static_cast<float>(first[0]), e[1] - static_cast<float>(first[1]));
-                ph[i >> 2][2 * (i & 3)] = first[0];
-                ph[i >> 2][2 * (i & 3) + 1] = first[1];
-                pl[i >> 2][2 * (i & 3)] = rest[0];
-                pl[i >> 2][2 * (i & 3) + 1] = rest[1];
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        }
-        __syncthreads();
-    }
-    if (pending) add_values(tiles - 1);
-    if (GROUPS == 2 && !grp) __syncthreads();
 
     l += __shfl_xor(l, 32);
     if (m == -INFINITY && l != l) m = 0.0f;                                // a NaN score alone leaves no reference
     const bool whole = chunk.count == 1;
+    const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
     const long long part = (static_cast<long long>(w) * p.v.H * p.row_groups + item) * kRowsBlock + 32 * wave;
-    // The groups' states in one reference; O through LDS, so that whole lines are stored: rounds of two blocks of dims
-    // (D = 64: of one), a wave's own [32 rows][block of h][32]. Accumulator j of tile dt is row
-    // 32 dt + 8 (j / 4) + 4h + j % 4 of V^T: nibble 2 dt + j / 8 of piece n = 8 (j / 4 % 2) + 4h + j % 4.
+    if (!whole && h == 0 && w0 + nl < r1) *reinterpret_cast<float2 *>(p.part_ml + (part + nl) * 2) = make_float2(m, l);
+    __syncthreads();                                                       // every wave is done with the tiles
+    // O through LDS, so that whole lines are stored: rounds of two blocks of dims (D = 64: of one), a wave's own
+    // [32 rows][block of h][32]. Accumulator j of tile dt is row 32 dt + 8 (j / 4) + 4h + j % 4 of V^T: nibble
+    // 2 dt + j / 8 of piece n = 8 (j / 4 % 2) + 4h + j % 4.
     constexpr int SPAN = D == 64 ? 32 : 64, STRIDE = SPAN + 4, ROUNDS = D / SPAN, LPR = SPAN / 4;
-    static_assert(sizeof(lds) >= kRowsBlock * STRIDE * sizeof(float), "room for a round");
     float *st = reinterpret_cast<float *>(lds) + wave * 32 * STRIDE;
-    float f = 1.0f;
-    if constexpr (GROUPS == 2) {
-        const int lr = 32 * wave + nl;
-        // First the second group's state, then the joint one.
-        if (grp && h == 0) {
-            joint[0][lr] = m;
-            joint[1][lr] = l;
-            joint[2][lr] = __uint_as_float(poison);
-        }
-        __syncthreads();
-        float m2 = 0.0f, l2 = 0.0f;
-        if (!grp) {
-            m2 = joint[0][lr];
-            l2 = joint[1][lr];
-            poison |= __float_as_uint(joint[2][lr]);
-        }
-        __syncthreads();
-        if (!grp) {
-            const float M = fmaxf(m, m2);
-            f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-            const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - M);
-            l = fmaf(l, f, l2 * f2);
-            m = M;
-            const float norm = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-            f *= norm;
-            if (h == 0) joint[0][lr] = f2 * norm;
-        }
-        __syncthreads();
-        if (grp) f = joint[0][lr];
-    } else {
-        f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-        __syncthreads();                                                   // every wave is done with the tiles
-    }
-    if (!grp && !whole && h == 0 && w0 + nl < r1) *reinterpret_cast<float2 *>(p.part_ml + (part + nl) * 2) = make_float2(m, l);
 #pragma unroll
     for (int rd = 0; rd < ROUNDS; ++rd) {
         const int u = D == 256 ? rd >> 1 : rd, sub = rd & 1;               // D = 256: j % 4 / 2 == sub
-        // This lane's values of the round into its places, added to what the second group left there.
-        auto put = [&](bool add) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if ((j >> 2 & 1) != u || (D == 256 && (j >> 1 & 1) != sub)) continue;
-                const int odd = j >> 3;
-                if constexpr (D == 64) {
-                    float2 *at = reinterpret_cast<float2 *>(st + nl * STRIDE + 16 * odd + 4 * (2 * h + (j >> 1 & 1)) + 2 * (j & 1));
-                    const float2 y = add ? *at : make_float2(0.0f, 0.0f);
-                    *at = make_float2(fmaf(o[0][j], f, y.x), fmaf(o[1][j], f, y.y));
-                } else {
+        for (int j = 0; j < 16; ++j) {
+            if ((j >> 2 & 1) != u || (D == 256 && (j >> 1 & 1) != sub)) continue;
+            const int odd = j >> 3;
+            if constexpr (D == 64) {
+                *reinterpret_cast<float2 *>(st + nl * STRIDE + 16 * odd + 4 * (2 * h + (j >> 1 & 1)) + 2 * (j & 1)) =
+                    make_float2(o[0][j] * f, o[1][j] * f);
+            } else {
 #pragma unroll
-                    for (int c = 0; c < DT / 4; ++c) {
-                        float4 *at = reinterpret_cast<float4 *>(st + nl * STRIDE + 32 * h + 16 * odd +
-                                                                (D == 128 ? 4 * (j & 3) : 8 * (j & 1) + 4 * c));
-                        const float4 y = add ? *at : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        *at = make_float4(fmaf(o[4 * c][j], f, y.x), fmaf(o[4 * c + 1][j], f, y.y), fmaf(o[4 * c + 2][j], f, y.z),
-                                          fmaf(o[4 * c + 3][j], f, y.w));
-                    }
-                }
+                for (int c = 0; c < DT / 4; ++c)
+                    *reinterpret_cast<float4 *>(st + nl * STRIDE + 32 * h + 16 * odd +
+                                                (D == 128 ? 4 * (j & 3) : 8 * (j & 1) + 4 * c)) =
+                        make_float4(o[4 * c][j] * f, o[4 * c + 1][j] * f, o[4 * c + 2][j] * f, o[4 * c + 3][j] * f);
             }
-        };
-        if constexpr (GROUPS == 2) {
-            if (grp) put(false);
-            __syncthreads();
-            if (!grp) put(true);
-        } else {
-            put(false);
         }
-        if (!grp) {
-            if (poison && (D != 64 || h == 0)) {
-                const int own = D == 64 ? u : D == 128 ? 2 * u + h : 4 * u + 2 * h + sub;
-                if (poison >> own & 1)
-                    for (int i = 0; i < 32; ++i) st[nl * STRIDE + (D == 64 ? 0 : 32 * h) + i] = NAN;
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // the wave's own writes
-#pragma unroll
-            for (int i = 0; i < 32 * LPR / 64; ++i) {
-                const int lr = (64 * i + lane) / LPR, d = 4 * ((64 * i + lane) % LPR), rr = w0 + lr;
-                if (rr < r1) {
-                    const float4 val = *reinterpret_cast<const float4 *>(st + lr * STRIDE + d);
-                    const int block = D == 64 ? u : D == 128 ? 2 * u + (d >> 5) : 4 * u + 2 * (d >> 5) + sub;
-                    const int tt = p.by_g(rr);
-                    float *dst = whole ? p.out + ((static_cast<long long>(b) * p.T + tt) * p.Hq + kvh * p.G + (rr - tt * p.G)) * D
-                                       : p.part_o + (part + lr) * D;
-                    *reinterpret_cast<float4 *>(dst + 32 * block + (d & 31)) = val;
-                }
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // read before the next round's writes
+        if (poison && (D != 64 || h == 0)) {
+            const int own = D == 64 ? u : D == 128 ? 2 * u + h : 4 * u + 2 * h + sub;
+            if (poison >> own & 1)
+                for (int i = 0; i < 32; ++i) st[nl * STRIDE + (D == 64 ? 0 : 32 * h) + i] = NAN;
         }
-        if constexpr (GROUPS == 2) __syncthreads();
-    }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the wave's own writes
+#pragma unroll
+        for (int i = 0; i < 32 * LPR / 64; ++i) {
+            const int lr = (64 * i + lane) / LPR, d = 4 * ((64 * i + lane) % LPR), rr = w0 + lr;
+            if (rr < r1) {
+                const float4 val = *reinterpret_cast<const float4 *>(st + lr * STRIDE + d);
+                const int block = D == 64 ? u : D == 128 ? 2 * u + (d >> 5) : 4 * u + 2 * (d >> 5) + sub;
+                const int tt = p.by_g(rr);
+                float *dst = whole ? p.out + ((static_cast<long long>(b) * p.T + tt) * p.Hq + kvh * p.G + (rr - tt * p.G)) * D
+                                   : p.part_o + (part + lr) * D;
+                *reinterpret_cast<float4 *>(dst + 32 * block + (d & 31)) = val;
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // read before the next round's writes
     }
 }
 
@@ -520,12 +458,11 @@ __global__ __launch_bounds__(256) void kv4_merge_rows_kernel(Params p, long long
 
 template <int D, bool PAGED>
 void launch_typed(const Params &p, hipStream_t s) {
-    const int items = p.v.H * (p.pairs ? (p.row_groups + 1) / 2 : p.row_groups);
-    const dim3 grid(items * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B)), block(Shape<D>::kThreads);
+    const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
     if (p.soft_cap > 0.0f)
-        hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, true>), grid, block, 0, s, p);
+        hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, true>), grid, dim3(kThreads), 0, s, p);
     else
-        hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, false>), grid, block, 0, s, p);
+        hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, false>), grid, dim3(kThreads), 0, s, p);
     const long long rows = static_cast<long long>(p.v.B) * p.T * p.Hq;
     if (p.quota)
         hipLaunchKernelGGL((kv4_merge_rows_kernel<D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, p, rows);
