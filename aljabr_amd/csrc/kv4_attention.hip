@@ -447,7 +447,13 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
     }
 }
 
-// Rows a workgroup stacks: 8 or 16 in the split kernel, kRowsBlock in the rows kernel.
+// Rows a workgroup stacks: 8 or 16 in the split kernel, kRowsBlock in the rows
+// kernel, which decodes a tile once for all its rows but leaves waves idle
+// below 128. From 33 rows a KV head on it wins or draws (4 sequences of 2048
+// keys, D = 128: 40 rows 24.0 us against 26.2, 96 rows 27.3 against 39.9; 16 of
+// 4096: 40 rows 91 against 99, 64 rows 94 against 81, 96 rows 98 against 117);
+// below, the split kernel does (16 of 4096: 12 rows 35 us against 85, 32 rows
+// 52 against 88).
 constexpr int kManyRows = 33;
 int stacked_rows(long long rows, int D) { return rows >= kManyRows ? kRowsBlock : rows > 8 && D < 256 ? 16 : 8; }
 
@@ -472,7 +478,9 @@ void launch(const Params &p, hipStream_t s) {
 // How a call's work is laid out: stacked rows of a workgroup, row groups, and
 // the chunks that the keys are cut into (all sequences together, per KV head
 // and row group): two workgroups a CU, of 128 rows one (256 rows of a 2048-key
-// chunk: 38.3 us against 40.0 with two).
+// chunk: 38.3 us against 40.0 with two), of D = 256 three, whose workgroups have
+// two waves (16 sequences of 4096 keys: 47.8 us against 54.5; a draft of 5 over a
+// window of 1024 in 8 sequences: 26.8 against 31.9, with four 28.3).
 struct Plan {
     int rows, groups, quota;
 };
@@ -484,7 +492,7 @@ Plan make_plan(const Kv4View &v, int T, int Hq) {
     const long long items = static_cast<long long>(v.H) * s.groups;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const long long most = v.B * ((static_cast<long long>(kv4_capacity(v)) + kTile * waves(v.D) - 1) / (kTile * waves(v.D)));
-    s.quota = static_cast<int>(std::min((s.rows == kRowsBlock ? 1 : 2) * cus / items, most));
+    s.quota = static_cast<int>(std::min((s.rows == kRowsBlock ? 1 : v.D == 256 ? 3 : 2) * cus / items, most));
     if (s.quota <= 1) s.quota = 0;                         // heads and row groups fill the chip, or there is one chunk
     return s;
 }
