@@ -265,8 +265,8 @@ int kv4_view(const aljabr_rocm_kv4_cache *c, const char *who, Kv4View &v) {
                 "%s: sequences, n_kv_heads, head_dim and rows must be positive", who);
     ALJ_REQUIRE(c->rows % 16 == 0 && c->rows <= (1 << 26), "%s: rows = %d must be a multiple of 16, at most 2^26", who, c->rows);
     if (c->block_table)
-        ALJ_REQUIRE(c->num_blocks > 0 && c->max_blocks > 0 && static_cast<long long>(c->max_blocks) * c->rows < (1LL << 31),
-                    "%s: a paged cache needs num_blocks and max_blocks, max_blocks * rows below 2^31", who);
+        ALJ_REQUIRE(c->num_blocks > 0 && c->max_blocks > 0 && static_cast<long long>(c->max_blocks) * c->rows <= (1LL << 30),
+                    "%s: a paged cache needs num_blocks and max_blocks, max_blocks * rows at most 2^30", who);
     ALJ_REQUIRE(c->sequences <= 65535 && c->n_kv_heads <= 16384, "%s: more than 65535 sequences or 16384 heads", who);
     ALJ_REQUIRE(aligned(c->k_codes, 16) && aligned(c->v_codes, 16) && aligned(c->k_scales, 16) && aligned(c->v_scales, 16),
                 "%s: the cache's planes must be 16-byte aligned", who);

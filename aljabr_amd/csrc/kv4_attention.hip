@@ -523,9 +523,9 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.scale = a.scale;
     p.soft_cap = a.soft_cap;
     p.causal = a.causal;
-    p.window = a.window;
+    p.window = std::min(a.window, 1 << 30);                // past every key; pos - window stays in 32 bits
     const Plan plan = make_plan(v, a.T, a.Hq);
-    if (a.T > 65535 || static_cast<double>(v.H) * plan.groups * (plan.quota + static_cast<double>(v.B)) > 0x7fffff)
+    if (static_cast<double>(v.H) * plan.groups * (plan.quota + static_cast<double>(v.B)) > 0x7fffff)
         return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv4_attention: T = %d rows of %d heads are more than one launch takes", a.T, a.Hq);
     p.row_groups = plan.groups;
     p.quota = plan.quota;
@@ -572,6 +572,8 @@ int check_attention(const aljabr_rocm_kv4_cache *cache, int T, int Hq, Kv4View &
     ALJ_REQUIRE(T > 0 && Hq > 0 && Hq % v.H == 0, "kv4_attention: T = %d must be positive and Hq = %d a multiple of %d KV heads",
                 T, Hq, v.H);
     ALJ_REQUIRE(static_cast<long long>(T) * Hq <= (1 << 30), "kv4_attention: T * Hq exceeds 2^30");
+    ALJ_REQUIRE(static_cast<long long>(v.B) * kv4_capacity(v) <= (1LL << 35),
+                "kv4_attention: sequences * the positions of each exceeds 2^35");   // find_chunk adds up their tiles
     return ALJABR_ROCM_OK;
 }
 

@@ -264,7 +264,8 @@ int aljabr_rocm_paged_attention_gqa_windowed(void *out, const void *Q, const voi
  * Without a block table S = sequences and a sequence holds `rows` positions.
  * With one S = num_blocks: position j of sequence b is row j % rows of block
  * block_table[b * max_blocks + j / rows], as in the paged attention. rows is a
- * multiple of 16, head_dim 64, 128 or 256 (else -3), planes 16-byte aligned.
+ * multiple of 16, at most 2^26, max_blocks * rows at most 2^30, head_dim 64,
+ * 128 or 256 (else -3), planes 16-byte aligned.
  *
  * The calls below read positions, lengths and the table on the device, wait
  * for nothing there and can be captured: a position outside the cache, or on a
@@ -309,7 +310,8 @@ int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, c
  * rows verify a draft, many are a prompt or a chunk of one. soft_cap > 0 caps
  * scores as cap * tanh(score / cap); scale <= 0: 1 / sqrt(head_dim). A row
  * that sees no key gives zeros; rows from counts[b] on are left as they were.
- * Keys on a bad block are not seen. fp32-accurate.
+ * Keys on a bad block are not seen. fp32-accurate. T * Hq is at most 2^30,
+ * sequences * the positions of each at most 2^35.
  * workspace: device scratch for split partials, of
  * aljabr_rocm_kv4_attention_workspace bytes (fewer: fewer splits), not shared
  * by calls that may run at once, captured graphs among them. NULL: the

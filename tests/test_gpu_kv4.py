@@ -352,6 +352,94 @@ def test_workspace_of_any_size(rocm, t):
     check(attend(rocm, dev, q, lens), *want)
 
 
+@pytest.mark.parametrize("t,g", [(1, 4), (3, 8), (20, 4)])
+@pytest.mark.parametrize("b,page", [(65, 0), (130, 16)])
+def test_many_uneven_sequences(rocm, b, page, t, g):
+    """More sequences than a wave has lanes, from no key to all of them."""
+    rng = np.random.default_rng(b + t)
+    lens = rng.integers(0, 200, b)
+    lens[3], lens[64], lens[b - 1] = 200, 200, 1
+    counts = rng.integers(0, t + 1, b)
+    host = plain.Cache(b, 1, 64, 208, page)
+    host.fill(lens)
+    q = query(b, b, t, g, 64)
+    got = attend(rocm, Device(rocm, host), q, lens, counts)
+    check(got, *plain.attention(host, q, lens, counts))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("g", [33, 64, 130])
+def test_one_token_of_many_heads(rocm, d, g):
+    """Groups of more heads than the split kernel stacks."""
+    lens = [500, 31, 0]
+    host = plain.Cache(3, 1, d, 512)
+    host.fill(lens)
+    q = query(g, 3, 1, g, d)
+    got = attend(rocm, Device(rocm, host), q, lens)
+    check(got, *plain.attention(host, q, lens))
+
+
+def test_windows_of_any_size(rocm):
+    host = plain.Cache(2, 2, 64, 64)
+    host.fill([40, 2])
+    dev = Device(rocm, host)
+    for t in (1, 5, 40):
+        q = query(t, 2, t, 4, 64)
+        for causal in (1, 0):
+            for window in (-3, 1, 2 ** 31 - 1):
+                check(attend(rocm, dev, q, [40, 2], causal=causal, window=window),
+                      *plain.attention(host, q, [40, 2], causal=bool(causal), window=window))
+
+
+def test_prompt_of_more_rows_than_a_grid_dimension(rocm):
+    n, d = 70000, 64
+    host = plain.Cache(1, 1, d, 70016)
+    host.codes["k"][:], host.codes["v"][:] = (np.random.default_rng(i).integers(0, 256, host.codes["k"].shape) for i in (1, 2))
+    for w in "kv":
+        host.scales[w][:] = np.float16(0.25)
+    dev = Device(rocm, host)
+    q = query(1, 1, n, 1, d)
+    got = attend(rocm, dev, q, [n], window=40)
+    for at in (0, 65535, 65536, n - 1):                               # four rows, each as the last of a shorter sequence
+        want, bound, live = plain.attention(host, q[:, at:at + 1], [at + 1], window=40)
+        check(got[:, at:at + 1], want, bound, live)
+    assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("paged", [0, 1])
+@pytest.mark.parametrize("t,g", [(1, 2), (5, 8)])
+def test_planes_past_32_bits(rocm, paged, t, g):
+    """Rows at the end of planes of 8 GiB, seen through a window."""
+    h, d, n, seen = 2, 256, 1 << 25, 80
+    rows, blocks = (16, n // 16) if paged else (n, 1)
+    small = plain.Cache(1, h, d, 96)                                   # the last rows alone
+    codes = {w: torch.empty(blocks * h * rows * d // 2, dtype=torch.uint8, device="cuda") for w in "kv"}
+    scales = {w: torch.empty(blocks * h * rows * d // 32, dtype=torch.float16, device="cuda") for w in "kv"}
+    table = torch.arange(n // 16, dtype=torch.int32, device="cuda") if paged else None
+    desc = rocm.Kv4Cache(codes["k"].data_ptr(), scales["k"].data_ptr(), codes["v"].data_ptr(), scales["v"].data_ptr(), ptr(table),
+                         1, h, d, rows, blocks if paged else 0, n // 16 if paged else 0)
+    need, sc = ctypes.c_size_t(), ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv4_cache_bytes", ctypes.byref(desc), ctypes.byref(need), ctypes.byref(sc))
+    assert need.value == codes["k"].numel() and sc.value == 2 * scales["k"].numel()
+    x = np.random.default_rng(t).standard_normal((2, seen, h, d)).astype(np.float32)
+    for i in range(seen):
+        small.write("k", 0, i, x[0, i])
+        small.write("v", 0, i, x[1, i])
+    xd, pos, lens = torch.from_numpy(x).cuda(), ints([n - seen]), ints([n])
+    back = torch.empty(1, seen, h, d, device="cuda")
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_write", ctypes.byref(desc), xd[0].data_ptr(), xd[1].data_ptr(), pos.data_ptr(), None, seen, 0, 0, 0,
+              F32)
+    rocm.call("aljabr_rocm_kv4_read", None, back.data_ptr(), ctypes.byref(desc), pos.data_ptr(), None, seen, 0, 0, 0, F32)
+    assert np.array_equal(back[0].cpu().numpy(), small.rows_of("v", 0, seen)[0].transpose(1, 0, 2).astype(np.float32))
+    q = query(2, 1, t, h * g, d)
+    qd, out = torch.from_numpy(q).cuda(), torch.full(q.shape, POISON, device="cuda")
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_attention", out.data_ptr(), qd.data_ptr(), ctypes.byref(desc), lens.data_ptr(), None, t, h * g, 0.0, 1,
+              64, 0.0, None, 0)
+    check(out.cpu().numpy(), *plain.attention(small, q, [seen], window=64))
+
+
 def test_same_call_same_bits(rocm):
     host = plain.Cache(2, 4, 128, 1024)
     host.fill([1024, 513])

@@ -96,3 +96,15 @@ def test_encoder_is_within_half_a_step():
     # Half a step; a whole one and the scale's rounding (2^-9 of 8 steps) for a value as large as the top one, of the other sign.
     top = np.abs(x).reshape(64, 8, 32) > 7.5 * step * (1 - 2.0 ** -8)
     assert (err <= np.where(top, 1 + 2.0 ** -6, 0.5) * step + 2.0 ** -25 * 8).all()
+
+
+def test_limits_of_sizes():
+    lib, n = abi.load(), ctypes.c_size_t()
+    ask = lambda c, t=1, hq=32: lib.aljabr_rocm_kv4_attention(P, P, ctypes.byref(c), P, None, t, hq, 0.0, 1, 0, 0.0, None, 0)
+    paged = dict(block_table=0x50000, num_blocks=1 << 20)
+    assert ask(cache(rows=(1 << 26) + 16)) == -2
+    assert ask(cache(max_blocks=(1 << 24) + 1, **paged)) == -2                     # 2^30 positions and a block
+    assert ask(cache(sequences=33, max_blocks=1 << 24, **paged)) == -2             # 33 of 2^30: past 2^35
+    assert ask(cache(), t=1 << 26) == -2                                           # T * Hq
+    assert lib.aljabr_rocm_kv4_write(ctypes.byref(cache(max_blocks=(1 << 24) + 1, **paged)), P, P, P, None, 1, 0, 0, 0, 0) == -2
+    assert "2^30" in abi.last_error()
