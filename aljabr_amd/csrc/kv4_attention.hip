@@ -33,7 +33,7 @@
 //
 // Bound by the vector ALU (55 to 59 % of the kernel's time): about 364
 // instructions a tile of 32 keys and 8 rows at D = 128, most of them decoding,
-// against 34 matrix products that run beside them. Measured with the merge: one
+// against 17 matrix products that run beside them. Measured with the merge: one
 // sequence of 131072 keys 39.5 us (151 MB, 3.8 TB/s), 16 of 4096 23.8 us, 512
 // keys 8.9 us. Three workgroups a CU at D <= 128 with 8 rows (registers allow
 // no more): a wave of another workgroup covers a wave's waits.
