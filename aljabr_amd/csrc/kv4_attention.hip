@@ -27,8 +27,8 @@
 // V product, of ones, so numerator and denominator hold the same weights.
 //
 // Keys a row does not see get weight 0, and V rows past a sequence's end may
-// hold anything: their scales are taken as 0. A scale that is not finite among
-// keys that only some rows see is taken as 0 too and remembered for the rows
+// hold anything: their scales are taken as 0. A scale that is not finite, or so
+// large that its values may not be, among keys that only some rows see is taken as 0 too and remembered for the rows
 // that see it: their values of its block are made NaN at the end.
 //
 // Bound by the vector ALU (55 to 59 % of the kernel's time): about 364

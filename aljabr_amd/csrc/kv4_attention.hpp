@@ -208,8 +208,9 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)p));
 }
 
+// A scale that is not finite, or past the writer's largest (8160): a code times it may leave fp16.
 __device__ __forceinline__ bool not_finite(_Float16 x) {
-    return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) == 0x7c00u;
+    return (__builtin_bit_cast(uint16_t, x) & 0x7fffu) > 0x6ff8u;
 }
 
 // x of the lane 8 columns away (the row's other fp16 part).

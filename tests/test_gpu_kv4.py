@@ -333,6 +333,23 @@ def test_window_leaves_nan_behind(rocm):
     check(got[:, 1:], want[:, 1:], bound[:, 1:], np.ones((1, 2), bool))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", [1, 6, 40])
+@pytest.mark.parametrize("scale", [8190.0, 30000.0, -65504.0, np.inf])
+def test_scales_past_fp16_outside_the_window(rocm, d, t, scale):
+    """Finite scales whose values overflow, among keys of the first tiles that no row sees."""
+    host = plain.Cache(1, 2, d, 208)
+    host.fill([200])
+    q = query(d, 1, t, 8, d)
+    want = plain.attention(host, q, [200], window=48)
+    first = 200 - t - 48 + 1                                           # the first key that a row sees
+    for w in "kv":
+        host.codes[w][:, :, :first] = np.random.default_rng(t).integers(0, 256, host.codes[w][:, :, :first].shape)
+        host.scales[w][..., :first] = scale
+        host.scales[w][..., 200:] = scale                              # and past the end
+    check(attend(rocm, Device(rocm, host), q, [200], window=48), *want)
+
+
 @pytest.mark.parametrize("t", [1, 20])
 def test_workspace_of_any_size(rocm, t):
     host = plain.Cache(2, 2, 128, 1024, 32)
