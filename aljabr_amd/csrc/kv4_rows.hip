@@ -15,11 +15,12 @@
 //   S^T = K Q^T, O^T += V^T P^T, rows along the lanes: a row's query parts,
 // maximum and sum stay in its two lanes.
 // Two products a score and a value, for the two fp16 parts of queries and
-// weights. Measured: a causal prompt of 2048 rows of 32 heads of 128 98.8 us (0.35
+// weights. Measured: a causal prompt of 2048 rows of 32 heads of 128 98 us (0.35
 // PFLOP/s, 0.70 with both parts; matrix cores 25 %, vector ALU 34 %), 256 rows
-// over 2048 keys 38.3 us. The waves' products, decoding and softmax go in turn:
+// over 2048 keys 37.6 us. The waves' products and softmax go in turn:
 // what a CU's other workgroup covers is lost where the last rows of a causal
-// prompt, of the most keys, run alone.
+// prompt, of the most keys, run alone. The next tile's decoding is laid between
+// the score products (3 % of a prompt of 4096 rows).
 #include "kv4_attention.hpp"
 
 namespace aljabr {
@@ -116,19 +117,10 @@ __device__ __forceinline__ bool both_ok(const Params &p, int b, int n_keys, int 
     return !PAGED || half_ok<PAGED>(p, b, n_keys, kt) == 3;
 }
 
-// Decodes a thread's share into the tile's fragments. `edge`: some row does not see some key; scales of V rows past
-// the end, or on no block, are then taken as 0, and one that is not finite too, with its key's bit set in bad[block].
+// The scales of a thread's two V rows. `edge`: some row does not see some key; scales of V rows past the end, or on
+// no block, are then taken as 0, and one that is not finite too, with its key's bit set in bad[block].
 template <int D>
-__device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, int k0, int n_keys, bool edge, int tid,
-                                            _Float16 *buf, uint32_t *bad) {
-    const int key = tid >> 3, kd = (tid & 7) * (D / 64);
-    const half2v kdup = as_half2(__builtin_amdgcn_perm(x.ks, x.ks, 0x01000100u));
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-        uint32_t f[4];
-        decode8(g, x.k[i], kdup, f);
-        *reinterpret_cast<uint4 *>(buf + key * Shape<D>::kKStride + 8 * (kd + i)) = make_uint4(f[0], f[1], f[2], f[3]);
-    }
+__device__ __forceinline__ half2v value_scales(const Raw<D> &x, int k0, int n_keys, bool edge, int tid, uint32_t *bad) {
     const int pr = tid >> 4, n = tid & 15;                                 // pair of keys 2 pr, 2 pr + 1
     half2v vd = as_half2(x.vs);
     if (edge) {
@@ -142,6 +134,21 @@ __device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, int
             }
         }
     }
+    return vd;
+}
+
+// Decodes a thread's share into the tile's fragments.
+template <int D>
+__device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, half2v vd, int tid, _Float16 *buf) {
+    const int key = tid >> 3, kd = (tid & 7) * (D / 64);
+    const half2v kdup = as_half2(__builtin_amdgcn_perm(x.ks, x.ks, 0x01000100u));
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        uint32_t f[4];
+        decode8(g, x.k[i], kdup, f);
+        *reinterpret_cast<uint4 *>(buf + key * Shape<D>::kKStride + 8 * (kd + i)) = make_uint4(f[0], f[1], f[2], f[3]);
+    }
+    const int pr = tid >> 4, n = tid & 15;                                 // pair of keys 2 pr, 2 pr + 1
     _Float16 *vt = buf + kTile * Shape<D>::kKStride + n * kVStride + 2 * pr;
 #pragma unroll
     for (int i = 0; i < Shape<D>::kPieces; ++i)
@@ -249,7 +256,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     if (BUFS == 2 && t0 < t1) {
         __syncthreads();                                                   // `bad` is clear
         ok_next = both_ok<PAGED>(p, b, seq.n, t0);
-        decode_tile<D>(g, raw, t0 * kTile, seq.n, edge_of(t0) || !ok_next, tid, lds, bad[0]);
+        decode_tile<D>(g, raw, value_scales<D>(raw, t0 * kTile, seq.n, edge_of(t0) || !ok_next, tid, bad[0]), tid, lds);
         if (t0 + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, t0 + 1, tid, raw);
     }
     for (int kt = t0, i = 0; kt < t1; ++kt, i = i == 2 ? 0 : i + 1) {
@@ -263,30 +270,46 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             for (int st = 0; st < STEPS; ++st) ka[st] = *reinterpret_cast<const half8 *>(kl + nl * KS + 16 * st + 8 * h);
             __builtin_amdgcn_sched_barrier(0);
         };
+        // S^T: accumulator j is key k0 + 8 (j / 4) + 4h + j % 4 of this lane's row.
+        f32x16 s = {};
+        auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], s, 0, 0, 0);
+            }
+        };
+        const bool unseen = idle || k0 >= w_hi || k0 + kTile <= w_lo;      // by the wave's rows
         if constexpr (BUFS == 2) {
-            read_keys();                                                   // they arrive while the next tile is decoded
+            read_keys();
             if (tid < 8) bad[ahead == 2 ? 0 : ahead + 1][tid] = 0;         // the tile before this one's
+            half2v vd = {};
             if (kt + 1 < t1) {
                 ok_next = both_ok<PAGED>(p, b, seq.n, kt + 1);
-                decode_tile<D>(g, raw, k0 + kTile, seq.n, edge_of(kt + 1) || !ok_next, tid,
-                               lds + ((kt + 1 - t0) & 1) * Shape<D>::kHalves, bad[ahead]);
-                if (kt + 2 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 2, tid, raw);
+                vd = value_scales<D>(raw, k0 + kTile, seq.n, edge_of(kt + 1) || !ok_next, tid, bad[ahead]);
             }
+            // The next tile is decoded between the products (past the last one, what it holds is not used).
+            __builtin_amdgcn_sched_barrier(0);
+            scores();
+            decode_tile<D>(g, raw, vd, tid, lds + ((kt + 1 - t0) & 1) * Shape<D>::kHalves);
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);         // a product,
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);         // six vector instructions (about its 32 cycles),
+                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);         // a store to LDS
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (kt + 2 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 2, tid, raw);
+            if (unseen) continue;
         } else {
             ok = both_ok<PAGED>(p, b, seq.n, kt);
             if (tid < 8) bad[ahead][tid] = 0;
-            decode_tile<D>(g, raw, k0, seq.n, edge_of(kt) || !ok, tid, lds, bad[i]);
+            decode_tile<D>(g, raw, value_scales<D>(raw, k0, seq.n, edge_of(kt) || !ok, tid, bad[i]), tid, lds);
             if (kt + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 1, tid, raw);
             __syncthreads();
             read_keys();
-        }
-        if (idle || k0 >= w_hi || k0 + kTile <= w_lo) continue;
-        // S^T: accumulator j is key k0 + 8 (j / 4) + 4h + j % 4 of this lane's row.
-        f32x16 s = {};
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], s, 0, 0, 0);
+            if (unseen) continue;
+            scores();
         }
         // V's fragments arrive while the weights are computed.
         half8 va[2][DT];
