@@ -270,6 +270,9 @@ int kv4_view(const aljabr_rocm_kv4_cache *c, const char *who, Kv4View &v) {
     if (c->block_table)
         ALJ_REQUIRE(c->num_blocks > 0 && c->max_blocks > 0 && static_cast<long long>(c->max_blocks) * c->rows <= (1LL << 30),
                     "%s: a paged cache needs num_blocks and max_blocks, max_blocks * rows at most 2^30", who);
+    else
+        // kv4_cache_bytes counts such a description's blocks: as a contiguous cache its sequences may pass the planes.
+        ALJ_REQUIRE(c->num_blocks == 0 && c->max_blocks == 0, "%s: num_blocks and max_blocks without a block_table", who);
     ALJ_REQUIRE(c->sequences <= 65535 && c->n_kv_heads <= 16384, "%s: more than 65535 sequences or 16384 heads", who);
     ALJ_REQUIRE(aligned(c->k_codes, 16) && aligned(c->v_codes, 16) && aligned(c->k_scales, 16) && aligned(c->v_scales, 16),
                 "%s: the cache's planes must be 16-byte aligned", who);

@@ -276,7 +276,7 @@ typedef struct aljabr_rocm_kv4_cache {
     const void *block_table;                         /* device int32 [sequences][max_blocks], or NULL */
     int32_t sequences, n_kv_heads, head_dim;
     int32_t rows;                                    /* positions of a sequence, or of a block */
-    int32_t num_blocks, max_blocks;                  /* with a block table */
+    int32_t num_blocks, max_blocks;                  /* with a block table, else 0 */
 } aljabr_rocm_kv4_cache;
 
 /* Bytes of one codes and one scales plane (K's; V's are alike) of a cache with

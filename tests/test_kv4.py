@@ -108,3 +108,15 @@ def test_limits_of_sizes():
     assert ask(cache(), t=1 << 26) == -2                                           # T * Hq
     assert lib.aljabr_rocm_kv4_write(ctypes.byref(cache(max_blocks=(1 << 24) + 1, **paged)), P, P, P, None, 1, 0, 0, 0, 0) == -2
     assert "2^30" in abi.last_error()
+
+
+@pytest.mark.parametrize("blocks", [dict(num_blocks=4), dict(max_blocks=4), dict(num_blocks=1, max_blocks=2), dict(num_blocks=-1)])
+def test_blocks_without_a_table_are_refused(blocks):
+    """kv4_cache_bytes sizes such planes by num_blocks: taken as contiguous, `sequences` may reach past them."""
+    lib, c = abi.load(), ctypes.byref(cache(**blocks))
+    n = ctypes.c_size_t()
+    assert lib.aljabr_rocm_kv4_write(c, P, P, P, None, 1, 0, 0, 0, abi.TYPE_F32) == -2
+    assert lib.aljabr_rocm_kv4_read(P, P, c, P, None, 1, 0, 0, 0, abi.TYPE_F32) == -2
+    assert lib.aljabr_rocm_kv4_attention(P, P, c, P, None, 1, 32, 0.0, 1, 0, 0.0, None, 0) == -2
+    assert lib.aljabr_rocm_kv4_attention_workspace(c, 1, 32, ctypes.byref(n)) == -2
+    assert "block_table" in abi.last_error()
