@@ -315,9 +315,13 @@ int aljabr_rocm_kv4_cache_bytes(const aljabr_rocm_kv4_cache *cache, size_t *code
                 "sequences (or num_blocks) and n_kv_heads must be positive, rows a positive multiple of 16");
     if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
         return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv4_cache_bytes: head_dim %d is not 64, 128 or 256", cache->head_dim);
-    const size_t rows = static_cast<size_t>(paged ? cache->num_blocks : cache->sequences) * cache->n_kv_heads * cache->rows;
-    *codes_bytes = rows * (cache->head_dim / 2);
-    *scales_bytes = rows * (cache->head_dim / 32) * 2;
+    const size_t of_each = static_cast<size_t>(cache->n_kv_heads) * cache->rows;      // below 2^62
+    size_t rows, codes;
+    ALJ_REQUIRE(!__builtin_mul_overflow(static_cast<size_t>(paged ? cache->num_blocks : cache->sequences), of_each, &rows) &&
+                    !__builtin_mul_overflow(rows, static_cast<size_t>(cache->head_dim / 2), &codes),
+                "kv4_cache_bytes: a plane of this shape has 2^64 bytes or more");
+    *codes_bytes = codes;
+    *scales_bytes = codes / 8;                               // 2 bytes for every 16 of codes
     return ALJABR_ROCM_OK;
 }
 

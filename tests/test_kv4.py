@@ -120,3 +120,15 @@ def test_blocks_without_a_table_are_refused(blocks):
     assert lib.aljabr_rocm_kv4_attention(P, P, c, P, None, 1, 32, 0.0, 1, 0, 0.0, None, 0) == -2
     assert lib.aljabr_rocm_kv4_attention_workspace(c, 1, 32, ctypes.byref(n)) == -2
     assert "block_table" in abi.last_error()
+
+
+def test_cache_bytes_past_64_bits_are_refused():
+    lib, codes, scales = abi.load(), ctypes.c_size_t(7), ctypes.c_size_t(7)
+    ask = lambda **kw: lib.aljabr_rocm_kv4_cache_bytes(ctypes.byref(cache(**kw)), ctypes.byref(codes), ctypes.byref(scales))
+    top = 2 ** 31 - 1
+    assert ask(num_blocks=top, n_kv_heads=top, rows=top - 15, head_dim=256) == -2
+    assert ask(num_blocks=1 << 30, n_kv_heads=1 << 14, rows=1 << 20, head_dim=64) == -2     # 2^69: 0 in 64 bits
+    assert ask(sequences=1 << 29, n_kv_heads=1 << 15, rows=1 << 15, head_dim=64) == -2      # codes 2^64
+    assert (codes.value, scales.value) == (7, 7)
+    assert ask(sequences=1 << 28, n_kv_heads=1 << 15, rows=1 << 15, head_dim=64) == 0       # codes 2^63
+    assert (codes.value, scales.value) == (1 << 63, 1 << 60)
