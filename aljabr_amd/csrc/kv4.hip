@@ -247,6 +247,8 @@ int check_rows(const char *who, const Kv4View &v, const void *k, const void *vv,
     ALJ_REQUIRE(T > 0 && T <= (1 << 30), "%s: T = %d is outside [1, 2^30]", who, T);
     if (type != ALJABR_ROCM_TYPE_F32 && type != ALJABR_ROCM_TYPE_F16)
         return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "%s: K/V type %d is not F32 or F16", who, type);
+    ALJ_REQUIRE(static_cast<long long>(T) * (v.D / 8) <= 0xffffff00LL,      // lanes of a launch, whole workgroups
+                "%s: T = %d rows of %d values are more than one launch takes", who, T, v.D);
     ALJ_REQUIRE(sb >= 0 && st >= 0 && sh >= 0, "%s: strides must not be negative", who);
     if (!sb && !st && !sh) {
         sh = v.D;

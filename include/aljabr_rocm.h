@@ -288,7 +288,8 @@ int aljabr_rocm_kv4_cache_bytes(const aljabr_rocm_kv4_cache *cache, size_t *code
  * adjacent; all three 0: dense) into the cache: row t of sequence b goes to
  * position positions[b] + t, for t < counts[b] (counts NULL: T). Rows that the
  * cache does not have are dropped. K or V may be NULL: only the other is
- * written. Rows of one call must be different rows of the cache.
+ * written. Rows of one call must be different rows of the cache. T *
+ * head_dim is below 2^35.
  * Per block: top = its smallest value if that is at least as large in
  * magnitude as its largest, else its largest; scale = -top / 8 rounded to 8
  * significant bits (ties to even; a multiple of 2^-24; at most 8160); code =

@@ -132,3 +132,12 @@ def test_cache_bytes_past_64_bits_are_refused():
     assert (codes.value, scales.value) == (7, 7)
     assert ask(sequences=1 << 28, n_kv_heads=1 << 15, rows=1 << 15, head_dim=64) == 0       # codes 2^63
     assert (codes.value, scales.value) == (1 << 63, 1 << 60)
+
+
+@pytest.mark.parametrize("d,t", [(64, 1 << 29), (128, 1 << 28), (256, 1 << 27), (256, 1 << 30)])
+def test_rows_of_more_than_one_launch_are_refused(d, t):
+    """T rows of D / 8 lanes each: a launch takes fewer than 2^32."""
+    lib, c = abi.load(), ctypes.byref(cache(head_dim=d))
+    assert lib.aljabr_rocm_kv4_write(c, P, P, P, None, t, 0, 0, 0, abi.TYPE_F32) == -2
+    assert "launch" in abi.last_error()
+    assert lib.aljabr_rocm_kv4_read(P, P, c, P, None, t, 0, 0, 0, abi.TYPE_F16) == -2
