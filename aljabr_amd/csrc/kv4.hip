@@ -342,6 +342,9 @@ int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, c
     Kv4View v;
     int rc = kv4_view(cache, "kv4_read", v);
     if (rc == ALJABR_ROCM_OK) rc = check_rows("kv4_read", v, K, V, positions, T, stride_b, stride_t, stride_h, type);
+    if (rc == ALJABR_ROCM_OK)      // rows read to one place: which stays would be chance
+        ALJ_REQUIRE((stride_b || v.B == 1) && (stride_t || T == 1) && (stride_h || v.H == 1),
+                    "kv4_read: a stride of 0 over several sequences, tokens or heads");
     if (rc == ALJABR_ROCM_OK) rc = ensure_ready();
     if (rc == ALJABR_ROCM_OK) rc = enqueue_kv4_read(v, K, V, positions, counts, T, stride_b, stride_t, stride_h, type);
     return rc == ALJABR_ROCM_OK ? finish_launch("kv4_read") : rc;

@@ -299,8 +299,9 @@ int aljabr_rocm_kv4_write(const aljabr_rocm_kv4_cache *cache, const void *K, con
                           const int *counts, int T, long long stride_b, long long stride_t, long long stride_h,
                           int type);
 /* The values of rows positions[b] + t, t < counts[b], as F32 or F16 (both
- * exact), with the layout rules of kv4_write. Rows that the cache does not
- * have read as zeros; rows from counts[b] on are left as they were. */
+ * exact), with the layout rules of kv4_write; the rows must not overlap (-2 for
+ * a stride of 0 over several). Rows that the cache does not have read as
+ * zeros; rows from counts[b] on are left as they were. */
 int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, const int *positions, const int *counts,
                          int T, long long stride_b, long long stride_t, long long stride_h, int type);
 /* GQA attention over the cache: Q and out [sequences][T][Hq][head_dim] fp32,

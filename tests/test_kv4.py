@@ -141,3 +141,14 @@ def test_rows_of_more_than_one_launch_are_refused(d, t):
     assert lib.aljabr_rocm_kv4_write(c, P, P, P, None, t, 0, 0, 0, abi.TYPE_F32) == -2
     assert "launch" in abi.last_error()
     assert lib.aljabr_rocm_kv4_read(P, P, c, P, None, t, 0, 0, 0, abi.TYPE_F16) == -2
+
+
+@pytest.mark.parametrize("strides,shape", [((0, 128, 256), (2, 5, 2)), ((4096, 0, 128), (2, 5, 2)), ((4096, 128, 0), (2, 5, 2)),
+                                           ((4096, 128, 0), (1, 1, 2))])
+def test_read_into_rows_on_one_place_is_refused(strides, shape):
+    """A stride of 0 reads a shared source row for several heads, tokens or sequences; what is read back has no such place."""
+    lib = abi.load()
+    b, t, h = shape
+    c = ctypes.byref(cache(sequences=b, n_kv_heads=h))
+    assert lib.aljabr_rocm_kv4_read(P, P, c, P, None, t, *strides, abi.TYPE_F32) == -2
+    assert "stride" in abi.last_error()
