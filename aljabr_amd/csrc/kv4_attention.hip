@@ -498,9 +498,10 @@ Plan make_plan(const Kv4View &v, int T, int Hq) {
     s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
     const long long items = static_cast<long long>(v.H) * s.groups;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const long long most = v.B * ((static_cast<long long>(kv4_capacity(v)) + kTile * waves(v.D) - 1) / (kTile * waves(v.D)));
-    s.quota = static_cast<int>(std::min((s.rows == kRowsBlock ? 1 : v.D == 256 ? 3 : 2) * cus / items, most));
-    if (s.quota <= 1) s.quota = 0;                         // heads and row groups fill the chip, or there is one chunk
+    const int least = kTile * (s.rows == kRowsBlock ? kRowsLeast : waves(v.D));          // keys of the smallest chunk
+    const long long most = (static_cast<long long>(kv4_capacity(v)) + least - 1) / least;   // chunks of a sequence
+    s.quota = static_cast<int>(std::min((s.rows == kRowsBlock ? 1 : v.D == 256 ? 3 : 2) * cus / items, v.B * most));
+    if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
     return s;
 }
 

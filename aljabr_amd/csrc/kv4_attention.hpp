@@ -18,6 +18,7 @@ constexpr int kTile = 32;                    // keys a wave takes at once
 // Waves of a workgroup, and tiles it takes at the least (two at D = 256, whose ring of tiles is twice as large).
 __host__ __device__ constexpr int waves(int D) { return D == 256 ? 2 : 4; }
 constexpr int kRowsBlock = 128;              // rows a workgroup of the rows kernel stacks
+constexpr int kRowsLeast = 4;                // tiles it takes at the least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightScale = 8192.0f;      // weights are at most 4
 

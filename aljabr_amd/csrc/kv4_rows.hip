@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     work_of(p, blockIdx.x, item, w);
     const int group = group_of(p, p.by_heads(item)), kvh = item - p.by_heads(item) * p.v.H;
     const int r0 = group * kRowsBlock;
-    const Chunk chunk = find_chunk(p, w, r0, kRowsBlock, 4);
+    const Chunk chunk = find_chunk(p, w, r0, kRowsBlock, kRowsLeast);
     if (chunk.b < 0) return;
     const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
     if (p.quota && w == chunk.first && tid == 0)

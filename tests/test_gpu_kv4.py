@@ -577,3 +577,44 @@ def test_two_streams_at_once(rocm):
         for i, outs in enumerate(pool.map(work, (0, 1))):
             for got in outs:
                 assert np.array_equal(got, want[i])
+
+
+def workspace_bytes(rocm, dev, t, hq):
+    n = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv4_attention_workspace", dev.ref(), t, hq, ctypes.byref(n))
+    return n.value
+
+
+@pytest.mark.parametrize("d,cap,t,g", [(64, 128, 1, 4), (128, 128, 5, 4), (128, 128, 20, 4), (256, 64, 1, 2), (256, 128, 40, 1)])
+def test_caches_of_one_chunk_take_no_scratch(rocm, d, cap, t, g):
+    """Sequences too short to be split: no partials, so a call under capture needs no workspace."""
+    b = 7
+    lens = [cap, 1, 33, 0, cap - 1, 64, 17]
+    host = plain.Cache(b, 2, d, cap, 16)
+    host.fill(lens)
+    dev, q = Device(rocm, host), query(d + t, b, t, 2 * g, d)
+    assert workspace_bytes(rocm, dev, t, 2 * g) == 0
+    want = plain.attention(host, q, lens)
+    qd, ld, out = torch.from_numpy(q).cuda(), ints(lens), torch.zeros(b, t, 2 * g, d, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def body():
+        rocm.call("aljabr_rocm_set_stream", s.cuda_stream)
+        rocm.call("aljabr_rocm_set_sync_mode", 0)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+            rocm.call("aljabr_rocm_kv4_attention", out.data_ptr(), qd.data_ptr(), dev.ref(), ld.data_ptr(), None, t, 2 * g, 0.0, 1,
+                      0, 0.0, None, 0)
+        for _ in range(3):
+            out.fill_(POISON)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            check(out.cpu().numpy(), *want)
+        held = scratch_held(rocm)
+        rocm.call("aljabr_rocm_set_stream", None)
+        rocm.call("aljabr_rocm_set_sync_mode", 1)
+        return held
+
+    assert fresh_thread(body) == 0
