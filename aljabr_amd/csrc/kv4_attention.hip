@@ -205,7 +205,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
     if (chunk.b < 0) return;
     const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
     if (p.quota && w == chunk.first && threadIdx.x == 0)
-        p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.first, chunk.count);
+        p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.slot, chunk.count);
     const Seq seq = chunk.seq;
     const int r1 = min(r0 + ROWS, seq.cnt * p.G);
 
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
             const int t = p.by_g(r), g = r - t * p.G;
             p.out[((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D + dd] = L == 0.0f ? 0.0f : O / L;
         } else {
-            const long long row = (static_cast<long long>(w) * p.v.H * p.row_groups + item) * ROWS + i / D;
+            const long long row = (static_cast<long long>(chunk.slot + w - chunk.first) * p.v.H * p.row_groups + item) * ROWS + i / D;
             p.part_o[row * D + dd] = O;
             if (dd == 0) *reinterpret_cast<float2 *>(p.part_ml + row * 2) = make_float2(M, L);
         }
@@ -505,10 +505,15 @@ Plan make_plan(const Kv4View &v, int T, int Hq) {
     return s;
 }
 
+// Slots of partials that so many chunks need at the most: sequence b of x_b > 1 chunk sizes takes ceil(x_b), fewer
+// than 2 x_b and than x_b + 1, and the x_b add up to at most the quota.
+size_t partial_slots(const Kv4View &v, int quota) {
+    return quota ? static_cast<size_t>(std::min<long long>(2LL * quota - 1, static_cast<long long>(quota) + v.B - 1)) : 0;
+}
 // Bytes of partials with this many chunks.
 size_t partial_bytes(const Kv4View &v, const Plan &s, int quota) {
-    return static_cast<size_t>(v.H) * s.groups * ((static_cast<size_t>(quota) + v.B) * s.rows * (v.D + 2) * sizeof(float) +
-                                                  v.B * sizeof(int2));
+    return static_cast<size_t>(v.H) * s.groups *
+           (partial_slots(v, quota) * s.rows * (v.D + 2) * sizeof(float) + v.B * sizeof(int2));
 }
 
 }  // namespace
@@ -546,15 +551,18 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
         float *part = a.scratch;
         if (a.scratch) {
             // As many chunks as the caller's workspace holds the partials of.
-            const size_t none = partial_bytes(v, plan, 0), one = partial_bytes(v, plan, 1) - none;
-            const size_t fit = a.scratch_bytes < none ? 0 : (a.scratch_bytes - none) / one;
-            if (fit < static_cast<size_t>(p.quota)) p.quota = fit < 2 ? 0 : static_cast<int>(fit);
+            const size_t none = partial_bytes(v, plan, 0), slot = partial_bytes(v, plan, 1) - none;
+            const size_t fit = a.scratch_bytes < none ? 0 : (a.scratch_bytes - none) / slot;
+            if (fit < partial_slots(v, p.quota)) {
+                const size_t most = std::max((fit + 1) / 2, fit + 1 > static_cast<size_t>(v.B) ? fit + 1 - v.B : 0);
+                p.quota = most < 2 ? 0 : static_cast<int>(most);
+            }
         } else {
             part = static_cast<float *>(stream_scratch(partial_bytes(v, plan, p.quota)));
             if (!part) return ALJABR_ROCM_ERR_BUFFER;
         }
         p.part_o = part;
-        const size_t all = (static_cast<size_t>(p.quota) + v.B) * v.H * plan.groups * plan.rows;
+        const size_t all = partial_slots(v, p.quota) * v.H * plan.groups * plan.rows;
         p.part_ml = part + all * v.D;
         p.chunks = reinterpret_cast<int2 *>(p.part_ml + 2 * all);
     }

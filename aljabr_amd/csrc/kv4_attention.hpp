@@ -46,8 +46,8 @@ struct Params {
     float scale, soft_cap;
     int causal, window;
     int quota;                               // chunks that the keys of all sequences are cut into (about), 0: one each
-    float *part_o, *part_ml;                 // per chunk, KV head, row group and stacked row: D sums, and (m, l)
-    int2 *chunks;                            // per sequence, KV head and row group: its first chunk and their number
+    float *part_o, *part_ml;                 // per slot, KV head, row group and stacked row: D sums, and (m, l)
+    int2 *chunks;                            // per sequence, KV head and row group: its first slot and its chunks
 };
 
 // A sequence's keys and its rows.
@@ -94,16 +94,20 @@ __device__ __forceinline__ int wave_scan(int v) {
 // One chunk of the work of a row group: tiles [t0, t1) of sequence b. The
 // tiles of all sequences are cut into chunks of one size, a multiple of
 // `least`, about `quota` of them: a batch of uneven lengths keeps every
-// workgroup busy alike. Chunks are numbered through the sequences.
+// workgroup busy alike. Chunks are numbered through the sequences, and slots
+// of partials through those of several chunks (a single chunk writes its rows
+// itself): fewer than 2 quota, as each of these is longer than one chunk, and
+// fewer than quota + B (partial_slots).
 struct Chunk {
     int b, t0, t1;
     int first, count;        // of the sequence's chunks
+    int slot;                // of the first
     Seq seq;
 };
 
 // Chunk number w; b < 0 past the end. Called by whole waves.
 __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int rows, int least) {
-    Chunk c{-1, 0, 0, 0, 0, {0, 0}};
+    Chunk c{-1, 0, 0, 0, 0, 0, {0, 0}};
     const int lane = threadIdx.x & 63, B = p.v.B;
     if (p.quota == 0 || B == 1) {
         const int b = p.quota ? 0 : w;
@@ -141,7 +145,7 @@ __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int 
     int per = max(p.by_chunks(total + p.quota - 1), least);
     per = (per + least - 1) / least * least;
     const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
-    int before = 0;
+    int before = 0, slots = 0;
     for (int b0 = 0; b0 <= last; b0 += 64) {
         if (last) {
             a = z = 0;
@@ -157,12 +161,13 @@ __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int 
         n -= n > 0 && (n - 1) * per >= z - a ? 1 : 0;
         n += n * per < z - a ? 1 : 0;
         n = r0 < s.cnt * p.G ? max(n, 1) : 0;
-        const int end = before + wave_scan(n);
+        const int end = before + wave_scan(n), slot_end = slots + wave_scan(n > 1 ? n : 0);
         const uint64_t hit = __ballot(w >= end - n && w < end);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             c.count = __builtin_amdgcn_readlane(n, l);
             c.first = __builtin_amdgcn_readlane(end, l) - c.count;
+            c.slot = __builtin_amdgcn_readlane(slot_end, l) - c.count;       // of one chunk: not used
             a = __builtin_amdgcn_readlane(a, l);
             z = __builtin_amdgcn_readlane(z, l);
             c.seq.n = __builtin_amdgcn_readlane(s.n, l);
@@ -173,6 +178,7 @@ __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int 
             return c;
         }
         before = __builtin_amdgcn_readlane(end, 63);
+        slots = __builtin_amdgcn_readlane(slot_end, 63);
     }
     return c;
 }

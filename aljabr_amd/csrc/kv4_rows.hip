@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     if (chunk.b < 0) return;
     const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
     if (p.quota && w == chunk.first && tid == 0)
-        p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.first, chunk.count);
+        p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.slot, chunk.count);
     const Seq seq = chunk.seq;
     const int r1 = min(r0 + kRowsBlock, seq.cnt * p.G);
     const int w0 = r0 + 32 * wave;
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     if (m == -INFINITY && l != l) m = 0.0f;                                // a NaN score alone leaves no reference
     const bool whole = chunk.count == 1;
     const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-    const long long part = (static_cast<long long>(w) * p.v.H * p.row_groups + item) * kRowsBlock + 32 * wave;
+    const long long part = (static_cast<long long>(chunk.slot + w - chunk.first) * p.v.H * p.row_groups + item) * kRowsBlock + 32 * wave;
     if (!whole && h == 0 && w0 + nl < r1) *reinterpret_cast<float2 *>(p.part_ml + (part + nl) * 2) = make_float2(m, l);
     __syncthreads();                                                       // every wave is done with the tiles
     // O through LDS, so that whole lines are stored: rounds of two blocks of dims (D = 64: of one), a wave's own

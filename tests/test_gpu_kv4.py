@@ -618,3 +618,44 @@ def test_caches_of_one_chunk_take_no_scratch(rocm, d, cap, t, g):
         return held
 
     assert fresh_thread(body) == 0
+
+
+def scratch_test(rocm, b, t, hkv, g, d, lens, counts=None, page=0):
+    """A call on exactly the workspace that was asked for, on half and a third of it; nothing past it is written."""
+    host = plain.Cache(b, hkv, d, -(-max(lens) // 16) * 16, page)
+    host.fill(lens)
+    dev, q = Device(rocm, host), query(b + t, b, t, hkv * g, d)
+    size = workspace_bytes(rocm, dev, t, hkv * g)
+    assert size > 0
+    want = plain.attention(host, q, lens, counts)
+    for part in (1, 2, 3):
+        ws = torch.full((size + 4096,), 0xCD, dtype=torch.uint8, device="cuda")
+        check(attend(rocm, dev, q, lens, counts, workspace=ws[:size // part]), *want)
+        assert (ws[size // part:] == 0xCD).all()
+
+
+@pytest.mark.parametrize("d,t,g", [(64, 1, 3), (128, 1, 4), (128, 12, 4), (256, 2, 2)])
+@pytest.mark.parametrize("page", [0, 32])
+def test_workspace_of_uneven_batches(rocm, d, t, g, page):
+    """A few long sequences among many short ones, in several groups of 64: only the long ones are split."""
+    b = 150
+    lens = [20 + 3 * (i % 7) for i in range(b)]
+    for i, n in ((0, 700), (63, 1100), (64, 900), (100, 0), (127, 800), (128, 1500), (149, 1024)):
+        lens[i] = n
+    scratch_test(rocm, b, t, 1, g, d, lens, page=page)
+
+
+def test_workspace_of_an_even_batch(rocm):
+    scratch_test(rocm, 5, 1, 2, 4, 128, [900] * 5)
+
+
+@pytest.mark.parametrize("b,t,hkv,g,d,block", [(64, 256, 8, 4, 128, 128), (64, 32, 8, 2, 64, 128), (1024, 1, 1, 8, 128, 8),
+                                               (4096, 1, 8, 4, 256, 8)])
+def test_workspace_grows_with_the_chunks_not_the_batch(rocm, b, t, hkv, g, d, block):
+    """Partials of twice the chunks that fill the chip, and a first chunk and number for each sequence."""
+    desc = rocm.Kv4Cache(0x10000, 0x20000, 0x30000, 0x40000, None, b, hkv, d, 4096, 0, 0)
+    n = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv4_attention_workspace", ctypes.byref(desc), t, hkv * g, ctypes.byref(n))
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    groups = -(-t * g // block)
+    assert n.value <= 2 * 3 * cus * block * (d + 2) * 4 + 8 * hkv * groups * b
