@@ -547,8 +547,8 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.by_rows.set(v.R);
     p.by_items.set(v.H * plan.groups);
     p.by_heads.set(v.H);
+    float *part = a.scratch;
     if (p.quota) {
-        float *part = a.scratch;
         if (a.scratch) {
             // As many chunks as the caller's workspace holds the partials of.
             const size_t none = partial_bytes(v, plan, 0), slot = partial_bytes(v, plan, 1) - none;
@@ -558,9 +558,14 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
                 p.quota = most < 2 ? 0 : static_cast<int>(most);
             }
         } else {
-            part = static_cast<float *>(stream_scratch(partial_bytes(v, plan, p.quota)));
-            if (!part) return ALJABR_ROCM_ERR_BUFFER;
+            part = static_cast<float *>(stream_scratch_try(partial_bytes(v, plan, p.quota), 0));
+            hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+            if (!part && (hipStreamIsCapturing(current_stream(), &cs) != hipSuccess || cs != hipStreamCaptureStatusNone))
+                return fail(ALJABR_ROCM_ERR_BUFFER, "kv4_attention: a call under stream capture needs a workspace");
+            if (!part) p.quota = 0;                        // no memory: one chunk a sequence needs none
         }
+    }
+    if (p.quota) {
         p.part_o = part;
         const size_t all = partial_slots(v, p.quota) * v.H * plan.groups * plan.rows;
         p.part_ml = part + all * v.D;

@@ -659,3 +659,25 @@ def test_workspace_grows_with_the_chunks_not_the_batch(rocm, b, t, hkv, g, d, bl
     cus = torch.cuda.get_device_properties(0).multi_processor_count
     groups = -(-t * g // block)
     assert n.value <= 2 * 3 * cus * block * (d + 2) * 4 + 8 * hkv * groups * b
+
+
+@pytest.mark.parametrize("d,t", [(64, 1), (128, 20), (256, 3)])
+@pytest.mark.parametrize("nbytes", [0, 8, 1000])
+def test_a_workspace_too_small_to_split_with(rocm, d, t, nbytes):
+    """A pointer with (next to) no bytes behind it: one chunk a sequence, and the stream's scratch stays untouched."""
+    lens = [700, 31, 0]
+    host = plain.Cache(3, 2, d, 704, 16)
+    host.fill(lens)
+    dev, q = Device(rocm, host), query(t, 3, t, 8, d)
+    qd, ld, out = torch.from_numpy(q).cuda(), ints(lens), torch.full(q.shape, POISON, device="cuda")
+    ws = torch.full((4096,), 0xCD, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+
+    def body():
+        rocm.call("aljabr_rocm_kv4_attention", out.data_ptr(), qd.data_ptr(), dev.ref(), ld.data_ptr(), None, t, 8, 0.0, 1, 0, 0.0,
+                  ws.data_ptr(), nbytes)
+        return scratch_held(rocm)
+
+    assert fresh_thread(body) == 0
+    check(out.cpu().numpy(), *plain.attention(host, q, lens))
+    assert (ws == 0xCD).all()
