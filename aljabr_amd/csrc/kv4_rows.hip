@@ -446,12 +446,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
 // partial as float4s (64 / (D/4) chunks at once), folded in order, then across
 // the lane groups.
 template <int D>
-__global__ __launch_bounds__(256) void kv4_merge_rows_kernel(Params p, long long rows) {
+__global__ __launch_bounds__(256) void kv4_merge_rows_kernel(Params p) {
     constexpr int LPS = D / 4, SG = 64 / LPS;
-    const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int bt = static_cast<int>(row / p.Hq), hq = static_cast<int>(row - static_cast<long long>(bt) * p.Hq);
-    const int b = bt / p.T, t = bt - b * p.T;
+    const int of_seq = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
+    const int t = of_seq / p.Hq, hq = of_seq - t * p.Hq;
+    if (t >= p.T) return;
+    const long long row = static_cast<long long>(b) * p.T * p.Hq + of_seq;
     const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
     const int item = group_of(p, r / kRowsBlock) * p.v.H + kvh;
     const int2 chunk = p.chunks[static_cast<long long>(item) * p.v.B + b];   // written for the rows that exist
@@ -492,9 +492,8 @@ void launch_typed(const Params &p, hipStream_t s) {
         hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, true>), grid, dim3(kThreads), 0, s, p);
     else
         hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, false>), grid, dim3(kThreads), 0, s, p);
-    const long long rows = static_cast<long long>(p.v.B) * p.T * p.Hq;
-    if (p.quota)
-        hipLaunchKernelGGL((kv4_merge_rows_kernel<D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, p, rows);
+    if (p.quota)                                           // few row groups, so few rows of a sequence
+        hipLaunchKernelGGL((kv4_merge_rows_kernel<D>), dim3((p.T * p.Hq + 3) / 4, p.v.B), dim3(256), 0, s, p);
 }
 
 template <int D>

@@ -681,3 +681,33 @@ def test_a_workspace_too_small_to_split_with(rocm, d, t, nbytes):
     assert fresh_thread(body) == 0
     check(out.cpu().numpy(), *plain.attention(host, q, lens))
     assert (ws == 0xCD).all()
+
+
+def test_merge_of_more_rows_than_a_launch_has_lanes(rocm):
+    """2^26 rows of 4096 sequences, all but four of them padding: as one dimension the merge would have 2^32 lanes."""
+    b, t, g, d, cap = 4096, 128, 128, 64, 144
+    assert b * t * g * 64 >= 1 << 32
+    small = plain.Cache(2, 1, d, cap)
+    small.fill([20, cap])
+    at = torch.tensor([0, b - 1])                                      # the last sequence has two chunks
+    planes = {}
+    for w in "kv":
+        planes[w + "c"] = torch.zeros(b, 1, cap, d // 2, dtype=torch.uint8, device="cuda")
+        planes[w + "s"] = torch.zeros(b, 1, d // 32, cap, dtype=torch.float16, device="cuda")
+        planes[w + "c"][at] = torch.from_numpy(small.codes[w]).cuda()
+        planes[w + "s"][at] = torch.from_numpy(small.scales[w]).cuda()
+    desc = rocm.Kv4Cache(*[planes[n].data_ptr() for n in ("kc", "ks", "vc", "vs")], None, b, 1, d, cap, 0, 0)
+    lens, counts = torch.full((b,), cap, dtype=torch.int32), torch.zeros(b, dtype=torch.int32)
+    lens[0], counts[at] = 20, 2
+    lens, counts = lens.cuda(), counts.cuda()
+    q = query(1, 2, 2, g, d)
+    qd, out = torch.empty(b, t, g, d, device="cuda"), torch.full((b, t, g, d), POISON, device="cuda")
+    qd[at, :2] = torch.from_numpy(q).cuda()
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv4_attention", out.data_ptr(), qd.data_ptr(), ctypes.byref(desc), lens.data_ptr(), counts.data_ptr(), t, g,
+              0.0, 1, 0, 0.0, None, 0)
+    torch.cuda.synchronize()
+    check(out[at, :2].cpu().numpy(), *plain.attention(small, q, [20, cap]))
+    assert (out[at, 2:] == POISON).all()
+    assert all(bool((out[s:s + 128] == POISON).all()) for s in range(128, b - 128, 128))
+    assert (out[1:128] == POISON).all() and (out[b - 128:b - 1] == POISON).all()
