@@ -27,9 +27,10 @@
 // V product, of ones, so numerator and denominator hold the same weights.
 //
 // Keys a row does not see get weight 0, and V rows past a sequence's end may
-// hold anything: their scales are taken as 0. A scale that is not finite, or so
-// large that its values may not be, among keys that only some rows see is taken as 0 too and remembered for the rows
-// that see it: their values of its block are made NaN at the end.
+// hold anything: their scales are taken as 0. In a tile with keys that not every
+// row sees, a scale that makes one of a lane's values not finite is taken as 0
+// too and remembered for the rows that see the key: their values of these dims
+// are made NaN at the end.
 //
 // Bound by the vector ALU (55 to 59 % of the kernel's time): about 364
 // instructions a tile of 32 keys and 8 rows at D = 128, most of them decoding,
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
 
     f32x4 o[NT][OT], l[NT];                                // l: the sum of the weights, in every accumulator
     float m[NT];
-    uint32_t poison[NT];                                   // per lane n: its block of a key this column sees is not finite
+    uint32_t poison[NT];                                   // per lane n: a value of its dims, of a key this column sees, is not finite
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         m[c] = -INFINITY;
@@ -376,12 +377,16 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (16 * (i >> 2) + (i & 3) >= end || !here.ok[i >> 2]) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
-                odd |= not_finite(vd[i >> 1][i & 1]);
+                odd |= may_overflow(vd[i >> 1][i & 1]);
             }
             if (__any(odd)) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint64_t bad = __ballot(not_finite(vd[i >> 1][i & 1]));
+                    const _Float16 d = vd[i >> 1][i & 1];
+                    const uint32_t w = xv.v[i >> 2][i & 3][0];
+                    bool over = overflows(g, D == 64 ? __builtin_amdgcn_perm(w, w, vsel) : w, d);
+                    if constexpr (D == 256) over |= overflows(g, xv.v[i >> 2][i & 3][1], d);
+                    const uint64_t bad = __ballot(over);
 #pragma unroll 1
                     for (int hh = 0; hh < 4; ++hh) {
                         const int key = k0 + 16 * (i >> 2) + 4 * hh + (i & 3);
@@ -389,7 +394,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
                         for (int c = 0; c < NT; ++c)
                             if (key >= lo[c] && key < hi[c]) poison[c] |= static_cast<uint32_t>(bad >> (16 * hh)) & 0xffffu;
                     }
-                    if (not_finite(vd[i >> 1][i & 1])) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
+                    if (over) vd[i >> 1][i & 1] = static_cast<_Float16>(0.0f);
                 }
             }
         }
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int piece = 4 * h + r;                   // the lane n whose V codes these are
-            const float bad = poison[c] >> (D == 64 ? piece & 8 : D == 128 ? piece & 12 : piece & 14) & 1 ? NAN : 0.0f;
+            const float bad = poison[c] >> piece & 1 ? NAN : 0.0f;
 #pragma unroll
             for (int j = 0; j < OT; ++j) {
                 const float val = o[c][j][r] + other_part(o[c][j][r]) + bad;

@@ -216,8 +216,17 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 }
 
 // A scale that is not finite, or past the writer's largest (8160): a code times it may leave fp16.
-__device__ __forceinline__ bool not_finite(_Float16 x) {
+__device__ __forceinline__ bool may_overflow(_Float16 x) {
     return (__builtin_bit_cast(uint16_t, x) & 0x7fffu) > 0x6ff8u;
+}
+
+// Whether one of the 8 values of w's nibbles is not a finite fp16 number.
+__device__ __forceinline__ bool overflows(const Magic &g, uint32_t w, _Float16 d) {
+    uint32_t f[4], all_ones = 0;
+    decode8(g, w, half2v{d, d}, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all_ones |= (f[i] & 0x7fff7fffu) + 0x04000400u;      // the exponent's carry
+    return all_ones & 0x80008000u;
 }
 
 // x of the lane 8 columns away (the row's other fp16 part).

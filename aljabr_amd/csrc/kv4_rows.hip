@@ -118,9 +118,10 @@ __device__ __forceinline__ bool both_ok(const Params &p, int b, int n_keys, int 
 }
 
 // The scales of a thread's two V rows. `edge`: some row does not see some key; scales of V rows past the end, or on
-// no block, are then taken as 0, and one that is not finite too, with its key's bit set in bad[block].
+// no block, are then taken as 0, and one that makes a value of the thread's not finite too, with its key's bit set in
+// bad[block].
 template <int D>
-__device__ __forceinline__ half2v value_scales(const Raw<D> &x, int k0, int n_keys, bool edge, int tid, uint32_t *bad) {
+__device__ __forceinline__ half2v value_scales(const Magic &g, const Raw<D> &x, int k0, int n_keys, bool edge, int tid, uint32_t *bad) {
     const int pr = tid >> 4, n = tid & 15;                                 // pair of keys 2 pr, 2 pr + 1
     half2v vd = as_half2(x.vs);
     if (edge) {
@@ -128,9 +129,14 @@ __device__ __forceinline__ half2v value_scales(const Raw<D> &x, int k0, int n_ke
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             if (k0 + 2 * pr + r >= n_keys || !x.ok) vd[r] = static_cast<_Float16>(0.0f);
-            if (not_finite(vd[r])) {
-                vd[r] = static_cast<_Float16>(0.0f);
-                atomicOr(bad + vg, 1u << (2 * pr + r));
+            if (may_overflow(vd[r])) {
+                const uint32_t w = x.v[r][0];
+                bool over = overflows(g, D == 64 ? __builtin_amdgcn_perm(w, w, n & 1 ? 0x03020302u : 0x01000100u) : w, vd[r]);
+                if constexpr (D == 256) over |= overflows(g, x.v[r][1], vd[r]);
+                if (over) {
+                    vd[r] = static_cast<_Float16>(0.0f);
+                    atomicOr(bad + vg, 1u << (2 * pr + r));
+                }
             }
         }
     }
@@ -256,7 +262,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     if (BUFS == 2 && t0 < t1) {
         __syncthreads();                                                   // `bad` is clear
         ok_next = both_ok<PAGED>(p, b, seq.n, t0);
-        decode_tile<D>(g, raw, value_scales<D>(raw, t0 * kTile, seq.n, edge_of(t0) || !ok_next, tid, bad[0]), tid, lds);
+        decode_tile<D>(g, raw, value_scales<D>(g, raw, t0 * kTile, seq.n, edge_of(t0) || !ok_next, tid, bad[0]), tid, lds);
         if (t0 + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, t0 + 1, tid, raw);
     }
     for (int kt = t0, i = 0; kt < t1; ++kt, i = i == 2 ? 0 : i + 1) {
@@ -286,7 +292,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             half2v vd = {};
             if (kt + 1 < t1) {
                 ok_next = both_ok<PAGED>(p, b, seq.n, kt + 1);
-                vd = value_scales<D>(raw, k0 + kTile, seq.n, edge_of(kt + 1) || !ok_next, tid, bad[ahead]);
+                vd = value_scales<D>(g, raw, k0 + kTile, seq.n, edge_of(kt + 1) || !ok_next, tid, bad[ahead]);
             }
             // The next tile is decoded between the products (past the last one, what it holds is not used).
             __builtin_amdgcn_sched_barrier(0);
@@ -304,7 +310,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
         } else {
             ok = both_ok<PAGED>(p, b, seq.n, kt);
             if (tid < 8) bad[ahead][tid] = 0;
-            decode_tile<D>(g, raw, value_scales<D>(raw, k0, seq.n, edge_of(kt) || !ok, tid, bad[i]), tid, lds);
+            decode_tile<D>(g, raw, value_scales<D>(g, raw, k0, seq.n, edge_of(kt) || !ok, tid, bad[i]), tid, lds);
             if (kt + 1 < t1) load_raw<D, PAGED>(p, b, kvh, seq.n, kt + 1, tid, raw);
             __syncthreads();
             read_keys();

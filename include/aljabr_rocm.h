@@ -313,8 +313,9 @@ int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, c
  * scores as cap * tanh(score / cap); scale <= 0: 1 / sqrt(head_dim). A row
  * that sees no key gives zeros; rows from counts[b] on are left as they were.
  * Keys on a bad block are not seen, and what keys hold that a row does not see
- * never reaches it; a scale past 8160, which kv4_write does not make, may count
- * as NaN to rows that do. fp32-accurate. T * Hq is at most 2^30,
+ * never reaches it; a block with a value past fp16's range (its scale past
+ * 8160, which kv4_write does not make) may count as NaN to rows that do.
+ * fp32-accurate. T * Hq is at most 2^30,
  * sequences * the positions of each at most 2^35.
  * workspace: device scratch for split partials, of
  * aljabr_rocm_kv4_attention_workspace bytes (fewer: fewer splits), not shared

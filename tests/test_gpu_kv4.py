@@ -711,3 +711,45 @@ def test_merge_of_more_rows_than_a_launch_has_lanes(rocm):
     assert (out[at, 2:] == POISON).all()
     assert all(bool((out[s:s + 128] == POISON).all()) for s in range(128, b - 128, 128))
     assert (out[1:128] == POISON).all() and (out[b - 128:b - 1] == POISON).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", [1, 6, 40])
+@pytest.mark.parametrize("n", [200, 224])
+@pytest.mark.parametrize("scale,most", [(8192.0, 7), (-12000.0, 5), (30000.0, 2), (65504.0, 1)])
+def test_scales_past_the_writers_with_finite_values(rocm, d, t, n, scale, most):
+    """Visible keys of another writer: a scale past 8160 whose codes keep every value within fp16, wherever tiles end."""
+    host = plain.Cache(1, 2, d, 240)
+    host.fill([n])
+    q = query(d + n, 1, t, 8, d)
+    rng = np.random.default_rng(most)
+    for pos in (0, 31, 100, n - t, n - 5, n - 1):                      # of 40 rows, the last are seen by some only
+        at = rng.integers(0, d // 32)                                  # one block
+        c = rng.integers(8 - most, 9 + most, (2, 32)).astype(np.uint8)
+        host.codes["v"][0, :, pos, 16 * at:16 * at + 16] = c[:, :16] | c[:, 16:] << 4
+        host.scales["v"][0, :, at, pos] = scale
+    want, bound, live = plain.attention(host, q, [n])
+    assert np.isfinite(want).all()
+    check(attend(rocm, Device(rocm, host), q, [n]), want, bound, live)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", [6, 40])
+def test_values_past_fp16_reach_only_rows_that_see_them(rocm, d, t):
+    """One value of a key that two rows see leaves fp16: those rows' block may be NaN, nothing else."""
+    host = plain.Cache(1, 1, d, 128)
+    host.fill([101])
+    q = query(d + t, 1, t, 4, d)
+    want, bound, live = plain.attention(host, q, [101])
+    for block in range(d // 32):
+        saved = [host.codes["v"].copy(), host.scales["v"].copy()]
+        c = np.full(32, 9, np.uint8)
+        c[(7 * block + 3) % 32] = 0                                    # -8 of a scale of 30000
+        host.codes["v"][0, 0, 99, 16 * block:16 * block + 16] = c[:16] | c[16:] << 4
+        host.scales["v"][0, 0, block, 99] = 30000.0
+        got = attend(rocm, Device(rocm, host), q, [101])
+        check(got[:, :t - 2], want[:, :t - 2], bound[:, :t - 2], live[:, :t - 2])
+        other = [i for i in range(d) if i // 32 != block]
+        assert (np.abs(got - want)[0, t - 2:][..., other] <= bound[0, t - 2:][..., other]).all()
+        assert (~np.isfinite(got[0, t - 2:, :, 32 * block + (7 * block + 3) % 32])).all()
+        host.codes["v"], host.scales["v"] = saved
