@@ -331,7 +331,7 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
                 y[i] = raw + other_part(raw);
             }
             if constexpr (CAP) {
-                const float cap = p.soft_cap * kLog2e, in = unscale[c] / cap;
+                const float cap = p.soft_cap * kLog2e, in = fminf(unscale[c] / cap, 3e38f);    // finite: 0 stays 0
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = cap * tanhf(y[i] * in);
             }
@@ -539,7 +539,9 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.Hq = a.Hq;
     p.G = a.Hq / v.H;
     p.scale = a.scale;
-    p.soft_cap = a.soft_cap;
+    // Within fp32's range with the scores' scaling, and to fp32 the same: past 2^64 a cap is none for every score that
+    // softmax tells from its neighbours, below 2^-30 all weights are equal.
+    p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;
     p.causal = a.causal;
     p.window = std::min(a.window, 1 << 30);                // past every key; pos - window stays in 32 bits
     const Plan plan = make_plan(v, a.T, a.Hq);

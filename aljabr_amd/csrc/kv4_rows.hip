@@ -328,7 +328,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (CAP) {
-            const float cap = p.soft_cap * kLog2e, in = unscale / cap;
+            const float cap = p.soft_cap * kLog2e, in = fminf(unscale / cap, 3e38f);       // finite: 0 stays 0
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[j] = cap * tanhf(s[j] * in);
         }

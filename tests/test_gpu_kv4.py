@@ -753,3 +753,32 @@ def test_values_past_fp16_reach_only_rows_that_see_them(rocm, d, t):
         assert (np.abs(got - want)[0, t - 2:][..., other] <= bound[0, t - 2:][..., other]).all()
         assert (~np.isfinite(got[0, t - 2:, :, 32 * block + (7 * block + 3) % 32])).all()
         host.codes["v"], host.scales["v"] = saved
+
+
+@pytest.mark.parametrize("d,t", [(64, 1), (128, 5), (256, 1), (128, 40), (256, 40)])
+@pytest.mark.parametrize("cap", [3.4e38, 1e38, 1e30, 2.0 ** 64, 1e10])
+def test_soft_caps_past_every_score(rocm, d, t, cap):
+    """cap tanh(score / cap) of a cap far past the scores is the score; the bound is that without a cap (its terms in cap are
+    bounds for |score| near cap), and 4 roundings of each score for the cap's products and tanh."""
+    host = plain.Cache(2, 1, d, 208)
+    host.fill([200, 9])
+    q = query(t, 2, t, 4, d)
+    want, bound, live = plain.attention(host, q, [200, 9])
+    k = host.rows_of("k", 0, 200)[0].astype(np.float64)
+    top = (np.abs(k) @ np.abs(q[0].reshape(-1, d).T)).max() * d ** -0.5
+    v = np.abs(host.rows_of("v", 0, 200)[0].astype(np.float64)).max()
+    check(attend(rocm, Device(rocm, host), q, [200, 9], cap=cap), want, bound + 2 * v * 4 * top * 2.0 ** -24, live)
+
+
+@pytest.mark.parametrize("d,t", [(64, 1), (128, 5), (256, 1), (128, 40), (256, 40)])
+@pytest.mark.parametrize("cap,size", [(1e-6, 1.0), (1e-20, 1.0), (1e-38, 1.0), (1e-44, 1.0), (1e-6, 1e30), (1e-30, 1e25), (1e-44, 1e30)])
+def test_soft_caps_next_to_zero(rocm, d, t, cap, size):
+    """Scores of at most 1e-6: every key weighs the same to 2e-6. Keys of zeros, whose scores are 0, are among them."""
+    host = plain.Cache(2, 1, d, 208)
+    host.fill([200, 9])
+    for pos in (0, 8):
+        host.write("k", 1, pos, np.zeros((1, d), np.float32))
+    q = query(t, 2, t, 4, d) * np.float32(size)
+    want, bound, live = plain.attention(host, np.zeros_like(q), [200, 9])
+    v = np.abs(host.rows_of("v", 0, 200)[0].astype(np.float64)).max()
+    check(attend(rocm, Device(rocm, host), q, [200, 9], cap=cap), want, bound + 2 * 2 * 1e-6 * v, live)
