@@ -235,7 +235,6 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
         key_range(p, seq, t, lo[c], hi[c]);
         const float *qr = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D;
         float x[ND][8], top = 0.0f;
-        const float qs = p.scale * kLog2e;
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
             const int w = h * ND + i;
@@ -248,17 +247,17 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
         }
         top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32)) * qs;
+        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale * kLog2e;
         int e = 0;
         if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
         e = e < -100 ? -100 : e;
-        const float up = ldexpf(1.0f, 15 - e);
+        const float up = ldexpf(1.0f, 15 - e);             // a power of two: y is the same number wherever it is used
         unscale[c] = ldexpf(1.0f, e - 15);
 #pragma unroll
         for (int i = 0; i < ND; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = x[i][j] * qs * up;
+                const float y = x[i][j] * p.scale * kLog2e * up;
                 const _Float16 first = static_cast<_Float16>(y);
                 qf[c][i][j] = n < 8 ? first : static_cast<_Float16>(y - static_cast<float>(first));
             }

@@ -213,7 +213,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     float unscale;
     {
         const float *qr = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D + 4 * h;
-        const float qs = p.scale * kLog2e;
         float top = 0.0f;
         float4 qa[STEPS], qc[STEPS];
 #pragma unroll
@@ -227,11 +226,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
                                    fmaxf(fmaxf(fabsf(c.x), fabsf(c.y)), fmaxf(fabsf(c.z), fabsf(c.w)))));
         }
-        top = fmaxf(top, __shfl_xor(top, 32)) * qs;
+        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale * kLog2e;
         int e = 0;
         if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
         e = e < -100 ? -100 : e;
-        const float up = ldexpf(1.0f, 15 - e);
+        const float up = ldexpf(1.0f, 15 - e);             // a power of two: y is the same number wherever it is used
         unscale = ldexpf(1.0f, e - 15);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             const float y[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = y[i] * qs * up;
+                const float v = y[i] * p.scale * kLog2e * up;
                 qh[s][i] = static_cast<_Float16>(v);
                 ql[s][i] = static_cast<_Float16>(v - static_cast<float>(qh[s][i]));
             }

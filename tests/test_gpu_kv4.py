@@ -782,3 +782,23 @@ def test_soft_caps_next_to_zero(rocm, d, t, cap, size):
     want, bound, live = plain.attention(host, np.zeros_like(q), [200, 9])
     v = np.abs(host.rows_of("v", 0, 200)[0].astype(np.float64)).max()
     check(attend(rocm, Device(rocm, host), q, [200, 9], cap=cap), want, bound + 2 * 2 * 1e-6 * v, live)
+
+
+@pytest.mark.parametrize("d,t", [(64, 1), (128, 5), (256, 1), (128, 40), (256, 40)])
+@pytest.mark.parametrize("scale,size", [(3.4e38, 1e-39), (2.5e38, 1e-38), (1e-38, 2e37), (2e-39, 1e38), (1e30, 1e-31)])
+def test_scales_at_the_ends_of_fp32(rocm, d, t, scale, size):
+    host = plain.Cache(1, 1, d, 208)
+    host.fill([200])
+    with np.errstate(over="ignore"):
+        q = query(t, 1, t, 4, d) * np.float32(size)
+    scale = float(np.float32(scale))
+    want, bound, live = plain.attention(host, q, [200], scale=scale)
+    # Scores are far apart here: a weight's second fp16 part, of 2^13 times the weight or more, is off by up to 2^-25, so a
+    # weight by up to 2^-38 of the largest, which a dim where the largest weight's value is 0 shows: 200 of them, on values
+    # of at most v, over a sum of at least the largest.
+    v = np.abs(host.rows_of("v", 0, 200)[0].astype(np.float64)).max()
+    got = attend(rocm, Device(rocm, host), q, [200], scale=scale)
+    past = ~np.isfinite(q).all(-1)                                     # at 1e38 some element is infinite: its row is NaN
+    assert np.isnan(got[past]).all() and np.isnan(want[past]).all()
+    got, want, bound = (np.where(past[..., None], 0.0, x) for x in (got, want, bound))
+    check(got, want, bound + 200 * 2.0 ** -38 * v, live)
