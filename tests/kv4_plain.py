@@ -140,3 +140,41 @@ def attention(cache, q, lens, counts=None, causal=True, window=0, cap=0.0, scale
                     mean = w @ np.abs(vv)
                     bound[b, t, h] = 2 * mean * (off.max() + 2.0 ** -21 + (see.sum() / 16 + 64) * 2.0 ** -24)
     return out, bound, live
+
+
+def one_hot_keys(d, n=40, seed=0):
+    """A cache whose keys are one number in [1, 2) and zeros: a score is one product, off by all of its query element's
+    error, where the bound allows a sum of D of them. Queries for it: one_hot_query."""
+    rng = np.random.default_rng(seed)
+    host = Cache(1, 1, d, -(-n // 16) * 16)
+    for pos in range(n):
+        k = np.zeros((1, d), np.float32)
+        k[0, rng.integers(0, d)] = rng.choice([-1.0, 1.0]) * rng.uniform(1, 2)
+        host.write("k", 0, pos, k)
+        host.write("v", 0, pos, rng.standard_normal((1, d)).astype(np.float32))
+    return host
+
+
+def one_hot_query(d, t, g):
+    rng = np.random.default_rng(d + t)
+    return (rng.uniform(1, 2, (1, t, g, d)) * rng.choice([-1, 1], (1, t, g, d))).astype(np.float32)
+
+
+def in_fp16_parts(cache, q, n, scale, query_parts, weight_parts):
+    """Causal attention of one sequence and KV head with queries and weights in one or two fp16 parts, else in float64."""
+    k, v = (cache.rows_of(w, 0, n)[0][0].astype(np.float64) for w in "kv")
+
+    def parts(x, count):
+        first = x.astype(np.float16).astype(np.float64)
+        return first if count == 1 else first + (x - first).astype(np.float16).astype(np.float64)
+
+    out = np.zeros(q.shape)
+    for t in range(q.shape[1]):
+        seen = n - q.shape[1] + t + 1
+        for h in range(q.shape[2]):
+            x = q[0, t, h].astype(np.float64) * scale / np.log(2.0)
+            e = int(np.frexp(np.abs(x).max())[1])
+            s = k[:seen] @ parts(np.ldexp(x, 15 - e), query_parts) * 2.0 ** (e - 15)
+            w = parts(np.exp2(s - s.max()) * 8192, weight_parts)
+            out[0, t, h] = w @ v[:seen] / w.sum()
+    return out

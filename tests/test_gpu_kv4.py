@@ -802,3 +802,55 @@ def test_scales_at_the_ends_of_fp32(rocm, d, t, scale, size):
     assert np.isnan(got[past]).all() and np.isnan(want[past]).all()
     got, want, bound = (np.where(past[..., None], 0.0, x) for x in (got, want, bound))
     check(got, want, bound + 200 * 2.0 ** -38 * v, live)
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("t", [1, 6, 40])
+def test_bad_blocks_at_other_head_sizes(rocm, d, t):
+    lens = [90, 90, 90, 20]
+    host = plain.Cache(4, 2, d, 96, 16)
+    host.fill(lens)
+    host.table[0, 2], host.table[1, 0], host.table[1, 5], host.table[3, :] = -1, host.s, 2 ** 31 - 1, -5
+    q = query(6, 4, t, 8, d)
+    got = attend(rocm, Device(rocm, host), q, lens)
+    check(got, *plain.attention(host, q, lens))
+    assert not got[3].any()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,window", [(4, 0), (40, 0), (4, 50), (40, 60)])
+def test_nan_in_each_block_reaches_its_dims_of_the_rows_that_see_it(rocm, d, t, window):
+    """V of one key the last two rows see, and of one that leaves the windows after the first: NaN in one block of 32 dims
+    after the other, which those rows have there, and the others nowhere."""
+    n = 100
+    host = plain.Cache(1, 2, d, 128)
+    host.fill([n])
+    q = query(8, 1, t, 4, d)
+    clean = plain.attention(host, q, [n], window=window)
+    keys = [n - 2] + ([n - t - window + 1] if window else [])
+    rng = np.random.default_rng(d)
+    for block in range(d // 32):
+        saved = [host.codes["v"].copy(), host.scales["v"].copy()]
+        for key in keys:
+            x = rng.standard_normal((2, d)).astype(np.float32)
+            x[1, 32 * block + 5] = np.nan
+            host.write("v", 0, key, x)
+        want, bound, _ = plain.attention(host, q, [n], window=window)
+        got = attend(rocm, Device(rocm, host), q, [n], window=window)
+        hurt = np.zeros(got.shape, bool)
+        hurt[0, t - 2:, 2:, 32 * block:32 * block + 32] = True
+        if window:
+            hurt[0, 0, 2:, 32 * block:32 * block + 32] = True
+        assert np.array_equal(np.isnan(want), hurt) and np.array_equal(np.isnan(got), hurt)
+        assert (np.abs(got - want)[~hurt] <= bound[~hurt]).all()
+        host.codes["v"], host.scales["v"] = saved
+    check(attend(rocm, Device(rocm, host), q, [n], window=window), *clean)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,g", [(1, 4), (5, 4), (40, 2)])
+@pytest.mark.parametrize("scale", [1.0, 0.01])
+def test_queries_and_weights_have_two_parts(rocm, d, t, g, scale):
+    """Keys of one number each, for which the bound does not hold with one fp16 part (tests/test_kv4.py)."""
+    host, q = plain.one_hot_keys(d), plain.one_hot_query(d, t, g)
+    check(attend(rocm, Device(rocm, host), q, [40], scale=scale), *plain.attention(host, q, [40], scale=scale))

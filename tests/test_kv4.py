@@ -152,3 +152,16 @@ def test_read_into_rows_on_one_place_is_refused(strides, shape):
     c = ctypes.byref(cache(sequences=b, n_kv_heads=h))
     assert lib.aljabr_rocm_kv4_read(P, P, c, P, None, t, *strides, abi.TYPE_F32) == -2
     assert "stride" in abi.last_error()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,g", [(1, 4), (5, 4), (40, 2)])
+def test_the_bound_tells_two_parts_from_one(d, t, g):
+    """With keys of one number each the bound of kv4_plain.attention holds for queries and weights in two fp16 parts, with
+    most of it to spare, and not for either in one."""
+    host, q = plain.one_hot_keys(d), plain.one_hot_query(d, t, g)
+    over = lambda scale, *parts: (np.abs(plain.in_fp16_parts(host, q, 40, scale, *parts) - want[scale][0]) / (want[scale][1] + 1e-30)).max()
+    want = {scale: plain.attention(host, q, [40], scale=scale) for scale in (1.0, 0.01)}
+    assert over(1.0, 2, 2) < 0.1 and over(0.01, 2, 2) < 0.1
+    assert over(1.0, 1, 2) > 2                                 # queries in one part: scores of some size
+    assert over(0.01, 2, 1) > 4                                # weights in one part: scores next to 0
