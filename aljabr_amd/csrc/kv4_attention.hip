@@ -564,11 +564,14 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
                 p.quota = most < 2 ? 0 : static_cast<int>(most);
             }
         } else {
-            part = static_cast<float *>(stream_scratch_try(partial_bytes(v, plan, p.quota), 0));
-            hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-            if (!part && (hipStreamIsCapturing(current_stream(), &cs) != hipSuccess || cs != hipStreamCaptureStatusNone))
-                return fail(ALJABR_ROCM_ERR_BUFFER, "kv4_attention: a call under stream capture needs a workspace");
-            if (!part) p.quota = 0;                        // no memory: one chunk a sequence needs none
+            part = static_cast<float *>(stream_scratch(partial_bytes(v, plan, p.quota)));
+            if (!part) {
+                hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+                if (hipStreamIsCapturing(current_stream(), &cs) != hipSuccess || cs != hipStreamCaptureStatusNone)
+                    return ALJABR_ROCM_ERR_BUFFER;
+                (void)hipGetLastError();                   // no memory: one chunk a sequence needs none
+                p.quota = 0;
+            }
         }
     }
     if (p.quota) {
