@@ -247,17 +247,17 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
         }
         top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale * kLog2e;
+        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale;
         int e = 0;
         if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
         e = e < -100 ? -100 : e;
         const float up = ldexpf(1.0f, 15 - e);             // a power of two: y is the same number wherever it is used
-        unscale[c] = ldexpf(1.0f, e - 15);
+        unscale[c] = ldexpf(p.unscale, e - 15);
 #pragma unroll
         for (int i = 0; i < ND; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = x[i][j] * p.scale * kLog2e * up;
+                const float y = x[i][j] * p.scale * up;
                 const _Float16 first = static_cast<_Float16>(y);
                 qf[c][i][j] = n < 8 ? first : static_cast<_Float16>(y - static_cast<float>(first));
             }
@@ -537,7 +537,13 @@ int enqueue_kv4_attention(const Kv4View &v, const Kv4Attention &a) {
     p.T = a.T;
     p.Hq = a.Hq;
     p.G = a.Hq / v.H;
-    p.scale = a.scale;
+    // scale * log2(e) as p.scale p.unscale, the first between 2^-61 and 2^100: where scores are in fp32's range, so is a
+    // query element times it.
+    int k;
+    const double m = std::frexp(static_cast<double>(a.scale) * 1.4426950408889634, &k);
+    const int in = std::min(std::max(k, -60), 100);
+    p.scale = static_cast<float>(std::ldexp(m, in));
+    p.unscale = static_cast<float>(std::ldexp(1.0, k - in));
     // Within fp32's range with the scores' scaling, and to fp32 the same: past 2^64 a cap is none for every score that
     // softmax tells from its neighbours, below 2^-30 all weights are equal.
     p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;

@@ -43,7 +43,8 @@ struct Params {
     const int *lens, *counts;
     int T, Hq, G, row_groups;
     FastDiv by_g, by_groups, by_rows, by_chunks, by_items, by_heads;   // G, row_groups, rows of a block, chunks that vary fastest, H * row_groups, H
-    float scale, soft_cap;
+    float scale, unscale;                    // their product is the call's scale times log2(e)
+    float soft_cap;
     int causal, window;
     int quota;                               // chunks that the keys of all sequences are cut into (about), 0: one each
     float *part_o, *part_ml;                 // per slot, KV head, row group and stacked row: D sums, and (m, l)

@@ -226,19 +226,19 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
             top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
                                    fmaxf(fmaxf(fabsf(c.x), fabsf(c.y)), fmaxf(fabsf(c.z), fabsf(c.w)))));
         }
-        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale * kLog2e;
+        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale;
         int e = 0;
         if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
         e = e < -100 ? -100 : e;
         const float up = ldexpf(1.0f, 15 - e);             // a power of two: y is the same number wherever it is used
-        unscale = ldexpf(1.0f, e - 15);
+        unscale = ldexpf(p.unscale, e - 15);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const float4 a = qa[s], c = qc[s];
             const float y[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = y[i] * p.scale * kLog2e * up;
+                const float v = y[i] * p.scale * up;
                 qh[s][i] = static_cast<_Float16>(v);
                 ql[s][i] = static_cast<_Float16>(v - static_cast<float>(qh[s][i]));
             }
