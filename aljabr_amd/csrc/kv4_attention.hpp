@@ -146,7 +146,7 @@ __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int 
     int per = max(p.by_chunks(total + p.quota - 1), least);
     per = (per + least - 1) / least * least;
     const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
-    int before = 0, slots = 0;
+    int before = 0, singles = 0;                           // chunks, and sequences of one, of the groups of 64 before
     for (int b0 = 0; b0 <= last; b0 += 64) {
         if (last) {
             a = z = 0;
@@ -162,13 +162,14 @@ __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int 
         n -= n > 0 && (n - 1) * per >= z - a ? 1 : 0;
         n += n * per < z - a ? 1 : 0;
         n = r0 < s.cnt * p.G ? max(n, 1) : 0;
-        const int end = before + wave_scan(n), slot_end = slots + wave_scan(n > 1 ? n : 0);
+        const int end = before + wave_scan(n);
+        const uint64_t single = __ballot(n == 1);
         const uint64_t hit = __ballot(w >= end - n && w < end);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             c.count = __builtin_amdgcn_readlane(n, l);
             c.first = __builtin_amdgcn_readlane(end, l) - c.count;
-            c.slot = __builtin_amdgcn_readlane(slot_end, l) - c.count;       // of one chunk: not used
+            c.slot = c.first - singles - __builtin_popcountll(single & ((uint64_t{1} << l) - 1));   // of one chunk: not used
             a = __builtin_amdgcn_readlane(a, l);
             z = __builtin_amdgcn_readlane(z, l);
             c.seq.n = __builtin_amdgcn_readlane(s.n, l);
@@ -179,7 +180,7 @@ __device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int 
             return c;
         }
         before = __builtin_amdgcn_readlane(end, 63);
-        slots = __builtin_amdgcn_readlane(slot_end, 63);
+        singles += __builtin_popcountll(single);
     }
     return c;
 }
