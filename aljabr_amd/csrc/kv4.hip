@@ -16,9 +16,10 @@
 // Work: one lane per code dword (8 values: 4q..4q+3 and 16+4q..+3 of a block,
 // two 16-byte loads), four lanes a block (its minimum and maximum in two DPP
 // steps), D/8 lanes a row. Bound by the bytes: 4 in and 0.5625 out a value.
-// Measured: 4 prompts of 2048 rows of 8 x 128, fp32, written in 13 us and read
-// back in 12; 16 sequences of 8192 read as fp16 in 166 us (688 MB, 4.15 TB/s,
-// near a copy's 4.7); one token in 2.4 us, a launch's time.
+// Measured: 4 prompts of 2048 rows of 8 x 128 written in 16 us from fp32 (4.7
+// TB/s) and in 15 from fp16, 16 of 8192 in 275 (4.45 TB/s) and 185 (3.7 TB/s);
+// 16 sequences of 8192 read as fp16 in 164 us (688 MB, 4.2 TB/s, near a copy's
+// 4.7); one token in 3.1 us (2.4 in a trace), a launch's time.
 #include "device.hpp"
 #include "internal.hpp"
 #include "kv4.hpp"

@@ -23,8 +23,9 @@
 // Precision: K and V enter as the fp16 numbers they stand for. A query row is
 // scaled by a power of two to a largest magnitude in [2^14, 2^15) and split
 // into two fp16 parts (2^-22 of each element), a weight, scaled to at most
-// 2^15, likewise; sums are fp32. The sum of the weights is one more row of the
-// V product, of ones, so numerator and denominator hold the same weights.
+// 2^15, likewise (what it has below 2^-38 of the largest is lost); sums are
+// fp32. The sum of the weights is one more row of the V product, of ones, so
+// numerator and denominator hold the same weights.
 //
 // Keys a row does not see get weight 0, and V rows past a sequence's end may
 // hold anything: their scales are taken as 0. In a tile with keys that not every
@@ -32,12 +33,15 @@
 // too and remembered for the rows that see the key: their values of these dims
 // are made NaN at the end.
 //
-// Bound by the vector ALU (55 to 59 % of the kernel's time): about 364
-// instructions a tile of 32 keys and 8 rows at D = 128, most of them decoding,
-// against 17 matrix products that run beside them. Measured with the merge: one
-// sequence of 131072 keys 39.5 us (151 MB, 3.8 TB/s), 16 of 4096 23.8 us, 512
-// keys 8.9 us. Three workgroups a CU at D <= 128 with 8 rows (registers allow
-// no more): a wave of another workgroup covers a wave's waits.
+// Most of the time goes into the vector ALU (55 to 59 % of the issue slots):
+// about 364 instructions a tile of 32 keys and 8 rows at D = 128, most of them
+// decoding, against 17 matrix products that run beside them. The rest is waits
+// (22 to 30 % of the waves' cycles) that 1.6 to 1.7 waves a SIMD do not cover:
+// make_plan cuts the keys for two workgroups a CU, of which registers (120 to
+// 125 at D = 128, 90 to 93 at D = 64) and the rings would let four run; more
+// chunks have not been measured. Measured with the merge: one sequence of
+// 131072 keys 39.6 us (151 MB, 3.8 TB/s), 16 of 4096 23.8 us (D = 64 18.5 us,
+// D = 256 48 us), 512 keys 8.9 us.
 #include <algorithm>
 #include <cmath>
 
@@ -460,11 +464,23 @@ __global__ __launch_bounds__(waves(D) * 64, D == 256 ? 2 : NT == 1 || D == 64 ? 
 
 // Rows a workgroup stacks: 8 or 16 in the split kernel, kRowsBlock in the rows
 // kernel, which decodes a tile once for all its rows but leaves waves idle
-// below 128. From 33 rows a KV head on it wins or draws (4 sequences of 2048
-// keys, D = 128: 40 rows 24.0 us against 26.2, 96 rows 27.3 against 39.9; 16 of
-// 4096: 40 rows 91 against 99, 64 rows 94 against 81, 96 rows 98 against 117);
-// below, the split kernel does (16 of 4096: 12 rows 35 us against 85, 32 rows
-// 52 against 88).
+// below 128. It is taken from 33 rows a KV head on. Rows kernel / split kernel,
+// us, 8 KV heads:
+//   rows               20       32       40       48       64       80       96
+//   D = 64
+//   4 x 2048 keys  16.5/15.8 17.1/17.0 17.8/19.2 18.3/19.3 19.2/19.8 20.6/23.1 21.4/29.9
+//   16 x 4096        62/38     63/39     65/66     66/67     67/58     70/77     71/79
+//   D = 128
+//   1 x 4096       18.9/18.1 19.8/19.0 20.7/21.9 21.3/22.1 22.4/21.7 23.7/24.3 24.8/26.4
+//   4 x 2048       21.2/21.9 22.4/23.5 23.5/26.5 24.3/27.1 25.7/28.0 26.7/32.4 26.6/40.4
+//   16 x 4096        82/52     84/53     86/100    87/101    88/82     92/116    94/119
+//   D = 256
+//   1 x 4096       33.1/23.9 35.0/26.4 36.5/30.1 37.4/30.0 39.5/34.2 39.9/40.1 40.3/40.4
+//   4 x 2048       36.8/29.6 39.1/35.7 40.3/41.3 41.0/41.9 42.4/48.4 43.7/61.5 45.3/61.7
+//   16 x 4096       168/100   173/131   177/200   179/176   183/193   187/266   191/345
+// So it loses at 49 to 64 rows of many long sequences at D <= 128 (four full
+// row groups of 16; 7 to 14 %), at D = 256 over one sequence up to 64 rows
+// (16 to 25 %), and below the threshold 4 % in one of the rows above.
 constexpr int kManyRows = 33;
 int stacked_rows(long long rows, int D) { return rows >= kManyRows ? kRowsBlock : rows > 8 && D < 256 ? 16 : 8; }
 

@@ -15,12 +15,15 @@
 //   S^T = K Q^T, O^T += V^T P^T, rows along the lanes: a row's query parts,
 // maximum and sum stay in its two lanes.
 // Two products a score and a value, for the two fp16 parts of queries and
-// weights. Measured: a causal prompt of 2048 rows of 32 heads of 128 98 us (0.35
-// PFLOP/s, 0.70 with both parts; matrix cores 25 %, vector ALU 34 %), 256 rows
-// over 2048 keys 37.6 us. The waves' products and softmax go in turn:
+// weights. Measured: a causal prompt of 2048 rows of 32 heads of 128 99 us (0.35
+// PFLOP/s, 0.70 with both parts; matrix cores 26 %, vector ALU 35 %), 256 rows
+// over 2048 keys 36.6 us with the merge (19 %, 30 %); with heads of 64 68 and
+// 31 us. The waves' products and softmax go in turn:
 // what a CU's other workgroup covers is lost where the last rows of a causal
 // prompt, of the most keys, run alone. The next tile's decoding is laid between
-// the score products (3 % of a prompt of 4096 rows).
+// the score products (3 % of a prompt of 4096 rows). D = 256 has one buffer and
+// two barriers a tile, one workgroup a CU (512 registers; with a soft cap 24
+// bytes a lane spill), and takes 212 us and 70 us.
 #include "kv4_attention.hpp"
 
 namespace aljabr {
@@ -40,7 +43,6 @@ struct Shape {
     static constexpr int kKStride = D + 8;                                 // halves
     static constexpr int kHalves = kTile * kKStride + D * kVStride;        // of a decoded tile
     static constexpr int kBuffers = D == 256 ? 1 : 2;                      // as many as fit 64 KB
-    static constexpr int kDwords = D / 64;                                 // of K a thread decodes
     static constexpr int kPieces = D == 256 ? 2 : 1;                       // dwords of a V row a thread decodes
 };
 

@@ -285,7 +285,7 @@ typedef struct aljabr_rocm_kv4_cache {
 int aljabr_rocm_kv4_cache_bytes(const aljabr_rocm_kv4_cache *cache, size_t *codes_bytes, size_t *scales_bytes);
 /* Quantises K and V rows [sequences][T][n_kv_heads][head_dim] (type F32 or
  * F16; element strides of a sequence, a token and a head, the values of a row
- * adjacent; all three 0: dense) into the cache: row t of sequence b goes to
+ * adjacent, 0 for a row that several share; all three 0: dense) into the cache: row t of sequence b goes to
  * position positions[b] + t, for t < counts[b] (counts NULL: T). Rows that the
  * cache does not have are dropped. K or V may be NULL: only the other is
  * written. Rows of one call must be different rows of the cache. T *
@@ -315,12 +315,15 @@ int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, c
  * Keys on a bad block are not seen, and what keys hold that a row does not see
  * never reaches it; a block with a value past fp16's range (its scale past
  * 8160, which kv4_write does not make) may count as NaN to rows that do.
- * fp32-accurate. T * Hq is at most 2^30,
- * sequences * the positions of each at most 2^35.
+ * fp32-accurate; of a weight, what is below 2^-38 of the row's largest is lost.
+ * T * Hq is at most 2^30, sequences * the positions of each at most 2^35; a
+ * workgroup takes up to 128 of the T * Hq / n_kv_heads rows of a sequence and
+ * KV head (8 or 16 of up to 32), and a call of 2^23 and more is refused (-3).
  * workspace: device scratch for split partials, of
  * aljabr_rocm_kv4_attention_workspace bytes (fewer: fewer splits), not shared
  * by calls that may run at once, captured graphs among them. NULL: the
- * stream's scratch, which a call under stream capture is refused (-4). */
+ * stream's scratch (no memory for it: no splits), which a call under stream
+ * capture is refused (-4) unless it needs none (0 bytes). */
 int aljabr_rocm_kv4_attention(void *out, const void *Q, const aljabr_rocm_kv4_cache *cache, const int *context_lens,
                               const int *counts, int T, int Hq, float scale, int is_causal, int window, float soft_cap,
                               void *workspace, size_t workspace_bytes);
