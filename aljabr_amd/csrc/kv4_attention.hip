@@ -494,7 +494,7 @@ void launch_split(const Params &p, hipStream_t s) {
         hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, true>), grid, dim3(kWaves * 64), lds, s, p);
     else
         hipLaunchKernelGGL((kv4_split_kernel<D, NT, PAGED, false>), grid, dim3(kWaves * 64), lds, s, p);
-    if (p.quota) hipLaunchKernelGGL((kv4_merge_kernel<D, 8 * NT>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
+    if (p.quota) hipLaunchKernelGGL((merge_kernel<Params, D, 8 * NT>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
 }
 
 template <int D, int NT>

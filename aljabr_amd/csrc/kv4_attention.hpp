@@ -1,14 +1,17 @@
 // kv4_attention.hpp - what the two kernels of attention over the 4-bit cache
-// share: the rows' key ranges, the cut of the keys into chunks, the decoder of
-// codes and the merge of chunks' partials. Included by the two .hip files only.
+// share: the rows' key ranges and the decoder of codes. Included by the two
+// .hip files only.
 #pragma once
 
 #include "device.hpp"
 #include "internal.hpp"
 #include "kv4.hpp"
+#include "kv_chunks.hpp"
 
 namespace aljabr {
 namespace kv4 {
+
+using namespace kv;
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -21,20 +24,6 @@ constexpr int kRowsBlock = 128;              // rows a workgroup of the rows ker
 constexpr int kRowsLeast = 4;                // tiles it takes at the least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightScale = 8192.0f;      // weights are at most 4
-
-// n / d for 0 <= n < 2^31 without a division.
-struct FastDiv {
-    uint32_t mul, shift;
-    void set(uint32_t d) {
-        uint32_t l = 0;
-        while ((uint64_t{1} << l) < d) ++l;
-        shift = 31 + l;
-        mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);   // off by less than 1: n / 2^shift of it is below 1 / d
-    }
-    __device__ __forceinline__ int operator()(int n) const {
-        return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul >> shift);
-    }
-};
 
 struct Params {
     Kv4View v;
@@ -51,10 +40,6 @@ struct Params {
     int2 *chunks;                            // per sequence, KV head and row group: its first slot and its chunks
 };
 
-// A sequence's keys and its rows.
-struct Seq {
-    int n, cnt;
-};
 __device__ __forceinline__ Seq sequence(const Params &p, int b) {
     Seq s;
     s.n = min(max(p.lens[b], 0), kv4_capacity(p.v));
@@ -79,110 +64,6 @@ __device__ __forceinline__ bool row_tiles(const Params &p, const Seq &s, int r0,
     a = lo / kTile;
     z = hi > lo ? (hi + kTile - 1) / kTile : a;
     return true;
-}
-
-// Inclusive sum over the lanes up to this one.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // row 0's and 2's sums into 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // the first half's into the second
-    return v;
-}
-
-// One chunk of the work of a row group: tiles [t0, t1) of sequence b. The
-// tiles of all sequences are cut into chunks of one size, a multiple of
-// `least`, about `quota` of them: a batch of uneven lengths keeps every
-// workgroup busy alike. Chunks are numbered through the sequences, and slots
-// of partials through those of several chunks (a single chunk writes its rows
-// itself): fewer than 2 quota, as each of these is longer than one chunk, and
-// fewer than quota + B (partial_slots).
-struct Chunk {
-    int b, t0, t1;
-    int first, count;        // of the sequence's chunks
-    int slot;                // of the first
-    Seq seq;
-};
-
-// Chunk number w; b < 0 past the end. Called by whole waves.
-__device__ __forceinline__ Chunk find_chunk(const Params &p, int w, int r0, int rows, int least) {
-    Chunk c{-1, 0, 0, 0, 0, 0, {0, 0}};
-    const int lane = threadIdx.x & 63, B = p.v.B;
-    if (p.quota == 0 || B == 1) {
-        const int b = p.quota ? 0 : w;
-        int a, z;
-        c.seq = sequence(p, b);
-        if (!row_tiles(p, c.seq, r0, rows, a, z)) return c;
-        int per = max(z - a, 1);
-        if (p.quota) {
-            per = max(p.by_chunks(z - a + p.quota - 1), least);
-            per = (per + least - 1) / least * least;
-            c.count = max((z - a + per - 1) / per, 1);
-        } else {
-            c.count = 1;
-        }
-        const int i = p.quota ? w : 0;
-        if (i >= c.count) return c;
-        c.b = b;
-        c.first = p.quota ? 0 : b;
-        c.t0 = a + i * per;
-        c.t1 = min(c.t0 + per, z);
-        return c;
-    }
-    // A lane a sequence; the last (for B <= 64 the only) 64 stay in registers.
-    const int last = (B - 1) & ~63;
-    Seq s{0, 0};
-    int a = 0, z = 0, total = 0;
-    for (int b0 = 0; b0 <= last; b0 += 64) {
-        a = z = 0;
-        if (b0 + lane < B) {
-            s = sequence(p, b0 + lane);
-            row_tiles(p, s, r0, rows, a, z);
-        }
-        total += __builtin_amdgcn_readlane(wave_scan(z - a), 63);
-    }
-    int per = max(p.by_chunks(total + p.quota - 1), least);
-    per = (per + least - 1) / least * least;
-    const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
-    int before = 0, singles = 0;                           // chunks, and sequences of one, of the groups of 64 before
-    for (int b0 = 0; b0 <= last; b0 += 64) {
-        if (last) {
-            a = z = 0;
-            s.cnt = 0;
-            if (b0 + lane < B) {
-                s = sequence(p, b0 + lane);
-                row_tiles(p, s, r0, rows, a, z);
-            }
-        }
-        // ceil((z - a) / per): the estimate is at most one off.
-        int n = static_cast<int>(static_cast<float>(z - a) * inv);
-        n += n * per < z - a ? 1 : 0;
-        n -= n > 0 && (n - 1) * per >= z - a ? 1 : 0;
-        n += n * per < z - a ? 1 : 0;
-        n = r0 < s.cnt * p.G ? max(n, 1) : 0;
-        const int end = before + wave_scan(n);
-        const uint64_t single = __ballot(n == 1);
-        const uint64_t hit = __ballot(w >= end - n && w < end);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            c.count = __builtin_amdgcn_readlane(n, l);
-            c.first = __builtin_amdgcn_readlane(end, l) - c.count;
-            c.slot = c.first - singles - __builtin_popcountll(single & ((uint64_t{1} << l) - 1));   // of one chunk: not used
-            a = __builtin_amdgcn_readlane(a, l);
-            z = __builtin_amdgcn_readlane(z, l);
-            c.seq.n = __builtin_amdgcn_readlane(s.n, l);
-            c.seq.cnt = __builtin_amdgcn_readlane(s.cnt, l);
-            c.b = b0 + l;
-            c.t0 = a + (w - c.first) * per;
-            c.t1 = min(c.t0 + per, z);
-            return c;
-        }
-        before = __builtin_amdgcn_readlane(end, 63);
-        singles += __builtin_popcountll(single);
-    }
-    return c;
 }
 
 __device__ __forceinline__ half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
@@ -263,99 +144,6 @@ __device__ __forceinline__ Place place(const Params &p, int b, int kvh, int n_ke
         x.scale[u] = head * (D / 32) * p.v.R + row;
     }
     return x;
-}
-
-// The item and chunk number of a workgroup: `quota` chunks of every item, the
-// chunk varying fastest, then the numbers that only uneven batches need (no CU
-// is left half full by workgroups that find none).
-__device__ __forceinline__ void work_of(const Params &p, int id, int &item, int &w) {
-    const int most = p.quota ? p.quota : p.v.B, items = p.v.H * p.row_groups;
-    item = p.by_chunks(id);
-    w = id - item * most;
-    if (item >= items) {
-        w = most + p.by_items(id - items * most);
-        item = id - w * items;
-    }
-}
-
-// Folds the state (m2, l2, o2) into (m, l, o); a state without keys has m = -inf.
-__device__ __forceinline__ void fold(float &m, float &l, float4 &o, float m2, float l2, const float4 &o2) {
-    const float mn = fmaxf(m, m2);
-    if (mn == -INFINITY) return;
-    const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float e = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
-    l = fmaf(l, a, l2 * e);
-    o.x = fmaf(o.x, a, o2.x * e);
-    o.y = fmaf(o.y, a, o2.y * e);
-    o.z = fmaf(o.z, a, o2.z * e);
-    o.w = fmaf(o.w, a, o2.w * e);
-    m = mn;
-}
-
-// One workgroup a row of a sequence with several chunks: D/4 lanes take a
-// chunk's partial as float4s, 256 / (D/4) chunks at once, folded in order and
-// then across the lane groups.
-template <int D, int ROWS>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Params p) {
-    constexpr int LPS = D / 4, SG = 256 / LPS;
-    __shared__ float st[SG * (D + 2)];
-    const int hq = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-    const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
-    const int item = kvh * p.row_groups + r / ROWS;
-    const int2 chunk = p.chunks[static_cast<long long>(item) * p.v.B + b];   // written for the rows that exist
-    if (t >= sequence(p, b).cnt || chunk.y <= 1) return;   // no row, or its one chunk wrote it
-    const int used = chunk.y;
-    const long long row = (static_cast<long long>(b) * p.T + t) * p.Hq + hq;
-    const long long step = static_cast<long long>(p.v.H) * p.row_groups * ROWS;      // rows from chunk to chunk
-    const long long first = chunk.x * step + static_cast<long long>(item) * ROWS + r % ROWS;
-    const float *po = p.part_o + first * D, *pm = p.part_ml + first * 2;
-    const int sg = threadIdx.x / LPS, j = threadIdx.x % LPS;
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int U = 8;                                   // splits in flight per lane group
-    for (int s0 = sg; s0 < used; s0 += U * SG) {
-        float ms[U], ls[U];
-        float4 os[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long s = s0 + u * SG < used ? s0 + u * SG : s0;
-            const float2 ml = *reinterpret_cast<const float2 *>(pm + 2 * s * step);
-            ms[u] = ml.x;
-            ls[u] = ml.y;
-            os[u] = *reinterpret_cast<const float4 *>(po + s * step * D + 4 * j);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (s0 + u * SG >= used) break;
-            fold(m, l, o, ms[u], ls[u], os[u]);
-        }
-    }
-    float *my = st + sg * (D + 2);
-    my[4 * j] = o.x;
-    my[4 * j + 1] = o.y;
-    my[4 * j + 2] = o.z;
-    my[4 * j + 3] = o.w;
-    if (j == 0) {
-        my[D] = m;
-        my[D + 1] = l;
-    }
-    __syncthreads();
-    for (int dd = threadIdx.x; dd < D; dd += 256) {
-        float M = -INFINITY, L = 0.0f, O = 0.0f;
-#pragma unroll
-        for (int g = 0; g < SG; ++g) M = fmaxf(M, st[g * (D + 2) + D]);
-        if (M != -INFINITY) {
-#pragma unroll
-            for (int g = 0; g < SG; ++g) {
-                const float mg = st[g * (D + 2) + D];
-                if (mg == -INFINITY) continue;
-                const float e = __builtin_amdgcn_exp2f(mg - M);
-                L = fmaf(st[g * (D + 2) + D + 1], e, L);
-                O = fmaf(st[g * (D + 2) + dd], e, O);
-            }
-        }
-        p.out[row * D + dd] = L == 0.0f ? 0.0f : O / L;
-    }
 }
 
 // The rows kernel (kv4_rows.hip), p.row_groups blocks of kRowsBlock rows, and the merge.

@@ -170,9 +170,6 @@ __device__ __forceinline__ void decode_tile(const Magic &g, const Raw<D> &x, hal
         }
 }
 
-// The row group of the item group i, and the other way round: the last, of most keys when causal, first.
-__device__ __forceinline__ int group_of(const Params &p, int i) { return p.row_groups - 1 - i; }
-
 template <int D, bool PAGED, bool CAP>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Params p) {
     constexpr int STEPS = D / 16, DT = D / 32, KS = Shape<D>::kKStride, BUFS = Shape<D>::kBuffers;
@@ -449,49 +446,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_rows_kernel(Pa
     }
 }
 
-// A wave a row of a sequence with several chunks: D/4 lanes take a chunk's
-// partial as float4s (64 / (D/4) chunks at once), folded in order, then across
-// the lane groups.
-template <int D>
-__global__ __launch_bounds__(256) void kv4_merge_rows_kernel(Params p) {
-    constexpr int LPS = D / 4, SG = 64 / LPS;
-    const int of_seq = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
-    const int t = of_seq / p.Hq, hq = of_seq - t * p.Hq;
-    if (t >= p.T) return;
-    const long long row = static_cast<long long>(b) * p.T * p.Hq + of_seq;
-    const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
-    const int item = group_of(p, r / kRowsBlock) * p.v.H + kvh;
-    const int2 chunk = p.chunks[static_cast<long long>(item) * p.v.B + b];   // written for the rows that exist
-    if (t >= sequence(p, b).cnt || chunk.y <= 1) return;   // no row, or its one chunk wrote it
-    const long long step = static_cast<long long>(p.v.H) * p.row_groups * kRowsBlock;
-    const long long first = chunk.x * step + static_cast<long long>(item) * kRowsBlock + r % kRowsBlock;
-    const int lane = threadIdx.x & 63, sg = lane / LPS, j = lane % LPS;
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int U = 4;                                   // chunks in flight per lane group
-    for (int s0 = sg; s0 < chunk.y; s0 += U * SG) {
-        float2 ml[U];
-        float4 os[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long s = s0 + u * SG < chunk.y ? s0 + u * SG : s0;
-            ml[u] = *reinterpret_cast<const float2 *>(p.part_ml + (first + s * step) * 2);
-            os[u] = *reinterpret_cast<const float4 *>(p.part_o + (first + s * step) * D + 4 * j);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (s0 + u * SG < chunk.y) fold(m, l, o, ml[u].x, ml[u].y, os[u]);
-    }
-#pragma unroll
-    for (int off = LPS; off < 64; off <<= 1) {
-        const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
-        const float4 o2 = make_float4(__shfl_xor(o.x, off), __shfl_xor(o.y, off), __shfl_xor(o.z, off), __shfl_xor(o.w, off));
-        fold(m, l, o, m2, l2, o2);
-    }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    if (sg == 0) *reinterpret_cast<float4 *>(p.out + row * D + 4 * j) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-}
-
 template <int D, bool PAGED>
 void launch_typed(const Params &p, hipStream_t s) {
     const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
@@ -500,7 +454,7 @@ void launch_typed(const Params &p, hipStream_t s) {
     else
         hipLaunchKernelGGL((kv4_rows_kernel<D, PAGED, false>), grid, dim3(kThreads), 0, s, p);
     if (p.quota)                                           // few row groups, so few rows of a sequence
-        hipLaunchKernelGGL((kv4_merge_rows_kernel<D>), dim3((p.T * p.Hq + 3) / 4, p.v.B), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((merge_rows_kernel<Params, D, kRowsBlock>), dim3((p.T * p.Hq + 3) / 4, p.v.B), dim3(256), 0, s, p);
 }
 
 template <int D>
