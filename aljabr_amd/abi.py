@@ -108,6 +108,21 @@ class Kv4Cache(ctypes.Structure):
 _KV = ctypes.POINTER(Kv4Cache)
 
 
+class KvCache(ctypes.Structure):
+    """aljabr_rocm_kv_cache: the planes and shape of an fp16 or fp32 KV cache."""
+    _fields_ = [("k", _P), ("v", _P), ("block_table", _P)] + [(n, ctypes.c_int32) for n in (
+        "type", "layers", "sequences", "n_kv_heads", "head_dim", "rows", "num_blocks", "max_blocks")]
+
+
+class Rotation(ctypes.Structure):
+    """aljabr_rocm_rotation: how positions turn pairs of a row's values."""
+    _fields_ = [("base", ctypes.c_float), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("freq_divisors", _P)]
+
+
+_KC = ctypes.POINTER(KvCache)
+
+
 # name -> (restype, argtypes); every symbol declared in include/aljabr_rocm.h.
 class KernelStat(ctypes.Structure):
     """aljabr_rocm_kernel_stat: one launch group of a profiled decode step."""
@@ -154,6 +169,11 @@ SIGNATURES = {
     "aljabr_rocm_kv4_read": (_I, [_P, _P, _KV, _P, _P, _I, _LL, _LL, _LL, _I]),
     "aljabr_rocm_kv4_attention": (_I, [_P, _P, _KV, _P, _P, _I, _I, _F, _I, _I, _F, _P, _SZ]),
     "aljabr_rocm_kv4_attention_workspace": (_I, [_KV, _I, _I, ctypes.POINTER(_SZ)]),
+    "aljabr_rocm_kv_cache_bytes": (_I, [_KC, ctypes.POINTER(_SZ)]),
+    "aljabr_rocm_kv_append": (_I, [_KC, _I] + [_P] * 7 + [_I, _I] + [_LL] * 6 + [_I, ctypes.POINTER(Rotation)]),
+    "aljabr_rocm_kv_tree_attention": (_I, [_P, _P, _KC, _I, _P, _P, _P, _I, _I, _F, _I, _F, _P, _SZ]),
+    "aljabr_rocm_kv_tree_attention_workspace": (_I, [_KC, _I, _I, ctypes.POINTER(_SZ)]),
+    "aljabr_rocm_kv_tree_accept": (_I, [_KC] + [_P] * 9 + [_I]),
     "aljabr_rocm_matvec_tb_pair": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
     "aljabr_rocm_matvec_tb_triple": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I]),
     "aljabr_rocm_matvec_tb_triple_batch": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I]),

@@ -1,0 +1,634 @@
+// kv_tree.hip - attention of a draft's rows over an fp16 or fp32 cache (layout
+// and trees: kv_cache.hpp).
+//
+//   out[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(s_j - max s),
+//   s_j = cap(scale * q[t, h] . k_j), over the keys j that row t sees.
+//
+// The rows of a KV head are stacked, r = t * G + g (G = Hq / Hkv), 16 or 32 a
+// workgroup. A wave walks tiles of 16 U keys, whose fragments come straight
+// from the cache into registers, each refilled for the wave's next tile as soon
+// as the matrix cores have taken it: no LDS, no barrier in the loop.
+//   S[key][row]   = K Q^T: lane (n, h) holds key n, 16 bytes at every step;
+//   O^T[d][row] += V^T P^T on v_mfma_f32_16x16x4_f32, whose operands are one
+//     number a lane: V's is V[4h' + r][its dims] as loaded (whole rows a load,
+//     no transposition), P's the weight that the lane computed itself, as fp32.
+// The fp32 products run at 1/16 of fp16's rate; for up to 32 rows they take
+// less time than the bytes, and they keep the weights whole.
+//
+// Precision: an fp16 K enters as it is against a query row scaled by a power of
+// two to a largest magnitude in [2^14, 2^15) and split into two fp16 parts
+// (2^-22 of each element); everything else is fp32.
+//
+// Keys a row does not see get weight 0. In a tile that not every row sees
+// whole, V rows past the end are taken as 0, and values that are not finite are
+// taken out of the product and added by hand for the rows that see them. A
+// score that comes out as NaN is computed again in fp32: the parts of a query
+// times an infinity make a NaN where the sum has none.
+#include <algorithm>
+#include <cmath>
+
+#include "kv_tree.hpp"
+
+namespace aljabr {
+
+using namespace kvt;
+
+namespace {
+
+template <bool F16, int D>
+struct Shape {
+    static constexpr int kSize = F16 ? 2 : 4, kRow = D * kSize;
+    static constexpr int U = kRow >= 512 ? 1 : 2;          // groups of 16 keys of a tile: 16 KB of K and V, D = 256 of fp32 32 KB
+    static constexpr int KT = 16 * U;
+    static constexpr int VE = F16 && D > 64 ? 8 : 4;       // dims of a lane's piece of a V row
+    static constexpr int VP = D / 16 / VE;                 // pieces
+    static constexpr int KL = D * kSize / 64;              // K's 16-byte loads of a group
+    static constexpr int OT = D / 16;                      // output tiles
+};
+
+// A piece of a V row as loaded.
+template <bool F16, int D>
+struct Piece {
+    static constexpr int kWords = Shape<F16, D>::VE * Shape<F16, D>::kSize / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const char *at) {
+        if constexpr (kWords == 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(at);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(at);
+            w[0] = x.x; w[1] = x.y;
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (F16) return f16_bits_to_f32(w[e >> 1] >> (16 * (e & 1)) & 0xffffu);
+        else return __uint_as_float(w[e]);
+    }
+    // The bits of values that are not finite have an exponent of ones.
+    __device__ __forceinline__ bool finite() const {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) bad |= F16 ? ((w[i] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u : ((w[i] & 0x7fffffffu) + 0x00800000u) & 0x80000000u;
+        return !bad;
+    }
+    __device__ __forceinline__ void drop() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    // Values that are not finite become 0.
+    __device__ __forceinline__ void clean() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (F16) {
+                if ((w[i] & 0x7c00u) == 0x7c00u) w[i] &= 0xffff0000u;
+                if ((w[i] & 0x7c000000u) == 0x7c000000u) w[i] &= 0x0000ffffu;
+            } else {
+                if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] = 0;
+            }
+        }
+    }
+};
+
+// grid: chunks of KV heads and row groups (work_of).
+template <bool F16, int D, int NT>
+__global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
+    using S = Shape<F16, D>;
+    constexpr int U = S::U, KT = S::KT, VE = S::VE, VP = S::VP, KL = S::KL, OT = S::OT, ROWS = 16 * NT, STEPS = D / 32;
+    extern __shared__ float smem[];                        // states on their way, and weights of odd tiles
+    __shared__ Tree tree;
+    const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int item, w;
+    work_of(p, blockIdx.x, item, w);
+    const int kvh = p.by_groups(item), r0 = (item - kvh * p.row_groups) * ROWS;
+    const Chunk chunk = find_chunk(p, w, r0, ROWS, kWaves);
+    if (chunk.b < 0) return;
+    const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
+    if (p.quota && w == chunk.first && threadIdx.x == 0)
+        p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.slot, chunk.count);
+    const Seq seq = chunk.seq;
+    const int base = seq.n - seq.cnt, r1 = min(r0 + ROWS, seq.cnt * p.G);
+
+    // The first tile goes out before anything else is read.
+    uint4 kf[U][KL];
+    Piece<F16, D> vf[U][4][VP];
+    Place<U> here = {}, next = {};
+    auto load_keys = [&](const Place<U> &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const char *at = x.k[u] + (min(n, x.last[u]) * S::kRow + 16 * h);
+#pragma unroll
+            for (int s = 0; s < KL; ++s) kf[u][s] = *reinterpret_cast<const uint4 *>(at + 64 * s);
+        }
+    };
+    auto load_values = [&](const Place<U> &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const char *at = x.v[u] + (min(4 * h + r, x.last[u]) * S::kRow + n * VE * S::kSize);
+#pragma unroll
+                for (int c = 0; c < VP; ++c) vf[u][r][c].load(at + c * 16 * VE * S::kSize);
+            }
+    };
+    if (t0 + wave < t1) {
+        here = place<U>(p, S::kRow, b, kvh, seq.n, t0 + wave);
+        load_keys(here);
+        load_values(here);
+    }
+    const bool filled = p.parents && (p.window > 0 || t1 * KT > base);
+    if (filled) fill_tree(tree, p.parents + static_cast<long long>(b) * p.T, seq.cnt, p.window);
+
+    // This lane's columns: row, what it sees, the query times scale * log2(e).
+    Range range[NT];
+    int row_t[NT];
+    half8 qh[F16 ? NT : 1][STEPS], ql[F16 ? NT : 1][STEPS];
+    float qf[F16 ? 1 : NT][D / 4];
+    float unscale[NT], up[NT];
+    const float *qrow[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const int r = min(r0 + 16 * c + n, r1 - 1);        // columns past the rows repeat the last and are not stored
+        const int t = p.by_g(r), g = r - t * p.G;
+        row_t[c] = t;
+        range[c] = range_of(p, seq, t, tree, filled);
+        qrow[c] = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D;
+        if constexpr (F16) {
+            float4 x[STEPS][2];
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    x[s][i] = *reinterpret_cast<const float4 *>(qrow[c] + 32 * s + 8 * h + 4 * i);
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x[s][i].x), fabsf(x[s][i].y)), fmaxf(fabsf(x[s][i].z), fabsf(x[s][i].w))));
+                }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32)) * p.scale;
+            int e = 0;
+            if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
+            e = e < -100 ? -100 : e;
+            up[c] = ldexpf(1.0f, 15 - e);
+            unscale[c] = ldexpf(p.unscale, e - 15);
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const float y[8] = {x[s][0].x, x[s][0].y, x[s][0].z, x[s][0].w, x[s][1].x, x[s][1].y, x[s][1].z, x[s][1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float z = y[i] * p.scale * up[c];
+                    qh[c][s][i] = static_cast<_Float16>(z);
+                    ql[c][s][i] = static_cast<_Float16>(z - static_cast<float>(qh[c][s][i]));
+                }
+            }
+        } else {
+            up[c] = 1.0f;
+            unscale[c] = p.unscale;
+#pragma unroll
+            for (int s = 0; s < KL; ++s) {
+                const float4 x = *reinterpret_cast<const float4 *>(qrow[c] + 16 * s + 4 * h);
+                qf[c][4 * s] = x.x * p.scale;
+                qf[c][4 * s + 1] = x.y * p.scale;
+                qf[c][4 * s + 2] = x.z * p.scale;
+                qf[c][4 * s + 3] = x.w * p.scale;
+            }
+        }
+    }
+    // Keys that every row sees: a tree's rows stand at most at their places.
+    const int full_lo = p.window > 0 ? base + p.by_g(r1 - 1) - p.window + 1 : 0;
+    const int full_hi = p.parents ? base : base + p.by_g(r0) + 1;
+
+    f32x4 o[NT][OT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        m[c] = -INFINITY;
+        l[c] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < OT; ++j) o[c][j] = f32x4{};
+    }
+
+    for (int kt = t0 + wave; kt < t1; kt += kWaves) {
+        const int k0 = kt * KT;
+        const bool more = kt + kWaves < t1;
+        if (more) next = place<U>(p, S::kRow, b, kvh, seq.n, kt + kWaves);
+        const bool whole = k0 >= full_lo && k0 + KT <= full_hi && here.ok == (1u << U) - 1;   // every row sees every key
+
+        // S: accumulator r of group u is key k0 + 16u + 4h + r of this lane's column.
+        f32x4 s[NT][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) s[c][u] = f32x4{};
+            if constexpr (F16) {
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const half8 a = __builtin_bit_cast(half8, kf[u][i]);
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) {
+                        s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[c][i], s[c][u], 0, 0, 0);
+                        s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[c][i], s[c][u], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    const float a[4] = {__uint_as_float(kf[u][i].x), __uint_as_float(kf[u][i].y), __uint_as_float(kf[u][i].z),
+                                        __uint_as_float(kf[u][i].w)};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+                            s[c][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], qf[c][4 * i + e], s[c][u], 0, 0, 0);
+                }
+            }
+        }
+        if (more) load_keys(next);
+        uint32_t see[NT];
+        float pw[NT][U][4];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            float mx = -INFINITY;
+            see[c] = 0xffffffffu;
+            if (!whole) {
+                see[c] = seen(p, seq, range[c], row_t[c], k0, tree);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (!(here.ok >> u & 1)) see[c] &= ~(0xffffu << 16 * u);
+            }
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < 4 * U; ++i) {
+                pw[c][i >> 2][i & 3] = s[c][i >> 2][i & 3];
+                nan |= pw[c][i >> 2][i & 3] != pw[c][i >> 2][i & 3];
+            }
+            if (__any(nan)) {
+                float *mine = smem + wave * (ROWS * KT) + lane;
+#pragma unroll
+                for (int i = 0; i < 4 * U; ++i) mine[64 * i] = pw[c][i >> 2][i & 3];
+                int keys = 4 * U, dims = D;
+                asm("" : "+s"(keys), "+s"(dims));          // loops that stay loops
+                for (int i = 0; i < keys; ++i) {
+                    const int r = 4 * h + (i & 3);
+                    if (mine[64 * i] == mine[64 * i] || !(see[c] >> (16 * (i >> 2) + r) & 1)) continue;
+                    const char *kr = i >= 4 ? here.k[U - 1] + min(r, here.last[U - 1]) * S::kRow : here.k[0] + min(r, here.last[0]) * S::kRow;
+                    float sum = 0.0f;
+                    for (int d = 0; d < dims; ++d) {
+                        const float x = F16 ? static_cast<float>(reinterpret_cast<const _Float16 *>(kr)[d]) : reinterpret_cast<const float *>(kr)[d];
+                        sum = fmaf(qrow[c][d] * p.scale * up[c], x, sum);
+                    }
+                    mine[64 * i] = sum;
+                }
+#pragma unroll
+                for (int i = 0; i < 4 * U; ++i) pw[c][i >> 2][i & 3] = mine[64 * i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * U; ++i) {
+                const int u = i >> 2, key = 16 * u + 4 * h + (i & 3);
+                float y = pw[c][u][i & 3];
+                if (p.soft_cap > 0.0f) {
+                    const float cap = p.soft_cap * kLog2e;
+                    y = cap * tanhf(y * fminf(unscale[c] / cap, 3e38f));       // finite: 0 stays 0
+                }
+                if (!(see[c] >> key & 1)) y = -INFINITY;
+                mx = fmaxf(mx, y);
+                pw[c][u][i & 3] = y;
+            }
+            const float us = p.soft_cap > 0.0f ? 1.0f : unscale[c];
+            mx *= us;
+            // The reference m of a column is raised only when a score exceeds it by more than 2.
+            if (__any(mx > m[c] + 2.0f)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float to = mx > m[c] + 2.0f ? mx : m[c];
+                const float alpha = to == m[c] ? 1.0f : __builtin_amdgcn_exp2f(m[c] - to);     // 0 while m is -inf
+                l[c] *= alpha;
+#pragma unroll
+                for (int j = 0; j < OT; ++j) o[c][j] *= alpha;
+                m[c] = to;
+            }
+            const float ref = m[c] == -INFINITY ? 0.0f : m[c];
+#pragma unroll
+            for (int i = 0; i < 4 * U; ++i) {
+                float &y = pw[c][i >> 2][i & 3];
+                y = __builtin_amdgcn_exp2f(fmaf(y, us, -ref));
+                l[c] += y;
+            }
+        }
+        if (!whole) {
+            bool odd = false;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < VP; ++c) {
+                        if (k0 + 16 * u + 4 * h + r >= seq.n || !(here.ok >> u & 1)) vf[u][r][c].drop();
+                        odd |= !vf[u][r][c].finite();
+                    }
+            if (__any(odd)) {
+                float *pl = smem + wave * (ROWS * KT);     // the wave's weights, [column tile][key][row]
+#pragma unroll
+                for (int c = 0; c < NT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4 * U; ++i) pl[(c * KT + 16 * (i >> 2) + 4 * h + (i & 3)) * 16 + n] = pw[c][i >> 2][i & 3];
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the wave's own writes
+                int keys = KT;
+                asm("" : "+s"(keys));                      // a loop that stays one
+                for (int i = 0; i < keys; ++i) {
+                    if (k0 + i >= seq.n || !(here.ok >> (i >> 4) & 1)) continue;
+                    const char *vr = (U == 2 && i >= 16 ? here.v[U - 1] : here.v[0]) + (i & 15) * S::kRow;
+#pragma unroll
+                    for (int x = 0; x < VP; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            Piece<F16, D> v;
+                            v.load(vr + (x * 16 + 4 * h + r) * VE * S::kSize);
+                            if (!__any(!v.finite())) continue;
+#pragma unroll
+                            for (int e = 0; e < VE; ++e) {
+                                const float val = v.get(e);
+#pragma unroll
+                                for (int c = 0; c < NT; ++c)
+                                    o[c][x * VE + e][r] += val - val != 0.0f && (see[c] >> i & 1) ? pl[(c * KT + i) * 16 + n] * val : 0.0f;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int c = 0; c < VP; ++c) vf[u][r][c].clean();
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int x = 0; x < VP; ++x)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        const float a = vf[u][r][x].get(e);
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+                            o[c][x * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pw[c][u][r], o[c][x * VE + e], 0, 0, 0);
+                    }
+        if (more) load_values(next);
+        here = next;
+    }
+
+    // The four waves' states become one: 2 and 3 hand theirs to 0 and 1, then 1 to 0. O^T tile x VE + e, accumulator r:
+    // dim 16 VE x + VE (4h + r) + e of the row.
+    constexpr int kState = NT * (OT * 256 + 64 * 2);       // floats of a wave's state
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        if (m[c] == -INFINITY && l[c] != l[c]) m[c] = 0.0f;            // a NaN score alone leaves no reference: any finite one carries it
+    }
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            float *st = smem + (wave - half) * kState;
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+#pragma unroll
+                for (int j = 0; j < OT; ++j) *reinterpret_cast<f32x4 *>(st + ((c * OT + j) * 64 + lane) * 4) = o[c][j];
+                *reinterpret_cast<float2 *>(st + NT * OT * 256 + (c * 64 + lane) * 2) = make_float2(m[c], l[c]);
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float *st = smem + wave * kState;
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const float2 ml = *reinterpret_cast<const float2 *>(st + NT * OT * 256 + (c * 64 + lane) * 2);
+                const float to = fmaxf(m[c], ml.x);
+                const float a = m[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[c] - to);
+                const float e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - to);
+                l[c] = fmaf(l[c], a, ml.y * e);
+                m[c] = to;
+#pragma unroll
+                for (int j = 0; j < OT; ++j) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(st + ((c * OT + j) * 64 + lane) * 4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[c][j][r] = fmaf(o[c][j][r], a, x[r] * e);
+                }
+            }
+        }
+    }
+    if (wave) return;
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const int r = r0 + 16 * c + n;
+        if (r >= r1) continue;
+        const bool whole = chunk.count == 1;
+        const long long part = (static_cast<long long>(chunk.slot + w - chunk.first) * p.v.H * p.row_groups + item) * ROWS + 16 * c + n;
+        const int t = p.by_g(r), g = r - t * p.G;
+        float *dst = whole ? p.out + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D : p.part_o + part * D;
+        const float f = whole ? (l[c] == 0.0f ? 0.0f : 1.0f / l[c]) : 1.0f;
+#pragma unroll
+        for (int x = 0; x < VP; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VE; e += 4)
+                    *reinterpret_cast<float4 *>(dst + 16 * VE * x + VE * (4 * h + i) + e) =
+                        make_float4(o[c][x * VE + e][i] * f, o[c][x * VE + e + 1][i] * f, o[c][x * VE + e + 2][i] * f, o[c][x * VE + e + 3][i] * f);
+        if (!whole && h == 0) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(m[c], l[c]);
+    }
+}
+
+template <bool F16, int D, int NT>
+void launch_split(const Params &p, hipStream_t s) {
+    using S = Shape<F16, D>;
+    constexpr size_t states = 2 * NT * (S::OT * 256 + 128) * 4, weights = kWaves * 16 * NT * S::KT * 4;
+    constexpr size_t lds = states > weights ? states : weights;
+    static_assert(lds + sizeof(Tree) <= 65536, "LDS of a workgroup");
+    const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
+    hipLaunchKernelGGL((kv_split_kernel<F16, D, NT>), grid, dim3(kThreads), lds, s, p);
+    if (p.quota) hipLaunchKernelGGL((merge_kernel<Params, D, 16 * NT>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
+}
+
+template <bool F16, int D>
+void launch_d(const Params &p, int rows, hipStream_t s) {
+    if constexpr (D < 256) {
+        if (rows == 32) return launch_split<F16, D, 2>(p, s);
+    }
+    launch_split<F16, D, 1>(p, s);
+}
+
+template <bool F16>
+void launch(const Params &p, int rows, hipStream_t s) {
+    if (p.v.D == 64) launch_d<F16, 64>(p, rows, s);
+    else if (p.v.D == 128) launch_d<F16, 128>(p, rows, s);
+    else launch_d<F16, 256>(p, rows, s);
+}
+
+// How a call's work is laid out: stacked rows of a workgroup, row groups, keys of a tile, and the chunks that the keys
+// are cut into (all sequences together, per KV head and row group): two workgroups a CU.
+struct Plan {
+    int rows, groups, tile, quota;
+};
+Plan make_plan(const KvView &v, int T, int Hq) {
+    Plan s;
+    const long long rows = static_cast<long long>(T) * (Hq / v.H);
+    s.rows = rows > 16 && v.D < 256 ? 32 : 16;
+    s.tile = v.D * (v.f16 ? 2 : 4) >= 512 ? 16 : 32;
+    s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
+    const long long items = static_cast<long long>(v.H) * s.groups;
+    const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    const int least = s.tile * kWaves;                     // keys of the smallest chunk
+    const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
+    s.quota = static_cast<int>(std::min(2 * cus / items, v.B * most));
+    if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
+    return s;
+}
+
+// Slots of partials that so many chunks need at the most: sequence b of x_b > 1 chunk sizes takes ceil(x_b), fewer
+// than 2 x_b and than x_b + 1, and the x_b add up to at most the quota.
+size_t partial_slots(const KvView &v, int quota) {
+    return quota ? static_cast<size_t>(std::min<long long>(2LL * quota - 1, static_cast<long long>(quota) + v.B - 1)) : 0;
+}
+// Bytes of partials with this many chunks.
+size_t partial_bytes(const KvView &v, const Plan &s, int quota) {
+    return static_cast<size_t>(v.H) * s.groups *
+           (partial_slots(v, quota) * s.rows * (v.D + 2) * sizeof(float) + v.B * sizeof(int2));
+}
+
+}  // namespace
+
+size_t kv_tree_attention_scratch_bytes(const KvView &v, int T, int Hq) {
+    const Plan s = make_plan(v, T, Hq);
+    return s.quota ? partial_bytes(v, s, s.quota) : 0;
+}
+
+int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
+    Params p{};
+    p.v = v;
+    p.out = a.out;
+    p.q = a.q;
+    p.lens = a.lens;
+    p.counts = a.counts;
+    p.parents = a.T > 1 ? a.parents : nullptr;             // one row is its own line
+    p.T = a.T;
+    p.Hq = a.Hq;
+    p.G = a.Hq / v.H;
+    // scale * log2(e) as p.scale p.unscale, the first between 2^-61 and 2^100: where scores are in fp32's range, so is a
+    // query element times it.
+    int k;
+    const double m = std::frexp(static_cast<double>(a.scale) * 1.4426950408889634, &k);
+    const int in = std::min(std::max(k, -60), 100);
+    p.scale = static_cast<float>(std::ldexp(m, in));
+    p.unscale = static_cast<float>(std::ldexp(1.0, k - in));
+    // Within fp32's range with the scores' scaling, and to fp32 the same: past 2^64 a cap is none for every score that
+    // softmax tells from its neighbours, below 2^-30 all weights are equal.
+    p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;
+    p.window = std::min(a.window, 1 << 30);                // past every key; positions less it stay in 32 bits
+    const Plan plan = make_plan(v, a.T, a.Hq);
+    if (static_cast<double>(v.H) * plan.groups * (plan.quota + static_cast<double>(v.B)) > 0x7fffff)
+        return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv_tree_attention: T = %d rows of %d heads are more than one launch takes", a.T, a.Hq);
+    p.row_groups = plan.groups;
+    p.quota = plan.quota;
+    p.tile_shift = log2_exact(plan.tile);
+    p.by_g.set(p.G);
+    p.by_groups.set(plan.groups);
+    p.by_rows.set(v.R);
+    p.by_items.set(v.H * plan.groups);
+    p.by_heads.set(v.H);
+    float *part = a.scratch;
+    if (p.quota) {
+        if (a.scratch) {
+            // As many chunks as the caller's workspace holds the partials of.
+            const size_t none = partial_bytes(v, plan, 0), slot = partial_bytes(v, plan, 1) - none;
+            const size_t fit = a.scratch_bytes < none ? 0 : (a.scratch_bytes - none) / slot;
+            if (fit < partial_slots(v, p.quota)) {
+                const size_t most = std::max((fit + 1) / 2, fit + 1 > static_cast<size_t>(v.B) ? fit + 1 - v.B : 0);
+                p.quota = most < 2 ? 0 : static_cast<int>(most);
+            }
+        } else {
+            part = static_cast<float *>(stream_scratch(partial_bytes(v, plan, p.quota)));
+            if (!part) {
+                hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+                if (hipStreamIsCapturing(current_stream(), &cs) != hipSuccess || cs != hipStreamCaptureStatusNone)
+                    return ALJABR_ROCM_ERR_BUFFER;
+                (void)hipGetLastError();                   // no memory: one chunk a sequence needs none
+                p.quota = 0;
+            }
+        }
+    }
+    if (p.quota) {
+        p.part_o = part;
+        const size_t all = partial_slots(v, p.quota) * v.H * plan.groups * plan.rows;
+        p.part_ml = part + all * v.D;
+        p.chunks = reinterpret_cast<int2 *>(p.part_ml + 2 * all);
+    }
+    p.by_chunks.set(p.quota ? p.quota : v.B);
+    v.f16 ? launch<true>(p, plan.rows, current_stream()) : launch<false>(p, plan.rows, current_stream());
+    return ALJABR_ROCM_OK;
+}
+
+}  // namespace aljabr
+
+using namespace aljabr;
+
+namespace {
+
+int check_attention(const aljabr_rocm_kv_cache *cache, int layer, int T, int Hq, KvView &v) {
+    const int rc = kv_view(cache, layer, "kv_tree_attention", v);
+    if (rc != ALJABR_ROCM_OK) return rc;
+    ALJ_REQUIRE(T > 0 && Hq > 0 && Hq % v.H == 0, "kv_tree_attention: T = %d must be positive and Hq = %d a multiple of %d KV heads",
+                T, Hq, v.H);
+    ALJ_REQUIRE(static_cast<long long>(T) * Hq <= (1 << 30), "kv_tree_attention: T * Hq exceeds 2^30");
+    ALJ_REQUIRE(static_cast<long long>(v.B) * kv_capacity(v) <= (1LL << 35),
+                "kv_tree_attention: sequences * the positions of each exceeds 2^35");   // find_chunk adds up their tiles
+    return ALJABR_ROCM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int aljabr_rocm_kv_tree_attention_workspace(const aljabr_rocm_kv_cache *cache, int T, int Hq, size_t *bytes) {
+    ALJ_REQUIRE(bytes, "kv_tree_attention_workspace: bytes is null");
+    KvView v;
+    const int rc = check_attention(cache, 0, T, Hq, v);
+    if (rc != ALJABR_ROCM_OK) return rc;
+    ALJ_CHECK_READY();
+    *bytes = kv_tree_attention_scratch_bytes(v, T, Hq);
+    return ALJABR_ROCM_OK;
+}
+
+int aljabr_rocm_kv_tree_attention(void *out, const void *Q, const aljabr_rocm_kv_cache *cache, int layer,
+                                  const int *context_lens, const int *counts, const int *parents, int T, int Hq, float scale,
+                                  int window, float soft_cap, void *workspace, size_t workspace_bytes) {
+    KvView v;
+    int rc = check_attention(cache, layer, T, Hq, v);
+    if (rc != ALJABR_ROCM_OK) return rc;
+    ALJ_REQUIRE(out && Q && context_lens, "kv_tree_attention: out, Q and context_lens must be device pointers");
+    ALJ_REQUIRE(aligned(out, 16) && aligned(Q, 16) && aligned(workspace, 16),
+                "kv_tree_attention: out, Q and workspace must be 16-byte aligned");
+    ALJ_REQUIRE(std::isfinite(scale) && std::isfinite(soft_cap), "kv_tree_attention: scale and soft_cap must be finite");
+    if (parents && T > kTreeMost)
+        return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv_tree_attention: a tree of T = %d rows exceeds %d", T, kTreeMost);
+    ALJ_CHECK_READY();
+    KvTreeAttention a{};
+    a.out = static_cast<float *>(out);
+    a.q = static_cast<const float *>(Q);
+    a.lens = context_lens;
+    a.counts = counts;
+    a.parents = parents;
+    a.T = T;
+    a.Hq = Hq;
+    a.scale = scale > 0.0f ? scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(v.D)));
+    a.window = window;
+    a.soft_cap = soft_cap;
+    a.scratch = static_cast<float *>(workspace);
+    a.scratch_bytes = workspace ? workspace_bytes : 0;
+    rc = enqueue_kv_tree_attention(v, a);
+    return rc == ALJABR_ROCM_OK ? finish_launch("kv_tree_attention") : rc;
+}
+
+}  // extern "C"

@@ -1,0 +1,122 @@
+// kv_tree.hpp - what the kernels of attention over fp16 and fp32 caches share:
+// the rows' key ranges, their lines in a tree, where a tile's keys are.
+// Included by the kv_tree .hip files only.
+#pragma once
+
+#include "device.hpp"
+#include "internal.hpp"
+#include "kv_cache.hpp"
+#include "kv_chunks.hpp"
+
+namespace aljabr {
+namespace kvt {
+
+using namespace kv;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+    KvView v;
+    float *out;
+    const float *q;
+    const int *lens, *counts, *parents;
+    int T, Hq, G, row_groups;
+    FastDiv by_g, by_groups, by_rows, by_chunks, by_items, by_heads;   // G, row_groups, rows of a block, chunks that vary fastest, H * row_groups, H
+    float scale, unscale;                    // their product is the call's scale times log2(e)
+    float soft_cap;
+    int window;
+    int tile_shift;                          // log2 of the keys of a tile
+    int quota;                               // chunks that the keys of all sequences are cut into (about), 0: one each
+    float *part_o, *part_ml;                 // per slot, KV head, row group and stacked row: D sums, and (m, l)
+    int2 *chunks;                            // per sequence, KV head and row group: its first slot and its chunks
+};
+
+__device__ __forceinline__ Seq sequence(const Params &p, int b) {
+    Seq s;
+    s.n = min(max(p.lens[b], 0), kv_capacity(p.v));
+    s.cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+    return s;
+}
+
+// The tiles that rows [r0, r0 + rows) see together. A row of a tree may stand anywhere between its root and its place,
+// so the window is taken from the root and the last key from the place.
+__device__ __forceinline__ bool row_tiles(const Params &p, const Seq &s, int r0, int rows, int &a, int &z) {
+    a = z = 0;
+    if (r0 >= s.cnt * p.G) return false;
+    const int base = s.n - s.cnt, hi = base + min(p.by_g(r0 + rows - 1), s.cnt - 1) + 1;
+    const int lo = p.window > 0 ? max(base + (p.parents ? 0 : p.by_g(r0)) - p.window + 1, 0) : 0;
+    a = lo >> p.tile_shift;
+    z = hi > lo ? (hi + (1 << p.tile_shift) - 1) >> p.tile_shift : a;
+    return true;
+}
+
+// What a row sees: keys [lo, hi), and of a tree's rows those in its line.
+struct Range {
+    int lo, hi;
+};
+__device__ __forceinline__ Range range_of(const Params &p, const Seq &s, int t, const Tree &tree, bool filled) {
+    const int base = s.n - s.cnt;
+    Range x;
+    x.hi = max(p.parents ? base : base + t + 1, 0);
+    x.lo = p.window > 0 ? max(base + (p.parents ? (filled ? tree.depth[t] : 0) : t) - p.window + 1, 0) : 0;
+    return x;
+}
+
+// Bits of keys k0 .. k0 + 31 that row t sees.
+__device__ __forceinline__ uint32_t seen(const Params &p, const Seq &s, const Range &x, int t, int k0, const Tree &tree) {
+    const int a = max(x.lo - k0, 0), z = min(x.hi - k0, 32);
+    uint32_t bits = z <= a ? 0 : (z == 32 ? 0xffffffffu : (1u << z) - 1) & ~((1u << a) - 1);
+    if (p.parents) {
+        const int at = k0 - (s.n - s.cnt);                   // of the tree's rows
+        if (at >= 0 && at < s.cnt) {
+            const int w = at >> 5;
+            bits |= funnel_shift_right(w + 1 < kTreeWords ? tree.mask[(w + 1) * kTreeMost + t] : 0, tree.mask[w * kTreeMost + t], at & 31);
+        } else if (at < 0 && at > -32) {
+            bits |= tree.mask[t] << -at;
+        }
+    }
+    return bits;
+}
+
+// Where a tile's groups of 16 keys are (uniform over the wave).
+template <int U>
+struct Place {
+    const char *k[U], *v[U];
+    int last[U];                             // the last of the 16 rows that is in the plane
+    uint32_t ok;                             // bit u: the group's block exists
+};
+
+template <int U>
+__device__ __forceinline__ Place<U> place(const Params &p, int row_bytes, int b, int kvh, int n_keys, int kt) {
+    Place<U> x;
+    x.ok = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        int key = (kt * U + u) * 16;
+        if (key >= n_keys) key = kt * U * 16;                // past the end: the tile's first group again, masked
+        int s = b, row = key;
+        x.last[u] = 15;
+        if (p.v.table) {
+            const int blk = p.by_rows(key);
+            // A scalar load: nothing writes the table while the kernel runs.
+            s = ((const __attribute__((address_space(4))) int *)p.v.table)[static_cast<long long>(b) * p.v.max_blocks + blk];
+            row = key - blk * p.v.R;
+            if (s >= 0 && s < p.v.num_blocks) x.ok |= 1u << u;
+            else s = 0;
+        } else {
+            x.ok |= 1u << u;
+            x.last[u] = min(15, p.v.R - 1 - row);
+        }
+        const long long at = ((static_cast<long long>(s) * p.v.H + kvh) * p.v.R + row) * row_bytes;
+        x.k[u] = p.v.k + at;
+        x.v[u] = p.v.v + at;
+    }
+    return x;
+}
+
+}  // namespace kvt
+}  // namespace aljabr

@@ -330,6 +330,110 @@ int aljabr_rocm_kv4_attention(void *out, const void *Q, const aljabr_rocm_kv4_ca
 int aljabr_rocm_kv4_attention_workspace(const aljabr_rocm_kv4_cache *cache, int T, int Hq, size_t *bytes);
 
 /* ======================================================================== */
+/* fp16 and fp32 KV caches: rows appended, drafts verified                   */
+/* ======================================================================== */
+/*
+ * K and V as planes [layers][S][n_kv_heads][rows][head_dim] of type F32 or
+ * F16 in device memory, 16-byte aligned: the layout of aljabr_rocm_llama_kv_cache
+ * (its planes can be described here), of attention_gqa's K and V (one layer),
+ * and, with a block table, of the paged attention above. Without a table S =
+ * sequences and a sequence holds `rows` positions (any number up to 2^30).
+ * With one S = num_blocks: position j of sequence b is row j % rows of block
+ * block_table[b * max_blocks + j / rows], rows a multiple of 16, max_blocks *
+ * rows at most 2^30. head_dim is 64, 128 or 256 (else -3). No counterpart in
+ * the reference, whose decode rotates, appends and attends a token at a time.
+ *
+ * A draft of T rows a sequence is a tree: parents[b * T + t] is an earlier row
+ * of the sequence, any other number (-1) none; a row's line is the row and its
+ * ancestors, its depth the number of those. Row t of sequence b lies at place
+ * context_lens[b] - counts[b] + t of the cache, context_lens counting the
+ * draft's rows too, and stands at position context_lens[b] - counts[b] + depth.
+ * parents NULL: a chain, row t - 1 before row t (a decode step, a chunk of a
+ * prompt). A tree has at most 256 rows (-3), a chain in attention any number.
+ *
+ * The calls read positions, lengths, trees and the table on the device, wait
+ * for nothing there and can be captured: a place outside the cache, or on a
+ * block index outside [0, num_blocks), is a row that the cache does not have.
+ */
+typedef struct aljabr_rocm_kv_cache {
+    void *k, *v;                                     /* device */
+    const void *block_table;                         /* device int32 [sequences][max_blocks], or NULL */
+    int32_t type;                                    /* ALJABR_ROCM_TYPE_F32 or F16 */
+    int32_t layers, sequences, n_kv_heads, head_dim;
+    int32_t rows;                                    /* positions of a sequence, or of a block */
+    int32_t num_blocks, max_blocks;                  /* with a block table, else 0 */
+} aljabr_rocm_kv_cache;
+
+/* Bytes of K's plane, all layers (V's is alike): num_blocks > 0 counts blocks,
+ * else sequences. The pointers are not read; no device is needed. */
+int aljabr_rocm_kv_cache_bytes(const aljabr_rocm_kv_cache *cache, size_t *bytes);
+
+/* A rotation of positions: pair i of the first rotary_dim (0: head_dim; a
+ * multiple of 8, else -3) values turns by position * base^(-2i / rotary_dim),
+ * divided by freq_divisors[i] where that is positive (device fp32
+ * [rotary_dim / 2], or NULL). Pairs are (i, i + rotary_dim / 2), interleaved:
+ * (2i, 2i + 1). Angles are computed in 64 bits: at far positions they differ
+ * from aljabr_rocm_rope's, which rounds them to fp32 as the reference does. */
+typedef struct aljabr_rocm_rotation {
+    float base;
+    int32_t rotary_dim, interleaved;
+    const void *freq_divisors;
+} aljabr_rocm_rotation;
+
+/* The rows of T tokens a sequence on their way to attention: Q [sequences][T]
+ * [Hq][head_dim] and K [sequences][T][n_kv_heads][head_dim] rotated, V as it
+ * is; Q to q_out (fp32, dense), K and V into the cache, row t of sequence b at
+ * place positions[b] + t, for t < counts[b] (NULL: T). Q, K and V are of type
+ * F32 or F16, at element strides of a sequence, a token and a head, the values
+ * of a row adjacent (all three 0: dense; slices of a stacked Q/K/V product have
+ * its row as token stride). angles: the position a row turns by (device int32
+ * [sequences][T], e.g. a tree's), NULL: its place. rotation NULL: none. Q with
+ * q_out, K or V may be NULL. q_out may be Q if that is fp32 and dense, and is
+ * left as it was from row counts[b] on. Rows that the cache does not have are
+ * dropped (their Q is not). Rows of one call must be different rows of the
+ * cache. Values past F16's range become infinities in an F16 cache. */
+int aljabr_rocm_kv_append(const aljabr_rocm_kv_cache *cache, int layer, void *q_out, const void *Q, const void *K,
+                          const void *V, const int *positions, const int *counts, const int *angles, int T, int Hq,
+                          long long q_stride_b, long long q_stride_t, long long q_stride_h, long long kv_stride_b,
+                          long long kv_stride_t, long long kv_stride_h, int type, const aljabr_rocm_rotation *rotation);
+
+/* GQA attention of a draft's rows over a layer of the cache: Q and out
+ * [sequences][T][Hq][head_dim] fp32, Hq a multiple of n_kv_heads. Of the
+ * context_lens[b] keys (clamped to what the sequence can hold) the last
+ * counts[b] (NULL: T) are the draft's rows. Row t sees the keys before those
+ * and its line; with window > 0 only keys whose position is less than window
+ * before its own. soft_cap > 0 caps scores as cap * tanh(score / cap); scale
+ * <= 0: 1 / sqrt(head_dim). A row that sees no key (or none with a score above
+ * -inf) gives zeros; rows from counts[b] on are left as they were. Keys on a
+ * bad block are not seen, and what keys hold that a row does not see never
+ * reaches it. fp32-accurate. T * Hq is at most 2^30, sequences * the positions
+ * of each at most 2^35, and a call of more workgroups than a launch takes is
+ * refused (-3). workspace: device scratch for split partials, of
+ * aljabr_rocm_kv_tree_attention_workspace bytes (fewer: fewer splits), not
+ * shared by calls that may run at once, captured graphs among them. NULL: the
+ * stream's scratch (no memory for it: no splits), which a call under stream
+ * capture is refused (-4) unless it needs none (0 bytes). */
+int aljabr_rocm_kv_tree_attention(void *out, const void *Q, const aljabr_rocm_kv_cache *cache, int layer,
+                                  const int *context_lens, const int *counts, const int *parents, int T, int Hq,
+                                  float scale, int window, float soft_cap, void *workspace, size_t workspace_bytes);
+int aljabr_rocm_kv_tree_attention_workspace(const aljabr_rocm_kv_cache *cache, int T, int Hq, size_t *bytes);
+
+/* Accepts the drafted rows that the model agrees with. tokens [sequences][T]
+ * are the drafted tokens, choices [sequences][T] the model's token after each
+ * row (aljabr_rocm_argmax of its logits), device int32. Row 0 is accepted (the
+ * last token known before the draft); after an accepted row its first child
+ * whose token is the row's choice. path[b * T + i] is the i-th accepted row (-1
+ * behind the last), accepted[b] their number, next_token[b] the choice of the
+ * last (-1 for a sequence without rows), new_lens[b] = context_lens[b] -
+ * counts[b] + accepted[b]. The accepted rows' K and V are moved to the first
+ * places of the draft in every layer of the cache, where their positions say
+ * they belong; what is behind them is left over. T is at most 256, the draft's
+ * rows are different rows of the cache, and the outputs are none of the inputs. */
+int aljabr_rocm_kv_tree_accept(const aljabr_rocm_kv_cache *cache, int *new_lens, int *path, int *accepted,
+                               int *next_token, const int *context_lens, const int *counts, const int *parents,
+                               const int *tokens, const int *choices, int T);
+
+/* ======================================================================== */
 /* Several matrices over one input (replaces MTLC/aljabr_metal_matvec_api.h: */
 /* 83-120): device pointers; types F32 0, F16 1, Q4_0 2, Q8_0 8, Q4_K 12,    */
 /* Q6_K 14. Matrices of one type share a launch.                             */
