@@ -38,12 +38,13 @@ namespace {
 template <bool F16, int D>
 struct Shape {
     static constexpr int kSize = F16 ? 2 : 4, kRow = D * kSize;
-    static constexpr int U = kRow >= 512 ? 1 : 2;          // groups of 16 keys of a tile: 16 KB of K and V, D = 256 of fp32 32 KB
+    static constexpr int U = F16 || D == 64 ? 2 : 1;       // groups of 16 keys of a tile: at most 32 KB of K and V
     static constexpr int KT = 16 * U;
     static constexpr int VE = F16 && D > 64 ? 8 : 4;       // dims of a lane's piece of a V row
     static constexpr int VP = D / 16 / VE;                 // pieces
-    static constexpr int KL = D * kSize / 64;              // K's 16-byte loads of a group
+    static constexpr int KL = D * kSize / 64;              // K's 16-byte loads of a group, a step of the contraction each
     static constexpr int OT = D / 16;                      // output tiles
+    static constexpr int kQuery = KL * (F16 ? 2 : 1);      // 16-byte pieces of a lane's query
 };
 
 // A piece of a V row as loaded.
@@ -89,13 +90,74 @@ struct Piece {
     }
 };
 
+// The 8 halves of dim e of a piece, of the 8 keys that a lane holds.
+template <int D, int W>
+__device__ __forceinline__ half8 dim_of(const Piece<true, D> (&v)[2][4][W], int x, int e) {
+    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+    uint32_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        f[i] = __builtin_amdgcn_perm(v[i >> 1][2 * (i & 1) + 1][x].w[e >> 1], v[i >> 1][2 * (i & 1)][x].w[e >> 1], sel);
+    return __builtin_bit_cast(half8, make_uint4(f[0], f[1], f[2], f[3]));
+}
+
+// A row's query as a lane's pieces: fp16 the two parts of each step, fp32 as it is. up: the power of two it was scaled by.
+template <bool F16, int D>
+__device__ __forceinline__ void load_query(const float *row, float scale, int h, uint4 (&q)[Shape<F16, D>::kQuery], float &up, int &e) {
+    up = 1.0f;
+    e = 15;
+    if constexpr (F16) {
+        constexpr int STEPS = D / 32;
+        float4 x[STEPS][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[s][i] = *reinterpret_cast<const float4 *>(row + 32 * s + 8 * h + 4 * i);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[s][i].x), fabsf(x[s][i].y)), fmaxf(fabsf(x[s][i].z), fabsf(x[s][i].w))));
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+        e = 0;
+        if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);         // top in [2^(e-1), 2^e)
+        e = e < -100 ? -100 : e;
+        up = ldexpf(1.0f, 15 - e);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const float y[8] = {x[s][0].x, x[s][0].y, x[s][0].z, x[s][0].w, x[s][1].x, x[s][1].y, x[s][1].z, x[s][1].w};
+            half8 first, rest;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float z = y[i] * scale * up;
+                first[i] = static_cast<_Float16>(z);
+                rest[i] = static_cast<_Float16>(z - static_cast<float>(first[i]));
+            }
+            q[2 * s] = __builtin_bit_cast(uint4, first);
+            q[2 * s + 1] = __builtin_bit_cast(uint4, rest);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < Shape<F16, D>::KL; ++s) {
+            const float4 x = *reinterpret_cast<const float4 *>(row + 16 * s + 4 * h);
+            q[s] = make_uint4(__float_as_uint(x.x * scale), __float_as_uint(x.y * scale), __float_as_uint(x.z * scale), __float_as_uint(x.w * scale));
+        }
+    }
+}
+
+// Whether the queries are kept in LDS: in registers they would be D / 4 of each column tile.
+constexpr bool query_in_lds(int D, int NT) { return NT * D >= 256; }
+
 // grid: chunks of KV heads and row groups (work_of).
 template <bool F16, int D, int NT>
-__global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_split_kernel(Params p) {
     using S = Shape<F16, D>;
-    constexpr int U = S::U, KT = S::KT, VE = S::VE, VP = S::VP, KL = S::KL, OT = S::OT, ROWS = 16 * NT, STEPS = D / 32;
-    extern __shared__ float smem[];                        // states on their way, and weights of odd tiles
+    constexpr int U = S::U, KT = S::KT, VE = S::VE, VP = S::VP, KL = S::KL, OT = S::OT, ROWS = 16 * NT, QL = S::kQuery;
+    constexpr bool QLDS = query_in_lds(D, NT);
+    extern __shared__ float smem[];                        // queries, states on their way, weights of odd tiles
     __shared__ Tree tree;
+    __shared__ float2 query_scale[QLDS ? ROWS : 1];
+    float *work = smem + (QLDS ? NT * QL * 256 : 0);
     const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int item, w;
@@ -142,10 +204,10 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
     // This lane's columns: row, what it sees, the query times scale * log2(e).
     Range range[NT];
     int row_t[NT];
-    half8 qh[F16 ? NT : 1][STEPS], ql[F16 ? NT : 1][STEPS];
-    float qf[F16 ? 1 : NT][D / 4];
+    uint4 qr[QLDS ? 1 : NT][QL];
     float unscale[NT], up[NT];
     const float *qrow[NT];
+    uint4 *qlds = reinterpret_cast<uint4 *>(smem) + lane;
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         const int r = min(r0 + 16 * c + n, r1 - 1);        // columns past the rows repeat the last and are not stored
@@ -153,52 +215,34 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
         row_t[c] = t;
         range[c] = range_of(p, seq, t, tree, filled);
         qrow[c] = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D;
-        if constexpr (F16) {
-            float4 x[STEPS][2];
-            float top = 0.0f;
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[s][i] = *reinterpret_cast<const float4 *>(qrow[c] + 32 * s + 8 * h + 4 * i);
-                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x[s][i].x), fabsf(x[s][i].y)), fmaxf(fabsf(x[s][i].z), fabsf(x[s][i].w))));
-                }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32)) * p.scale;
-            int e = 0;
-            if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
-            e = e < -100 ? -100 : e;
-            up[c] = ldexpf(1.0f, 15 - e);
+        int e;
+        if constexpr (!QLDS) {
+            load_query<F16, D>(qrow[c], p.scale, h, qr[c], up[c], e);
             unscale[c] = ldexpf(p.unscale, e - 15);
+        } else if (c % kWaves == wave) {
+            load_query<F16, D>(qrow[c], p.scale, h, qr[0], up[c], e);
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const float y[8] = {x[s][0].x, x[s][0].y, x[s][0].z, x[s][0].w, x[s][1].x, x[s][1].y, x[s][1].z, x[s][1].w};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float z = y[i] * p.scale * up[c];
-                    qh[c][s][i] = static_cast<_Float16>(z);
-                    ql[c][s][i] = static_cast<_Float16>(z - static_cast<float>(qh[c][s][i]));
-                }
-            }
-        } else {
-            up[c] = 1.0f;
-            unscale[c] = p.unscale;
-#pragma unroll
-            for (int s = 0; s < KL; ++s) {
-                const float4 x = *reinterpret_cast<const float4 *>(qrow[c] + 16 * s + 4 * h);
-                qf[c][4 * s] = x.x * p.scale;
-                qf[c][4 * s + 1] = x.y * p.scale;
-                qf[c][4 * s + 2] = x.z * p.scale;
-                qf[c][4 * s + 3] = x.w * p.scale;
-            }
+            for (int i = 0; i < QL; ++i) qlds[(c * QL + i) * 64] = qr[0][i];
+            if (lane < 16) query_scale[16 * c + n] = make_float2(ldexpf(p.unscale, e - 15), up[c]);
         }
     }
+    if constexpr (QLDS) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            unscale[c] = query_scale[16 * c + n].x;
+            up[c] = query_scale[16 * c + n].y;
+        }
+    }
+    auto query = [&](int c, int i) __attribute__((always_inline)) { return QLDS ? qlds[(c * QL + i) * 64] : qr[QLDS ? 0 : c][i]; };
     // Keys that every row sees: a tree's rows stand at most at their places.
     const int full_lo = p.window > 0 ? base + p.by_g(r1 - 1) - p.window + 1 : 0;
     const int full_hi = p.parents ? base : base + p.by_g(r0) + 1;
 
     f32x4 o[NT][OT];
     float m[NT], l[NT];
+    bool careful = false;
+again:
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         m[c] = -INFINITY;
@@ -211,37 +255,37 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
         const int k0 = kt * KT;
         const bool more = kt + kWaves < t1;
         if (more) next = place<U>(p, S::kRow, b, kvh, seq.n, kt + kWaves);
-        const bool whole = k0 >= full_lo && k0 + KT <= full_hi && here.ok == (1u << U) - 1;   // every row sees every key
+        // Every row sees every key.
+        const bool whole = !careful && k0 >= full_lo && k0 + KT <= full_hi && here.ok == (1u << U) - 1;
 
         // S: accumulator r of group u is key k0 + 16u + 4h + r of this lane's column.
         f32x4 s[NT][U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int c = 0; c < NT; ++c)
 #pragma unroll
-            for (int c = 0; c < NT; ++c) s[c][u] = f32x4{};
-            if constexpr (F16) {
+            for (int u = 0; u < U; ++u) s[c][u] = f32x4{};
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
-                    const half8 a = __builtin_bit_cast(half8, kf[u][i]);
+        for (int i = 0; i < KL; ++i)
 #pragma unroll
-                    for (int c = 0; c < NT; ++c) {
-                        s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[c][i], s[c][u], 0, 0, 0);
-                        s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[c][i], s[c][u], 0, 0, 0);
+            for (int c = 0; c < NT; ++c) {
+                if constexpr (F16) {
+                    const half8 q0 = __builtin_bit_cast(half8, query(c, 2 * i)), q1 = __builtin_bit_cast(half8, query(c, 2 * i + 1));
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const half8 a = __builtin_bit_cast(half8, kf[u][i]);
+                        s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q1, s[c][u], 0, 0, 0);
+                        s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q0, s[c][u], 0, 0, 0);
+                    }
+                } else {
+                    const f32x4 q = __builtin_bit_cast(f32x4, query(c, i));
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const f32x4 a = __builtin_bit_cast(f32x4, kf[u][i]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[c][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], q[e], s[c][u], 0, 0, 0);
                     }
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < KL; ++i) {
-                    const float a[4] = {__uint_as_float(kf[u][i].x), __uint_as_float(kf[u][i].y), __uint_as_float(kf[u][i].z),
-                                        __uint_as_float(kf[u][i].w)};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int c = 0; c < NT; ++c)
-                            s[c][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], qf[c][4 * i + e], s[c][u], 0, 0, 0);
-                }
             }
-        }
         if (more) load_keys(next);
         uint32_t see[NT];
         float pw[NT][U][4];
@@ -262,7 +306,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
                 nan |= pw[c][i >> 2][i & 3] != pw[c][i >> 2][i & 3];
             }
             if (__any(nan)) {
-                float *mine = smem + wave * (ROWS * KT) + lane;
+                float *mine = work + wave * (ROWS * KT) + lane;
 #pragma unroll
                 for (int i = 0; i < 4 * U; ++i) mine[64 * i] = pw[c][i >> 2][i & 3];
                 int keys = 4 * U, dims = D;
@@ -310,7 +354,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
 #pragma unroll
             for (int i = 0; i < 4 * U; ++i) {
                 float &y = pw[c][i >> 2][i & 3];
-                y = __builtin_amdgcn_exp2f(fmaf(y, us, -ref));
+                y = __builtin_amdgcn_exp2f(fmaf(y, us, -ref)) * kWeightScale<F16>;
                 l[c] += y;
             }
         }
@@ -326,7 +370,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
                         odd |= !vf[u][r][c].finite();
                     }
             if (__any(odd)) {
-                float *pl = smem + wave * (ROWS * KT);     // the wave's weights, [column tile][key][row]
+                float *pl = work + wave * (ROWS * KT);     // the wave's weights, [column tile][key][row]
 #pragma unroll
                 for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -361,21 +405,63 @@ __global__ __launch_bounds__(kThreads, 2) void kv_split_kernel(Params p) {
                         for (int c = 0; c < VP; ++c) vf[u][r][c].clean();
             }
         }
+        if constexpr (F16) {
+            half8 p0[NT], p1[NT];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int c = 0; c < NT; ++c)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+                for (int i = 0; i < 4 * U; ++i) {
+                    const float y = pw[c][i >> 2][i & 3];
+                    p0[c][i] = static_cast<_Float16>(y);
+                    p1[c][i] = static_cast<_Float16>(fmaf(static_cast<float>(p0[c][i]), -1.0f, y));
+                }
 #pragma unroll
-                for (int x = 0; x < VP; ++x)
+            for (int x = 0; x < VP; ++x)
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        const float a = vf[u][r][x].get(e);
+                for (int e = 0; e < VE; ++e) {
+                    const half8 a = dim_of<D, VP>(vf, x, e);
 #pragma unroll
-                        for (int c = 0; c < NT; ++c)
-                            o[c][x * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pw[c][u][r], o[c][x * VE + e], 0, 0, 0);
+                    for (int c = 0; c < NT; ++c) {
+                        f32x4 &acc = o[c][x * VE + e];
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p1[c], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p0[c], acc, 0, 0, 0);
                     }
+                }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int x = 0; x < VP; ++x)
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) {
+                            const float a = vf[u][r][x].get(e);
+#pragma unroll
+                            for (int c = 0; c < NT; ++c)
+                                o[c][x * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pw[c][u][r], o[c][x * VE + e], 0, 0, 0);
+                        }
+        }
         if (more) load_values(next);
         here = next;
+    }
+    if (F16 && !careful) {
+        // Parts of a weight times an infinity may make a NaN: sums that are not finite are made again with every tile
+        // treated as one that not every row sees.
+        float probe = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int j = 0; j < OT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) probe = fmaf(o[c][j][r], 0.0f, probe);
+        if (__any(probe != probe)) {
+            careful = true;
+            here = place<U>(p, S::kRow, b, kvh, seq.n, t0 + wave);       // the wave had a tile: its sums are not zeros
+            load_keys(here);
+            load_values(here);
+            goto again;
+        }
     }
 
     // The four waves' states become one: 2 and 3 hand theirs to 0 and 1, then 1 to 0. O^T tile x VE + e, accumulator r:
@@ -445,8 +531,11 @@ template <bool F16, int D, int NT>
 void launch_split(const Params &p, hipStream_t s) {
     using S = Shape<F16, D>;
     constexpr size_t states = 2 * NT * (S::OT * 256 + 128) * 4, weights = kWaves * 16 * NT * S::KT * 4;
-    constexpr size_t lds = states > weights ? states : weights;
-    static_assert(lds + sizeof(Tree) <= 65536, "LDS of a workgroup");
+    constexpr size_t loop = weights + (query_in_lds(D, NT) ? NT * S::kQuery * 1024 : 0), lds = states > loop ? states : loop;
+    static_assert(lds + sizeof(Tree) + NT * 128 <= 160 * 1024, "LDS of a workgroup");
+    if (lds + sizeof(Tree) + NT * 128 > 65536)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_split_kernel<F16, D, NT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(lds));
     const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
     hipLaunchKernelGGL((kv_split_kernel<F16, D, NT>), grid, dim3(kThreads), lds, s, p);
     if (p.quota) hipLaunchKernelGGL((merge_kernel<Params, D, 16 * NT>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
@@ -454,10 +543,9 @@ void launch_split(const Params &p, hipStream_t s) {
 
 template <bool F16, int D>
 void launch_d(const Params &p, int rows, hipStream_t s) {
-    if constexpr (D < 256) {
-        if (rows == 32) return launch_split<F16, D, 2>(p, s);
-    }
-    launch_split<F16, D, 1>(p, s);
+    if (rows == 16) return launch_split<F16, D, 1>(p, s);
+    if (rows == 32) return launch_split<F16, D, 2>(p, s);
+    if constexpr (D < 256) launch_split<F16, D, 4>(p, s);
 }
 
 template <bool F16>
@@ -475,14 +563,15 @@ struct Plan {
 Plan make_plan(const KvView &v, int T, int Hq) {
     Plan s;
     const long long rows = static_cast<long long>(T) * (Hq / v.H);
-    s.rows = rows > 16 && v.D < 256 ? 32 : 16;
-    s.tile = v.D * (v.f16 ? 2 : 4) >= 512 ? 16 : 32;
+    s.rows = v.f16 && rows > 64 ? kRowsBlock : rows > 32 && v.D < 256 ? 64 : rows > 16 ? 32 : 16;
+    s.tile = v.f16 || v.D == 64 ? 32 : 16;
     s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
     const long long items = static_cast<long long>(v.H) * s.groups;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const int least = s.tile * kWaves;                     // keys of the smallest chunk
+    const int least = s.tile * kWaves;                     // keys of the smallest chunk (kRowsLeast tiles as well)
     const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
-    s.quota = static_cast<int>(std::min(2 * cus / items, v.B * most));
+    const int per_cu = s.rows == 64 || (v.D == 256 && s.rows < 64) ? 1 : 2;
+    s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
     if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
     return s;
 }
@@ -566,7 +655,9 @@ int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
         p.chunks = reinterpret_cast<int2 *>(p.part_ml + 2 * all);
     }
     p.by_chunks.set(p.quota ? p.quota : v.B);
-    v.f16 ? launch<true>(p, plan.rows, current_stream()) : launch<false>(p, plan.rows, current_stream());
+    hipStream_t s = current_stream();
+    if (plan.rows == kRowsBlock) launch_rows(p, s);
+    else v.f16 ? launch<true>(p, plan.rows, s) : launch<false>(p, plan.rows, s);
     return ALJABR_ROCM_OK;
 }
 

@@ -17,7 +17,12 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kWaves = 4;
+constexpr int kRowsBlock = 128;              // rows a workgroup of the rows kernel stacks
+constexpr int kRowsLeast = 4;                // tiles it takes at the least
 constexpr float kLog2e = 1.4426950408889634f;
+// Weights, at most 4, are kept times this: as two fp16 parts they keep what is not below 2^-38 of the row's largest.
+template <bool F16>
+constexpr float kWeightScale = F16 ? 8192.0f : 1.0f;
 
 struct Params {
     KvView v;
@@ -117,6 +122,9 @@ __device__ __forceinline__ Place<U> place(const Params &p, int row_bytes, int b,
     }
     return x;
 }
+
+// The rows kernel (kv_tree_rows.hip), p.row_groups blocks of kRowsBlock rows, and the merge.
+void launch_rows(const Params &p, hipStream_t s);
 
 }  // namespace kvt
 }  // namespace aljabr
