@@ -21,9 +21,10 @@
 //
 // Keys a row does not see get weight 0. In a tile that not every row sees
 // whole, V rows past the end are taken as 0, and values that are not finite are
-// taken out of the product and added by hand for the rows that see them. A
-// score that comes out as NaN is computed again in fp32: the parts of a query
-// times an infinity make a NaN where the sum has none.
+// taken out of the product and added by hand for the rows that see them. The
+// two fp16 parts of a query or a weight times an infinity may make a NaN where
+// the sum has none: a wave whose sums are not finite walks its tiles again, with
+// scores that are NaN computed in fp32 and every tile treated as above.
 #include <algorithm>
 #include <cmath>
 
@@ -174,8 +175,26 @@ __global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_spli
     // The first tile goes out before anything else is read.
     uint4 kf[U][KL];
     Piece<F16, D> vf[U][4][VP];
-    Place<U> here = {}, next = {};
-    auto load_keys = [&](const Place<U> &x) __attribute__((always_inline)) {
+    struct Place {
+        const char *k[U], *v[U];
+        int last[U];                                       // the last of the 16 rows that is in the plane
+        uint32_t ok;                                       // bit u: the group's block exists
+    } here = {}, next = {};
+    Places<U> places{t0 + wave, kWaves};
+    auto place = [&](int i) __attribute__((always_inline)) {
+        Place x;
+        const int key = (t0 + wave + i * kWaves) * KT;
+        x.ok = places.ok(i);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long at = places.offset(i, u);
+            x.k[u] = p.v.k + at;
+            x.v[u] = p.v.v + at;
+            x.last[u] = last_row(p, u && key + 16 * u >= seq.n ? key : key + 16 * u);
+        }
+        return x;
+    };
+    auto load_keys = [&](const Place &x) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const char *at = x.k[u] + (min(n, x.last[u]) * S::kRow + 16 * h);
@@ -183,7 +202,7 @@ __global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_spli
             for (int s = 0; s < KL; ++s) kf[u][s] = *reinterpret_cast<const uint4 *>(at + 64 * s);
         }
     };
-    auto load_values = [&](const Place<U> &x) __attribute__((always_inline)) {
+    auto load_values = [&](const Place &x) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -194,7 +213,8 @@ __global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_spli
             }
     };
     if (t0 + wave < t1) {
-        here = place<U>(p, S::kRow, b, kvh, seq.n, t0 + wave);
+        places.load(p, S::kRow, b, kvh, seq.n, 0);
+        here = place(0);
         load_keys(here);
         load_values(here);
     }
@@ -251,10 +271,13 @@ again:
         for (int j = 0; j < OT; ++j) o[c][j] = f32x4{};
     }
 
-    for (int kt = t0 + wave; kt < t1; kt += kWaves) {
+    for (int kt = t0 + wave, i = 0; kt < t1; kt += kWaves, ++i) {
         const int k0 = kt * KT;
         const bool more = kt + kWaves < t1;
-        if (more) next = place<U>(p, S::kRow, b, kvh, seq.n, kt + kWaves);
+        if (more) {
+            if (i + 1 == places.held + 64 / U) places.load(p, S::kRow, b, kvh, seq.n, i + 1);
+            next = place(i + 1);
+        }
         // Every row sees every key.
         const bool whole = !careful && k0 >= full_lo && k0 + KT <= full_hi && here.ok == (1u << U) - 1;
 
@@ -299,13 +322,9 @@ again:
                 for (int u = 0; u < U; ++u)
                     if (!(here.ok >> u & 1)) see[c] &= ~(0xffffu << 16 * u);
             }
-            bool nan = false;
 #pragma unroll
-            for (int i = 0; i < 4 * U; ++i) {
-                pw[c][i >> 2][i & 3] = s[c][i >> 2][i & 3];
-                nan |= pw[c][i >> 2][i & 3] != pw[c][i >> 2][i & 3];
-            }
-            if (__any(nan)) {
+            for (int i = 0; i < 4 * U; ++i) pw[c][i >> 2][i & 3] = s[c][i >> 2][i & 3];
+            if (F16 && careful) {                          // scores that are NaN, in fp32
                 float *mine = work + wave * (ROWS * KT) + lane;
 #pragma unroll
                 for (int i = 0; i < 4 * U; ++i) mine[64 * i] = pw[c][i >> 2][i & 3];
@@ -316,10 +335,7 @@ again:
                     if (mine[64 * i] == mine[64 * i] || !(see[c] >> (16 * (i >> 2) + r) & 1)) continue;
                     const char *kr = i >= 4 ? here.k[U - 1] + min(r, here.last[U - 1]) * S::kRow : here.k[0] + min(r, here.last[0]) * S::kRow;
                     float sum = 0.0f;
-                    for (int d = 0; d < dims; ++d) {
-                        const float x = F16 ? static_cast<float>(reinterpret_cast<const _Float16 *>(kr)[d]) : reinterpret_cast<const float *>(kr)[d];
-                        sum = fmaf(qrow[c][d] * p.scale * up[c], x, sum);
-                    }
+                    for (int d = 0; d < dims; ++d) sum = fmaf(qrow[c][d] * p.scale * up[c], static_cast<float>(reinterpret_cast<const _Float16 *>(kr)[d]), sum);
                     mine[64 * i] = sum;
                 }
 #pragma unroll
@@ -446,8 +462,7 @@ again:
         here = next;
     }
     if (F16 && !careful) {
-        // Parts of a weight times an infinity may make a NaN: sums that are not finite are made again with every tile
-        // treated as one that not every row sees.
+        // Sums that are not finite are made again, carefully.
         float probe = 0.0f;
 #pragma unroll
         for (int c = 0; c < NT; ++c)
@@ -457,7 +472,8 @@ again:
                 for (int r = 0; r < 4; ++r) probe = fmaf(o[c][j][r], 0.0f, probe);
         if (__any(probe != probe)) {
             careful = true;
-            here = place<U>(p, S::kRow, b, kvh, seq.n, t0 + wave);       // the wave had a tile: its sums are not zeros
+            places.load(p, S::kRow, b, kvh, seq.n, 0);     // the wave had a tile: its sums are not zeros
+            here = place(0);
             load_keys(here);
             load_values(here);
             goto again;

@@ -87,41 +87,49 @@ __device__ __forceinline__ uint32_t seen(const Params &p, const Seq &s, const Ra
     return bits;
 }
 
-// Where a tile's groups of 16 keys are (uniform over the wave).
+// Where the groups of 16 keys of a wave's tiles first, first + step, .. are: lane i holds the byte offset of group i % U
+// of the wave's tile i / U, 64 groups at once, so that a tile's address costs two lane reads and waits for no load.
 template <int U>
-struct Place {
-    const char *k[U], *v[U];
-    int last[U];                             // the last of the 16 rows that is in the plane
-    uint32_t ok;                             // bit u: the group's block exists
-};
+struct Places {
+    int first, step, held;                   // the wave's tiles [held, held + 64 / U) are held
+    int lo, hi;                              // this lane's offset
+    uint64_t there;                          // lanes whose group's block exists
 
-template <int U>
-__device__ __forceinline__ Place<U> place(const Params &p, int row_bytes, int b, int kvh, int n_keys, int kt) {
-    Place<U> x;
-    x.ok = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        int key = (kt * U + u) * 16;
-        if (key >= n_keys) key = kt * U * 16;                // past the end: the tile's first group again, masked
-        int s = b, row = key;
-        x.last[u] = 15;
+    __device__ __forceinline__ void load(const Params &p, int row_bytes, int b, int kvh, int n_keys, int i) {
+        held = i;
+        const int lane = threadIdx.x & 63;
+        const long long tile = (first + static_cast<long long>(i + lane / U) * step) * (16 * U), last = n_keys - 1;
+        long long key = tile + 16 * (lane % U);              // past the end: the tile's first group again, masked; or any
+        if (key > last) key = tile;
+        if (key > last) key = max(last, 0LL) & ~15;
+        int s = b, row = static_cast<int>(key);
+        bool ok = true;
         if (p.v.table) {
-            const int blk = p.by_rows(key);
-            // A scalar load: nothing writes the table while the kernel runs.
-            s = ((const __attribute__((address_space(4))) int *)p.v.table)[static_cast<long long>(b) * p.v.max_blocks + blk];
-            row = key - blk * p.v.R;
-            if (s >= 0 && s < p.v.num_blocks) x.ok |= 1u << u;
-            else s = 0;
-        } else {
-            x.ok |= 1u << u;
-            x.last[u] = min(15, p.v.R - 1 - row);
+            const int blk = p.by_rows(row);
+            s = p.v.table[static_cast<long long>(b) * p.v.max_blocks + blk];
+            row -= blk * p.v.R;
+            ok = s >= 0 && s < p.v.num_blocks;
+            if (!ok) s = 0;
         }
         const long long at = ((static_cast<long long>(s) * p.v.H + kvh) * p.v.R + row) * row_bytes;
-        x.k[u] = p.v.k + at;
-        x.v[u] = p.v.v + at;
+        lo = static_cast<int>(at);
+        hi = static_cast<int>(at >> 32);
+        there = __ballot(ok);
     }
-    return x;
-}
+    // Group u of the wave's i-th tile.
+    __device__ __forceinline__ long long offset(int i, int u) const {
+        const int l = (i - held) * U + u;
+        return static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, l))) << 32 |
+                                      static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, l)));
+    }
+    // Bit u: group u's block exists.
+    __device__ __forceinline__ uint32_t ok(int i) const {
+        return static_cast<uint32_t>(there >> ((i - held) * U)) & ((1u << U) - 1);
+    }
+};
+
+// The last of the 16 rows from `key` on that is in the plane.
+__device__ __forceinline__ int last_row(const Params &p, int key) { return p.v.table ? 15 : min(15, p.v.R - 1 - key); }
 
 // The rows kernel (kv_tree_rows.hip), p.row_groups blocks of kRowsBlock rows, and the merge.
 void launch_rows(const Params &p, hipStream_t s);

@@ -19,8 +19,9 @@
 //
 // Values that are not finite: a tile that not every row sees whole is cleaned
 // of them in LDS first, and they are added by hand for the rows that see them.
-// In any other tile they make sums that are not finite; the workgroup then
-// walks its keys again with every tile treated so.
+// In any other tile, and in keys, they make sums that are not finite; the
+// workgroup then walks its keys again with every tile treated so, and scores
+// that are NaN computed in fp32.
 #include "kv_tree.hpp"
 
 namespace aljabr {
@@ -97,23 +98,36 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
     const int own = lane / R::CPR, slot = lane % R::CPR;
     const uint32_t ring = lds_address(lds);
     uint32_t ok = 0, ok_next = 0;                          // of the tile at hand and the next: halves whose block exists
+    Places<2> places{t0, 1};
     auto copy = [&](int kt, int buffer) __attribute__((always_inline)) {
-        const Place<2> x = place<2>(p, R::kRow, b, kvh, seq.n, kt);
-        const int u = wave >> 1, first = 8 * (wave & 1);
-        const char *k = wave >= 2 ? x.k[1] : x.k[0], *v = wave >= 2 ? x.v[1] : x.v[0];
-        const int last = wave >= 2 ? x.last[1] : x.last[0];
+        const int i = kt - t0, u = wave >> 1, first = 8 * (wave & 1);
+        if (i == places.held + 32) places.load(p, R::kRow, b, kvh, seq.n, i);
+        const long long at = places.offset(i, u);
+        const int last = last_row(p, kt * kTile + (kt * kTile + 16 * u < seq.n ? 16 * u : 0));
         const uint32_t dst = ring + buffer * R::kBuffer + (16 * u + first) * R::kRow;
 #pragma unroll
         for (int j = 0; j < R::kCopies; ++j) {
-            const int row = first + j * R::RPL + own, at = min(row, last) * R::kRow;
-            dma16(k + at + 16 * (slot ^ R::k_swap(row)), dst + 1024 * j);
-            dma16(v + at + 16 * (slot ^ R::v_swap(row)), dst + R::kPlane + 1024 * j);
+            const int row = first + j * R::RPL + own, in = min(row, last) * R::kRow;
+            dma16(p.v.k + at + (in + 16 * (slot ^ R::k_swap(row))), dst + 1024 * j);
+            dma16(p.v.v + at + (in + 16 * (slot ^ R::v_swap(row))), dst + R::kPlane + 1024 * j);
         }
-        return x.ok;
+        return places.ok(i);
     };
     auto start = [&]() __attribute__((always_inline)) {
+        places.load(p, R::kRow, b, kvh, seq.n, 0);
         if (t0 < t1) ok = copy(t0, 0);
         if (t0 + 1 < t1) ok_next = copy(t0 + 1, 1);
+    };
+    // A tile's rows by hand, for the paths that are rarely taken.
+    auto row_of = [&](int kt, int key, bool of_v) __attribute__((always_inline)) {
+        int at = min(kt * kTile + key, seq.n - 1), s = b;
+        if (p.v.table) {
+            const int blk = p.by_rows(at);
+            s = p.v.table[static_cast<long long>(b) * p.v.max_blocks + blk];
+            at -= blk * p.v.R;
+            if (s < 0 || s >= p.v.num_blocks) s = 0;
+        }
+        return (of_v ? p.v.v : p.v.k) + ((static_cast<long long>(s) * p.v.H + kvh) * p.v.R + at) * R::kRow;
     };
     start();
     const bool filled = p.parents && (p.window > 0 || t1 * kTile > base);
@@ -182,6 +196,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
             else wait_copies<0>();
             lds_barrier();                                 // the tile is there; the buffer after the next is free
             char *kl = lds + cur * R::kBuffer, *vl = kl + R::kPlane;
+            const bool seen_here = !(idle || k0 >= w_hi || k0 + kTile <= w_lo);
+            half8 ka[STEPS];
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) ka[st] = *reinterpret_cast<const half8 *>(kl + nl * R::kRow + 16 * (2 * st + h ^ R::k_swap(nl)));
+            __builtin_amdgcn_sched_barrier(0);
             uint32_t ok_after = 0;
             if (kt + 2 < t1) ok_after = copy(kt + 2, cur == 0 ? 2 : cur - 1);
             const bool edge = careful || k0 < all_lo || k0 + kTile > all_hi || ok != 3;
@@ -204,7 +223,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                 lds_barrier();
                 odd = odd_tile == kt + 1;
             }
-            const bool seen_here = !(idle || k0 >= w_hi || k0 + kTile <= w_lo);
             half8 ph[2], pl[2];
             uint32_t see = 0xffffffffu;
             if (seen_here) {
@@ -212,27 +230,42 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                 f32x16 s = {};
 #pragma unroll
                 for (int st = 0; st < STEPS; ++st) {
-                    const half8 a = *reinterpret_cast<const half8 *>(kl + nl * R::kRow + 16 * (2 * st + h ^ R::k_swap(nl)));
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[st], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[st], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], s, 0, 0, 0);
+                }
+                // V's fragments arrive while the weights are computed (D = 256 has no registers for them).
+                auto read_values = [&](int dt, int j) __attribute__((always_inline)) {
+                    fp16x4 a[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = 16 * j + 8 * i + vrow;
+                        a[i] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(
+                            vl + row * R::kRow + 16 * (4 * dt + vchunk ^ R::v_swap(row)) + vbyte));
+                    }
+                    return __builtin_bit_cast(half8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                };
+                half8 va[DT][2];
+                if constexpr (D < 256) {
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) va[dt][j] = read_values(dt, j);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 if (k0 < full_lo || k0 + kTile > full_hi || ok != 3) {
                     see = seen(p, seq, range, t, k0, tree);
                     if (!(ok & 1)) see &= 0xffff0000u;
                     if (!(ok & 2)) see &= 0x0000ffffu;
                 }
-                float probe = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) probe += s[j];
-                if (__any(probe != probe)) {               // scores that are NaN, in fp32
-                    const Place<2> x = place<2>(p, R::kRow, b, kvh, seq.n, kt);
+                if (careful) {                             // scores that are NaN, in fp32
                     int dims = D;
                     asm("" : "+s"(dims));                  // a loop that stays one
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const int key = 8 * (j >> 2) + 4 * h + (j & 3);
                         if (s[j] != s[j] && (see >> key & 1)) {
-                            const _Float16 *kr = reinterpret_cast<const _Float16 *>(x.k[j >> 3] + min(key & 15, x.last[j >> 3]) * R::kRow);
+                            const _Float16 *kr = reinterpret_cast<const _Float16 *>(row_of(kt, key, false));
                             float sum = 0.0f;
                             for (int d = 0; d < dims; ++d) sum = fmaf(qrow[d] * p.scale * up, static_cast<float>(kr[d]), sum);
                             s[j] = sum;
@@ -288,21 +321,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        fp16x4 a[2];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int row = 16 * j + 8 * i + vrow;
-                            a[i] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(
-                                vl + row * R::kRow + 16 * (4 * dt + vchunk ^ R::v_swap(row)) + vbyte));
-                        }
-                        const half8 v = __builtin_bit_cast(half8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[j], o[dt], 0, 0, 0);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[j], o[dt], 0, 0, 0);
+                        if constexpr (D == 256) va[dt][j] = read_values(dt, j);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][j], pl[j], o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][j], ph[j], o[dt], 0, 0, 0);
                     }
             }
             if (odd) {
                 // The values that were taken out, times the rows' weights, which go through the tile's LDS.
-                const Place<2> x = place<2>(p, R::kRow, b, kvh, seq.n, kt);
                 float *wt = reinterpret_cast<float *>(kl) + wave * 512;
                 for (int u = 0; u < 2; ++u) {
                     lds_barrier();                         // every wave has left the tile, or the other half's weights
@@ -316,7 +341,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                     asm("" : "+s"(keys));                  // a loop that stays one
                     for (int i = 0; i < keys; ++i) {
                         if (k0 + 16 * u + i >= seq.n || !(ok >> u & 1)) continue;
-                        const char *vr = (u ? x.v[1] : x.v[0]) + i * R::kRow + 8 * h;
+                        const char *vr = row_of(kt, 16 * u + i, true) + 8 * h;
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
