@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_spli
             }
     };
     if (t0 + wave < t1) {
-        places.load(p, S::kRow, b, kvh, seq.n, 0);
+        places.load(p, lane, S::kRow, b, kvh, seq.n, 0);
         here = place(0);
         load_keys(here);
         load_values(here);
@@ -275,7 +275,7 @@ again:
         const int k0 = kt * KT;
         const bool more = kt + kWaves < t1;
         if (more) {
-            if (i + 1 == places.held + 64 / U) places.load(p, S::kRow, b, kvh, seq.n, i + 1);
+            if (i + 1 == places.held + 64 / U) places.load(p, lane, S::kRow, b, kvh, seq.n, i + 1);
             next = place(i + 1);
         }
         // Every row sees every key.
@@ -355,11 +355,11 @@ again:
             }
             const float us = p.soft_cap > 0.0f ? 1.0f : unscale[c];
             mx *= us;
-            // The reference m of a column is raised only when a score exceeds it by more than 2.
-            if (__any(mx > m[c] + 2.0f)) {
+            // The reference m of a column is raised only when a score exceeds it by more than kRaise.
+            if (__any(mx > m[c] + kRaise)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float to = mx > m[c] + 2.0f ? mx : m[c];
+                const float to = mx > m[c] + kRaise ? mx : m[c];
                 const float alpha = to == m[c] ? 1.0f : __builtin_amdgcn_exp2f(m[c] - to);     // 0 while m is -inf
                 l[c] *= alpha;
 #pragma unroll
@@ -472,7 +472,7 @@ again:
                 for (int r = 0; r < 4; ++r) probe = fmaf(o[c][j][r], 0.0f, probe);
         if (__any(probe != probe)) {
             careful = true;
-            places.load(p, S::kRow, b, kvh, seq.n, 0);     // the wave had a tile: its sums are not zeros
+            places.load(p, lane, S::kRow, b, kvh, seq.n, 0);     // the wave had a tile: its sums are not zeros
             here = place(0);
             load_keys(here);
             load_values(here);

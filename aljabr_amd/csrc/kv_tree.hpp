@@ -20,9 +20,12 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRowsBlock = 128;              // rows a workgroup of the rows kernel stacks
 constexpr int kRowsLeast = 4;                // tiles it takes at the least
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights, at most 4, are kept times this: as two fp16 parts they keep what is not below 2^-38 of the row's largest.
+// The reference that weights are relative to is raised only when a score (times log2(e)) exceeds it by more than kRaise:
+// weights are at most 2^kRaise, and are kept times kWeightScale, as two fp16 parts that keep what is not below 2^-36 of the
+// row's largest. (Raised at 2, with weights times 2^13: 2^-38, and a fifth more of the vector work in the rows kernel.)
+constexpr float kRaise = 4.0f;
 template <bool F16>
-constexpr float kWeightScale = F16 ? 8192.0f : 1.0f;
+constexpr float kWeightScale = F16 ? 2048.0f : 1.0f;
 
 struct Params {
     KvView v;
@@ -95,9 +98,8 @@ struct Places {
     int lo, hi;                              // this lane's offset
     uint64_t there;                          // lanes whose group's block exists
 
-    __device__ __forceinline__ void load(const Params &p, int row_bytes, int b, int kvh, int n_keys, int i) {
+    __device__ __forceinline__ void load(const Params &p, int lane, int row_bytes, int b, int kvh, int n_keys, int i) {
         held = i;
-        const int lane = threadIdx.x & 63;
         const long long tile = (first + static_cast<long long>(i + lane / U) * step) * (16 * U), last = n_keys - 1;
         long long key = tile + 16 * (lane % U);              // past the end: the tile's first group again, masked; or any
         if (key > last) key = tile;

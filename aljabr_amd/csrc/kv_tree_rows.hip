@@ -41,14 +41,13 @@ template <int D>
 struct Rows {
     static constexpr int kRow = 2 * D;                     // bytes
     static constexpr int kPlane = kTile * kRow;            // of K's (or V's) tile
-    static constexpr int kBuffer = 2 * kPlane;
-    static constexpr int kBuffers = 3;
+    static constexpr int kValues = 3 * kPlane;             // three tiles of K, then three of V
     static constexpr int CPR = kRow / 16;                  // chunks of a row
     static constexpr int RPL = 64 / CPR;                   // rows of a wave-wide copy
     static constexpr int kCopies = 8 / RPL;                // of a wave's 8 rows of K (and of V)
     static constexpr int kSpan = D == 64 ? 32 : 64, kStride = kSpan + 4;   // dims of a round of the output, and its rows in LDS
     static constexpr int kOut = kWaves * 32 * kStride * 4;
-    static constexpr int kBytes = kBuffers * kBuffer > kOut ? kBuffers * kBuffer : kOut;
+    static constexpr int kBytes = 6 * kPlane > kOut ? 6 * kPlane : kOut;
     __device__ static __forceinline__ int k_swap(int row) { return D == 64 ? row >> 1 & 7 : row & 15; }
     __device__ static __forceinline__ int v_swap(int row) { return D == 64 ? 4 * (row >> 1 & 1) : 4 * (row & 3); }
 };
@@ -65,6 +64,21 @@ __device__ __forceinline__ void wait_copies() {
 
 __device__ __forceinline__ half2v pair(float a, float b) { return half2v{static_cast<_Float16>(a), static_cast<_Float16>(b)}; }
 
+// The larger of x in this lane and in the one 32 lanes away.
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// 16 bytes a lane from base + offset to LDS at dst + 16 * lane (dma16 of device.hpp with a base that the wave shares).
+__device__ __forceinline__ void dma16(const char *base, uint32_t offset, uint32_t dst) {
+    uint32_t save;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save)
+                 : "s"(dst), "v"(offset), "s"(base)
+                 : "memory");
+}
+
 // A dword of two fp16 numbers: bits of those whose exponent is all ones.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7fff7fffu) + 0x04000400u) & 0x80008000u; }
 __device__ __forceinline__ uint32_t clean(uint32_t w) {
@@ -78,9 +92,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
     constexpr int STEPS = D / 16, DT = D / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ Tree tree;
+    __shared__ int4 row_info[kThreads];                    // of a lane's row: t, its range, the power of two it was scaled by
     __shared__ int odd_tile;                               // the last tile that held values which are not finite, plus 1
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, nl = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // For the paths that are rarely taken: the thread's number, of which the compiler keeps nothing in registers.
+    auto fresh_tid = []() __attribute__((always_inline)) {
+        int x = threadIdx.x;
+        asm volatile("" : "+v"(x));
+        return x;
+    };
     int item, w;
     work_of(p, blockIdx.x, item, w);
     const int group = group_of(p, p.by_heads(item)), kvh = item - p.by_heads(item) * p.v.H;
@@ -94,29 +115,44 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
     const int base = seq.n - seq.cnt, r1 = min(r0 + kRowsBlock, seq.cnt * p.G), w0 = r0 + 32 * wave;
     const bool idle = w0 >= r1;                            // a wave without rows only copies
 
-    // This wave copies rows 8 wave .. + 7 of a tile, of its half wave / 2. A lane's chunk and row of each copy:
-    const int own = lane / R::CPR, slot = lane % R::CPR;
     const uint32_t ring = lds_address(lds);
-    uint32_t ok = 0, ok_next = 0;                          // of the tile at hand and the next: halves whose block exists
     Places<2> places{t0, 1};
-    auto copy = [&](int kt, int buffer) __attribute__((always_inline)) {
-        const int i = kt - t0, u = wave >> 1, first = 8 * (wave & 1);
-        if (i == places.held + 32) places.load(p, R::kRow, b, kvh, seq.n, i);
-        const long long at = places.offset(i, u);
-        const int last = last_row(p, kt * kTile + (kt * kTile + 16 * u < seq.n ? 16 * u : 0));
-        const uint32_t dst = ring + buffer * R::kBuffer + (16 * u + first) * R::kRow;
-#pragma unroll
-        for (int j = 0; j < R::kCopies; ++j) {
-            const int row = first + j * R::RPL + own, in = min(row, last) * R::kRow;
-            dma16(p.v.k + at + (in + 16 * (slot ^ R::k_swap(row))), dst + 1024 * j);
-            dma16(p.v.v + at + (in + 16 * (slot ^ R::v_swap(row))), dst + R::kPlane + 1024 * j);
-        }
-        return places.ok(i);
+    // This wave copies rows 8 wave .. + 7 of a tile, of its half wave / 2. A lane's part of the half's rows, copy j:
+    const int u = wave >> 1, first = 8 * (wave & 1);
+    auto share = [&](int lane, int j, int last, bool of_v) __attribute__((always_inline)) {
+        const int row = first + j * R::RPL + lane / R::CPR, slot = lane % R::CPR;
+        return min(row, last) * R::kRow + 16 * (slot ^ (of_v ? R::v_swap(row) : R::k_swap(row)));
     };
+    int k_from[R::kCopies], v_from[R::kCopies];
+#pragma unroll
+    for (int j = 0; j < R::kCopies; ++j) {
+        k_from[j] = share(lane, j, 15, false);
+        v_from[j] = share(lane, j, 15, true);
+    }
+    // Tile i of the chunk's K, or V, into its third of the ring.
+    auto copy = [&](int i, int third, bool of_v) __attribute__((always_inline)) {
+        const int key = (t0 + i) * kTile;
+        if (i == places.held + 32) places.load(p, fresh_tid() & 63, R::kRow, b, kvh, seq.n, i - 16);
+        const char *at = (of_v ? p.v.v : p.v.k) + places.offset(i, u);
+        const int last = last_row(p, key + 16 * u < seq.n ? key + 16 * u : key);
+        const uint32_t dst = ring + (of_v ? R::kValues : 0) + third * R::kPlane + (16 * u + first) * R::kRow;
+        if (last < 15) {                                   // the end of a contiguous plane
+            const int lane = fresh_tid() & 63;
+#pragma unroll
+            for (int j = 0; j < R::kCopies; ++j) dma16(at, share(lane, j, last, of_v), __builtin_amdgcn_readfirstlane(dst + 1024 * j));
+        } else {
+#pragma unroll
+            for (int j = 0; j < R::kCopies; ++j) dma16(at, of_v ? v_from[j] : k_from[j], __builtin_amdgcn_readfirstlane(dst + 1024 * j));
+        }
+    };
+    const int tiles = t1 - t0;
+    // The first tiles: two of K, then a third of K with the first of V.
     auto start = [&]() __attribute__((always_inline)) {
-        places.load(p, R::kRow, b, kvh, seq.n, 0);
-        if (t0 < t1) ok = copy(t0, 0);
-        if (t0 + 1 < t1) ok_next = copy(t0 + 1, 1);
+        places.load(p, fresh_tid() & 63, R::kRow, b, kvh, seq.n, 0);
+        if (tiles > 0) copy(0, 0, false);
+        if (tiles > 1) copy(1, 1, false);
+        if (tiles > 2) copy(2, 2, false);
+        if (tiles > 0) copy(0, 0, true);
     };
     // A tile's rows by hand, for the paths that are rarely taken.
     auto row_of = [&](int kt, int key, bool of_v) __attribute__((always_inline)) {
@@ -135,20 +171,19 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
     if (filled) fill_tree(tree, p.parents + static_cast<long long>(b) * p.T, seq.cnt, p.window);
     else __syncthreads();
 
-    // This lane's row, what it sees; the wave's keys, and those that all rows of the wave and of the workgroup see.
+    // This lane's row, what it sees; the keys that all rows of the wave, and of the workgroup, see.
     const int r = min(w0 + nl, r1 - 1);                    // lanes past the rows repeat the last and are not stored
     const int t = p.by_g(r);
-    const Range range = range_of(p, seq, t, tree, filled);
+    const Range seen_range = range_of(p, seq, t, tree, filled);
     const int t_first = p.by_g(min(w0, r1 - 1)), t_last = p.by_g(min(w0 + 31, r1 - 1));
-    const int w_lo = p.window > 0 ? base + (p.parents ? 0 : t_first) - p.window + 1 : 0, w_hi = base + t_last + 1;
     const int full_lo = p.window > 0 ? base + t_last - p.window + 1 : 0, full_hi = p.parents ? base : base + t_first + 1;
     const int all_lo = p.window > 0 ? base + p.by_g(r1 - 1) - p.window + 1 : 0, all_hi = p.parents ? base : base + p.by_g(r0) + 1;
 
     // The row times scale * log2(e) as two fp16 parts: step s holds dims 16s + 8h .. + 7.
     half8 qh[STEPS], ql[STEPS];
-    float unscale, up;
-    const float *qrow = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
+    float unscale;
     {
+        const float *qrow = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
         float top = 0.0f;
         float4 qa[STEPS], qc[STEPS];
 #pragma unroll
@@ -166,7 +201,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
         int e = 0;
         if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
         e = e < -100 ? -100 : e;
-        up = ldexpf(1.0f, 15 - e);
+        const float up = ldexpf(1.0f, 15 - e);
+        row_info[tid] = make_int4(t, seen_range.lo, seen_range.hi, __float_as_int(up));        // read by this thread alone
         unscale = ldexpf(p.unscale, e - 15);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -183,33 +219,72 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
 
     f32x16 o[DT];
     float m, l;
-    // A lane's share of V's transposed reads: of 16 lanes, row i / 4 and dims 4 (i % 4) .. + 3 of 16.
-    const int vrow = 4 * h + (lane >> 2 & 3), vchunk = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vbyte = 8 * (lane & 1);
+    // A lane's part of K's fragment 0, its row's chunk h, and of V's transposed reads: of 16 lanes, row i / 4 and dims
+    // 4 (i % 4) .. + 3 of 16. Further chunks of the row are an exclusive or away.
+    const int vrow = 4 * h + (lane >> 2 & 3);
+    const int k_part = nl * R::kRow + 16 * (h ^ R::k_swap(nl));
+    const int v_part = vrow * R::kRow + 16 * (2 * (lane >> 4 & 1) + (lane >> 1 & 1) ^ R::v_swap(vrow)) + 8 * (lane & 1);
     for (bool careful = false;; careful = true) {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
-        for (int kt = t0, cur = 0; kt < t1; ++kt, cur = cur == 2 ? 0 : cur + 1) {
-            const int k0 = kt * kTile;
-            if (kt + 1 < t1) wait_copies<2 * R::kCopies>();
-            else wait_copies<0>();
-            lds_barrier();                                 // the tile is there; the buffer after the next is free
-            char *kl = lds + cur * R::kBuffer, *vl = kl + R::kPlane;
-            const bool seen_here = !(idle || k0 >= w_hi || k0 + kTile <= w_lo);
-            half8 ka[STEPS];
+        half8 ka[STEPS];
+        f32x16 s = {};
+        int k_at = 0;
+        auto read_key = [&](int st) __attribute__((always_inline)) { ka[st] = *reinterpret_cast<const half8 *>(lds + (k_at ^ 32 * st)); };
+        auto keys_at = [&](int third) __attribute__((always_inline)) {
+            k_at = third * R::kPlane + k_part;
+            asm("" : "+v"(k_at));                          // one register, not one for each fragment
+        };
+        // S^T: accumulator j is key k0 + 8 (j / 4) + 4h + j % 4 of this lane's row.
+        auto scores = [&]() __attribute__((always_inline)) {
+            f32x16 x = {};
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st) ka[st] = *reinterpret_cast<const half8 *>(kl + nl * R::kRow + 16 * (2 * st + h ^ R::k_swap(nl)));
-            __builtin_amdgcn_sched_barrier(0);
-            uint32_t ok_after = 0;
-            if (kt + 2 < t1) ok_after = copy(kt + 2, cur == 0 ? 2 : cur - 1);
+            for (int st = 0; st < STEPS; ++st) {
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], x, 0, 0, 0);
+            }
+            return x;
+        };
+        if (tiles > 0) {
+            if (tiles > 2) wait_copies<2 * R::kCopies>();
+            else wait_copies<0>();
+            lds_barrier();                                 // the first two tiles of K are there
+            if (!idle) {
+                keys_at(0);
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) read_key(st);
+                s = scores();
+                keys_at(1);
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) read_key(st);
+            }
+            lds_barrier();                                 // every wave has read the first
+            if (tiles > 3) copy(3, 0, false);
+            if (tiles > 1) copy(1, 1, true);
+        }
+        // Tile i: its scores are in s, the next one's K in registers. Behind it lie V of i and K of i + 2, copied two trips
+        // ago, and in flight V of i + 1 and K of i + 3; V of i + 2 and K of i + 4 go where those of i - 1 and i + 1 lay.
+        for (int i = 0, cur = 0; i < tiles; ++i, cur = cur == 2 ? 0 : cur + 1) {
+            const int k0 = (t0 + i) * kTile;
+            if (i + 3 < tiles) wait_copies<2 * R::kCopies>();
+            else if (i + 1 < tiles) wait_copies<R::kCopies>();
+            else wait_copies<0>();
+            lds_barrier();                                 // ... and every wave has left V of i - 1 and K of i + 1
+            const uint32_t ok = places.ok(i);
+            const int before = cur == 0 ? 2 : cur - 1, after = cur == 2 ? 0 : cur + 1;
+            if (i + 4 < tiles) copy(i + 4, after, false);
+            if (i + 2 < tiles) copy(i + 2, before, true);
+            char *vl = lds + R::kValues + cur * R::kPlane;
             const bool edge = careful || k0 < all_lo || k0 + kTile > all_hi || ok != 3;
             bool odd = false;
             if (edge) {
                 bool found = false;
+                const int thread = fresh_tid();
 #pragma unroll
                 for (int j = 0; j < R::kPlane / 4096; ++j) {
-                    const int at = 16 * (tid + kThreads * j), row = at / R::kRow;
+                    const int at = 16 * (thread + kThreads * j), row = at / R::kRow;
                     uint4 x = *reinterpret_cast<const uint4 *>(vl + at);
                     const bool gone = k0 + row >= seq.n || !(ok >> (row >> 4) & 1);
                     const bool bad = not_finite(x.x) | not_finite(x.y) | not_finite(x.z) | not_finite(x.w);
@@ -219,53 +294,45 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                         *reinterpret_cast<uint4 *>(vl + at) = x;
                     }
                 }
-                if (found) odd_tile = kt + 1;
+                if (found) odd_tile = i + 1;
                 lds_barrier();
-                odd = odd_tile == kt + 1;
+                odd = odd_tile == i + 1;
             }
             half8 ph[2], pl[2];
             uint32_t see = 0xffffffffu;
-            if (seen_here) {
-                // S^T: accumulator j is key k0 + 8 (j / 4) + 4h + j % 4 of this lane's row.
-                f32x16 s = {};
+            if (!idle) {
+                int v_at = R::kValues + cur * R::kPlane + v_part;
+                asm("" : "+v"(v_at));
+                auto read_values = [&](int dt, half8 (&v)[2]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st) {
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], ql[st], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[st], qh[st], s, 0, 0, 0);
-                }
-                // V's fragments arrive while the weights are computed (D = 256 has no registers for them).
-                auto read_values = [&](int dt, int j) __attribute__((always_inline)) {
-                    fp16x4 a[2];
+                    for (int j = 0; j < 2; ++j) {
+                        fp16x4 a[2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int row = 16 * j + 8 * i + vrow;
-                        a[i] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(
-                            vl + row * R::kRow + 16 * (4 * dt + vchunk ^ R::v_swap(row)) + vbyte));
+                        for (int c = 0; c < 2; ++c)
+                            a[c] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(
+                                lds + (v_at ^ 64 * dt) + (16 * j + 8 * c) * R::kRow));
+                        v[j] = __builtin_bit_cast(half8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
                     }
-                    return __builtin_bit_cast(half8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
                 };
-                half8 va[DT][2];
-                if constexpr (D < 256) {
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) va[dt][j] = read_values(dt, j);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
                 if (k0 < full_lo || k0 + kTile > full_hi || ok != 3) {
-                    see = seen(p, seq, range, t, k0, tree);
+                    const int4 info = row_info[fresh_tid()];
+                    see = seen(p, seq, Range{info.y, info.z}, info.x, k0, tree);
                     if (!(ok & 1)) see &= 0xffff0000u;
                     if (!(ok & 2)) see &= 0x0000ffffu;
                 }
                 if (careful) {                             // scores that are NaN, in fp32
                     int dims = D;
                     asm("" : "+s"(dims));                  // a loop that stays one
+                    const int thread = fresh_tid(), h = thread >> 5 & 1;
+                    const int4 info = row_info[thread];
+                    const int r = min(w0 + (thread & 31), r1 - 1), t = info.x;
+                    const float *qrow = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
+                    const float up = __int_as_float(info.w);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const int key = 8 * (j >> 2) + 4 * h + (j & 3);
                         if (s[j] != s[j] && (see >> key & 1)) {
-                            const _Float16 *kr = reinterpret_cast<const _Float16 *>(row_of(kt, key, false));
+                            const _Float16 *kr = reinterpret_cast<const _Float16 *>(row_of(t0 + i, key, false));
                             float sum = 0.0f;
                             for (int d = 0; d < dims; ++d) sum = fmaf(qrow[d] * p.scale * up, static_cast<float>(kr[d]), sum);
                             s[j] = sum;
@@ -279,7 +346,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                 }
                 const float us = p.soft_cap > 0.0f ? 1.0f : unscale;
                 if (see != 0xffffffffu) {
-                    const uint32_t mine = see >> (4 * h);
+                    const uint32_t mine = see >> (4 * (fresh_tid() >> 5 & 1));
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (!(mine >> (8 * (j >> 2) + (j & 3)) & 1)) s[j] = -INFINITY;
@@ -288,10 +355,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
 #pragma unroll
                 for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
                 mx *= us;
-                // The reference m of a row is raised only when a score exceeds it by more than 2.
-                if (__any(mx > m + 2.0f)) {
-                    mx = fmaxf(mx, __shfl_xor(mx, 32));
-                    const float to = mx > m + 2.0f ? mx : m;
+                // The reference m of a row is raised only when a score exceeds it by more than kRaise.
+                if (__any(mx > m + kRaise)) {
+                    mx = half_max(mx);
+                    const float to = mx > m + kRaise ? mx : m;
                     const float alpha = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);           // 0 while m is -inf
                     l *= alpha;
 #pragma unroll
@@ -299,6 +366,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                     m = to;
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
+                half8 va[2][2];
+                read_values(0, va[0]);
+                // The next tile's scores on the matrix cores, between them this one's weights.
+                __builtin_amdgcn_sched_barrier(0);
+                const f32x16 after_s = scores();
                 float sum[4] = {};
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -316,50 +388,68 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
                     pl[j >> 2][2 * (j & 3) + 1] = rest[1];
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                // Lane half h supplies contraction entries 0..3 -> key 16j + 4h + e and 4..7 -> key 16j + 8 + 4h + e - 4.
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int j = 0; j < 2 * STEPS; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                 // a product,
+                    __builtin_amdgcn_sched_group_barrier(0x402, 104 / (2 * STEPS), 0); // vector instructions for its 32 cycles
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                s = after_s;
+                // Lane half h supplies contraction entries 0..3 -> key 16j + 4h + e and 4..7 -> key 16j + 8 + 4h + e - 4. Behind
+                // the products go the reads of the next dims and of K of i + 2.
+                keys_at(before);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    if (dt + 1 < DT) read_values(dt + 1, va[(dt + 1) & 1]);
+                    read_key(2 * dt);
+                    read_key(2 * dt + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if constexpr (D == 256) va[dt][j] = read_values(dt, j);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][j], pl[j], o[dt], 0, 0, 0);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][j], ph[j], o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt & 1][j], pl[j], o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt & 1][j], ph[j], o[dt], 0, 0, 0);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             if (odd) {
-                // The values that were taken out, times the rows' weights, which go through the tile's LDS.
-                float *wt = reinterpret_cast<float *>(kl) + wave * 512;
-                for (int u = 0; u < 2; ++u) {
-                    lds_barrier();                         // every wave has left the tile, or the other half's weights
-                    if (!seen_here) continue;
+                // The values that were taken out, times the rows' weights, which go through the tile's LDS, 8 keys at once.
+                float *wt = reinterpret_cast<float *>(vl) + wave * 256;
+                const int thread = fresh_tid(), h = thread >> 5 & 1, nl = thread & 31;
+                for (int q = 0; q < 4; ++q) {
+                    lds_barrier();                         // every wave has left the tile, or the last weights
+                    if (idle) continue;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        wt[(8 * (j >> 2) + 4 * h + (j & 3)) * 32 + nl] =
-                            u ? static_cast<float>(ph[1][j]) + static_cast<float>(pl[1][j]) : static_cast<float>(ph[0][j]) + static_cast<float>(pl[0][j]);
+                    for (int j = 0; j < 4; ++j) {
+                        const float w0 = static_cast<float>(ph[0][j]) + static_cast<float>(pl[0][j]);
+                        const float w1 = static_cast<float>(ph[0][4 + j]) + static_cast<float>(pl[0][4 + j]);
+                        const float w2 = static_cast<float>(ph[1][j]) + static_cast<float>(pl[1][j]);
+                        const float w3 = static_cast<float>(ph[1][4 + j]) + static_cast<float>(pl[1][4 + j]);
+                        wt[(4 * h + j) * 32 + nl] = q & 2 ? (q & 1 ? w3 : w2) : (q & 1 ? w1 : w0);
+                    }
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the wave's own writes
-                    int keys = 16;
+                    int keys = 8;
                     asm("" : "+s"(keys));                  // a loop that stays one
-                    for (int i = 0; i < keys; ++i) {
-                        if (k0 + 16 * u + i >= seq.n || !(ok >> u & 1)) continue;
-                        const char *vr = row_of(kt, 16 * u + i, true) + 8 * h;
+                    for (int c = 0; c < keys; ++c) {
+                        const int key = 8 * q + c;
+                        if (k0 + key >= seq.n || !(ok >> (q >> 1) & 1)) continue;
+                        const char *vr = row_of(t0 + i, key, true) + 8 * h;
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const uint2 v = *reinterpret_cast<const uint2 *>(vr + 64 * dt + 16 * q);
+                            for (int x = 0; x < 4; ++x) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(vr + 64 * dt + 16 * x);
                                 if (!__any((not_finite(v.x) | not_finite(v.y)) != 0)) continue;
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     const float val = f16_bits_to_f32((e < 2 ? v.x : v.y) >> (16 * (e & 1)) & 0xffffu);
-                                    o[dt][4 * q + e] += val - val != 0.0f && (see >> (16 * u + i) & 1) ? wt[i * 32 + nl] * val : 0.0f;
+                                    o[dt][4 * x + e] += val - val != 0.0f && (see >> key & 1) ? wt[c * 32 + nl] * val : 0.0f;
                                 }
                             }
                     }
                 }
                 lds_barrier();
             }
-            ok = ok_next;
-            ok_next = ok_after;
         }
         if (careful) break;
         float probe = 0.0f;
@@ -412,7 +502,7 @@ template <int D>
 void launch(const Params &p, hipStream_t s) {
     using R = Rows<D>;
     const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
-    if (R::kBytes + sizeof(Tree) + 16 > 65536)
+    if (R::kBytes + sizeof(Tree) + kThreads * sizeof(int4) + 16 > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_rows_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
     hipLaunchKernelGGL((kv_rows_kernel<D>), grid, dim3(kThreads), R::kBytes, s, p);
     if (p.quota)                                           // few row groups, so few rows of a sequence

@@ -143,7 +143,7 @@ def attention(cache, q, lens, counts=None, parents=None, window=0, cap=0.0, scal
     The bound: a score is off by at most A (2^-22 + (D + 16) 2^-24), A = scale sum |q||k|: the query's two fp16 parts
     keep 2^-22 of each element, and its products' sum is rounded at most D + 16 times (scaling, chains, the exponent's
     argument); a soft cap adds 4 roundings of a number up to 2 cap. Weights are off by that, by 2^-22 for the exponential
-    and 2^-22 for two fp16 parts, which lose what is below 2^-38 of the largest weight; the sums over n keys by a
+    and 2^-22 for two fp16 parts, which lose what is below 2^-36 of the largest weight (weights, at most 16, times 2^11, next to fp16's 2^-25); the sums over n keys by a
     rounding a key and 64 for their joining. An output is a weighted mean, so all of it is relative to the weighted
     mean of |v|, twice for the denominator."""
     B, T, Hq, D = q.shape
@@ -183,7 +183,7 @@ def attention(cache, q, lens, counts=None, parents=None, window=0, cap=0.0, scal
                     out[b, t, kv * g:(kv + 1) * g] = w @ vv
                     size = np.abs(vv)
                     bound[b, t, kv * g:(kv + 1) * g] = (2 * (w @ size) * (off.max(-1, keepdims=True) + 2.0 ** -21 + (see.sum() + 64) * 2.0 ** -24)
-                                                        + see.sum() * 2.0 ** -38 * size.max(initial=0.0, where=np.isfinite(size)))
+                                                        + see.sum() * 2.0 ** -36 * size.max(initial=0.0, where=np.isfinite(size)))
     return out, bound, live
 
 
