@@ -26,6 +26,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kWeightScale = 8192.0f;      // weights are at most 4
 
 struct Params {
+    static constexpr bool kEvenChunks = false;
     Kv4View v;
     float *out;
     const float *q;
@@ -46,6 +47,8 @@ __device__ __forceinline__ Seq sequence(const Params &p, int b) {
     s.cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
     return s;
 }
+
+__device__ __forceinline__ int item_of(const Params &p, int kvh, int group) { return kvh * p.row_groups + group; }
 
 // Keys [lo, hi) that row t sees.
 __device__ __forceinline__ void key_range(const Params &p, const Seq &s, int t, int &lo, int &hi) {

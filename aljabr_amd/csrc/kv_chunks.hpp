@@ -5,11 +5,15 @@
 //
 // P, a kernel's parameters, has the cache's view v (sequences B, KV heads H),
 // T, G, Hq, row_groups, quota, the dividers by_g, by_chunks and by_items, the
-// partials part_o, part_ml and chunks, and out. Beside P stand
+// partials part_o, part_ml and chunks, and out; kEvenChunks: a sequence's
+// chunks are of one size, instead of its last one taking what is left. Beside P
+// stand
 //   Seq sequence(const P &, int b)
 //   bool row_tiles(const P &, const Seq &, int r0, int rows, int &a, int &z)
-// the latter: the tiles [a, z) that rows [r0, r0 + rows) of a sequence see
-// together; false when it has none of the rows.
+//   int item_of(const P &, int kvh, int group)
+// The second gives the tiles [a, z) that rows [r0, r0 + rows) of a sequence see
+// together; false when it has none of the rows. The third numbers KV heads and
+// row groups for merge_kernel.
 #pragma once
 
 #include "device.hpp"
@@ -61,6 +65,13 @@ struct Chunk {
     Seq seq;
 };
 
+// The size, a multiple of `least`, of `count` chunks of so many tiles. No more than the size that gave the count, so the
+// last one is not empty.
+__device__ __forceinline__ int even_size(int tiles, int count, int least) {
+    const int each = (tiles + count - 1) / count;
+    return (each + least - 1) / least * least;
+}
+
 // Chunk number w; b < 0 past the end. Called by whole waves.
 template <class P>
 __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows, int least) {
@@ -83,6 +94,7 @@ __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows,
         if (i >= c.count) return c;
         c.b = b;
         c.first = p.quota ? 0 : b;
+        if constexpr (P::kEvenChunks) per = even_size(z - a, c.count, least);
         c.t0 = a + i * per;
         c.t1 = min(c.t0 + per, z);
         return c;
@@ -101,7 +113,26 @@ __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows,
     }
     int per = max(p.by_chunks(total + p.quota - 1), least);
     per = (per + least - 1) / least * least;
-    const float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
+    float inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
+    // This lane's chunks, ceil((z - a) / per) and one for a sequence without keys: the estimate is at most one off.
+    auto chunks = [&]() __attribute__((always_inline)) {
+        int n = static_cast<int>(static_cast<float>(z - a) * inv);
+        n += n * per < z - a ? 1 : 0;
+        n -= n > 0 && (n - 1) * per >= z - a ? 1 : 0;
+        n += n * per < z - a ? 1 : 0;
+        return r0 < s.cnt * p.G ? max(n, 1) : 0;
+    };
+    if constexpr (P::kEvenChunks) {
+        // What sequences take beyond the quota for their last chunks makes the chunks larger (up to 64 sequences, twice):
+        // workgroups past what the chip holds at once would run alone.
+        for (int i = 0; i < 2 && last == 0; ++i) {
+            const int all = __builtin_amdgcn_readlane(wave_scan(chunks()), 63);
+            if (all <= p.quota || B > p.quota) break;
+            per = static_cast<int>(static_cast<float>(per) * static_cast<float>(all) * __builtin_amdgcn_rcpf(static_cast<float>(p.quota))) + 1;
+            per = (per + least - 1) / least * least;
+            inv = __builtin_amdgcn_rcpf(static_cast<float>(per));
+        }
+    }
     int before = 0, singles = 0;                           // chunks, and sequences of one, of the groups of 64 before
     for (int b0 = 0; b0 <= last; b0 += 64) {
         if (last) {
@@ -112,12 +143,7 @@ __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows,
                 row_tiles(p, s, r0, rows, a, z);
             }
         }
-        // ceil((z - a) / per): the estimate is at most one off.
-        int n = static_cast<int>(static_cast<float>(z - a) * inv);
-        n += n * per < z - a ? 1 : 0;
-        n -= n > 0 && (n - 1) * per >= z - a ? 1 : 0;
-        n += n * per < z - a ? 1 : 0;
-        n = r0 < s.cnt * p.G ? max(n, 1) : 0;
+        const int n = chunks();
         const int end = before + wave_scan(n);
         const uint64_t single = __ballot(n == 1);
         const uint64_t hit = __ballot(w >= end - n && w < end);
@@ -131,6 +157,7 @@ __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows,
             c.seq.n = __builtin_amdgcn_readlane(s.n, l);
             c.seq.cnt = __builtin_amdgcn_readlane(s.cnt, l);
             c.b = b0 + l;
+            if constexpr (P::kEvenChunks) per = even_size(z - a, c.count, least);
             c.t0 = a + (w - c.first) * per;
             c.t1 = min(c.t0 + per, z);
             return c;
@@ -178,7 +205,7 @@ __global__ __launch_bounds__(256) void merge_kernel(P p) {
     __shared__ float st[SG * (D + 2)];
     const int hq = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
     const int kvh = p.by_g(hq), r = t * p.G + hq - kvh * p.G;
-    const int item = kvh * p.row_groups + r / ROWS;
+    const int item = item_of(p, kvh, r / ROWS);
     const int2 chunk = p.chunks[static_cast<long long>(item) * p.v.B + b];   // written for the rows that exist
     if (t >= sequence(p, b).cnt || chunk.y <= 1) return;   // no row, or its one chunk wrote it
     const int used = chunk.y;

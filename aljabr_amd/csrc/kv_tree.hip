@@ -91,6 +91,14 @@ struct Piece {
     }
 };
 
+// The largest of x in the four lanes of a column.
+__device__ __forceinline__ float group_max(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+
 // The 8 halves of dim e of a piece, of the 8 keys that a lane holds.
 template <int D, int W>
 __device__ __forceinline__ half8 dim_of(const Piece<true, D> (&v)[2][4][W], int x, int e) {
@@ -151,19 +159,21 @@ constexpr bool query_in_lds(int D, int NT) { return NT * D >= 256; }
 
 // grid: chunks of KV heads and row groups (work_of).
 template <bool F16, int D, int NT>
-__global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_split_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Params p) {
     using S = Shape<F16, D>;
     constexpr int U = S::U, KT = S::KT, VE = S::VE, VP = S::VP, KL = S::KL, OT = S::OT, ROWS = 16 * NT, QL = S::kQuery;
     constexpr bool QLDS = query_in_lds(D, NT);
     extern __shared__ float smem[];                        // queries, states on their way, weights of odd tiles
     __shared__ Tree tree;
-    __shared__ float2 query_scale[QLDS ? ROWS : 1];
+    // Of a row: t, what it sees, the power of two it was scaled by (a wave's own copy); and what scales its scores back.
+    __shared__ int4 row_info[kWaves][ROWS];
+    __shared__ float query_scale[QLDS ? ROWS : 1];
     float *work = smem + (QLDS ? NT * QL * 256 : 0);
     const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int item, w;
     work_of(p, blockIdx.x, item, w);
-    const int kvh = p.by_groups(item), r0 = (item - kvh * p.row_groups) * ROWS;
+    const int group = p.by_heads(item), kvh = item - group * p.v.H, r0 = group * ROWS;
     const Chunk chunk = find_chunk(p, w, r0, ROWS, kWaves);
     if (chunk.b < 0) return;
     const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
@@ -176,84 +186,88 @@ __global__ __launch_bounds__(kThreads, NT == 4 || D == 256 ? 1 : 2) void kv_spli
     uint4 kf[U][KL];
     Piece<F16, D> vf[U][4][VP];
     struct Place {
-        const char *k[U], *v[U];
-        int last[U];                                       // the last of the 16 rows that is in the plane
+        long long at[U];                                   // of its groups of 16 keys in the planes
         uint32_t ok;                                       // bit u: the group's block exists
     } here = {}, next = {};
     Places<U> places{t0 + wave, kWaves};
     auto place = [&](int i) __attribute__((always_inline)) {
         Place x;
-        const int key = (t0 + wave + i * kWaves) * KT;
         x.ok = places.ok(i);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long at = places.offset(i, u);
-            x.k[u] = p.v.k + at;
-            x.v[u] = p.v.v + at;
-            x.last[u] = last_row(p, u && key + 16 * u >= seq.n ? key : key + 16 * u);
-        }
+        for (int u = 0; u < U; ++u) x.at[u] = places.offset(i, u);
         return x;
     };
-    auto load_keys = [&](const Place &x) __attribute__((always_inline)) {
+    // The last of the 16 rows of group u of tile kt that is in the plane.
+    auto last_of = [&](int kt, int u) __attribute__((always_inline)) {
+        return last_row(p, kt * KT + (kt * KT + 16 * u < seq.n ? 16 * u : 0));
+    };
+    // Offsets from an address that the wave shares, in 32 bits.
+    auto load_keys = [&](const Place &x, int kt) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const char *at = x.k[u] + (min(n, x.last[u]) * S::kRow + 16 * h);
+            const char *at = p.v.k + x.at[u];
+            const uint32_t off = min(n, last_of(kt, u)) * S::kRow + 16 * h;
 #pragma unroll
-            for (int s = 0; s < KL; ++s) kf[u][s] = *reinterpret_cast<const uint4 *>(at + 64 * s);
+            for (int s = 0; s < KL; ++s) kf[u][s] = *reinterpret_cast<const uint4 *>(at + off + 64 * s);
         }
     };
-    auto load_values = [&](const Place &x) __attribute__((always_inline)) {
+    auto load_values = [&](const Place &x, int kt) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            const char *at = p.v.v + x.at[u];
+            const int last = last_of(kt, u);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const char *at = x.v[u] + (min(4 * h + r, x.last[u]) * S::kRow + n * VE * S::kSize);
+                const uint32_t off = min(4 * h + r, last) * S::kRow + n * VE * S::kSize;
 #pragma unroll
-                for (int c = 0; c < VP; ++c) vf[u][r][c].load(at + c * 16 * VE * S::kSize);
+                for (int c = 0; c < VP; ++c) vf[u][r][c].load(at + off + c * 16 * VE * S::kSize);
             }
+        }
     };
     if (t0 + wave < t1) {
         places.load(p, lane, S::kRow, b, kvh, seq.n, 0);
         here = place(0);
-        load_keys(here);
-        load_values(here);
+        load_keys(here, t0 + wave);
+        load_values(here, t0 + wave);
     }
     const bool filled = p.parents && (p.window > 0 || t1 * KT > base);
     if (filled) fill_tree(tree, p.parents + static_cast<long long>(b) * p.T, seq.cnt, p.window);
 
-    // This lane's columns: row, what it sees, the query times scale * log2(e).
-    Range range[NT];
-    int row_t[NT];
+    // This lane's columns: the query times scale * log2(e), and in LDS what the paths that are rarely taken need of the row.
     uint4 qr[QLDS ? 1 : NT][QL];
-    float unscale[NT], up[NT];
-    const float *qrow[NT];
+    float unscale[NT];
     uint4 *qlds = reinterpret_cast<uint4 *>(smem) + lane;
+    auto row_at = [&](int t, int r) __attribute__((always_inline)) {
+        return p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
+    };
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         const int r = min(r0 + 16 * c + n, r1 - 1);        // columns past the rows repeat the last and are not stored
-        const int t = p.by_g(r), g = r - t * p.G;
-        row_t[c] = t;
-        range[c] = range_of(p, seq, t, tree, filled);
-        qrow[c] = p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D;
+        const int t = p.by_g(r);
+        const Range range = range_of(p, seq, t, tree, filled);
+        row_info[wave][16 * c + n] = make_int4(t, range.lo, range.hi, 0);                      // the same of four lanes
+        if (QLDS && c % kWaves != wave) continue;
+        float up;
         int e;
-        if constexpr (!QLDS) {
-            load_query<F16, D>(qrow[c], p.scale, h, qr[c], up[c], e);
-            unscale[c] = ldexpf(p.unscale, e - 15);
-        } else if (c % kWaves == wave) {
-            load_query<F16, D>(qrow[c], p.scale, h, qr[0], up[c], e);
+        load_query<F16, D>(row_at(t, r), p.scale, h, qr[QLDS ? 0 : c], up, e);
+        unscale[c] = ldexpf(p.unscale, e - 15);
+        if constexpr (QLDS) {
 #pragma unroll
             for (int i = 0; i < QL; ++i) qlds[(c * QL + i) * 64] = qr[0][i];
-            if (lane < 16) query_scale[16 * c + n] = make_float2(ldexpf(p.unscale, e - 15), up[c]);
+            if (lane < 16) query_scale[16 * c + n] = unscale[c];
         }
     }
     if constexpr (QLDS) {
         __syncthreads();
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            unscale[c] = query_scale[16 * c + n].x;
-            up[c] = query_scale[16 * c + n].y;
-        }
+        for (int c = 0; c < NT; ++c) unscale[c] = query_scale[16 * c + n];
     }
+    // For the paths that are rarely taken: the lane's number, of which the compiler keeps nothing in registers.
+    auto fresh_lane = [](int mask) __attribute__((always_inline)) {
+        int x = threadIdx.x;
+        asm volatile("" : "+v"(x));
+        return x & mask;
+    };
     auto query = [&](int c, int i) __attribute__((always_inline)) { return QLDS ? qlds[(c * QL + i) * 64] : qr[QLDS ? 0 : c][i]; };
     // Keys that every row sees: a tree's rows stand at most at their places.
     const int full_lo = p.window > 0 ? base + p.by_g(r1 - 1) - p.window + 1 : 0;
@@ -309,15 +323,15 @@ again:
                     }
                 }
             }
-        if (more) load_keys(next);
+        if (more) load_keys(next, kt + kWaves);
         uint32_t see[NT];
         float pw[NT][U][4];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-            float mx = -INFINITY;
             see[c] = 0xffffffffu;
             if (!whole) {
-                see[c] = seen(p, seq, range[c], row_t[c], k0, tree);
+                const int4 info = row_info[wave][16 * c + fresh_lane(15)];
+                see[c] = seen(p, seq, Range{info.y, info.z}, info.x, k0, tree);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (!(here.ok >> u & 1)) see[c] &= ~(0xffffu << 16 * u);
@@ -325,6 +339,9 @@ again:
 #pragma unroll
             for (int i = 0; i < 4 * U; ++i) pw[c][i >> 2][i & 3] = s[c][i >> 2][i & 3];
             if (F16 && careful) {                          // scores that are NaN, in fp32
+                const int lane = fresh_lane(63), h = lane >> 4, row = min(r0 + 16 * c + (lane & 15), r1 - 1);
+                const float *q = row_at(row_info[wave][16 * c + (lane & 15)].x, row);
+                const float up = p.unscale / unscale[c];   // powers of two
                 float *mine = work + wave * (ROWS * KT) + lane;
 #pragma unroll
                 for (int i = 0; i < 4 * U; ++i) mine[64 * i] = pw[c][i >> 2][i & 3];
@@ -333,32 +350,33 @@ again:
                 for (int i = 0; i < keys; ++i) {
                     const int r = 4 * h + (i & 3);
                     if (mine[64 * i] == mine[64 * i] || !(see[c] >> (16 * (i >> 2) + r) & 1)) continue;
-                    const char *kr = i >= 4 ? here.k[U - 1] + min(r, here.last[U - 1]) * S::kRow : here.k[0] + min(r, here.last[0]) * S::kRow;
+                    const _Float16 *kr = reinterpret_cast<const _Float16 *>(p.v.k + here.at[i >= 4 ? U - 1 : 0] + r * S::kRow);
                     float sum = 0.0f;
-                    for (int d = 0; d < dims; ++d) sum = fmaf(qrow[c][d] * p.scale * up[c], static_cast<float>(reinterpret_cast<const _Float16 *>(kr)[d]), sum);
+                    for (int d = 0; d < dims; ++d) sum = fmaf(q[d] * p.scale * up, static_cast<float>(kr[d]), sum);
                     mine[64 * i] = sum;
                 }
 #pragma unroll
                 for (int i = 0; i < 4 * U; ++i) pw[c][i >> 2][i & 3] = mine[64 * i];
             }
+            if (p.soft_cap > 0.0f) {
+                const float cap = p.soft_cap * kLog2e, in = fminf(unscale[c] / cap, 3e38f);    // finite: 0 stays 0
 #pragma unroll
-            for (int i = 0; i < 4 * U; ++i) {
-                const int u = i >> 2, key = 16 * u + 4 * h + (i & 3);
-                float y = pw[c][u][i & 3];
-                if (p.soft_cap > 0.0f) {
-                    const float cap = p.soft_cap * kLog2e;
-                    y = cap * tanhf(y * fminf(unscale[c] / cap, 3e38f));       // finite: 0 stays 0
-                }
-                if (!(see[c] >> key & 1)) y = -INFINITY;
-                mx = fmaxf(mx, y);
-                pw[c][u][i & 3] = y;
+                for (int i = 0; i < 4 * U; ++i) pw[c][i >> 2][i & 3] = cap * tanhf(pw[c][i >> 2][i & 3] * in);
             }
+            if (!whole) {
+                const uint32_t mine = see[c] >> (4 * (fresh_lane(63) >> 4));
+#pragma unroll
+                for (int i = 0; i < 4 * U; ++i)
+                    if (!(mine >> (16 * (i >> 2) + (i & 3)) & 1)) pw[c][i >> 2][i & 3] = -INFINITY;
+            }
+            float mx = pw[c][0][0];
+#pragma unroll
+            for (int i = 1; i < 4 * U; ++i) mx = fmaxf(mx, pw[c][i >> 2][i & 3]);
             const float us = p.soft_cap > 0.0f ? 1.0f : unscale[c];
             mx *= us;
             // The reference m of a column is raised only when a score exceeds it by more than kRaise.
             if (__any(mx > m[c] + kRaise)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                mx = group_max(mx);
                 const float to = mx > m[c] + kRaise ? mx : m[c];
                 const float alpha = to == m[c] ? 1.0f : __builtin_amdgcn_exp2f(m[c] - to);     // 0 while m is -inf
                 l[c] *= alpha;
@@ -367,14 +385,17 @@ again:
                 m[c] = to;
             }
             const float ref = m[c] == -INFINITY ? 0.0f : m[c];
+            float sum[2] = {};
 #pragma unroll
             for (int i = 0; i < 4 * U; ++i) {
                 float &y = pw[c][i >> 2][i & 3];
                 y = __builtin_amdgcn_exp2f(fmaf(y, us, -ref)) * kWeightScale<F16>;
-                l[c] += y;
+                sum[i & 1] += y;
             }
+            l[c] += sum[0] + sum[1];
         }
         if (!whole) {
+            const int lane = fresh_lane(63), n = lane & 15, h = lane >> 4;
             bool odd = false;
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -396,7 +417,7 @@ again:
                 asm("" : "+s"(keys));                      // a loop that stays one
                 for (int i = 0; i < keys; ++i) {
                     if (k0 + i >= seq.n || !(here.ok >> (i >> 4) & 1)) continue;
-                    const char *vr = (U == 2 && i >= 16 ? here.v[U - 1] : here.v[0]) + (i & 15) * S::kRow;
+                    const char *vr = p.v.v + here.at[U == 2 && i >= 16 ? U - 1 : 0] + (i & 15) * S::kRow;
 #pragma unroll
                     for (int x = 0; x < VP; ++x)
 #pragma unroll
@@ -458,7 +479,7 @@ again:
                                 o[c][x * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pw[c][u][r], o[c][x * VE + e], 0, 0, 0);
                         }
         }
-        if (more) load_values(next);
+        if (more) load_values(next, kt + kWaves);
         here = next;
     }
     if (F16 && !careful) {
@@ -474,8 +495,8 @@ again:
             careful = true;
             places.load(p, lane, S::kRow, b, kvh, seq.n, 0);     // the wave had a tile: its sums are not zeros
             here = place(0);
-            load_keys(here);
-            load_values(here);
+            load_keys(here, t0 + wave);
+            load_values(here, t0 + wave);
             goto again;
         }
     }
@@ -548,8 +569,8 @@ void launch_split(const Params &p, hipStream_t s) {
     using S = Shape<F16, D>;
     constexpr size_t states = 2 * NT * (S::OT * 256 + 128) * 4, weights = kWaves * 16 * NT * S::KT * 4;
     constexpr size_t loop = weights + (query_in_lds(D, NT) ? NT * S::kQuery * 1024 : 0), lds = states > loop ? states : loop;
-    static_assert(lds + sizeof(Tree) + NT * 128 <= 160 * 1024, "LDS of a workgroup");
-    if (lds + sizeof(Tree) + NT * 128 > 65536)
+    static_assert(lds + sizeof(Tree) + NT * 1088 <= 160 * 1024, "LDS of a workgroup");
+    if (lds + sizeof(Tree) + NT * 1088 > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_split_kernel<F16, D, NT>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(lds));
     const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
@@ -560,8 +581,7 @@ void launch_split(const Params &p, hipStream_t s) {
 template <bool F16, int D>
 void launch_d(const Params &p, int rows, hipStream_t s) {
     if (rows == 16) return launch_split<F16, D, 1>(p, s);
-    if (rows == 32) return launch_split<F16, D, 2>(p, s);
-    if constexpr (D < 256) launch_split<F16, D, 4>(p, s);
+    launch_split<F16, D, 2>(p, s);
 }
 
 template <bool F16>
@@ -572,21 +592,26 @@ void launch(const Params &p, int rows, hipStream_t s) {
 }
 
 // How a call's work is laid out: stacked rows of a workgroup, row groups, keys of a tile, and the chunks that the keys
-// are cut into (all sequences together, per KV head and row group): two workgroups a CU.
+// are cut into (all sequences together, per KV head and row group).
 struct Plan {
     int rows, groups, tile, quota;
 };
-Plan make_plan(const KvView &v, int T, int Hq) {
+Plan make_plan(const KvView &v, int T, int Hq, int window) {
     Plan s;
     const long long rows = static_cast<long long>(T) * (Hq / v.H);
-    s.rows = v.f16 && rows > 64 ? kRowsBlock : rows > 32 && v.D < 256 ? 64 : rows > 16 ? 32 : 16;
+    // What the cache may hold of visible keys, in bytes: the lengths themselves are on the device.
+    const long long seen = window > 0 ? std::min<long long>(kv_capacity(v), static_cast<long long>(window) + T) : kv_capacity(v);
+    const double bytes = 2.0 * v.B * seen * v.H * v.D * (v.f16 ? 2 : 4);
+    if (v.f16 && v.D < 256 && rows > 64 && rows * bytes >= 0x1p33) s.rows = kRowsBlock;
+    else if (rows > 32 ? rows * bytes >= 0x1p31 : rows > 16 && bytes >= 0x1p27) s.rows = 32;
+    else s.rows = 16;
     s.tile = v.f16 || v.D == 64 ? 32 : 16;
     s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
     const long long items = static_cast<long long>(v.H) * s.groups;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const int least = s.tile * kWaves;                     // keys of the smallest chunk (kRowsLeast tiles as well)
     const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
-    const int per_cu = s.rows == 64 || (v.D == 256 && s.rows < 64) ? 1 : 2;
+    const int per_cu = s.rows == kRowsBlock || (s.groups == 1 && v.D < 256 && bytes >= 0x1p28) ? 2 : 1;
     s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
     if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
     return s;
@@ -606,7 +631,7 @@ size_t partial_bytes(const KvView &v, const Plan &s, int quota) {
 }  // namespace
 
 size_t kv_tree_attention_scratch_bytes(const KvView &v, int T, int Hq) {
-    const Plan s = make_plan(v, T, Hq);
+    const Plan s = make_plan(v, T, Hq, 0);                 // with a window the partials are fewer
     return s.quota ? partial_bytes(v, s, s.quota) : 0;
 }
 
@@ -632,14 +657,13 @@ int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
     // softmax tells from its neighbours, below 2^-30 all weights are equal.
     p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;
     p.window = std::min(a.window, 1 << 30);                // past every key; positions less it stay in 32 bits
-    const Plan plan = make_plan(v, a.T, a.Hq);
+    const Plan plan = make_plan(v, a.T, a.Hq, p.window);
     if (static_cast<double>(v.H) * plan.groups * (plan.quota + static_cast<double>(v.B)) > 0x7fffff)
         return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv_tree_attention: T = %d rows of %d heads are more than one launch takes", a.T, a.Hq);
     p.row_groups = plan.groups;
     p.quota = plan.quota;
     p.tile_shift = log2_exact(plan.tile);
     p.by_g.set(p.G);
-    p.by_groups.set(plan.groups);
     p.by_rows.set(v.R);
     p.by_items.set(v.H * plan.groups);
     p.by_heads.set(v.H);

@@ -28,12 +28,13 @@ template <bool F16>
 constexpr float kWeightScale = F16 ? 2048.0f : 1.0f;
 
 struct Params {
+    static constexpr bool kEvenChunks = true;
     KvView v;
     float *out;
     const float *q;
     const int *lens, *counts, *parents;
     int T, Hq, G, row_groups;
-    FastDiv by_g, by_groups, by_rows, by_chunks, by_items, by_heads;   // G, row_groups, rows of a block, chunks that vary fastest, H * row_groups, H
+    FastDiv by_g, by_rows, by_chunks, by_items, by_heads;              // G, rows of a block, chunks that vary fastest, H * row_groups, H
     float scale, unscale;                    // their product is the call's scale times log2(e)
     float soft_cap;
     int window;
@@ -49,6 +50,10 @@ __device__ __forceinline__ Seq sequence(const Params &p, int b) {
     s.cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
     return s;
 }
+
+// Heads vary fastest: row groups that read the same keys are H chunks' numbers of workgroups apart, on one XCD (and its
+// L2) wherever that is a multiple of 8.
+__device__ __forceinline__ int item_of(const Params &p, int kvh, int group) { return group * p.v.H + kvh; }
 
 // The tiles that rows [r0, r0 + rows) see together. A row of a tree may stand anywhere between its root and its place,
 // so the window is taken from the root and the last key from the place.
