@@ -15,19 +15,32 @@ from conftest import fresh_thread, scratch_held
 pytestmark = pytest.mark.gpu
 
 F32, F16 = 0, 1
+ROOM = 1 << 28                                              # of a large cache, see Device
 POISON = -77.0
 
 
 class Device:
-    """A host cache's planes on the GPU and the description the calls take."""
+    """A host cache's planes on the GPU and the description the calls take. room: bytes that one layer's rows are to take at
+    the least, in which the host's are the first; attention shares its work out by what a cache has room for."""
 
-    def __init__(self, rocm, host):
+    def __init__(self, rocm, host, room=0):
         put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
         self.host = host
         self.planes = {w: put(host.planes[w]) for w in "kv"}
         self.table = None if host.table is None else put(host.table)
+        rows, per, cap = host.rows, host.per, -(-room // (2 * host.seqs * host.heads * host.d * host.planes["k"].itemsize))
+        if host.page and cap > host.cap:                    # a wider table, without blocks past the host's
+            per = -(-cap // host.page)
+            table = torch.full((host.seqs, per), -1, dtype=torch.int32, device="cuda")
+            table[:, :host.per] = self.table
+            self.table = table
+        elif cap > host.cap:
+            rows = cap
+            for w, x in self.planes.items():
+                self.planes[w] = torch.full((*x.shape[:3], rows, x.shape[4]), float("nan"), dtype=x.dtype, device="cuda")
+                self.planes[w][:, :, :, :host.rows] = x
         self.desc = rocm.KvCache(self.planes["k"].data_ptr(), self.planes["v"].data_ptr(), ptr(self.table), host.dtype, host.layers,
-                                 host.seqs, host.heads, host.d, host.rows, host.s if host.page else 0, host.per if host.page else 0)
+                                 host.seqs, host.heads, host.d, rows, host.s if host.page else 0, per if host.page else 0)
         torch.cuda.synchronize()
 
     def ref(self):
@@ -288,35 +301,38 @@ def test_decode(rocm, d, dtype, hkv, g, page):
     assert g == 3 or not got[3].any()                                 # no key: zeros
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 127, 128, 129, 255, 257, 511, 1000, 2047])
-def test_lengths(rocm, n, dtype):
+def test_lengths(rocm, room, n, dtype):
     host = plain.Cache(1, 2, 128, 2047, 0, dtype)
     host.fill([n], seed=n)
     q = normal(n, 1, 1, 8, 128)
-    check(attend(rocm, Device(rocm, host), q, [n]), *plain.attention(host, q, [n]))
+    check(attend(rocm, Device(rocm, host, room), q, [n]), *plain.attention(host, q, [n]))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("t,hkv,g", [(2, 2, 4), (5, 2, 2), (8, 1, 8), (9, 2, 1), (17, 2, 4), (40, 1, 3), (70, 2, 2)])
+@pytest.mark.parametrize("t,hkv,g", [(2, 2, 4), (5, 2, 2), (8, 1, 8), (9, 2, 1), (17, 2, 4), (26, 2, 1), (40, 1, 3), (70, 2, 2)])
 @pytest.mark.parametrize("window,cap", [(0, 0.0), (20, 0.0), (40, 5.0), (1, 0.0), (-3, 0.0), (2 ** 31 - 1, 0.0)])
 @pytest.mark.parametrize("tree", [0, 1, 2])
-def test_several_rows(rocm, d, dtype, t, hkv, g, window, cap, tree):
+def test_several_rows(rocm, room, d, dtype, t, hkv, g, window, cap, tree):
     lens, counts = [t, 100, 3, 150], [t, max(t - 3, 1), t, 0]         # the third: more rows than keys
     host = plain.Cache(4, hkv, d, 157, 16 if t % 2 else 0, dtype)
     host.fill(lens)
     parents = plain.random_parents(np.random.default_rng(t), 4, t, deep=tree == 2) if tree else None
     q = normal(t, 4, t, hkv * g, d)
-    got = attend(rocm, Device(rocm, host), q, lens, counts, parents, window, cap)
+    got = attend(rocm, Device(rocm, host, room), q, lens, counts, parents, window, cap)
     check(got, *plain.attention(host, q, lens, counts, parents, window, cap))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("t", [31, 32, 33, 64, 65, 128, 200, 255, 256])
 @pytest.mark.parametrize("shape", ["chain", "deep", "star", "forest", "wild"])
 @pytest.mark.parametrize("window", [0, 5, 33])
-def test_trees_of_every_size(rocm, t, shape, window, dtype):
+def test_trees_of_every_size(rocm, room, t, shape, window, dtype):
     rng = np.random.default_rng(t)
     b = 2
     if shape == "wild":                                               # numbers that are no earlier rows stand for none
@@ -331,22 +347,24 @@ def test_trees_of_every_size(rocm, t, shape, window, dtype):
     host = plain.Cache(b, 1, 64, t + 50, 16 if t % 2 else 0, dtype)
     host.fill(lens)
     q = normal(t, b, t, 2, 64)
-    got = attend(rocm, Device(rocm, host), q, lens, counts, parents, window)
+    got = attend(rocm, Device(rocm, host, room), q, lens, counts, parents, window)
     check(got, *plain.attention(host, q, lens, counts, parents, window))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("t", [1, 20])
-def test_scale_and_large_scores(rocm, dtype, t):
+@pytest.mark.parametrize("t", [1, 5, 20])
+def test_scale_and_large_scores(rocm, room, dtype, t):
     host = plain.Cache(1, 2, 128, 304, 0, dtype)
     host.fill([300])
-    dev = Device(rocm, host)
+    dev = Device(rocm, host, room)
     for scale, size in ((0.5, 1.0), (2.0, 30.0), (1e-3, 1e-20), (1e-4, 1e6)):
         q = normal(3, 1, t, 8, 128) * np.float32(size)
         check(attend(rocm, dev, q, [300], scale=scale), *plain.attention(host, q, [300], scale=scale))
 
 
-def test_fp32_values_of_any_size(rocm):
+@pytest.mark.parametrize("room", [0, ROOM])
+def test_fp32_values_of_any_size(rocm, room):
     """What fp16 does not hold: keys of 1e-9 against queries of 1e9, values from 1e-30 to 1e30."""
     host = plain.Cache(1, 2, 128, 90, 0, F32)
     host.fill([90])
@@ -354,20 +372,21 @@ def test_fp32_values_of_any_size(rocm):
     host.planes["v"] *= np.exp(np.random.default_rng(4).uniform(-60, 60, 128)).astype(np.float32)
     for t in (1, 20):
         q = normal(t, 1, t, 8, 128) * np.float32(1e9)
-        check(attend(rocm, Device(rocm, host), q, [90]), *plain.attention(host, q, [90]))
+        check(attend(rocm, Device(rocm, host, room), q, [90]), *plain.attention(host, q, [90]))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("t", [1, 6, 40])
-def test_bad_blocks_hold_no_keys(rocm, d, dtype, t):
+@pytest.mark.parametrize("t", [1, 6, 12, 40])
+def test_bad_blocks_hold_no_keys(rocm, room, d, dtype, t):
     lens = [90, 90, 90, 20]
     host = plain.Cache(4, 2, d, 96, 16, dtype)
     host.fill(lens)
     host.table[0, 2], host.table[1, 0], host.table[1, 5], host.table[3, :] = -1, host.s, 2 ** 31 - 1, -5
-    parents = plain.random_parents(np.random.default_rng(0), 4, t) if t == 6 else None
+    parents = plain.random_parents(np.random.default_rng(0), 4, t) if t in (6, 12) else None
     q = normal(6, 4, t, 8, d)
-    got = attend(rocm, Device(rocm, host), q, lens, None, parents)
+    got = attend(rocm, Device(rocm, host, room), q, lens, None, parents)
     check(got, *plain.attention(host, q, lens, None, parents))
     assert not got[3].any()
 
@@ -380,12 +399,13 @@ def test_lengths_past_the_cache_are_clamped(rocm):
     check(got, *plain.attention(host, q, [37, 0]))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("t,tree", [(4, 0), (40, 0), (4, 1), (40, 1)])
-def test_values_that_are_not_finite_reach_only_rows_that_see_them(rocm, value, which, d, dtype, t, tree):
+@pytest.mark.parametrize("t,tree", [(4, 0), (12, 0), (40, 0), (4, 1), (12, 1), (40, 1)])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(rocm, room, value, which, d, dtype, t, tree):
     """One element of one drafted row's key or value in one head: rows outside its line are as without it, and the others
     as float64 has them (an infinite score takes its row to NaN, or is a weight of zero)."""
     n = 100
@@ -399,7 +419,7 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(rocm, value, w
         x[1, 37] = value
         host.write(which, 0, n - t + row, x)
         want, bound, live = plain.attention(host, q, [n], None, parents)
-        got = attend(rocm, Device(rocm, host), q, [n], None, parents)
+        got = attend(rocm, Device(rocm, host, room), q, [n], None, parents)
         fine = np.isfinite(want)
         assert not fine.all() or which == "k"
         assert np.array_equal(got[~fine], want[~fine].astype(np.float32), equal_nan=True)
@@ -431,9 +451,10 @@ def test_window_leaves_values_behind_that_are_not_finite(rocm, value, dtype, d, 
     check(got[:, 1:], want[0][:, 1:], want[1][:, 1:], np.ones((1, t - 1), bool))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("t", [1, 40])
-def test_infinite_scores(rocm, dtype, t):
+@pytest.mark.parametrize("t", [1, 10, 40])
+def test_infinite_scores(rocm, room, dtype, t):
     """Keys whose score is -inf weigh nothing, rows of such keys alone are zeros; +inf makes NaN."""
     host = plain.Cache(1, 1, 64, 64, 0, dtype)
     host.fill([50])
@@ -443,19 +464,20 @@ def test_infinite_scores(rocm, dtype, t):
     q[..., 5] = -np.abs(q[..., 5])
     want = plain.attention(host, q, [50])
     assert np.isfinite(want[0]).all()
-    check(attend(rocm, Device(rocm, host), q, [50]), *want)
-    assert np.isnan(attend(rocm, Device(rocm, host), -q, [50])).all()
+    check(attend(rocm, Device(rocm, host, room), q, [50]), *want)
+    assert np.isnan(attend(rocm, Device(rocm, host, room), -q, [50])).all()
     host.planes["k"][0, 0, 0, :, 5] = np.inf
-    assert not attend(rocm, Device(rocm, host), q, [50]).any()
+    assert not attend(rocm, Device(rocm, host, room), q, [50]).any()
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("t", [1, 20, 50])
-def test_workspace_of_any_size(rocm, dtype, t):
+def test_workspace_of_any_size(rocm, room, dtype, t):
     host = plain.Cache(2, 2, 128, 1024, 32, dtype)
     lens = [1000, 700]
     host.fill(lens)
-    dev = Device(rocm, host)
+    dev = Device(rocm, host, room)
     q = normal(10, 2, t, 8, 128)
     want = plain.attention(host, q, lens)
     n = ctypes.c_size_t()
@@ -468,10 +490,11 @@ def test_workspace_of_any_size(rocm, dtype, t):
         assert (ws[size:] == 0xCD).all()
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("t,g", [(1, 4), (3, 8), (20, 4)])
 @pytest.mark.parametrize("b,page", [(65, 0), (130, 16)])
 @pytest.mark.parametrize("tree", [0, 1])
-def test_many_uneven_sequences(rocm, b, page, t, g, tree):
+def test_many_uneven_sequences(rocm, room, b, page, t, g, tree):
     """More sequences than a wave has lanes, from no key to all of them, a few of them long."""
     rng = np.random.default_rng(b + t)
     lens = rng.integers(0, 200, b)
@@ -481,36 +504,99 @@ def test_many_uneven_sequences(rocm, b, page, t, g, tree):
     host.fill(lens)
     parents = plain.random_parents(rng, b, t) if tree else None
     q = normal(b, b, t, g, 64)
-    got = attend(rocm, Device(rocm, host), q, lens, counts, parents)
+    got = attend(rocm, Device(rocm, host, room), q, lens, counts, parents)
     check(got, *plain.attention(host, q, lens, counts, parents))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("g", [17, 33, 64, 130])
-def test_one_token_of_many_heads(rocm, d, g):
+def test_one_token_of_many_heads(rocm, room, d, g):
     lens = [500, 31, 0]
     host = plain.Cache(3, 1, d, 512)
     host.fill(lens)
     q = normal(g, 3, 1, g, d)
-    check(attend(rocm, Device(rocm, host), q, lens), *plain.attention(host, q, lens))
+    check(attend(rocm, Device(rocm, host, room), q, lens), *plain.attention(host, q, lens))
 
 
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("t,ctx", [(300, 300), (130, 777)])
-def test_chunks_of_prompts(rocm, d, dtype, t, ctx):
+def test_chunks_of_prompts(rocm, room, d, dtype, t, ctx):
     host = plain.Cache(2, 2, d, ctx, 16, dtype)
     lens, counts = [ctx, ctx - 9], [t, t - 61]
     host.fill(lens)
     q = normal(t, 2, t, 8, d)
     for window in (0, 100):
-        check(attend(rocm, Device(rocm, host), q, lens, counts, window=window), *plain.attention(host, q, lens, counts, window=window))
+        check(attend(rocm, Device(rocm, host, room), q, lens, counts, window=window), *plain.attention(host, q, lens, counts, window=window))
 
 
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, F16), (256, F16), (128, F32)])
+@pytest.mark.parametrize("t,b,g,tree", [(520, 2, 8, 0), (256, 4, 16, 1)])
+def test_windows_of_many_rows(rocm, d, dtype, t, b, g, tree):
+    """Windows that end inside the cached keys, and inside the rows' own, of thousands of rows a KV head."""
+    lens, counts = [1300, 777, 650, 500][:b], [t, t - 71, t, t - 5][:b]
+    host = plain.Cache(b, 2, d, 1310, 16 if tree else 0, dtype)
+    host.fill(lens)
+    parents = plain.random_parents(np.random.default_rng(t), b, t, deep=True) if tree else None
+    q = normal(t, b, t, 2 * g, d)
+    for window in (610, 130):
+        got = attend(rocm, Device(rocm, host, ROOM), q, lens, counts, parents, window)
+        check(got, *plain.attention(host, q, lens, counts, parents, window))
+
+
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("d,t,g", [(128, 1, 4), (64, 6, 4), (256, 12, 4), (64, 40, 4), (128, 64, 4)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_replayed_with_other_lengths(rocm, page, d, t, g, dtype):
+    """A captured call reads lengths, counts and parents of its replay, and gives an eager call's bits."""
+    b, hkv = 3, 2
+    host = plain.Cache(b, hkv, d, 904, page, dtype)
+    host.fill([900] * b)
+    dev, q = Device(rocm, host, ROOM), normal(t, b, t, hkv * g, d)
+    need = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv_tree_attention_workspace", dev.ref(), t, hkv * g, ctypes.byref(need))
+    ws = [torch.empty(max(need.value, 16), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    rng = np.random.default_rng(t)
+    runs = [([900, 40 + t, 333], [t, max(t - 2, 1), t]), ([t, 0, 900], [t, 0, 0]), ([t + 1, 899, 700], [1, t, t])]
+    trees = [plain.random_parents(rng, b, t) for _ in runs]
+    eager = [attend(rocm, dev, q, lens, counts, up, workspace=ws[0]) for (lens, counts), up in zip(runs, trees)]
+    for got, (lens, counts), up in zip(eager, runs, trees):
+        check(got, *plain.attention(host, q, lens, counts, up))
+    qd, out = torch.from_numpy(q).cuda(), torch.empty(q.shape, device="cuda")
+    lens, counts, up = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((b,), (b,), (b, t)))
+    lib, stream = rocm.load(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def body():
+        rocm.call("aljabr_rocm_set_stream", stream.cuda_stream)
+        rocm.call("aljabr_rocm_set_sync_mode", 0)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            out.fill_(POISON)
+            rc = lib.aljabr_rocm_kv_tree_attention(out.data_ptr(), qd.data_ptr(), dev.ref(), 0, lens.data_ptr(), counts.data_ptr(),
+                                                   up.data_ptr(), t, hkv * g, 0.0, 0, 0.0, ws[1].data_ptr(), ws[1].numel())
+        rocm.call("aljabr_rocm_set_stream", None)
+        rocm.call("aljabr_rocm_set_sync_mode", 1)
+        assert rc == 0
+        for i in (0, 1, 2, 0, 2, 1):
+            for dst, src in ((lens, runs[i][0]), (counts, runs[i][1]), (up, trees[i])):
+                dst.copy_(ints(src))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(out.cpu().numpy(), eager[i])
+        return True
+
+    assert fresh_thread(body)
+
+
+@pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("cap", [3.4e38, 1e10, 1e-6, 1e-44])
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("t", [1, 40])
-def test_soft_caps_of_any_size(rocm, cap, dtype, t):
+@pytest.mark.parametrize("t", [1, 10, 40])
+def test_soft_caps_of_any_size(rocm, room, cap, dtype, t):
     """A cap far past the scores is none (4 roundings of each score for its products and tanh more than the bound without
     one); under one next to zero every key weighs the same to 2e-6."""
     host = plain.Cache(2, 1, 128, 208, 0, dtype)
@@ -521,13 +607,14 @@ def test_soft_caps_of_any_size(rocm, cap, dtype, t):
     v = np.abs(host.rows_of("v", 0, 200)[0]).max()
     top = (np.abs(k) @ np.abs(q[0].reshape(-1, 128).T)).max() * 128 ** -0.5
     more = 2 * v * 4 * top * 2.0 ** -24 if cap > 1 else 2 * 2 * 1e-6 * v
-    check(attend(rocm, Device(rocm, host), q, [200, 9], cap=cap), want, bound + more, live)
+    check(attend(rocm, Device(rocm, host, room), q, [200, 9], cap=cap), want, bound + more, live)
 
 
-@pytest.mark.parametrize("d,t", [(64, 1), (128, 5), (256, 1), (128, 40), (256, 40)])
+@pytest.mark.parametrize("room", [0, ROOM])
+@pytest.mark.parametrize("d,t", [(64, 1), (128, 5), (256, 1), (128, 40), (256, 40), (64, 12)])
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("scale,size", [(3.4e38, 1e-39), (2.5e38, 1e-38), (1e-38, 2e37), (2e-39, 1e38), (1e30, 1e-31)])
-def test_scales_at_the_ends_of_fp32(rocm, d, t, dtype, scale, size):
+def test_scales_at_the_ends_of_fp32(rocm, room, d, t, dtype, scale, size):
     """Queries and scales whose product alone is in range."""
     host = plain.Cache(1, 1, d, 208, 0, dtype)
     host.fill([200])
@@ -535,16 +622,17 @@ def test_scales_at_the_ends_of_fp32(rocm, d, t, dtype, scale, size):
         q = normal(t, 1, t, 4, d) * np.float32(size)
     scale = float(np.float32(scale))
     want, bound, live = plain.attention(host, q, [200], scale=scale)
-    got = attend(rocm, Device(rocm, host), q, [200], scale=scale)
+    got = attend(rocm, Device(rocm, host, room), q, [200], scale=scale)
     past = ~np.isfinite(q).all(-1)                                     # at 1e38 some element is infinite: its row is NaN
     assert np.isnan(got[past]).all() and np.isnan(want[past]).all()
     check(*(np.where(past[..., None], 0.0, x) for x in (got, want, bound)), live)
 
 
-def test_same_call_same_bits(rocm):
+@pytest.mark.parametrize("room", [0, ROOM])
+def test_same_call_same_bits(rocm, room):
     host = plain.Cache(2, 4, 128, 1024)
     host.fill([1024, 513])
-    dev = Device(rocm, host)
+    dev = Device(rocm, host, room)
     for t in (1, 30):
         q, parents = normal(11, 2, t, 16, 128), plain.random_parents(np.random.default_rng(1), 2, t)
         first = attend(rocm, dev, q, [1024, 513], None, parents)
