@@ -575,7 +575,7 @@ void launch_split(const Params &p, hipStream_t s) {
                                   static_cast<int>(lds));
     const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
     hipLaunchKernelGGL((kv_split_kernel<F16, D, NT>), grid, dim3(kThreads), lds, s, p);
-    if (p.quota) hipLaunchKernelGGL((merge_kernel<Params, D, 16 * NT>), dim3(p.Hq, p.T, p.v.B), dim3(256), 0, s, p);
+    if (p.quota) launch_merge<D, 16 * NT>(p, kWaves << p.tile_shift, s);
 }
 
 template <bool F16, int D>
@@ -613,7 +613,8 @@ Plan make_plan(const KvView &v, int T, int Hq, int window) {
     const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
     const int per_cu = s.rows == kRowsBlock || (s.groups == 1 && v.D < 256 && bytes >= 0x1p28) ? 2 : 1;
     s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
-    if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
+    // Heads and row groups fill the chip, no sequence is cut, or there are more than the merge's grid takes.
+    if (s.quota <= 1 || most == 1 || v.B > 65535) s.quota = 0;
     return s;
 }
 

@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t clean(uint32_t w) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
     using R = Rows<D>;
     constexpr int STEPS = D / 16, DT = D / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -105,6 +105,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_rows_kernel(Par
     int item, w;
     work_of(p, blockIdx.x, item, w);
     const int group = group_of(p, p.by_heads(item)), kvh = item - p.by_heads(item) * p.v.H;
+    item = item_of(p, kvh, group);
     const int r0 = group * kRowsBlock;
     const Chunk chunk = find_chunk(p, w, r0, kRowsBlock, kRowsLeast);
     if (chunk.b < 0) return;
@@ -505,16 +506,13 @@ void launch(const Params &p, hipStream_t s) {
     if (R::kBytes + sizeof(Tree) + kThreads * sizeof(int4) + 16 > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_rows_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
     hipLaunchKernelGGL((kv_rows_kernel<D>), grid, dim3(kThreads), R::kBytes, s, p);
-    if (p.quota)                                           // few row groups, so few rows of a sequence
-        hipLaunchKernelGGL((merge_rows_kernel<Params, D, kRowsBlock>), dim3((p.T * p.Hq + 3) / 4, p.v.B), dim3(256), 0, s, p);
+    if (p.quota) launch_merge<D, kRowsBlock>(p, kRowsLeast * kTile, s);
 }
 
 }  // namespace
 
 void kvt::launch_rows(const Params &p, hipStream_t s) {
-    if (p.v.D == 64) launch<64>(p, s);
-    else if (p.v.D == 128) launch<128>(p, s);
-    else launch<256>(p, s);
+    p.v.D == 64 ? launch<64>(p, s) : launch<128>(p, s);
 }
 
 }  // namespace aljabr
