@@ -201,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void kv_tree_accept_kernel(AcceptParams p
     __syncthreads();
     if (i > 0 && i < cnt && (!agrees || first[up] != i)) atomicOr(&disagree[i >> 5], 1u << (i & 31));
     if (p.parents) {
-        fill_tree(tree, p.parents + row0, cnt, 0);
+        fill_tree(tree, up, cnt, 0);
     } else {
         tree.depth[i] = i;
 #pragma unroll

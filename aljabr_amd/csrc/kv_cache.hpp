@@ -53,23 +53,20 @@ struct Tree {
     int depth[kTreeMost];
 };
 
-// Fills the tree of rows [0, n), n <= kTreeMost, from their parents (a number that is not an earlier row's stands for
-// none). With a window > 0, of a row's line only its last `window` rows are kept in mask. By a workgroup of kTreeMost
+// Fills the tree of rows [0, n), n <= kTreeMost, from the parent of each thread's row (a number that is not an earlier
+// row's stands for none). With a window > 0, of a row's line only its last `window` rows are kept in mask. By a workgroup of kTreeMost
 // threads, which it leaves in step.
 //
 // After step s a row knows the 2^(s+1) last rows of its line and the row before them: log2(n) steps whatever the depth,
 // each a row's masks joined with those of the row where its own end. A window is taken in parts of powers of two: the
 // steps whose bit it has, each from where the one before ended.
-__device__ __forceinline__ void fill_tree(Tree &t, const int *parents, int n, int window) {
+__device__ __forceinline__ void fill_tree(Tree &t, int parent, int n, int window) {
     const int i = threadIdx.x, words = (n + 31) >> 5;
     const bool mine = i < n;
     const int limit = window > 0 && window < n ? window : 0;
     int jump = -1, cur = mine ? i : -1;
     uint32_t own[kTreeWords], part[kTreeWords];
-    if (mine) {
-        const int p = parents[i];
-        jump = p >= 0 && p < i ? p : -1;
-    }
+    if (mine && parent >= 0 && parent < i) jump = parent;
 #pragma unroll
     for (int w = 0; w < kTreeWords; ++w) {
         own[w] = i >> 5 == w && mine ? 1u << (i & 31) : 0;

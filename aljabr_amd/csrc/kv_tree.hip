@@ -110,49 +110,48 @@ __device__ __forceinline__ half8 dim_of(const Piece<true, D> (&v)[2][4][W], int 
     return __builtin_bit_cast(half8, make_uint4(f[0], f[1], f[2], f[3]));
 }
 
-// A row's query as a lane's pieces: fp16 the two parts of each step, fp32 as it is. up: the power of two it was scaled by.
+// What a lane loads of a row's query: of fp16's steps dims 32s + 8h .. + 7, of fp32's 16s + 4h .. + 3.
 template <bool F16, int D>
-__device__ __forceinline__ void load_query(const float *row, float scale, int h, uint4 (&q)[Shape<F16, D>::kQuery], float &up, int &e) {
-    up = 1.0f;
-    e = 15;
-    if constexpr (F16) {
-        constexpr int STEPS = D / 32;
-        float4 x[STEPS][2];
-        float top = 0.0f;
+struct Query {
+    float4 x[D / 16];
+    __device__ __forceinline__ void load(const float *row, int h) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
+        for (int i = 0; i < D / 16; ++i) x[i] = *reinterpret_cast<const float4 *>(row + (F16 ? 32 * (i >> 1) + 8 * h + 4 * (i & 1) : 16 * i + 4 * h));
+    }
+    // The pieces that enter products: fp16 the two parts of each step, fp32 as it is, times scale. It was scaled by 2^(15 - e).
+    __device__ __forceinline__ void pieces(float scale, uint4 (&q)[Shape<F16, D>::kQuery], int &e) const {
+        e = 15;
+        if constexpr (F16) {
+            float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                x[s][i] = *reinterpret_cast<const float4 *>(row + 32 * s + 8 * h + 4 * i);
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[s][i].x), fabsf(x[s][i].y)), fmaxf(fabsf(x[s][i].z), fabsf(x[s][i].w))));
+            for (int i = 0; i < D / 16; ++i) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            top = group_max(top) * scale;
+            e = 0;
+            if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
+            e = e < -100 ? -100 : e;
+            const float up = ldexpf(1.0f, 15 - e);
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+                const float4 a = x[2 * s], c = x[2 * s + 1];
+                const float y[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+                half8 first, rest;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float z = y[i] * scale * up;
+                    first[i] = static_cast<_Float16>(z);
+                    rest[i] = static_cast<_Float16>(z - static_cast<float>(first[i]));
+                }
+                q[2 * s] = __builtin_bit_cast(uint4, first);
+                q[2 * s + 1] = __builtin_bit_cast(uint4, rest);
             }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-        e = 0;
-        if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);         // top in [2^(e-1), 2^e)
-        e = e < -100 ? -100 : e;
-        up = ldexpf(1.0f, 15 - e);
+        } else {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const float y[8] = {x[s][0].x, x[s][0].y, x[s][0].z, x[s][0].w, x[s][1].x, x[s][1].y, x[s][1].z, x[s][1].w};
-            half8 first, rest;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float z = y[i] * scale * up;
-                first[i] = static_cast<_Float16>(z);
-                rest[i] = static_cast<_Float16>(z - static_cast<float>(first[i]));
-            }
-            q[2 * s] = __builtin_bit_cast(uint4, first);
-            q[2 * s + 1] = __builtin_bit_cast(uint4, rest);
-        }
-    } else {
-#pragma unroll
-        for (int s = 0; s < Shape<F16, D>::KL; ++s) {
-            const float4 x = *reinterpret_cast<const float4 *>(row + 16 * s + 4 * h);
-            q[s] = make_uint4(__float_as_uint(x.x * scale), __float_as_uint(x.y * scale), __float_as_uint(x.z * scale), __float_as_uint(x.w * scale));
+            for (int s = 0; s < D / 16; ++s)
+                q[s] = make_uint4(__float_as_uint(x[s].x * scale), __float_as_uint(x[s].y * scale), __float_as_uint(x[s].z * scale),
+                                  __float_as_uint(x[s].w * scale));
         }
     }
-}
+};
 
 // Whether the queries are kept in LDS: in registers they would be D / 4 of each column tile.
 constexpr bool query_in_lds(int D, int NT) { return NT * D >= 256; }
@@ -182,14 +181,29 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
     const Seq seq = chunk.seq;
     const int base = seq.n - seq.cnt, r1 = min(r0 + ROWS, seq.cnt * p.G);
 
-    // The first tile goes out before anything else is read.
+    // The first tile's places, the tree's parents, the queries and then the tile: all on their way before any is used.
+    const int tile0 = t0 < t1 ? min(t0 + wave, t1 - 1) : 0;            // a wave without a tile loads one that is there
+    Places<U> places{tile0, kWaves};
+    const auto entry = places.fetch(p, lane, b, seq.n, 0);
+    const bool filled = p.parents && (p.window > 0 || t1 * KT > base);
+    int parent = -1;
+    if (filled && static_cast<int>(threadIdx.x) < seq.cnt) parent = p.parents[static_cast<long long>(b) * p.T + threadIdx.x];
+    auto row_at = [&](int t, int r) __attribute__((always_inline)) {
+        return p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
+    };
+    Query<F16, D> raw[QLDS ? 1 : NT];
+    static_assert(!QLDS || NT <= kWaves, "a wave loads one column tile's queries");
+#pragma unroll
+    for (int c = 0; c < (QLDS ? 1 : NT); ++c) {
+        const int r = min(r0 + 16 * (QLDS ? wave : c) + n, r1 - 1);    // columns past the rows repeat the last and are not stored
+        if (!QLDS || wave < NT) raw[c].load(row_at(p.by_g(r), r), h);
+    }
     uint4 kf[U][KL];
     Piece<F16, D> vf[U][4][VP];
     struct Place {
         long long at[U];                                   // of its groups of 16 keys in the planes
         uint32_t ok;                                       // bit u: the group's block exists
     } here = {}, next = {};
-    Places<U> places{t0 + wave, kWaves};
     auto place = [&](int i) __attribute__((always_inline)) {
         Place x;
         x.ok = places.ok(i);
@@ -224,32 +238,26 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
             }
         }
     };
-    if (t0 + wave < t1) {
-        places.load(p, lane, S::kRow, b, kvh, seq.n, 0);
-        here = place(0);
-        load_keys(here, t0 + wave);
-        load_values(here, t0 + wave);
-    }
-    const bool filled = p.parents && (p.window > 0 || t1 * KT > base);
-    if (filled) fill_tree(tree, p.parents + static_cast<long long>(b) * p.T, seq.cnt, p.window);
+    // By every wave, also one without a tile: loads that only some paths make would all be waited for before the first of
+    // the others is used.
+    places.hold(p, entry, S::kRow, kvh, 0);
+    here = place(0);
+    load_keys(here, tile0);
+    load_values(here, tile0);
+    if (filled) fill_tree(tree, parent, seq.cnt, p.window);
 
     // This lane's columns: the query times scale * log2(e), and in LDS what the paths that are rarely taken need of the row.
     uint4 qr[QLDS ? 1 : NT][QL];
     float unscale[NT];
     uint4 *qlds = reinterpret_cast<uint4 *>(smem) + lane;
-    auto row_at = [&](int t, int r) __attribute__((always_inline)) {
-        return p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
-    };
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
-        const int r = min(r0 + 16 * c + n, r1 - 1);        // columns past the rows repeat the last and are not stored
-        const int t = p.by_g(r);
+        const int t = p.by_g(min(r0 + 16 * c + n, r1 - 1));
         const Range range = range_of(p, seq, t, tree, filled);
         row_info[wave][16 * c + n] = make_int4(t, range.lo, range.hi, 0);                      // the same of four lanes
-        if (QLDS && c % kWaves != wave) continue;
-        float up;
+        if (QLDS && c != wave) continue;
         int e;
-        load_query<F16, D>(row_at(t, r), p.scale, h, qr[QLDS ? 0 : c], up, e);
+        raw[QLDS ? 0 : c].pieces(p.scale, qr[QLDS ? 0 : c], e);
         unscale[c] = ldexpf(p.unscale, e - 15);
         if constexpr (QLDS) {
 #pragma unroll

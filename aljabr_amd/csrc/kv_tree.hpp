@@ -105,25 +105,33 @@ struct Places {
     int lo, hi;                              // this lane's offset
     uint64_t there;                          // lanes whose group's block exists
 
-    __device__ __forceinline__ void load(const Params &p, int lane, int row_bytes, int b, int kvh, int n_keys, int i) {
-        held = i;
+    // What the table says of this lane's group, from the wave's i-th tile on: the block, or the sequence without a table.
+    struct Entry {
+        int s, row;
+    };
+    __device__ __forceinline__ Entry fetch(const Params &p, int lane, int b, int n_keys, int i) const {
         const long long tile = (first + static_cast<long long>(i + lane / U) * step) * (16 * U), last = n_keys - 1;
         long long key = tile + 16 * (lane % U);              // past the end: the tile's first group again, masked; or any
         if (key > last) key = tile;
         if (key > last) key = max(last, 0LL) & ~15;
-        int s = b, row = static_cast<int>(key);
-        bool ok = true;
+        Entry x{b, static_cast<int>(key)};
         if (p.v.table) {
-            const int blk = p.by_rows(row);
-            s = p.v.table[static_cast<long long>(b) * p.v.max_blocks + blk];
-            row -= blk * p.v.R;
-            ok = s >= 0 && s < p.v.num_blocks;
-            if (!ok) s = 0;
+            const int blk = p.by_rows(x.row);
+            x.s = p.v.table[static_cast<long long>(b) * p.v.max_blocks + blk];
+            x.row -= blk * p.v.R;
         }
-        const long long at = ((static_cast<long long>(s) * p.v.H + kvh) * p.v.R + row) * row_bytes;
+        return x;
+    }
+    __device__ __forceinline__ void hold(const Params &p, Entry x, int row_bytes, int kvh, int i) {
+        held = i;
+        const bool ok = !p.v.table || (x.s >= 0 && x.s < p.v.num_blocks);
+        const long long at = ((static_cast<long long>(ok ? x.s : 0) * p.v.H + kvh) * p.v.R + x.row) * row_bytes;
         lo = static_cast<int>(at);
         hi = static_cast<int>(at >> 32);
         there = __ballot(ok);
+    }
+    __device__ __forceinline__ void load(const Params &p, int lane, int row_bytes, int b, int kvh, int n_keys, int i) {
+        hold(p, fetch(p, lane, b, n_keys, i), row_bytes, kvh, i);
     }
     // Group u of the wave's i-th tile.
     __device__ __forceinline__ long long offset(int i, int u) const {

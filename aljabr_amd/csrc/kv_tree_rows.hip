@@ -166,10 +166,10 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
         }
         return (of_v ? p.v.v : p.v.k) + ((static_cast<long long>(s) * p.v.H + kvh) * p.v.R + at) * R::kRow;
     };
-    start();
     const bool filled = p.parents && (p.window > 0 || t1 * kTile > base);
+    start();
     if (tid == 0) odd_tile = 0;
-    if (filled) fill_tree(tree, p.parents + static_cast<long long>(b) * p.T, seq.cnt, p.window);
+    if (filled) fill_tree(tree, tid < seq.cnt ? p.parents[static_cast<long long>(b) * p.T + tid] : -1, seq.cnt, p.window);
     else __syncthreads();
 
     // This lane's row, what it sees; the keys that all rows of the wave, and of the workgroup, see.
