@@ -34,8 +34,7 @@ static_assert(kThreads == kTreeMost, "fill_tree takes a thread a row");
 struct AppendParams {
     KvView v;
     KvAppend a;
-    int per_token;           // lane groups that share a token's heads
-    kv::FastDiv by_token;
+    kv::FastDiv by_heads;    // Hq + 2 H, a token's rows
     double quarter;          // 2 / pi
     double step;             // log2(base) * -2 / rot
 };
@@ -110,59 +109,54 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendParams p) {
     const KvAppend &a = p.a;
     const int b = blockIdx.y, l = threadIdx.x % LPR;
     const int group = blockIdx.x * GPB + threadIdx.x / LPR;      // below 2^29
-    const int t = p.by_token(group), h0 = group - t * p.per_token;
+    const int heads = a.Hq + 2 * p.v.H, t = p.by_heads(group), h = group - t * heads;
     if (t >= (a.counts ? min(a.counts[b], a.T) : a.T)) return;
-    const long long pos = static_cast<long long>(a.positions[b]) + t;
-    int s = 0, row = 0;
-    const bool there = kv_locate(p.v, b, pos, s, row);
-    const int heads = a.Hq + 2 * p.v.H;
+    const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + p.v.H;
+    const void *src = is_q ? a.q : is_k ? a.k : a.v;
+    if (!src) return;
+    const int kv = is_q ? h : is_k ? h - a.Hq : h - a.Hq - p.v.H;
 
     // This lane's two units: of the rotated part l and its partner half a part on, behind it two neighbours.
     const int rot = a.rot, pairs = rot / 8;
     const bool turned = l < pairs;
     const int u0 = turned ? 4 * l : rot + 8 * (l - pairs), u1 = turned ? u0 + rot / 2 : u0 + 4;
-    float c[4], sn[4];
-    if (turned) {
-        const double at = static_cast<double>(a.angles ? a.angles[static_cast<long long>(b) * a.T + t] : pos) * p.quarter;
+    const long long at = is_q ? b * a.q_sb + t * a.q_st + h * a.q_sh : b * a.kv_sb + t * a.kv_st + kv * a.kv_sh;
+    float4 x = load_row4<WIDE>(src, at + u0, a.f16), y = load_row4<WIDE>(src, at + u1, a.f16);
+    const long long pos = static_cast<long long>(a.positions[b]) + t;
+    int s = 0, row = 0;
+    if (!is_q && !kv_locate(p.v, b, pos, s, row)) return;
+    if (turned && (is_q || is_k)) {
+        const double quarters = static_cast<double>(a.angles ? a.angles[static_cast<long long>(b) * a.T + t] : pos) * p.quarter;
         // Pairs 4l .. 4l + 3, or interleaved 2l, 2l + 1 and the same a quarter of the part on.
         const int first = a.interleaved ? 2 * l : 4 * l, skip = a.interleaved ? rot / 4 - 2 : 0;
+        float c[4], sn[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int i = first + j + (j >= 2 ? skip : 0);
             double f = exp2(p.step * i);
             if (a.divisors && a.divisors[i] > 0.0f) f /= static_cast<double>(a.divisors[i]);
-            cos_sin(at * f, c[j], sn[j]);
+            cos_sin(quarters * f, c[j], sn[j]);
+        }
+        if (a.interleaved) {
+            turn(x.x, x.y, c[0], sn[0]);
+            turn(x.z, x.w, c[1], sn[1]);
+            turn(y.x, y.y, c[2], sn[2]);
+            turn(y.z, y.w, c[3], sn[3]);
+        } else {
+            turn(x.x, y.x, c[0], sn[0]);
+            turn(x.y, y.y, c[1], sn[1]);
+            turn(x.z, y.z, c[2], sn[2]);
+            turn(x.w, y.w, c[3], sn[3]);
         }
     }
-    for (int h = h0; h < heads; h += p.per_token) {
-        const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + p.v.H;
-        const void *src = is_q ? a.q : is_k ? a.k : a.v;
-        if (!src || (!is_q && !there)) continue;
-        const int kv = is_q ? h : is_k ? h - a.Hq : h - a.Hq - p.v.H;
-        const long long at = is_q ? b * a.q_sb + t * a.q_st + h * a.q_sh : b * a.kv_sb + t * a.kv_st + kv * a.kv_sh;
-        float4 x = load_row4<WIDE>(src, at + u0, a.f16), y = load_row4<WIDE>(src, at + u1, a.f16);
-        if (turned && (is_q || is_k)) {
-            if (a.interleaved) {
-                turn(x.x, x.y, c[0], sn[0]);
-                turn(x.z, x.w, c[1], sn[1]);
-                turn(y.x, y.y, c[2], sn[2]);
-                turn(y.z, y.w, c[3], sn[3]);
-            } else {
-                turn(x.x, y.x, c[0], sn[0]);
-                turn(x.y, y.y, c[1], sn[1]);
-                turn(x.z, y.z, c[2], sn[2]);
-                turn(x.w, y.w, c[3], sn[3]);
-            }
-        }
-        if (is_q) {
-            float *dst = a.q_out + ((static_cast<long long>(b) * a.T + t) * a.Hq + h) * D;
-            *reinterpret_cast<float4 *>(dst + u0) = x;
-            *reinterpret_cast<float4 *>(dst + u1) = y;
-        } else {
-            const long long to = ((static_cast<long long>(s) * p.v.H + kv) * p.v.R + row) * D;
-            store_row4(is_k ? p.v.k : p.v.v, to + u0, x, p.v.f16);
-            store_row4(is_k ? p.v.k : p.v.v, to + u1, y, p.v.f16);
-        }
+    if (is_q) {
+        float *dst = a.q_out + ((static_cast<long long>(b) * a.T + t) * a.Hq + h) * D;
+        *reinterpret_cast<float4 *>(dst + u0) = x;
+        *reinterpret_cast<float4 *>(dst + u1) = y;
+    } else {
+        const long long to = ((static_cast<long long>(s) * p.v.H + kv) * p.v.R + row) * D;
+        store_row4(is_k ? p.v.k : p.v.v, to + u0, x, p.v.f16);
+        store_row4(is_k ? p.v.k : p.v.v, to + u1, y, p.v.f16);
     }
 }
 
@@ -327,15 +321,14 @@ int enqueue_kv_append(const KvView &v, const KvAppend &a) {
     p.v = v;
     p.a = a;
     const int heads = a.Hq + 2 * v.H;
-    p.per_token = heads;
-    p.by_token.set(p.per_token);
+    p.by_heads.set(heads);
     p.quarter = 2.0 / 3.14159265358979323846;
     p.step = a.rot ? std::log2(a.base) * -2.0 / a.rot : 0.0;
     const size_t unit = a.f16 ? 8 : 16;
     const bool wide = aligned(a.q, unit) && aligned(a.k, unit) && aligned(a.v, unit) && a.q_sb % 4 == 0 && a.q_st % 4 == 0 &&
                       a.q_sh % 4 == 0 && a.kv_sb % 4 == 0 && a.kv_st % 4 == 0 && a.kv_sh % 4 == 0;
     const int gpb = kThreads / (v.D / 8);
-    const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * p.per_token + gpb - 1) / gpb), v.B);
+    const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * heads + gpb - 1) / gpb), v.B);
     if (v.D == 64) launch_append<64>(p, wide, grid);
     else if (v.D == 128) launch_append<128>(p, wide, grid);
     else launch_append<256>(p, wide, grid);

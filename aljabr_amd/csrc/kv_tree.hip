@@ -621,8 +621,7 @@ Plan make_plan(const KvView &v, int T, int Hq, int window) {
     const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
     const int per_cu = s.rows == kRowsBlock || (s.groups == 1 && v.D < 256 && bytes >= 0x1p28) ? 2 : 1;
     s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
-    // Heads and row groups fill the chip, no sequence is cut, or there are more than the merge's grid takes.
-    if (s.quota <= 1 || most == 1 || v.B > 65535) s.quota = 0;
+    if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
     return s;
 }
 

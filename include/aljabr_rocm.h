@@ -340,8 +340,8 @@ int aljabr_rocm_kv4_attention_workspace(const aljabr_rocm_kv4_cache *cache, int 
  * sequences and a sequence holds `rows` positions (any number up to 2^30).
  * With one S = num_blocks: position j of sequence b is row j % rows of block
  * block_table[b * max_blocks + j / rows], rows a multiple of 16, max_blocks *
- * rows at most 2^30. head_dim is 64, 128 or 256 (else -3). No counterpart in
- * the reference, whose decode rotates, appends and attends a token at a time.
+ * rows at most 2^30. head_dim is 64, 128 or 256 (else -3), sequences are at
+ * most 65535. No counterpart in the reference, whose decode rotates, appends and attends a token at a time.
  *
  * A draft of T rows a sequence is a tree: parents[b * T + t] is an earlier row
  * of the sequence, any other number (-1) none; a row's line is the row and its
