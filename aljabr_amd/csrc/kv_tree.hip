@@ -5,19 +5,29 @@
 //   s_j = cap(scale * q[t, h] . k_j), over the keys j that row t sees.
 //
 // The rows of a KV head are stacked, r = t * G + g (G = Hq / Hkv), 16 or 32 a
-// workgroup. A wave walks tiles of 16 U keys, whose fragments come straight
-// from the cache into registers, each refilled for the wave's next tile as soon
-// as the matrix cores have taken it: no LDS, no barrier in the loop.
+// workgroup (65 and more over large caches: kv_tree_rows.hip). A wave walks
+// tiles of 16 U keys, whose fragments come straight from the cache into
+// registers, each refilled for the wave's next tile as soon as the matrix cores
+// have taken it: no LDS, no barrier in the loop.
 //   S[key][row]   = K Q^T: lane (n, h) holds key n, 16 bytes at every step;
-//   O^T[d][row] += V^T P^T on v_mfma_f32_16x16x4_f32, whose operands are one
-//     number a lane: V's is V[4h' + r][its dims] as loaded (whole rows a load,
-//     no transposition), P's the weight that the lane computed itself, as fp32.
-// The fp32 products run at 1/16 of fp16's rate; for up to 32 rows they take
-// less time than the bytes, and they keep the weights whole.
+//   O^T[d][row] += V^T P^T: a lane loads whole pieces of V's rows, 4 keys of
+//     each 16 and 8 (4) dims, and a weight of each row it computed itself.
+//     fp16: v_mfma_f32_16x16x32_f16 over the 32 keys, V transposed by a byte
+//       permutation of two keys' dwords (one a dword and key pair), weights as
+//       two fp16 parts;
+//     fp32: v_mfma_f32_16x16x4_f32, one number a lane, which needs no
+//       transposition. fp16 caches went this way first: a tree of 64 over
+//       8 x 8192 keys took 433 us, with fp16 products 180 us.
+// Bound by the bytes of the cache, read once a row group: 32 sequences of about
+// 2100 keys, 8 KV heads of 128, 20 rows each, 64 us with the merge (4.4 TB/s);
+// an fp32 cache of 4 x 2048 keys, 64 rows a head, 34 us, of which its products
+// at fp32's rate are 14; short calls by the chain lengths - table - tile -
+// states - merge: 8 drafted rows over 512 keys 12 us.
 //
 // Precision: an fp16 K enters as it is against a query row scaled by a power of
 // two to a largest magnitude in [2^14, 2^15) and split into two fp16 parts
-// (2^-22 of each element); everything else is fp32.
+// (2^-22 of each element); weights of an fp16 cache are two fp16 parts as well
+// (2^-22, nothing below 2^-36 of the largest); everything else is fp32.
 //
 // Keys a row does not see get weight 0. In a tile that not every row sees
 // whole, V rows past the end are taken as 0, and values that are not finite are
@@ -607,7 +617,22 @@ struct Plan {
 Plan make_plan(const KvView &v, int T, int Hq, int window) {
     Plan s;
     const long long rows = static_cast<long long>(T) * (Hq / v.H);
-    // What the cache may hold of visible keys, in bytes: the lengths themselves are on the device.
+    // The lengths are on the device: rules go by what the cache may hold of visible keys, in bytes. Measured with 8 KV
+    // heads of 128 in fp16 filled to the end, in us, the better of one and two workgroups a CU (one sequence of 1024 keys
+    // is 2^22 bytes, of 8192 2^25, four of 4096 2^26, 32 of 4096 2^29):
+    //   rows a KV head         16 a workgroup    32    rows kernel
+    //   20, one of 1024 keys             10.9  12.7           15.3
+    //   32, four of 4096                 21.9  23.5           27.8
+    //   20, 32 of 4096                  111.3 108.4          114.1
+    //   64, one of 1024                  12.3  14.1           16.7
+    //   64, one of 8192                  21.0  20.4           26.2
+    //   64, four of 4096                 31.9  27.6           32.9
+    //   256, one of 1024                 17.5  18.6           21.4
+    //   256, one of 8192                 48.5  36.2           37.2
+    //   160, four of 4096                67.5  43.9           44.9
+    //   128, 32 of 4096                 338.8 213.5          181.3
+    // Heads of 256 in the rows kernel (a ring of 96 KB, one workgroup a CU) took longer throughout: 256 rows over 8192 keys
+    // 109 us, with 32 rows a workgroup 65.
     const long long seen = window > 0 ? std::min<long long>(kv_capacity(v), static_cast<long long>(window) + T) : kv_capacity(v);
     const double bytes = 2.0 * v.B * seen * v.H * v.D * (v.f16 ? 2 : 4);
     if (v.f16 && v.D < 256 && rows > 64 && rows * bytes >= 0x1p33) s.rows = kRowsBlock;
@@ -619,6 +644,9 @@ Plan make_plan(const KvView &v, int T, int Hq, int window) {
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const int least = s.tile * kWaves;                     // keys of the smallest chunk (kRowsLeast tiles as well)
     const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
+    // Workgroups a CU: a second one covers the first one's waits where the bytes are many (20 rows over 32 of 4096 keys 112.5 ->
+    // 108.4 us; the rows kernel, 128 rows over the same, 202 -> 181), else it only splits more (48 rows over the same, two row
+    // groups, 125 -> 157 us; heads of 256, whose registers leave room for one, 31.8 -> 50.4 us).
     const int per_cu = s.rows == kRowsBlock || (s.groups == 1 && v.D < 256 && bytes >= 0x1p28) ? 2 : 1;
     s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
     if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
