@@ -749,8 +749,8 @@ int check_attention(const aljabr_rocm_kv_cache *cache, int layer, int T, int Hq,
     ALJ_REQUIRE(T > 0 && Hq > 0 && Hq % v.H == 0, "kv_tree_attention: T = %d must be positive and Hq = %d a multiple of %d KV heads",
                 T, Hq, v.H);
     ALJ_REQUIRE(static_cast<long long>(T) * Hq <= (1 << 30), "kv_tree_attention: T * Hq exceeds 2^30");
-    ALJ_REQUIRE(static_cast<long long>(v.B) * kv_capacity(v) <= (1LL << 35),
-                "kv_tree_attention: sequences * the positions of each exceeds 2^35");   // find_chunk adds up their tiles
+    ALJ_REQUIRE(static_cast<long long>(v.B) * kv_capacity(v) <= (1LL << 34),
+                "kv_tree_attention: sequences * the positions of each exceeds 2^34");   // find_chunk adds up tiles, of 16 keys and more
     return ALJABR_ROCM_OK;
 }
 

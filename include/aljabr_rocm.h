@@ -341,7 +341,8 @@ int aljabr_rocm_kv4_attention_workspace(const aljabr_rocm_kv4_cache *cache, int 
  * With one S = num_blocks: position j of sequence b is row j % rows of block
  * block_table[b * max_blocks + j / rows], rows a multiple of 16, max_blocks *
  * rows at most 2^30. head_dim is 64, 128 or 256 (else -3), sequences are at
- * most 65535. No counterpart in the reference, whose decode rotates, appends and attends a token at a time.
+ * most 65535. No counterpart in the reference, whose decode rotates, appends
+ * and attends a token at a time.
  *
  * A draft of T rows a sequence is a tree: parents[b * T + t] is an earlier row
  * of the sequence, any other number (-1) none; a row's line is the row and its
@@ -407,7 +408,7 @@ int aljabr_rocm_kv_append(const aljabr_rocm_kv_cache *cache, int layer, void *q_
  * -inf) gives zeros; rows from counts[b] on are left as they were. Keys on a
  * bad block are not seen, and what keys hold that a row does not see never
  * reaches it. fp32-accurate. T * Hq is at most 2^30, sequences * the positions
- * of each at most 2^35, and a call of more workgroups than a launch takes is
+ * of each at most 2^34, and a call of more workgroups than a launch takes is
  * refused (-3). workspace: device scratch for split partials, of
  * aljabr_rocm_kv_tree_attention_workspace bytes (fewer: fewer splits), not
  * shared by calls that may run at once, captured graphs among them. NULL: the

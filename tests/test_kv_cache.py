@@ -103,7 +103,10 @@ def test_bad_attention(kw):
 def test_sizes_that_attention_refuses():
     assert attend(cache(), t=257, parents=P) == -3
     big = dict(block_table=0x50000, num_blocks=1 << 20, rows=64, max_blocks=1 << 24)
-    assert attend(cache(**dict(big, sequences=33))) == -2                 # 33 of 2^30 positions: past 2^35
+    assert attend(cache(**dict(big, sequences=33))) == -2                 # 33 of 2^30 positions
+    # The positions' tiles, of 16 keys for fp32, are added up in 32 bits: 2^31 of them would pass those.
+    assert attend(cache(**dict(big, sequences=32, type=0))) == -2
+    assert attend(cache(**dict(big, sequences=17))) == -2 != attend(cache(**dict(big, sequences=16)))
     n = ctypes.c_size_t()
     assert abi.load().aljabr_rocm_kv_tree_attention_workspace(ctypes.byref(cache()), 1, 12, ctypes.byref(n)) == -2
     assert abi.load().aljabr_rocm_kv_tree_attention_workspace(ctypes.byref(cache()), 1, 32, None) == -2
