@@ -199,7 +199,9 @@ __global__ __launch_bounds__(kThreads) void kv_tree_accept_kernel(AcceptParams p
     __syncthreads();
     if (i > 0 && i < cnt && (!agrees || first[up] != i)) atomicOr(&disagree[i >> 5], 1u << (i & 31));
     if (p.parents) {
-        fill_tree(tree, up, cnt, 0);
+        const int row = tree_row(cnt);
+        fill_tree(tree, row < cnt ? p.parents[row0 + row] : -1, cnt, 0);
+        __syncthreads();
     } else {
         tree.depth[i] = i;
 #pragma unroll

@@ -53,9 +53,13 @@ struct Tree {
     int depth[kTreeMost];
 };
 
+// The row whose parent a thread gives fill_tree: of up to 64 rows every wave holds all.
+__device__ __forceinline__ int tree_row(int n) { return n <= 64 ? threadIdx.x & 63 : threadIdx.x; }
+
 // Fills the tree of rows [0, n), n <= kTreeMost, from the parent of each thread's row (a number that is not an earlier
-// row's stands for none). With a window > 0, of a row's line only its last `window` rows are kept in mask. By a workgroup of kTreeMost
-// threads, which it leaves in step.
+// row's stands for none). With a window > 0, of a row's line only its last `window` rows are kept in mask. By a workgroup
+// of kTreeMost threads, none of which waits for another where n <= 64: each wave then writes the whole tree, and what it
+// reads is its own.
 //
 // After step s a row knows the 2^(s+1) last rows of its line and the row before them: log2(n) steps whatever the depth,
 // each a row's masks joined with those of the row where its own end. A window is taken in parts of powers of two: the
@@ -64,6 +68,34 @@ __device__ __forceinline__ void fill_tree(Tree &t, int parent, int n, int window
     const int i = threadIdx.x, words = (n + 31) >> 5;
     const bool mine = i < n;
     const int limit = window > 0 && window < n ? window : 0;
+    if (n <= 64) {
+        const int lane = i & 63;
+        int to = lane < n && parent >= 0 && parent < lane ? parent : -1, at = lane;
+        uint32_t lo = lane < 32 ? 1u << lane : 0, hi = lane < 32 ? 0 : 1u << (lane - 32), in_lo = 0, in_hi = 0;
+        for (int s = 0; 1 << s < n; ++s) {
+            if (limit >> s & 1) {
+                const uint32_t x = __shfl(lo, at), y = __shfl(hi, at);
+                const int z = __shfl(to, at);
+                if (at >= 0) {
+                    in_lo |= x;
+                    in_hi |= y;
+                    at = z;
+                }
+            }
+            const uint32_t x = __shfl(lo, to), y = __shfl(hi, to);
+            const int z = __shfl(to, to);
+            if (to >= 0) {
+                lo |= x;
+                hi |= y;
+                to = z;
+            }
+        }
+        t.depth[lane] = __builtin_popcount(lo) + __builtin_popcount(hi) - 1;
+        t.mask[lane] = limit ? in_lo : lo;
+        t.mask[kTreeMost + lane] = limit ? in_hi : hi;
+        t.mask[2 * kTreeMost + lane] = 0;                  // a word of zeros behind the last
+        return;
+    }
     int jump = -1, cur = mine ? i : -1;
     uint32_t own[kTreeWords], part[kTreeWords];
     if (mine && parent >= 0 && parent < i) jump = parent;

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
     const auto entry = places.fetch(p, lane, b, seq.n, 0);
     const bool filled = p.parents && (p.window > 0 || t1 * KT > base);
     int parent = -1;
-    if (filled && static_cast<int>(threadIdx.x) < seq.cnt) parent = p.parents[static_cast<long long>(b) * p.T + threadIdx.x];
+    if (filled && tree_row(seq.cnt) < seq.cnt) parent = p.parents[static_cast<long long>(b) * p.T + tree_row(seq.cnt)];
     auto row_at = [&](int t, int r) __attribute__((always_inline)) {
         return p.q + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D;
     };
@@ -519,73 +519,69 @@ again:
         }
     }
 
-    // The four waves' states become one: 2 and 3 hand theirs to 0 and 1, then 1 to 0. O^T tile x VE + e, accumulator r:
-    // dim 16 VE x + VE (4h + r) + e of the row.
-    constexpr int kState = NT * (OT * 256 + 64 * 2);       // floats of a wave's state
+    // The four waves' states through LDS as rows, then a thread takes four dims of a row from all of them. O^T tile x VE + e,
+    // accumulator i: dim 16 VE x + VE (4h + i) + e of the row.
+    constexpr int kStride = D + 4;
+    float2 *ml = reinterpret_cast<float2 *>(smem + kWaves * ROWS * kStride);               // [wave][row]
+    __syncthreads();                                       // the queries and weights are done with
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
         if (m[c] == -INFINITY && l[c] != l[c]) m[c] = 0.0f;            // a NaN score alone leaves no reference: any finite one carries it
-    }
-#pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            float *st = smem + (wave - half) * kState;
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-#pragma unroll
-                for (int j = 0; j < OT; ++j) *reinterpret_cast<f32x4 *>(st + ((c * OT + j) * 64 + lane) * 4) = o[c][j];
-                *reinterpret_cast<float2 *>(st + NT * OT * 256 + (c * 64 + lane) * 2) = make_float2(m[c], l[c]);
-            }
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float *st = smem + wave * kState;
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-                const float2 ml = *reinterpret_cast<const float2 *>(st + NT * OT * 256 + (c * 64 + lane) * 2);
-                const float to = fmaxf(m[c], ml.x);
-                const float a = m[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[c] - to);
-                const float e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - to);
-                l[c] = fmaf(l[c], a, ml.y * e);
-                m[c] = to;
-#pragma unroll
-                for (int j = 0; j < OT; ++j) {
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(st + ((c * OT + j) * 64 + lane) * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[c][j][r] = fmaf(o[c][j][r], a, x[r] * e);
-                }
-            }
-        }
-    }
-    if (wave) return;
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-        const int r = r0 + 16 * c + n;
-        if (r >= r1) continue;
-        const bool whole = chunk.count == 1;
-        const long long part = (static_cast<long long>(chunk.slot + w - chunk.first) * p.v.H * p.row_groups + item) * ROWS + 16 * c + n;
-        const int t = p.by_g(r), g = r - t * p.G;
-        float *dst = whole ? p.out + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + g) * D : p.part_o + part * D;
-        const float f = whole ? (l[c] == 0.0f ? 0.0f : 1.0f / l[c]) : 1.0f;
+        float *row = smem + (wave * ROWS + 16 * c + n) * kStride + VE * 4 * h;
 #pragma unroll
         for (int x = 0; x < VP; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < VE; e += 4)
-                    *reinterpret_cast<float4 *>(dst + 16 * VE * x + VE * (4 * h + i) + e) =
-                        make_float4(o[c][x * VE + e][i] * f, o[c][x * VE + e + 1][i] * f, o[c][x * VE + e + 2][i] * f, o[c][x * VE + e + 3][i] * f);
-        if (!whole && h == 0) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(m[c], l[c]);
+                    *reinterpret_cast<float4 *>(row + 16 * VE * x + VE * i + e) =
+                        make_float4(o[c][x * VE + e][i], o[c][x * VE + e + 1][i], o[c][x * VE + e + 2][i], o[c][x * VE + e + 3][i]);
+        if (h == 0) ml[wave * ROWS + 16 * c + n] = make_float2(m[c], l[c]);
+    }
+    __syncthreads();
+    const bool all = chunk.count == 1;
+    const long long part = (static_cast<long long>(chunk.slot + w - chunk.first) * p.v.H * p.row_groups + item) * ROWS;
+    constexpr int LPR = D / 4;
+#pragma unroll
+    for (int i = 0; i < ROWS * LPR / kThreads; ++i) {
+        const int lr = (kThreads * i + static_cast<int>(threadIdx.x)) / LPR, d = 4 * (threadIdx.x % LPR), r = r0 + lr;
+        if (r >= r1) continue;
+        float2 of[kWaves];
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            of[k] = ml[k * ROWS + lr];
+            top = fmaxf(top, of[k].x);
+        }
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float e = of[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(of[k].x - top);
+            const float4 x = *reinterpret_cast<const float4 *>(smem + (k * ROWS + lr) * kStride + d);
+            sum = fmaf(of[k].y, e, sum);
+            y.x = fmaf(x.x, e, y.x);
+            y.y = fmaf(x.y, e, y.y);
+            y.z = fmaf(x.z, e, y.z);
+            y.w = fmaf(x.w, e, y.w);
+        }
+        if (all) {
+            const int t = p.by_g(r);
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<float4 *>(p.out + ((static_cast<long long>(b) * p.T + t) * p.Hq + kvh * p.G + (r - t * p.G)) * D + d) =
+                make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+        } else {
+            *reinterpret_cast<float4 *>(p.part_o + (part + lr) * D + d) = y;
+            if (d == 0) *reinterpret_cast<float2 *>(p.part_ml + (part + lr) * 2) = make_float2(top, sum);
+        }
     }
 }
 
 template <bool F16, int D, int NT>
 void launch_split(const Params &p, hipStream_t s) {
     using S = Shape<F16, D>;
-    constexpr size_t states = 2 * NT * (S::OT * 256 + 128) * 4, weights = kWaves * 16 * NT * S::KT * 4;
+    constexpr size_t states = kWaves * 16 * NT * (D + 6) * 4, weights = kWaves * 16 * NT * S::KT * 4;
     constexpr size_t loop = weights + (query_in_lds(D, NT) ? NT * S::kQuery * 1024 : 0), lds = states > loop ? states : loop;
     static_assert(lds + sizeof(Tree) + NT * 1088 <= 160 * 1024, "LDS of a workgroup");
     if (lds + sizeof(Tree) + NT * 1088 > 65536)

@@ -179,8 +179,11 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
     const bool filled = p.parents && (p.window > 0 || t1 * kTile > base);
     start();
     if (tid == 0) odd_tile = 0;
-    if (filled) fill_tree(tree, tid < seq.cnt ? p.parents[static_cast<long long>(b) * p.T + tid] : -1, seq.cnt, p.window);
-    else __syncthreads();
+    if (filled) {
+        const int row = tree_row(seq.cnt);
+        fill_tree(tree, row < seq.cnt ? p.parents[static_cast<long long>(b) * p.T + row] : -1, seq.cnt, p.window);
+    }
+    __syncthreads();
 
     // This lane's row, what it sees; the keys that all rows of the wave, and of the workgroup, see.
     const int r = min(w0 + nl, r1 - 1);                    // lanes past the rows repeat the last and are not stored
