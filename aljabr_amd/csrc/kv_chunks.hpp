@@ -4,7 +4,7 @@
 // over the 4-bit cache and over fp16 and fp32 caches.
 //
 // P, a kernel's parameters, has the cache's view v (sequences B, KV heads H),
-// T, G, Hq, row_groups, quota, the dividers by_g, by_chunks and by_items, the
+// T, G, Hq, row_groups, quota, the dividers by_g, by_chunks (work_of: and by_items), the
 // partials part_o, part_ml and chunks, and out; kEvenChunks: a sequence's
 // chunks are of one size, instead of its last one taking what is left. Beside P
 // stand

@@ -166,7 +166,7 @@ struct Query {
 // Whether the queries are kept in LDS: in registers they would be D / 4 of each column tile.
 constexpr bool query_in_lds(int D, int NT) { return NT * D >= 256; }
 
-// grid: chunks of KV heads and row groups (work_of).
+// grid: chunks of KV heads and row groups (work_at).
 template <bool F16, int D, int NT>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Params p) {
     using S = Shape<F16, D>;
@@ -180,9 +180,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
     float *work = smem + (QLDS ? NT * QL * 256 : 0);
     const int lane = threadIdx.x & 63, n = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int item, w;
-    work_of(p, blockIdx.x, item, w);
-    const int group = p.by_heads(item), kvh = item - group * p.v.H, r0 = group * ROWS;
+    const Work work_item = work_at(p, blockIdx.x);
+    const int kvh = work_item.kvh, group = work_item.group, w = work_item.w, item = item_of(p, kvh, group), r0 = group * ROWS;
+    if (!p.quota && w >= p.v.B) return;                    // numbers past the last unit
     const Chunk chunk = find_chunk(p, w, r0, ROWS, kWaves);
     if (chunk.b < 0) return;
     const int b = chunk.b, t0 = chunk.t0, t1 = chunk.t1;
@@ -587,8 +587,7 @@ void launch_split(const Params &p, hipStream_t s) {
     if (lds + sizeof(Tree) + NT * 1088 > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_split_kernel<F16, D, NT>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(lds));
-    const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
-    hipLaunchKernelGGL((kv_split_kernel<F16, D, NT>), grid, dim3(kThreads), lds, s, p);
+    hipLaunchKernelGGL((kv_split_kernel<F16, D, NT>), dim3(workgroups(p)), dim3(kThreads), lds, s, p);
     if (p.quota) launch_merge<D, 16 * NT>(p, kWaves << p.tile_shift, s);
 }
 
@@ -640,10 +639,12 @@ Plan make_plan(const KvView &v, int T, int Hq, int window) {
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const int least = s.tile * kWaves;                     // keys of the smallest chunk (kRowsLeast tiles as well)
     const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
-    // Workgroups a CU: a second one covers the first one's waits where the bytes are many (20 rows over 32 of 4096 keys 112.5 ->
-    // 108.4 us; the rows kernel, 128 rows over the same, 202 -> 181), else it only splits more (48 rows over the same, two row
-    // groups, 125 -> 157 us; heads of 256, whose registers leave room for one, 31.8 -> 50.4 us).
-    const int per_cu = s.rows == kRowsBlock || (s.groups == 1 && v.D < 256 && bytes >= 0x1p28) ? 2 : 1;
+    // Workgroups a CU: with a second one the chunks are finer and one's waits are covered by the other, which is worth its
+    // partials where the bytes are many and either lengths may differ or row groups share the keys. Of 8 KV heads of 128,
+    // one and two a CU: 20 rows over 32 fp16 sequences of about 2100 keys 80 and 66 us, fp32 178 and 126 (of 4096 keys each
+    // 99 and 104); 48 rows over one of 131072 132 and 121, 20 rows 98 and 106; 64 rows over one of 8192 19.0 and 20.1; the
+    // rows kernel, 128 rows over 32 of 4096, 202 and 181. Heads of 256 fill a CU's registers with one.
+    const int per_cu = s.rows == kRowsBlock || (v.D < 256 && bytes >= 0x1p27 && (v.B > 1 || s.groups > 1)) ? 2 : 1;
     s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
     if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
     return s;
@@ -690,14 +691,14 @@ int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
     p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;
     p.window = std::min(a.window, 1 << 30);                // past every key; positions less it stay in 32 bits
     const Plan plan = make_plan(v, a.T, a.Hq, p.window);
-    if (static_cast<double>(v.H) * plan.groups * (plan.quota + static_cast<double>(v.B)) > 0x7fffff)
+    if ((static_cast<double>(v.H) * (plan.quota + static_cast<double>(v.B)) + 7.0) * plan.groups > 0x7fffff)
         return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv_tree_attention: T = %d rows of %d heads are more than one launch takes", a.T, a.Hq);
     p.row_groups = plan.groups;
     p.quota = plan.quota;
     p.tile_shift = log2_exact(plan.tile);
     p.by_g.set(p.G);
     p.by_rows.set(v.R);
-    p.by_items.set(v.H * plan.groups);
+    p.by_groups.set(plan.groups);
     p.by_heads.set(v.H);
     float *part = a.scratch;
     if (p.quota) {
@@ -727,6 +728,8 @@ int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
         p.chunks = reinterpret_cast<int2 *>(p.part_ml + 2 * all);
     }
     p.by_chunks.set(p.quota ? p.quota : v.B);
+    const int units = v.H * (p.quota ? p.quota : v.B);     // in eights, or enough that a last part of eight is little
+    p.span_shift = units % 8 == 0 || units >= 64 ? 3 : 0;
     hipStream_t s = current_stream();
     if (plan.rows == kRowsBlock) launch_rows(p, s);
     else v.f16 ? launch<true>(p, plan.rows, s) : launch<false>(p, plan.rows, s);

@@ -112,10 +112,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
         asm volatile("" : "+v"(x));
         return x;
     };
-    int item, w;
-    work_of(p, blockIdx.x, item, w);
-    const int group = group_of(p, p.by_heads(item)), kvh = item - p.by_heads(item) * p.v.H;
-    item = item_of(p, kvh, group);
+    const Work work_item = work_at(p, blockIdx.x);
+    const int kvh = work_item.kvh, w = work_item.w, group = group_of(p, work_item.group), item = item_of(p, kvh, group);
+    if (!p.quota && w >= p.v.B) return;                    // numbers past the last unit
     const int r0 = group * kRowsBlock;
     const Chunk chunk = find_chunk(p, w, r0, kRowsBlock, kRowsLeast);
     if (chunk.b < 0) return;
@@ -515,10 +514,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
 template <int D>
 void launch(const Params &p, hipStream_t s) {
     using R = Rows<D>;
-    const dim3 grid(p.v.H * p.row_groups * (p.quota ? p.quota + (p.v.B > 1 ? p.v.B : 0) : p.v.B));
     if (R::kBytes + sizeof(Tree) + kThreads * sizeof(int4) + 16 > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_rows_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
-    hipLaunchKernelGGL((kv_rows_kernel<D>), grid, dim3(kThreads), R::kBytes, s, p);
+    hipLaunchKernelGGL((kv_rows_kernel<D>), dim3(workgroups(p)), dim3(kThreads), R::kBytes, s, p);
     if (p.quota) launch_merge<D, kRowsBlock>(p, kRowsLeast * kTile, s);
 }
 
