@@ -612,26 +612,28 @@ struct Plan {
 Plan make_plan(const KvView &v, int T, int Hq, int window) {
     Plan s;
     const long long rows = static_cast<long long>(T) * (Hq / v.H);
-    // The lengths are on the device: rules go by what the cache may hold of visible keys, in bytes. Measured with 8 KV
-    // heads of 128 in fp16 filled to the end, in us, the better of one and two workgroups a CU (one sequence of 1024 keys
-    // is 2^22 bytes, of 8192 2^25, four of 4096 2^26, 32 of 4096 2^29):
-    //   rows a KV head         16 a workgroup    32    rows kernel
-    //   20, one of 1024 keys             10.9  12.7           15.3
-    //   32, four of 4096                 21.9  23.5           27.8
-    //   20, 32 of 4096                  111.3 108.4          114.1
-    //   64, one of 1024                  12.3  14.1           16.7
-    //   64, one of 8192                  21.0  20.4           26.2
-    //   64, four of 4096                 31.9  27.6           32.9
-    //   256, one of 1024                 17.5  18.6           21.4
-    //   256, one of 8192                 48.5  36.2           37.2
-    //   160, four of 4096                67.5  43.9           44.9
-    //   128, 32 of 4096                 338.8 213.5          181.3
-    // Heads of 256 in the rows kernel (a ring of 96 KB, one workgroup a CU) took longer throughout: 256 rows over 8192 keys
-    // 109 us, with 32 rows a workgroup 65.
+    // The lengths are on the device: rules go by what the cache may hold of visible keys. More rows a workgroup read a key
+    // less often and start later. In us, 8 KV heads of 128 in fp16 filled to the end, in brackets w below:
+    //   rows a KV head, cache                16 a workgroup    32   128 (the rows kernel)
+    //   20, one of 1024 keys      (2^22)                11.4  12.7  16.0
+    //   32, four of 4096          (2^26)                19.6  21.5  27.0
+    //   20, one of 32768          (2^27)                34.7  32.3  38.0
+    //   20, 32 of 4096            (2^29)               107.3 104.1 111.4
+    //   64, one of 4096           (2^30 with the rows)  15.5  16.7  21.4
+    //   64, one of 8192           (2^31)                19.5  19.4  25.4
+    //   48, four of 4096          (2^31.6)              27.4  25.3  31.5
+    //   64, 32 of 1024            (2^33)                56.4  40.9  48.0
+    //   256, one of 8192          (2^33)                44.2  35.7  37.0
+    //   96, one of 32768          (2^33.6)              76.7  51.3  49.4
+    //   256, four of 4096         (2^34)                80.3  58.8  54.3
+    //   256, 32 of 4096           (2^37)               608.8 362.4 288.6
+    // fp32 and heads of 64 and 256 turn at the same w (of 259 shapes the rule is 0.3 % from the better choice, at most 8 %).
+    // Heads of 256 in a rows kernel (a ring of 96 KB, one workgroup a CU) took longer throughout: 256 rows over 8192 keys 109
+    // us, with 32 rows a workgroup 59.
     const long long seen = window > 0 ? std::min<long long>(kv_capacity(v), static_cast<long long>(window) + T) : kv_capacity(v);
-    const double bytes = 2.0 * v.B * seen * v.H * v.D * (v.f16 ? 2 : 4);
-    if (v.f16 && v.D < 256 && rows > 64 && rows * bytes >= 0x1p33) s.rows = kRowsBlock;
-    else if (rows > 32 ? rows * bytes >= 0x1p31 : rows > 16 && bytes >= 0x1p27) s.rows = 32;
+    const double keys = static_cast<double>(v.B) * seen * v.H, bytes = keys * v.D * (v.f16 ? 4 : 8), w = keys * std::max(v.D, 128) * 4;
+    if (v.f16 && v.D < 256 && rows > 64 && rows * w > 0x1p33) s.rows = kRowsBlock;
+    else if (rows > 32 ? rows * w > 0x1p31 : rows > 16 && w >= 0x1p27) s.rows = 32;
     else s.rows = 16;
     s.tile = v.f16 || v.D == 64 ? 32 : 16;
     s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
