@@ -19,10 +19,10 @@
 //       transposition. fp16 caches went this way first: a tree of 64 over
 //       8 x 8192 keys took 433 us, with fp16 products 180 us.
 // Bound by the bytes of the cache, read once a row group: 32 sequences of about
-// 2100 keys, 8 KV heads of 128, 20 rows each, 64 us with the merge (4.4 TB/s);
-// an fp32 cache of 4 x 2048 keys, 64 rows a head, 34 us, of which its products
-// at fp32's rate are 14; short calls by the chain lengths - table - tile -
-// states - merge: 8 drafted rows over 512 keys 12 us.
+// 2100 keys, 8 KV heads of 128, 20 rows each, 57 to 68 us with the merge (4.1 to
+// 4.9 TB/s); an fp32 cache of 4 x 2048 keys, 64 rows a head, 32.6 us, of which its
+// products at fp32's rate are 14; short calls by the chain lengths - table - tile
+// - states - merge: 8 drafted rows over 512 keys 10.5 us.
 //
 // Precision: an fp16 K enters as it is against a query row scaled by a power of
 // two to a largest magnitude in [2^14, 2^15) and split into two fp16 parts

@@ -12,11 +12,11 @@
 // the two fp16 parts of queries and weights. The next tile's scores are laid
 // between this one's weights, so that matrix cores and vector ALU work at once.
 //
-// Bound by the products: 256 rows of 8 KV heads of 128 over 8 x 8192 keys 162
+// Bound by the products: 256 rows of 8 KV heads of 128 over 8 x 8192 keys 157
 // us, 104 rows over 131072 keys 163 us, chunks of 512 rows of 32 heads over
-// 2 x 4096 keys 142 us, with the merges: 0.97 PFLOP/s with both parts, where the
-// library's product of 8192^3 reaches 1.2. Matrix cores 43 % of the cycles, vector
-// ALU 41 %, both at once 20 %; under this load the clock falls to 2.0 GHz. Tiles
+// 2 x 4096 keys 145 us, with the merges: 0.97 PFLOP/s with both parts, where the
+// library's product of 8192^3 reaches 1.2. Matrix cores 44 % of the cycles, vector
+// ALU 42 %, both at once 20 %; under this load the clock falls to 2.0 GHz. Tiles
 // of both operands shared in LDS by 128 rows took 157 us of the chunks where the
 // waves of 32 rows loaded their own (kv_tree.hip) 422; addresses of tiles held by
 // the lanes made that 149, the pipeline 143.

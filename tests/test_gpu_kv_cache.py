@@ -508,6 +508,60 @@ def test_many_uneven_sequences(rocm, room, b, page, t, g, tree):
     check(got, *plain.attention(host, q, lens, counts, parents))
 
 
+@pytest.mark.parametrize("b", [255, 256, 257, 320, 513, 900])
+@pytest.mark.parametrize("t,g", [(1, 4), (6, 8)])
+def test_hundreds_of_sequences(rocm, b, t, g):
+    """Lengths are looked through 256 at once: the long sequences are in the first, the last and at the edges between."""
+    rng = np.random.default_rng(b)
+    lens, counts = rng.integers(0, 60, b), rng.integers(0, t + 1, b)
+    for i in (0, 63, 64, 255, 256, 511, 512, b - 1):
+        if i < b:
+            lens[i], counts[i] = 300 + i % 7, t
+    host = plain.Cache(b, 1, 64, 320, 16, F16)
+    host.fill(lens)
+    q = normal(b, b, t, g, 64)
+    parents = plain.random_parents(rng, b, t)
+    check(attend(rocm, Device(rocm, host), q, lens, counts, parents), *plain.attention(host, q, lens, counts, parents))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("b,hkv", [(67, 1), (23, 3), (66, 1), (13, 5)])
+@pytest.mark.parametrize("t,g", [(1, 4), (11, 7)])
+def test_short_sequences_that_are_not_eights(rocm, b, hkv, dtype, t, g):
+    """Caches of one chunk a sequence, whose KV heads and sequences are no multiple of the 8 XCDs."""
+    rng = np.random.default_rng(b)
+    lens, counts = rng.integers(t, 101, b), rng.integers(0, t + 1, b)
+    host = plain.Cache(b, hkv, 64, 100, 0, dtype)
+    host.fill(lens)
+    q = normal(b, b, t, hkv * g, 64)
+    check(attend(rocm, Device(rocm, host), q, lens, counts), *plain.attention(host, q, lens, counts))
+
+
+def test_as_many_sequences_as_a_call_takes(rocm):
+    """65535 sequences of up to 3 keys of one block, the last of 250: each row is a mean of values, or one of them."""
+    b, d = 65535, 64
+    host = plain.Cache(1, 1, d, 256, 16)
+    host.fill([256])
+    one = Device(rocm, host)
+    table = one.table.expand(b, 16).contiguous()
+    desc = rocm.KvCache.from_buffer_copy(one.desc)
+    desc.sequences, desc.block_table = b, table.data_ptr()
+    lens = np.arange(b) % 3
+    lens[-1] = 250
+    q = normal(1, 1, 1, 2, d)
+    want = [plain.attention(host, q, [n]) for n in (0, 1, 2, 250)]
+    qd, ld = torch.from_numpy(q).cuda().expand(b, 1, 2, d).contiguous(), ints(lens)
+    out = torch.full((b, 1, 2, d), POISON, device="cuda")
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv_tree_attention", out.data_ptr(), qd.data_ptr(), ctypes.byref(desc), 0, ld.data_ptr(), None, None, 1, 2, 0.0, 0,
+              0.0, None, 0)
+    got = out.cpu().numpy()
+    for i in range(3):
+        err = np.abs(got[:-1][lens[:-1] == i] - want[i][0])
+        assert (err <= want[i][1] + 1e-30).all()
+    assert (np.abs(got[-1:] - want[3][0]) <= want[3][1]).all()
+
+
 @pytest.mark.parametrize("room", [0, ROOM])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("g", [17, 33, 64, 130])
