@@ -390,11 +390,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
                     float e[2];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        e[c] = __builtin_amdgcn_exp2f(fmaf(s[2 * j + c], us, -ref)) * kWeightScale<true>;
+                        e[c] = __builtin_amdgcn_exp2f(fmaf(s[2 * j + c], us, -ref));
                         sum[(2 * j + c) & 3] += e[c];
                     }
-                    const half2v first = pair(e[0], e[1]);
-                    const half2v rest = pair(fmaf(static_cast<float>(first[0]), -1.0f, e[0]), fmaf(static_cast<float>(first[1]), -1.0f, e[1]));
+                    constexpr float up = kWeightScale<true>;
+                    const half2v first = pair(e[0] * up, e[1] * up);
+                    const half2v rest = pair(fmaf(e[0], up, -static_cast<float>(first[0])), fmaf(e[1], up, -static_cast<float>(first[1])));
                     ph[j >> 2][2 * (j & 3)] = first[0];
                     ph[j >> 2][2 * (j & 3) + 1] = first[1];
                     pl[j >> 2][2 * (j & 3)] = rest[0];
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
         start();
     }
 
-    l += __shfl_xor(l, 32);
+    l = (l + __shfl_xor(l, 32)) * kWeightScale<true>;
     if (m == -INFINITY && l != l) m = 0.0f;                // a NaN score alone leaves no reference
     const bool whole = chunk.count == 1;
     const float f = (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
