@@ -393,6 +393,10 @@ int aljabr_rocm_kv_append(const aljabr_rocm_kv_cache *cache, int layer, void *q_
     const size_t elem = type == ALJABR_ROCM_TYPE_F16 ? 2 : 4;
     ALJ_REQUIRE(aligned(Q, elem) && aligned(K, elem) && aligned(V, elem), "kv_append: Q, K and V must be aligned to their elements");
     ALJ_REQUIRE(aligned(q_out, 16), "kv_append: q_out must be 16-byte aligned");
+    ALJ_REQUIRE(!Q || q_out != Q || (type == ALJABR_ROCM_TYPE_F32 && (Hq == 1 || q_stride_h == v.D) &&
+                                     (T == 1 || q_stride_t == static_cast<long long>(Hq) * v.D) &&
+                                     (v.B == 1 || q_stride_b == static_cast<long long>(T) * Hq * v.D)),
+                "kv_append: q_out is a Q that is not dense fp32 rows");
     ALJ_REQUIRE(static_cast<long long>(T) * (a.Hq + 2 * v.H) * (v.D / 8) <= 0xffffff00LL,       // lanes of a launch
                 "kv_append: T = %d rows of %d heads are more than one launch takes", T, a.Hq + 2 * v.H);
     ALJ_CHECK_READY();

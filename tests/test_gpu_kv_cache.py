@@ -710,6 +710,58 @@ def test_a_sessions_cache(rocm):
     assert np.abs(out.cpu().numpy().reshape(got.shape) - got).max() <= 1e-4
 
 
+def test_planes_of_a_llama_session(rocm):
+    """The planes a session decoded into, described to the calls: a tree over its last rows, and the rows it accepts moved
+    where the session's next step reads them."""
+    from aljabr_amd.llama import LLAMA3_8B, DeviceLlama, random_weights
+    cfg = dict(LLAMA3_8B, layers=2, dim=512, ffn=1024, n_heads=8, n_kv_heads=2, head_dim=64, vocab=512)
+    b, steps, t, room = 3, 9, 5, 24
+    model = DeviceLlama(cfg, random_weights(cfg, seed=3), max_batch=b, max_seq=room)
+    k, v = model.kv_cache_ptrs()
+    host = plain.Cache(b, 2, 64, room, 0, F16, 2)
+    for pos in range(steps):
+        model.decode(ints([7 + pos, 40 + pos, 90 + pos]), ints([pos] * b), b)
+
+    def read():
+        torch.cuda.synchronize()
+        for w, at in zip("kv", (k, v)):
+            plane = torch.empty(host.planes[w].size, dtype=torch.float16, device="cuda")
+            rocm.call("aljabr_rocm_memcpy_d2d", plane.data_ptr(), at, 2 * plane.numel())
+            rocm.call("aljabr_rocm_synchronize")
+            yield w, plane.cpu().numpy().reshape(host.planes[w].shape)
+
+    host.planes = dict(read())
+    desc = rocm.KvCache(k, v, None, F16, 2, b, 2, 64, room, 0, 0)
+    need = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv_cache_bytes", ctypes.byref(desc), ctypes.byref(need))
+    assert need.value == 2 * model.kv_cache_elems()
+    lens, parents = [steps] * b, np.array([[-1, 0, 0, 2, 1]] * b, np.int32)
+    q = normal(1, b, t, 8, 64)
+    qd, ld, pd, out = torch.from_numpy(q).cuda(), ints(lens), ints(parents), torch.full(q.shape, POISON, device="cuda")
+    torch.cuda.synchronize()
+    for layer in range(2):
+        rocm.call("aljabr_rocm_kv_tree_attention", out.data_ptr(), qd.data_ptr(), ctypes.byref(desc), layer, ld.data_ptr(), None,
+                  pd.data_ptr(), t, 8, 0.0, 0, 0.0, None, 0)
+        torch.cuda.synchronize()
+        check(out.cpu().numpy(), *plain.attention(host, q, lens, None, parents, layer=layer))
+    tokens, choices = np.array([[1, 2, 3, 4, 5]] * b), np.array([[3, 0, 4, 9, 0], [2, 5, 0, 0, 8], [7, 0, 0, 0, 0]])
+    outs = [torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((b,), (b, t), (b,), (b,))]
+    td, cd = ints(tokens), ints(choices)
+    torch.cuda.synchronize()
+    rocm.call("aljabr_rocm_kv_tree_accept", ctypes.byref(desc), *[o.data_ptr() for o in outs], ld.data_ptr(), None, pd.data_ptr(),
+              td.data_ptr(), cd.data_ptr(), t)
+    want = plain.accept(host, lens, None, parents, tokens, choices)
+    assert all(np.array_equal(x.cpu().numpy(), y) for x, y in zip(outs, want)) and want[2].tolist() == [3, 3, 1]
+    for w, plane in read():
+        assert np.array_equal(plane, host.planes[w], equal_nan=True)
+    model.decode(outs[3], outs[0], b)                                  # the next step writes behind the accepted rows
+    after = dict(read())
+    for i, n in enumerate(want[0]):
+        assert np.array_equal(after["k"][:, i, :, :n], host.planes["k"][:, i, :, :n])
+        assert not np.array_equal(after["k"][:, i, :, n], host.planes["k"][:, i, :, n])
+    model.close()
+
+
 # ---- accepted rows --------------------------------------------------------------------
 
 def take(rocm, dev, lens, counts, parents, tokens, choices):
