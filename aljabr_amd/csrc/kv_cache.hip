@@ -177,7 +177,7 @@ constexpr int kBatch = 4;                    // 16-byte pieces that a lane holds
 
 __global__ __launch_bounds__(kThreads) void kv_tree_accept_kernel(AcceptParams p) {
     __shared__ Tree tree;
-    __shared__ int first[kTreeMost], line[kTreeMost], count, last;
+    __shared__ int first[kTreeMost], line[kTreeMost], block[kTreeMost], in_block[kTreeMost], count, last;
     __shared__ uint32_t disagree[kTreeWords];
     const int i = threadIdx.x, b = blockIdx.y;
     const int n = min(max(p.lens[b], 0), kv_capacity(p.v));
@@ -190,6 +190,10 @@ __global__ __launch_bounds__(kThreads) void kv_tree_accept_kernel(AcceptParams p
         if (up < 0 || up >= i) up = -1;
         agrees = up >= 0 && p.tokens[row0 + i] == p.choices[row0 + up];
     }
+    int s = -1, row = 0;                                         // where the draft's row i lies, or nowhere
+    if (i < cnt && !kv_locate(p.v, b, static_cast<long long>(n) - cnt + i, s, row)) s = -1;
+    block[i] = s;
+    in_block[i] = row;
     first[i] = kTreeMost;
     line[i] = -1;
     if (i < kTreeWords) disagree[i] = 0;
@@ -245,12 +249,11 @@ __global__ __launch_bounds__(kThreads) void kv_tree_accept_kernel(AcceptParams p
             const int j = j0 + k * rows + mine;
             to[k] = nullptr;
             if (j >= kept || line[j] == j) continue;
-            int s, row, d, at;
-            if (!kv_locate(p.v, b, static_cast<long long>(n) - cnt + line[j], s, row) ||
-                !kv_locate(p.v, b, static_cast<long long>(n) - cnt + j, d, at))
-                continue;
-            x[k] = *reinterpret_cast<const uint4 *>(plane + ((static_cast<long long>(s) * p.v.H + head) * p.v.R + row) * p.row_bytes);
-            to[k] = plane + ((static_cast<long long>(d) * p.v.H + head) * p.v.R + at) * p.row_bytes;
+            const int from = line[j];
+            if (block[from] < 0 || block[j] < 0) continue;
+            x[k] = *reinterpret_cast<const uint4 *>(
+                plane + ((static_cast<long long>(block[from]) * p.v.H + head) * p.v.R + in_block[from]) * p.row_bytes);
+            to[k] = plane + ((static_cast<long long>(block[j]) * p.v.H + head) * p.v.R + in_block[j]) * p.row_bytes;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // a batch is read before any of it is written
 #pragma unroll
