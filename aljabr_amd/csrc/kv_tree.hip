@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
     constexpr bool QLDS = query_in_lds(D, NT);
     extern __shared__ float smem[];                        // queries, states on their way, weights of odd tiles
     __shared__ Tree tree;
-    // Of a row: t, what it sees, the power of two it was scaled by (a wave's own copy); and what scales its scores back.
+    // Of a row: t and what it sees (a wave's own copy); and what scales its scores back.
     __shared__ int4 row_info[kWaves][ROWS];
     __shared__ float query_scale[QLDS ? ROWS : 1];
     float *work = smem + (QLDS ? NT * QL * 256 : 0);
