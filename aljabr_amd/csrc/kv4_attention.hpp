@@ -45,6 +45,7 @@ __device__ __forceinline__ Seq sequence(const Params &p, int b) {
     Seq s;
     s.n = min(max(p.lens[b], 0), kv4_capacity(p.v));
     s.cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+    s.base = s.n - s.cnt;
     return s;
 }
 

@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void kv_tree_accept_kernel(AcceptParams p
     __shared__ int first[kTreeMost], line[kTreeMost], block[kTreeMost], in_block[kTreeMost], count, last;
     __shared__ uint32_t disagree[kTreeWords];
     const int i = threadIdx.x, b = blockIdx.y;
-    const int n = min(max(p.lens[b], 0), kv_capacity(p.v));
+    const int n = max(p.lens[b], 0);                             // past the cache too: its rows lie where it says
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
     const long long row0 = static_cast<long long>(b) * p.T;
     int up = -1;

@@ -35,9 +35,9 @@ struct FastDiv {
     }
 };
 
-// A sequence's keys and its rows.
+// A sequence's keys, its rows, and the position of the first of these.
 struct Seq {
-    int n, cnt;
+    int n, cnt, base;
 };
 
 // Inclusive sum over the lanes up to this one.
@@ -75,7 +75,7 @@ __device__ __forceinline__ int even_size(int tiles, int count, int least) {
 // Chunk number w; b < 0 past the end. Called by whole waves.
 template <class P>
 __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows, int least) {
-    Chunk c{-1, 0, 0, 0, 0, 0, {0, 0}};
+    Chunk c{-1, 0, 0, 0, 0, 0, {0, 0, 0}};
     const int lane = threadIdx.x & 63, B = p.v.B;
     if (p.quota == 0 || B == 1) {
         const int b = p.quota ? 0 : w;
@@ -101,7 +101,7 @@ __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows,
     }
     // A lane a sequence; the last (for B <= 64 the only) 64 stay in registers.
     const int last = (B - 1) & ~63;
-    Seq s{0, 0};
+    Seq s{0, 0, 0};
     int a = 0, z = 0, total = 0;
     for (int b0 = 0; b0 <= last; b0 += 64) {
         a = z = 0;
@@ -156,6 +156,7 @@ __device__ __forceinline__ Chunk find_chunk(const P &p, int w, int r0, int rows,
             z = __builtin_amdgcn_readlane(z, l);
             c.seq.n = __builtin_amdgcn_readlane(s.n, l);
             c.seq.cnt = __builtin_amdgcn_readlane(s.cnt, l);
+            c.seq.base = __builtin_amdgcn_readlane(s.base, l);
             c.b = b0 + l;
             if constexpr (P::kEvenChunks) per = even_size(z - a, c.count, least);
             c.t0 = a + (w - c.first) * per;

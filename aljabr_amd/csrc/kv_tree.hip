@@ -189,7 +189,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
     if (p.quota && w == chunk.first && threadIdx.x == 0)
         p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.slot, chunk.count);
     const Seq seq = chunk.seq;
-    const int base = seq.n - seq.cnt, r1 = min(r0 + ROWS, seq.cnt * p.G);
+    const int base = seq.base, r1 = min(r0 + ROWS, seq.cnt * p.G);
 
     // The first tile's places, the tree's parents, the queries and then the tile: all on their way before any is used.
     const int tile0 = t0 < t1 ? min(t0 + wave, t1 - 1) : 0;            // a wave without a tile loads one that is there
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
     };
     auto query = [&](int c, int i) __attribute__((always_inline)) { return QLDS ? qlds[(c * QL + i) * 64] : qr[QLDS ? 0 : c][i]; };
     // Keys that every row sees: a tree's rows stand at most at their places.
-    const int full_lo = p.window > 0 ? base + p.by_g(r1 - 1) - p.window + 1 : 0;
-    const int full_hi = p.parents ? base : base + p.by_g(r0) + 1;
+    const int full_lo = window_start(p, base + p.by_g(r1 - 1) + 1);
+    const int full_hi = min(p.parents ? base : base + p.by_g(r0) + 1, seq.n);
 
     f32x4 o[NT][OT];
     float m[NT], l[NT];
@@ -691,7 +691,7 @@ int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
     // Within fp32's range with the scores' scaling, and to fp32 the same: past 2^64 a cap is none for every score that
     // softmax tells from its neighbours, below 2^-30 all weights are equal.
     p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;
-    p.window = std::min(a.window, 1 << 30);                // past every key; positions less it stay in 32 bits
+    p.window = a.window;
     const Plan plan = make_plan(v, a.T, a.Hq, p.window);
     if ((static_cast<double>(v.H) * (plan.quota + static_cast<double>(v.B)) + 7.0) * plan.groups > 0x7fffff)
         return fail(ALJABR_ROCM_ERR_UNSUPPORTED, "kv_tree_attention: T = %d rows of %d heads are more than one launch takes", a.T, a.Hq);

@@ -47,10 +47,13 @@ struct Params {
     int2 *chunks;                            // per sequence, KV head and row group: its first slot and its chunks
 };
 
+// The rows lie where the length says, also past the cache's end, where it has no keys: base + cnt may exceed n.
 __device__ __forceinline__ Seq sequence(const Params &p, int b) {
     Seq s;
-    s.n = min(max(p.lens[b], 0), kv_capacity(p.v));
+    const int len = max(p.lens[b], 0);
+    s.n = min(len, kv_capacity(p.v));
     s.cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+    s.base = len - s.cnt;
     return s;
 }
 
@@ -76,15 +79,23 @@ inline unsigned workgroups(const Params &p) {
 // Numbers KV heads and row groups for partials.
 __device__ __forceinline__ int item_of(const Params &p, int kvh, int group) { return group * p.v.H + kvh; }
 
+// The first position less than `window` before the one in front of `next`; 0 without a window. No number leaves 32 bits: a
+// position may be anything up to 2^31 - 2, and, with more rows than keys, below 0.
+__device__ __forceinline__ int window_start(const Params &p, int next) {
+    return p.window > 0 && next > p.window ? next - p.window : 0;
+}
+
 // The tiles that rows [r0, r0 + rows) see together. A row of a tree may stand anywhere between its root and its place,
 // so the window is taken from the root and the last key from the place.
 __device__ __forceinline__ bool row_tiles(const Params &p, const Seq &s, int r0, int rows, int &a, int &z) {
     a = z = 0;
     if (r0 >= s.cnt * p.G) return false;
-    const int base = s.n - s.cnt, hi = base + min(p.by_g(r0 + rows - 1), s.cnt - 1) + 1;
-    const int lo = p.window > 0 ? max(base + (p.parents ? 0 : p.by_g(r0)) - p.window + 1, 0) : 0;
-    a = lo >> p.tile_shift;
-    z = hi > lo ? (hi + (1 << p.tile_shift) - 1) >> p.tile_shift : a;
+    const int hi = min(s.base + min(p.by_g(r0 + rows - 1), s.cnt - 1) + 1, s.n);
+    const int lo = window_start(p, s.base + (p.parents ? 0 : p.by_g(r0)) + 1);
+    if (hi > lo) {                                           // else no tile, which past the end would not be there
+        a = lo >> p.tile_shift;
+        z = (hi + (1 << p.tile_shift) - 1) >> p.tile_shift;
+    }
     return true;
 }
 
@@ -93,10 +104,9 @@ struct Range {
     int lo, hi;
 };
 __device__ __forceinline__ Range range_of(const Params &p, const Seq &s, int t, const Tree &tree, bool filled) {
-    const int base = s.n - s.cnt;
     Range x;
-    x.hi = max(p.parents ? base : base + t + 1, 0);
-    x.lo = p.window > 0 ? max(base + (p.parents ? (filled ? tree.depth[t] : 0) : t) - p.window + 1, 0) : 0;
+    x.hi = min(max(p.parents ? s.base : s.base + t + 1, 0), s.n);
+    x.lo = window_start(p, s.base + (p.parents ? (filled ? tree.depth[t] : 0) : t) + 1);
     return x;
 }
 
@@ -105,13 +115,14 @@ __device__ __forceinline__ uint32_t seen(const Params &p, const Seq &s, const Ra
     const int a = max(x.lo - k0, 0), z = min(x.hi - k0, 32);
     uint32_t bits = z <= a ? 0 : (z == 32 ? 0xffffffffu : (1u << z) - 1) & ~((1u << a) - 1);
     if (p.parents) {
-        const int at = k0 - (s.n - s.cnt);                   // of the tree's rows
+        const int at = k0 - s.base;                          // of the tree's rows
         if (at >= 0 && at < s.cnt) {
             const int w = at >> 5;
             bits |= funnel_shift_right(w + 1 < kTreeWords ? tree.mask[(w + 1) * kTreeMost + t] : 0, tree.mask[w * kTreeMost + t], at & 31);
         } else if (at < 0 && at > -32) {
             bits |= tree.mask[t] << -at;
         }
+        if (s.n - k0 < 32) bits &= (1u << (s.n - k0)) - 1;   // rows past the end
     }
     return bits;
 }

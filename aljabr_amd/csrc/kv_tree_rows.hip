@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
     if (p.quota && w == chunk.first && tid == 0)
         p.chunks[static_cast<long long>(item) * p.v.B + b] = make_int2(chunk.slot, chunk.count);
     const Seq seq = chunk.seq;
-    const int base = seq.n - seq.cnt, r1 = min(r0 + kRowsBlock, seq.cnt * p.G), w0 = r0 + 32 * wave;
+    const int base = seq.base, r1 = min(r0 + kRowsBlock, seq.cnt * p.G), w0 = r0 + 32 * wave;
     const bool idle = w0 >= r1;                            // a wave without rows only copies
 
     const uint32_t ring = lds_address(lds);
@@ -189,8 +189,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
     const int t = p.by_g(r);
     const Range seen_range = range_of(p, seq, t, tree, filled);
     const int t_first = p.by_g(min(w0, r1 - 1)), t_last = p.by_g(min(w0 + 31, r1 - 1));
-    const int full_lo = p.window > 0 ? base + t_last - p.window + 1 : 0, full_hi = p.parents ? base : base + t_first + 1;
-    const int all_lo = p.window > 0 ? base + p.by_g(r1 - 1) - p.window + 1 : 0, all_hi = p.parents ? base : base + p.by_g(r0) + 1;
+    const int full_lo = window_start(p, base + t_last + 1), full_hi = min(p.parents ? base : base + t_first + 1, seq.n);
+    const int all_lo = window_start(p, base + p.by_g(r1 - 1) + 1), all_hi = min(p.parents ? base : base + p.by_g(r0) + 1, seq.n);
 
     // The row times scale * log2(e) as two fp16 parts: step s holds dims 16s + 8h .. + 7.
     half8 qh[STEPS], ql[STEPS];

@@ -348,7 +348,8 @@ int aljabr_rocm_kv4_attention_workspace(const aljabr_rocm_kv4_cache *cache, int 
  * of the sequence, any other number (-1) none; a row's line is the row and its
  * ancestors, its depth the number of those. Row t of sequence b lies at place
  * context_lens[b] - counts[b] + t of the cache, context_lens counting the
- * draft's rows too, and stands at position context_lens[b] - counts[b] + depth.
+ * draft's rows too (a negative one counts as 0), and stands at position
+ * context_lens[b] - counts[b] + depth, also where its place is past the end.
  * parents NULL: a chain, row t - 1 before row t (a decode step, a chunk of a
  * prompt). A tree has at most 256 rows (-3), a chain in attention any number.
  *
@@ -400,10 +401,10 @@ int aljabr_rocm_kv_append(const aljabr_rocm_kv_cache *cache, int layer, void *q_
 
 /* GQA attention of a draft's rows over a layer of the cache: Q and out
  * [sequences][T][Hq][head_dim] fp32, Hq a multiple of n_kv_heads. Of the
- * context_lens[b] keys (clamped to what the sequence can hold) the last
- * counts[b] (NULL: T) are the draft's rows. Row t sees the keys before those
- * and its line; with window > 0 only keys whose position is less than window
- * before its own. soft_cap > 0 caps scores as cap * tanh(score / cap); scale
+ * context_lens[b] keys the last counts[b] (NULL: T) are the draft's rows. Row t
+ * sees the keys before those and its line, as far as the cache has them; with
+ * window > 0 only keys whose position is less than window before its own.
+ * soft_cap > 0 caps scores as cap * tanh(score / cap); scale
  * <= 0: 1 / sqrt(head_dim). A row that sees no key (or none with a score above
  * -inf) gives zeros; rows from counts[b] on are left as they were. Keys on a
  * bad block are not seen, and what keys hold that a row does not see never
@@ -428,8 +429,11 @@ int aljabr_rocm_kv_tree_attention_workspace(const aljabr_rocm_kv_cache *cache, i
  * last (-1 for a sequence without rows), new_lens[b] = context_lens[b] -
  * counts[b] + accepted[b]. The accepted rows' K and V are moved to the first
  * places of the draft in every layer of the cache, where their positions say
- * they belong; what is behind them is left over. T is at most 256, the draft's
- * rows are different rows of the cache, and the outputs are none of the inputs. */
+ * they belong; what is behind them is left over. Tokens alone decide: a row
+ * that the cache does not have may be accepted, but has nothing to move, and in
+ * attention it did not see itself. Where a draft may reach past the cache's
+ * end, counts says how many of its rows fit. T is at most 256, the draft's rows
+ * are different rows of the cache, and the outputs are none of the inputs. */
 int aljabr_rocm_kv_tree_accept(const aljabr_rocm_kv_cache *cache, int *new_lens, int *path, int *accepted,
                                int *next_token, const int *context_lens, const int *counts, const int *parents,
                                const int *tokens, const int *choices, int T);

@@ -1,0 +1,141 @@
+"""fp16 and fp32 KV caches at their ends and limits: drafts that reach past the
+last place, numbers at the ends of their types."""
+from __future__ import annotations
+
+import copy
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import kv_plain as plain
+from test_gpu_kv_cache import F16, F32, POISON, ROOM, Device, agreeing, append, attend, check, check_planes, ints, normal, ptr, take
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- drafts that reach past the end of the cache ----------------------------------------
+
+def unending(host):
+    """The host's cache as one that goes on past its end, where it has no rows: what lengths say is then not cut."""
+    far = copy.copy(host)
+    far.cap = 1 << 30
+    far.at = host.at
+    return far
+
+
+def overhanging(cap, t):
+    """Lengths and counts of four sequences: three rows in the cache, one, none, and none with a gap before them."""
+    return [cap - 3 + t, cap - 1 + t, cap + t, cap + 9 + t], [t, t, t, max(t - 1, 1)]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("cap,page", [(32, 16), (37, 0), (144, 48), (129, 0)])
+@pytest.mark.parametrize("t,g", [(1, 4), (5, 2), (12, 4), (40, 3)])
+@pytest.mark.parametrize("window", [0, 4, 30])
+@pytest.mark.parametrize("tree", [0, 1])
+def test_attention_of_drafts_past_the_end(rocm, d, dtype, cap, page, t, g, window, tree):
+    host = plain.Cache(4, 2, d, cap, page, dtype)
+    host.fill([cap] * 4)
+    lens, counts = overhanging(cap, t)
+    parents = plain.random_parents(np.random.default_rng(t), 4, t, window == 30) if tree else None
+    q = normal(t, 4, t, 2 * g, d)
+    got = attend(rocm, Device(rocm, host), q, lens, counts, parents, window)
+    check(got, *plain.attention(unending(host), q, lens, counts, parents, window))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [0, 64])
+@pytest.mark.parametrize("window", [0, 16470])
+@pytest.mark.parametrize("tree", [0, 1])
+def test_attention_of_many_rows_past_the_end(rocm, d, page, window, tree):
+    """As above for the kernel that many rows over a large cache take."""
+    t, cap = 33, 16512
+    host = plain.Cache(2, 4, d, cap, page, F16)
+    host.fill([cap] * 2)
+    parents = plain.random_parents(np.random.default_rng(d), 2, t, True) if tree else None
+    q = normal(d, 2, t, 16, d)
+    for lens, counts in (([cap - 3 + t, cap - 20 + t], [t, t]), ([cap + t, cap + 9 + t], [t, t - 1])):
+        got = attend(rocm, Device(rocm, host), q, lens, counts, parents, window)
+        check(got, *plain.attention(unending(host), q, lens, counts, parents, window))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("t,tree", [(1, 0), (7, 0), (7, 1), (40, 1)])
+def test_lengths_far_past_the_end(rocm, dtype, t, tree):
+    """At the largest length every row sees the whole cache, or none of it through a window."""
+    host = plain.Cache(2, 2, 128, 70, 0, dtype)
+    host.fill([70, 70])
+    parents = plain.random_parents(np.random.default_rng(1), 2, t) if tree else None
+    q, lens = normal(t, 2, t, 8, 128), [2 ** 31 - 1, 2 ** 31 - 1]
+    dev = Device(rocm, host)
+    check(attend(rocm, dev, q, lens, None, parents), *plain.attention(unending(host), q, [1000] * 2, None, parents))
+    assert not attend(rocm, dev, q, lens, None, parents, 2 ** 30).any()
+    assert not attend(rocm, dev, q, lens, None, parents, 5).any()
+    assert np.array_equal(attend(rocm, dev, q, lens, None, parents, 2 ** 31 - 1), attend(rocm, dev, q, lens, None, parents))
+
+
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_accept_at_the_end_of_the_cache(rocm, page, dtype):
+    """29 committed rows of 32 and a draft of 5: row 2 is moved to the second place of the draft, no committed row changes."""
+    host = plain.Cache(1, 2, 64, 32, page, dtype, 3)
+    host.fill([32])
+    before = [host.rows_of(w, 0, 32, layer)[0] for w in "kv" for layer in range(3)]
+    dev = Device(rocm, host)
+    got = take(rocm, dev, [34], None, np.array([[-1, 0, 0, 1, 2]]), np.array([[9, 1, 2, 3, 4]]), np.array([[2, 0, 8, 0, 0]]))
+    assert [x.tolist() for x in got] == [[31], [[0, 2, -1, -1, -1]], [2], [8]]
+    host.planes = {w: dev.plane(w) for w in "kv"}
+    after = [host.rows_of(w, 0, 32, layer)[0] for w in "kv" for layer in range(3)]
+    for x, y in zip(before, after):
+        assert np.array_equal(x[:, :30], y[:, :30]) and np.array_equal(x[:, 31:], y[:, 31:])
+        assert np.array_equal(y[:, 30], x[:, 31])
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, F32), (256, F16)])
+@pytest.mark.parametrize("t,cap,page", [(5, 32, 16), (5, 33, 0), (33, 48, 16), (64, 100, 0), (256, 300, 0)])
+@pytest.mark.parametrize("deep", [0, 1])
+def test_accept_of_drafts_past_the_end(rocm, d, dtype, t, cap, page, deep):
+    rng = np.random.default_rng(t + d)
+    parents = plain.random_parents(rng, 6, t, bool(deep))
+    tokens, choices = agreeing(rng, parents, t, 0.97 if deep else 0.8, 4 if t < 9 else 50)
+    lens, counts = [*overhanging(cap, t)[0], cap + t // 2, 2 ** 31 - 1], [*overhanging(cap, t)[1], t, t]
+    host = plain.Cache(6, 3, d, cap, page, dtype, 2)
+    host.fill([host.cap] * 6)
+    dev = Device(rocm, host)
+    got = take(rocm, dev, lens, counts, parents, tokens, choices)
+    far = unending(host)
+    far.cap = 1 << 40
+    want = plain.accept(far, lens, counts, parents, tokens, choices)
+    for x, y in zip(got, want):
+        assert np.array_equal(x, y)
+    check_planes(dev)
+
+
+@pytest.mark.parametrize("page", [0, 16])
+def test_a_step_at_the_end_of_the_cache(rocm, page):
+    """Append, attention and accept of one draft that reaches past the end: they mean the same places."""
+    b, t, d, cap = 3, 12, 64, 64
+    rng = np.random.default_rng(page)
+    host = plain.Cache(b, 2, d, cap, page, F16)
+    base = [cap - 7, cap - 1, cap]
+    host.fill(base)
+    dev = Device(rocm, host)
+    parents = plain.random_parents(rng, b, t, True)
+    angles = np.array([[base[s] + len(plain.line(parents[s], i)) - 1 for i in range(t)] for s in range(b)])
+    q, k, v = normal(1, b, t, 8, d), normal(2, b, t, 2, d), normal(3, b, t, 2, d)
+    qd = append(rocm, dev, q, k, v, base, None, angles)
+    turned, off, live, k_bound = plain.append(host, q, k, v, base, None, angles)
+    assert (np.abs(qd - turned) <= off + 1e-30).all()
+    check_planes(dev, k_bound)
+    host.planes = {w: dev.plane(w) for w in "kv"}                      # from here on what the GPU's cache holds
+    lens = [x + t for x in base]
+    check(attend(rocm, dev, qd, lens, None, parents), *plain.attention(unending(host), qd, lens, None, parents))
+    tokens, choices = agreeing(rng, parents, t, 0.95)
+    got = take(rocm, dev, lens, None, parents, tokens, choices)
+    want = plain.accept(unending(host), lens, None, parents, tokens, choices)
+    for x, y in zip(got, want):
+        assert np.array_equal(x, y)
+    check_planes(dev)
