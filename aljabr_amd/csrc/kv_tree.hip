@@ -129,16 +129,15 @@ struct Query {
         for (int i = 0; i < D / 16; ++i) x[i] = *reinterpret_cast<const float4 *>(row + (F16 ? 32 * (i >> 1) + 8 * h + 4 * (i & 1) : 16 * i + 4 * h));
     }
     // The pieces that enter products: fp16 the two parts of each step, fp32 as it is, times scale. It was scaled by 2^(15 - e).
-    __device__ __forceinline__ void pieces(float scale, uint4 (&q)[Shape<F16, D>::kQuery], int &e) const {
+    __device__ __forceinline__ void pieces(const Params &p, uint4 (&q)[Shape<F16, D>::kQuery], int &e) const {
+        const float scale = p.scale;
         e = 15;
         if constexpr (F16) {
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
             top = group_max(top) * scale;
-            e = 0;
-            if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
-            e = e < -100 ? -100 : e;
+            e = query_exponent(p, top);
             const float up = ldexpf(1.0f, 15 - e);
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv_split_kernel(Pa
         row_info[wave][16 * c + n] = make_int4(t, range.lo, range.hi, 0);                      // the same of four lanes
         if (QLDS && c != wave) continue;
         int e;
-        raw[QLDS ? 0 : c].pieces(p.scale, qr[QLDS ? 0 : c], e);
+        raw[QLDS ? 0 : c].pieces(p, qr[QLDS ? 0 : c], e);
         unscale[c] = ldexpf(p.unscale, e - 15);
         if constexpr (QLDS) {
 #pragma unroll
@@ -687,7 +686,8 @@ int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {
     const double m = std::frexp(static_cast<double>(a.scale) * 1.4426950408889634, &k);
     const int in = std::min(std::max(k, -60), 100);
     p.scale = static_cast<float>(std::ldexp(m, in));
-    p.unscale = static_cast<float>(std::ldexp(1.0, k - in));
+    p.unscale = static_cast<float>(std::ldexp(1.0, k - in));           // at least 2^-88
+    p.least_exp = std::max(-100, 15 - 126 - (k - in));
     // Within fp32's range with the scores' scaling, and to fp32 the same: past 2^64 a cap is none for every score that
     // softmax tells from its neighbours, below 2^-30 all weights are equal.
     p.soft_cap = a.soft_cap > 0.0f ? std::min(std::max(a.soft_cap, 0x1p-30f), 0x1p64f) : 0.0f;

@@ -39,6 +39,7 @@ struct Params {
     FastDiv by_g, by_rows, by_chunks, by_heads, by_groups;             // G, rows of a block, quota (or sequences), H, row_groups
     int span_shift;                          // see work_at
     float scale, unscale;                    // their product is the call's scale times log2(e)
+    int least_exp;                           // of a scaled query row's largest, see query_exponent
     float soft_cap;
     int window;
     int tile_shift;                          // log2 of the keys of a tile
@@ -83,6 +84,15 @@ __device__ __forceinline__ int item_of(const Params &p, int kvh, int group) { re
 // position may be anything up to 2^31 - 2, and, with more rows than keys, below 0.
 __device__ __forceinline__ int window_start(const Params &p, int next) {
     return p.window > 0 && next > p.window ? next - p.window : 0;
+}
+
+// The e with which an fp16 cache's query row, times p.scale, is scaled by 2^(15 - e): its largest magnitude `top` is in
+// [2^(e-1), 2^e). Not less than p.least_exp, so that what scales the scores back, p.unscale 2^(e - 15), stays a normal number:
+// zero times a masked key's -inf would be NaN. Scores so small weigh all keys alike.
+__device__ __forceinline__ int query_exponent(const Params &p, float top) {
+    int e = 0;
+    if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);
+    return max(e, p.least_exp);
 }
 
 // The tiles that rows [r0, r0 + rows) see together. A row of a tree may stand anywhere between its root and its place,

@@ -211,9 +211,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
                                    fmaxf(fmaxf(fabsf(c.x), fabsf(c.y)), fmaxf(fabsf(c.z), fabsf(c.w)))));
         }
         top = fmaxf(top, __shfl_xor(top, 32)) * p.scale;
-        int e = 0;
-        if (top > 0.0f && top <= 3.4028235e38f) (void)frexpf(top, &e);     // top in [2^(e-1), 2^e)
-        e = e < -100 ? -100 : e;
+        const int e = query_exponent(p, top);
         const float up = ldexpf(1.0f, 15 - e);
         row_info[tid] = make_int4(t, seen_range.lo, seen_range.hi, __float_as_int(up));        // read by this thread alone
         unscale = ldexpf(p.unscale, e - 15);

@@ -139,3 +139,20 @@ def test_a_step_at_the_end_of_the_cache(rocm, page):
     for x, y in zip(got, want):
         assert np.array_equal(x, y)
     check_planes(dev)
+
+
+# ---- numbers at the ends of their types -------------------------------------------------
+
+@pytest.mark.parametrize("room", [0, ROOM])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("d,t,tree", [(64, 1, 0), (128, 5, 0), (128, 12, 1), (256, 1, 0), (64, 40, 1), (128, 40, 0), (256, 40, 1)])
+@pytest.mark.parametrize("scale,size", [(1e-38, 1e-3), (1e-44, 1.0), (1e-30, 1e-20), (1e-38, 1e-38), (1e-44, 3e38), (2e-20, 1e-30)])
+def test_small_scales_of_small_queries(rocm, room, dtype, d, t, tree, scale, size):
+    """Scores next to zero weigh all keys alike, and what a row does not see nothing."""
+    host = plain.Cache(2, 1, d, 208, 0, dtype)
+    host.fill([200, 77])
+    q = np.float32(size) * np.clip(normal(t, 2, t, 4, d), -1, 1)
+    parents = plain.random_parents(np.random.default_rng(t), 2, t) if tree else None
+    scale = float(np.float32(scale))
+    got = attend(rocm, Device(rocm, host, room), q, [200, 77], None, parents, scale=scale)
+    check(got, *plain.attention(host, q, [200, 77], None, parents, scale=scale))
