@@ -104,6 +104,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
     __shared__ Tree tree;
     __shared__ int4 row_info[kThreads];                    // of a lane's row: t, its range, the power of two it was scaled by
     __shared__ int odd_tile;                               // the last tile that held values which are not finite, plus 1
+    __shared__ uint32_t weighs[kThreads];                  // in such a tile, bits of a lane's 16 keys whose weight is not 0 in fp32
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, nl = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // For the paths that are rarely taken: the thread's number, of which the compiler keeps nothing in registers.
@@ -377,6 +378,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
                     m = to;
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
+                if (odd) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) bits |= __builtin_amdgcn_exp2f(fmaf(s[j], us, -ref)) > 0.0f ? 1u << j : 0;
+                    weighs[fresh_tid()] = bits;            // read by this thread alone
+                }
                 half8 va[2][2];
                 read_values(0, va[0]);
                 // The next tile's scores on the matrix cores, between them this one's weights.
@@ -425,7 +432,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
                 }
             }
             if (odd) {
-                // The values that were taken out, times the rows' weights, which go through the tile's LDS, 8 keys at once.
+                // The values that were taken out, times the rows' weights, which go through the tile's LDS, 8 keys at once. A
+                // weight that its two parts have lost is still not 0: an infinity times it is one.
                 float *wt = reinterpret_cast<float *>(vl) + wave * 256;
                 const int thread = fresh_tid(), h = thread >> 5 & 1, nl = thread & 31;
                 for (int q = 0; q < 4; ++q) {
@@ -437,7 +445,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
                         const float w1 = static_cast<float>(ph[0][4 + j]) + static_cast<float>(pl[0][4 + j]);
                         const float w2 = static_cast<float>(ph[1][j]) + static_cast<float>(pl[1][j]);
                         const float w3 = static_cast<float>(ph[1][4 + j]) + static_cast<float>(pl[1][4 + j]);
-                        wt[(4 * h + j) * 32 + nl] = q & 2 ? (q & 1 ? w3 : w2) : (q & 1 ? w1 : w0);
+                        const float w = q & 2 ? (q & 1 ? w3 : w2) : (q & 1 ? w1 : w0);
+                        wt[(4 * h + j) * 32 + nl] = w == 0.0f && (weighs[thread] >> (4 * q + j) & 1) ? 0x1p-126f : w;
                     }
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the wave's own writes
                     int keys = 8;
@@ -513,7 +522,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_rows_kernel(Params p) {
 template <int D>
 void launch(const Params &p, hipStream_t s) {
     using R = Rows<D>;
-    if (R::kBytes + sizeof(Tree) + kThreads * sizeof(int4) + 16 > 65536)
+    if (R::kBytes + sizeof(Tree) + kThreads * (sizeof(int4) + sizeof(uint32_t)) + 16 > 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_rows_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
     hipLaunchKernelGGL((kv_rows_kernel<D>), dim3(workgroups(p)), dim3(kThreads), R::kBytes, s, p);
     if (p.quota) launch_merge<D, kRowsBlock>(p, kRowsLeast * kTile, s);

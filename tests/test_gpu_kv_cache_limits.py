@@ -156,3 +156,29 @@ def test_small_scales_of_small_queries(rocm, room, dtype, d, t, tree, scale, siz
     scale = float(np.float32(scale))
     got = attend(rocm, Device(rocm, host, room), q, [200, 77], None, parents, scale=scale)
     check(got, *plain.attention(host, q, [200, 77], None, parents, scale=scale))
+
+
+@pytest.mark.parametrize("room", [0, ROOM])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,at", [(1, 40), (12, 40), (40, 40), (40, 95)])
+@pytest.mark.parametrize("less", [10, 30, 60])
+def test_infinite_values_of_small_weights(rocm, room, dtype, d, t, at, less):
+    """A value of a key whose score is far below the row's largest, `less` powers of e: its weight is not zero, and an
+    infinity times it stays one."""
+    n = 100
+    host = plain.Cache(1, 1, d, 128, 0, dtype)
+    host.fill([n])
+    host.planes["k"][0, 0, 0, :n, 7] = 0
+    host.planes["k"][0, 0, 0, at, :] = 0
+    host.planes["k"][0, 0, 0, at, 7] = -less
+    host.planes["v"][0, 0, 0, at, 33] = np.inf
+    host.planes["v"][0, 0, 0, at, 34] = -np.inf
+    q = 0.1 * normal(1000, 1, t, 4, d)
+    q[..., 7] = 1
+    want, bound, live = plain.attention(host, q, [n], scale=1.0)
+    got = attend(rocm, Device(rocm, host, room), q, [n], scale=1.0)
+    fine = np.isfinite(want)
+    assert (~fine).sum() == 2 * 4 * min(t, n - at)
+    assert np.array_equal(got[~fine], want[~fine].astype(np.float32))
+    assert (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
