@@ -408,9 +408,10 @@ int aljabr_rocm_kv_append(const aljabr_rocm_kv_cache *cache, int layer, void *q_
  * <= 0: 1 / sqrt(head_dim). A row that sees no key (or none with a score above
  * -inf) gives zeros; rows from counts[b] on are left as they were. Keys on a
  * bad block are not seen, and what keys hold that a row does not see never
- * reaches it. fp32-accurate. T * Hq is at most 2^30, sequences * the positions
- * of each at most 2^34, and a call of more workgroups than a launch takes is
- * refused (-3). workspace: device scratch for split partials, of
+ * reaches it. fp32-accurate; sums and weights are fp32 numbers (a weight below
+ * 2^-126 of the row's largest is 0). T * Hq is at most 2^30, sequences * the
+ * positions of each at most 2^34, and a call of more workgroups than a launch
+ * takes is refused (-3). workspace: device scratch for split partials, of
  * aljabr_rocm_kv_tree_attention_workspace bytes (fewer: fewer splits), not
  * shared by calls that may run at once, captured graphs among them. NULL: the
  * stream's scratch (no memory for it: no splits), which a call under stream
