@@ -608,8 +608,35 @@ void launch(const Params &p, int rows, hipStream_t s) {
 struct Plan {
     int rows, groups, tile, quota;
 };
-Plan make_plan(const KvView &v, int T, int Hq, int window) {
+
+// The plan with this many rows a workgroup, where the cache may hold so many bytes of visible keys.
+Plan plan_of(const KvView &v, int T, int Hq, int rows, double bytes) {
     Plan s;
+    s.rows = rows;
+    s.tile = v.f16 || v.D == 64 ? 32 : 16;
+    s.groups = static_cast<int>((static_cast<long long>(T) * (Hq / v.H) + rows - 1) / rows);
+    const long long items = static_cast<long long>(v.H) * s.groups;
+    const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    const int least = s.tile * kWaves;                     // keys of the smallest chunk (kRowsLeast tiles as well)
+    const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
+    // Workgroups a CU: with a second one the chunks are finer and one's waits are covered by the other, which is worth its
+    // partials where the bytes are many and either lengths may differ or row groups share the keys. Of 8 KV heads of 128,
+    // one and two a CU: 20 rows over 32 fp16 sequences of about 2100 keys 80 and 66 us, fp32 178 and 126 (of 4096 keys each
+    // 99 and 104); 48 rows over one of 131072 132 and 121, 20 rows 98 and 106; 64 rows over one of 8192 19.0 and 20.1; the
+    // rows kernel, 128 rows over 32 of 4096, 202 and 181. Heads of 256 fill a CU's registers with one.
+    const int per_cu = s.rows == kRowsBlock || (v.D < 256 && bytes >= 0x1p27 && (v.B > 1 || s.groups > 1)) ? 2 : 1;
+    s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
+    if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
+    return s;
+}
+
+// Bytes of the keys that the rows of a call may see.
+double seen_bytes(const KvView &v, int T, int window) {
+    const long long seen = window > 0 ? std::min<long long>(kv_capacity(v), static_cast<long long>(window) + T) : kv_capacity(v);
+    return static_cast<double>(v.B) * seen * v.H * v.D * (v.f16 ? 4 : 8);
+}
+
+Plan make_plan(const KvView &v, int T, int Hq, int window) {
     const long long rows = static_cast<long long>(T) * (Hq / v.H);
     // The lengths are on the device: rules go by what the cache may hold of visible keys. More rows a workgroup read a key
     // less often and start later. In us, 8 KV heads of 128 in fp16 filled to the end, in brackets w below:
@@ -629,26 +656,10 @@ Plan make_plan(const KvView &v, int T, int Hq, int window) {
     // fp32 and heads of 64 and 256 turn at the same w (of 259 shapes the rule is 0.3 % from the better choice, at most 8 %).
     // Heads of 256 in a rows kernel (a ring of 96 KB, one workgroup a CU) took longer throughout: 256 rows over 8192 keys 109
     // us, with 32 rows a workgroup 59.
-    const long long seen = window > 0 ? std::min<long long>(kv_capacity(v), static_cast<long long>(window) + T) : kv_capacity(v);
-    const double keys = static_cast<double>(v.B) * seen * v.H, bytes = keys * v.D * (v.f16 ? 4 : 8), w = keys * std::max(v.D, 128) * 4;
-    if (v.f16 && v.D < 256 && rows > 64 && rows * w > 0x1p33) s.rows = kRowsBlock;
-    else if (rows > 32 ? rows * w > 0x1p31 : rows > 16 && w >= 0x1p27) s.rows = 32;
-    else s.rows = 16;
-    s.tile = v.f16 || v.D == 64 ? 32 : 16;
-    s.groups = static_cast<int>((rows + s.rows - 1) / s.rows);
-    const long long items = static_cast<long long>(v.H) * s.groups;
-    const long long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    const int least = s.tile * kWaves;                     // keys of the smallest chunk (kRowsLeast tiles as well)
-    const long long most = (static_cast<long long>(kv_capacity(v)) + least - 1) / least;   // chunks of a sequence
-    // Workgroups a CU: with a second one the chunks are finer and one's waits are covered by the other, which is worth its
-    // partials where the bytes are many and either lengths may differ or row groups share the keys. Of 8 KV heads of 128,
-    // one and two a CU: 20 rows over 32 fp16 sequences of about 2100 keys 80 and 66 us, fp32 178 and 126 (of 4096 keys each
-    // 99 and 104); 48 rows over one of 131072 132 and 121, 20 rows 98 and 106; 64 rows over one of 8192 19.0 and 20.1; the
-    // rows kernel, 128 rows over 32 of 4096, 202 and 181. Heads of 256 fill a CU's registers with one.
-    const int per_cu = s.rows == kRowsBlock || (v.D < 256 && bytes >= 0x1p27 && (v.B > 1 || s.groups > 1)) ? 2 : 1;
-    s.quota = static_cast<int>(std::min(per_cu * cus / items, v.B * most));
-    if (s.quota <= 1 || most == 1) s.quota = 0;            // heads and row groups fill the chip, or no sequence is cut
-    return s;
+    const double bytes = seen_bytes(v, T, window), w = bytes / (v.D * (v.f16 ? 4 : 8)) * std::max(v.D, 128) * 4;
+    if (v.f16 && v.D < 256 && rows > 64 && rows * w > 0x1p33) return plan_of(v, T, Hq, kRowsBlock, bytes);
+    if (rows > 32 ? rows * w > 0x1p31 : rows > 16 && w >= 0x1p27) return plan_of(v, T, Hq, 32, bytes);
+    return plan_of(v, T, Hq, 16, bytes);
 }
 
 // Slots of partials that so many chunks need at the most: sequence b of x_b > 1 chunk sizes takes ceil(x_b), fewer
@@ -665,8 +676,16 @@ size_t partial_bytes(const KvView &v, const Plan &s, int quota) {
 }  // namespace
 
 size_t kv_tree_attention_scratch_bytes(const KvView &v, int T, int Hq) {
-    const Plan s = make_plan(v, T, Hq, 0);                 // with a window the partials are fewer
-    return s.quota ? partial_bytes(v, s, s.quota) : 0;
+    // Of the call without a window, or, as a window makes the visible keys fewer, of any plan for fewer: with fewer rows a
+    // workgroup there are more row groups, whose chunk table (and, in sequences of many chunks, slots) may be larger.
+    const double bytes = seen_bytes(v, T, 0);
+    size_t most = 0;
+    for (int rows : {16, 32, kRowsBlock}) {
+        if (rows > make_plan(v, T, Hq, 0).rows) break;
+        const Plan s = plan_of(v, T, Hq, rows, bytes);
+        if (s.quota) most = std::max(most, partial_bytes(v, s, s.quota));
+    }
+    return most;
 }
 
 int enqueue_kv_tree_attention(const KvView &v, const KvTreeAttention &a) {

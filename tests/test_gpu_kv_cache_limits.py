@@ -191,3 +191,30 @@ def test_infinite_values_of_small_weights(rocm, room, dtype, d, t, at, less, see
     rest = ~fine & ~ends
     assert (np.isnan(got[rest]) | (got[rest] == want[rest])).all()
     assert (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
+
+
+# ---- workspaces -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,t,g,d,cap", [(8, 5, 4, 128, 131072), (2, 8, 4, 64, 1 << 19), (8, 16, 4, 128, 65536), (4, 16, 8, 128, 65536),
+                                             (8, 6, 4, 256, 65536)])
+def test_the_advertised_workspace_is_enough_for_every_window(rocm, dtype, heads, t, g, d, cap):
+    """A window may change how a call's work is laid out: with the advertised bytes it is cut as with any larger workspace."""
+    page, blocks = 128, 64
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(blocks, heads, page, d, device="cuda", generator=gen).to([torch.float32, torch.float16][dtype]) for _ in "kv")
+    table = (torch.arange(cap // page, device="cuda", dtype=torch.int32) * 7 % blocks)[None].contiguous()
+    desc = rocm.KvCache(k.data_ptr(), v.data_ptr(), table.data_ptr(), dtype, 1, 1, heads, d, page, blocks, cap // page)
+    n = ctypes.c_size_t()
+    rocm.call("aljabr_rocm_kv_tree_attention_workspace", ctypes.byref(desc), t, heads * g, ctypes.byref(n))
+    assert n.value > 0
+    q, lens = torch.randn(1, t, heads * g, d, device="cuda", generator=gen), ints([cap - 5])
+    large = torch.zeros(2 * n.value + (1 << 20), dtype=torch.uint8, device="cuda")
+    outs = [torch.empty_like(q) for _ in "ab"]
+    for window in (0, cap - 1, cap // 2, cap // 4, 20000, 5000, 300, 20):
+        for out, size in zip(outs, (n.value, large.numel())):
+            torch.cuda.synchronize()
+            rocm.call("aljabr_rocm_kv_tree_attention", out.data_ptr(), q.data_ptr(), ctypes.byref(desc), 0, lens.data_ptr(), None, None, t,
+                      heads * g, 0.0, window, 0.0, large.data_ptr(), size)
+        torch.cuda.synchronize()
+        assert torch.equal(*outs), window
