@@ -218,3 +218,35 @@ def test_the_advertised_workspace_is_enough_for_every_window(rocm, dtype, heads,
                       heads * g, 0.0, window, 0.0, large.data_ptr(), size)
         torch.cuda.synchronize()
         assert torch.equal(*outs), window
+
+
+# ---- long chunks ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("page", [0, 16, 112])
+@pytest.mark.parametrize("t,g,room", [(1, 4, 0), (9, 2, 0), (20, 4, ROOM)])
+@pytest.mark.parametrize("odd", [0, 1])
+def test_one_chunk_of_many_keys(rocm, d, dtype, page, t, g, room, odd):
+    """A workspace too small to cut the keys: each workgroup walks through all of them, further than the addresses that
+    its lanes hold at once (the keys of 32 tiles a wave, or of 32 in all for many rows), blocks in any order, some of them
+    not there; odd: with values that are not finite, for which it walks them again."""
+    lens = [9841, 4300]
+    host = plain.Cache(2, 1, d, 9850, page, dtype)
+    host.fill(lens)
+    if page:
+        host.table[0, [2, 9000 // page]] = -1, host.s
+        host.table[1, 3000 // page] = -7
+    if odd:
+        host.write("v", 0, 7003, np.where(np.arange(d) == 5, np.inf, 1.0)[None])
+        host.write("v", 1, 4177, np.where(np.arange(d) == 50, np.nan, 1.0)[None])
+        host.write("k", 1, 4100, np.where(np.arange(d) == 3, -np.inf, 0.0)[None])
+    q = normal(t, 2, t, g, d)
+    q[1, ..., 3] = np.abs(q[1, ..., 3])
+    parents = plain.random_parents(np.random.default_rng(d), 2, t) if t > 1 else None
+    want, bound, live = plain.attention(host, q, lens, None, parents)
+    got = attend(rocm, Device(rocm, host, room), q, lens, None, parents, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+    fine = np.isfinite(want)
+    assert (~fine).sum() == (2 * t * g if odd else 0)
+    assert np.array_equal(got[~fine], want[~fine].astype(np.float32), equal_nan=True)
+    check(np.where(fine, got, 0), np.where(fine, want, 0), np.where(fine, bound, 0), live)
