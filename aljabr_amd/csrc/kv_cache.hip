@@ -5,14 +5,16 @@
 // interleaved, turned by theta = a base^(-2i/r) / divisor_i, the rest of the
 // row is copied. The angle is computed in fp64 as quarter turns, a times
 // base^(-2i/r) / divisor_i / (pi/2): its nearest integer picks the quadrant
-// exactly, and the rest, at most half a quarter, is what fp32 series take (at
-// a = 2^30 fp32 angles would be off by whole turns; here by 2^-25).
+// exactly, and the rest, at most half a quarter, is what fp32 series take. The
+// product and the frequency are rounded a few times by 2^-53 of the angle: at
+// a = 2^30, where fp32 angles would be off by whole turns, about 2^-22 radians.
 //
 // A row is D/8 lanes with two units of four values each, so that both halves
 // of four pairs meet in a lane; the row is on its way before its position and
 // angles are known. Bound by the bytes: 4 x 2048 tokens of 32 + 8 + 8 heads of
-// 128, fp32 to an fp16 cache, 41 to 46 us (5.0 to 5.6 TB/s, what a copy
-// reaches); one token of a sequence 3.5 us, a launch.
+// 128, fp32 to an fp16 cache, 66 us (369 MB, 5.6 TB/s, what a copy reaches;
+// four prompts of up to 2048, 231 MB in the mean, 36 to 51 us, part of it from
+// the last-level cache); one token of a sequence 3.5 to 4.3 us, a launch.
 //
 // Accept: a row is kept when it and all its ancestors up to row 0 agree with
 // the model, which the tree's masks say for all rows at once; a kept row's

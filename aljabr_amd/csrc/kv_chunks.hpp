@@ -1,7 +1,8 @@
 // kv_chunks.hpp - work cut along the keys, for attention over caches whose
 // lengths the host does not know: the cut of all sequences' keys into chunks
 // of one size, and the merge of the chunks' partials. Shared by the attention
-// over the 4-bit cache and over fp16 and fp32 caches.
+// over the 4-bit cache and over fp16 and fp32 caches (work_of and
+// merge_rows_kernel are the 4-bit cache's alone).
 //
 // P, a kernel's parameters, has the cache's view v (sequences B, KV heads H),
 // T, G, Hq, row_groups, quota, the dividers by_g, by_chunks (work_of: and by_items), the

@@ -22,7 +22,7 @@
 // 2100 keys, 8 KV heads of 128, 20 rows each, 57 to 68 us with the merge (4.1 to
 // 4.9 TB/s); an fp32 cache of 4 x 2048 keys, 64 rows a head, 32.6 us, of which its
 // products at fp32's rate are 14; short calls by the chain lengths - table - tile
-// - states - merge: 8 drafted rows over 512 keys 10.5 us.
+// - states - merge: 8 drafted rows over 512 keys 10.7 us.
 //
 // Precision: an fp16 K enters as it is against a query row scaled by a power of
 // two to a largest magnitude in [2^14, 2^15) and split into two fp16 parts

@@ -14,7 +14,8 @@
 //
 // Bound by the products: 256 rows of 8 KV heads of 128 over 8 x 8192 keys 157
 // us, 104 rows over 131072 keys 163 us, chunks of 512 rows of 32 heads over
-// 2 x 4096 keys 145 us, with the merges: 0.97 PFLOP/s with both parts, where the
+// 2 x 4096 keys 145 us, with the merges: of the rows that are there 0.88, 0.68
+// (104 of the 128 rows computed) and 0.95 PFLOP/s with both parts, where the
 // library's product of 8192^3 reaches 1.2. Matrix cores 44 % of the cycles, vector
 // ALU 42 %, both at once 20 %; under this load the clock falls to 2.0 GHz. Tiles
 // of both operands shared in LDS by 128 rows took 157 us of the chunks where the
