@@ -306,7 +306,8 @@ int aljabr_rocm_kv4_read(void *K, void *V, const aljabr_rocm_kv4_cache *cache, c
                          int T, long long stride_b, long long stride_t, long long stride_h, int type);
 /* GQA attention over the cache: Q and out [sequences][T][Hq][head_dim] fp32,
  * Hq a multiple of n_kv_heads. Sequence b has context_lens[b] keys (clamped to
- * what it can hold), the last counts[b] (NULL: T) of them its rows' own: row t
+ * what it can hold: lengths and counts leave out rows that kv4_write dropped),
+ * the last counts[b] (NULL: T) of them its rows' own: row t
  * sits at position p = context_lens[b] - counts[b] + t and sees keys j <= p
  * when is_causal, and j > p - window when window > 0. T = 1 decodes, a few
  * rows verify a draft, many are a prompt or a chunk of one. soft_cap > 0 caps
